@@ -147,7 +147,7 @@ def prepare(case, seed):
 def _prepare_copy(case, gen):
     n, page = case["pairs"], case["page"]
     n_pages = 2 * n + 3
-    # Layers x (K, V) pools of one allocation.
+    # Layers x (K, V) pools, as the cache allocates them.
     store = _rand(gen, case["layers"], 2, n_pages, case["kv_heads"], page, D)
     perm = torch.randperm(n_pages, generator=gen, device=DEV).to(torch.int32)
     slots = None
@@ -155,8 +155,8 @@ def _prepare_copy(case, gen):
         slots = torch.full((n,), case["slots"], dtype=torch.int32, device=DEV)
     elif case["slots"] < 0:
         slots = torch.randint(1, page, (n,), generator=gen, device=DEV).to(torch.int32)
-    return dict(case=case, store=store, pools=[(layer[0], layer[1]) for layer in store],
-                src=perm[:n].clone(), dst=perm[n:2 * n].clone(), slots=slots)
+    return dict(case=case, store=store, src=perm[:n].clone(), dst=perm[n:2 * n].clone(),
+                slots=slots)
 
 
 def _prepare_prefix(case, gen):
@@ -252,7 +252,7 @@ def _plain(s):
 def _own_copy(s):
     from qwenforge_amd import paged
 
-    paged.copy_pages(s["pools"], s["src"], s["dst"], slots=s["slots"])
+    paged.copy_pages(s["store"], s["src"], s["dst"], slots=s["slots"])
     return s["store"]
 
 
