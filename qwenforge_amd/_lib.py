@@ -1,5 +1,6 @@
 """ctypes binding of the C ABI in ``include/qf_attn.h``, ``include/qf_step.h``,
-``include/qf_wide.h``, ``include/qf_prefill.h``, ``include/qf_paged.h`` and ``include/qf_probe.h``.
+``include/qf_wide.h``, ``include/qf_prefill.h``, ``include/qf_paged.h``,
+``include/qf_prefix.h`` and ``include/qf_probe.h``.
 
 The shared object is built in-tree by ``qwenforge_amd.build``.  There is no
 fallback: if it is missing or does not load, every op raises.
@@ -265,6 +266,12 @@ SIGNATURES = {
         _vp, _i64, _f32,                # ws, ws_bytes, eps
         _i32, _i32, _i32, _i32, _i32,   # hidden_size, QH, KVH, D, I
         _vp,                            # stream
+    ],
+    # include/qf_prefix.h
+    "qf_copy_pages": [
+        C.POINTER(_vp), _i32, _i64, _i64, _i64,  # pools, n_pools, sp, sh, sn
+        _vp, _vp, _vp, _i32,            # src, dst, slots, n_pairs
+        _i32, _i32, _i32, _i32, _vp,    # n_pages, KVH, page_size, D, stream
     ],
     # include/qf_probe.h
     "qf_stream_read": [_vp, _i64, _vp, _i32, _vp],   # src, bytes, sink, workgroups, stream

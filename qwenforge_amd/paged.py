@@ -10,7 +10,8 @@ and can be admitted and retired independently.  The ops call the C ABI in
 ``include/qf_paged.h``; like ``ops``, nothing computes on the host.
 
 * ``PagedKvCache`` -- pools for every layer, the device block table and a
-  host free list of pages.
+  host free list of pages; rows forked from one another share whole pages.
+* ``copy_pages`` -- pages of every layer copied to other pages in one launch.
 * ``flash_decode_attention_paged`` / ``flash_decode_split_paged`` -- split-K
   decode (SE:834-874 semantics) through the block table.
 * ``rope_append_paged`` -- one-token RoPE + append at a per-row slot.
@@ -20,6 +21,8 @@ and can be admitted and retired independently.  The ops call the C ABI in
 """
 
 from __future__ import annotations
+
+import ctypes as C
 
 import torch
 
@@ -39,11 +42,19 @@ class PagedKvCache:
     """Page pools of ``layers`` layers plus the block table of up to ``max_rows`` rows.
 
     ``pools[i] = (k_pool, v_pool)``, each ``(n_pages, kv_heads, page_size, 64)``
-    fp16, zero-initialised.  ``table`` is ``(max_rows, pages_per_row)`` int32 on
-    the device; unmapped entries hold -1.  Pages are handed out from a host
-    free list (lowest id first); ``map_row`` / ``release_row`` update the
+    fp16, zero-initialised views of the one allocation ``store`` (layers, 2,
+    n_pages, kv_heads, page_size, 64).  ``table`` is ``(max_rows, pages_per_row)``
+    int32 on the device; unmapped entries hold -1.  Pages are handed out from a
+    host free list (lowest id first); ``map_row`` / ``release_row`` update the
     device table with one small copy each, so they belong between graph
     replays, not inside them.
+
+    ``fork_rows`` maps the whole pages of a row into other rows too: such a page
+    is shared, and goes back to the free list with the last row that holds it.
+    Nothing may be written to a shared page: a row that will write to slots it
+    shares takes the pages for itself first (``own_slots``).  The slots after a
+    fork's are its own.  Like ``map_row`` these belong between graph replays and
+    on the stream that the cache's kernels run on.
     """
 
     def __init__(self, layers: int, kv_heads: int, n_pages: int, page_size: int, max_rows: int,
@@ -56,12 +67,13 @@ class PagedKvCache:
         self.kv_heads = kv_heads
         self.pages_per_row = pages_per_row
         self.device = torch.device(device)
-        shape = (n_pages, kv_heads, page_size, HEAD_DIM)
-        self.pools = [(torch.zeros(shape, device=self.device, dtype=dtype),
-                       torch.zeros(shape, device=self.device, dtype=dtype)) for _ in range(layers)]
+        self.store = torch.zeros((layers, 2, n_pages, kv_heads, page_size, HEAD_DIM),
+                                 device=self.device, dtype=dtype)
+        self.pools = [(layer[0], layer[1]) for layer in self.store]
         self.table = torch.full((max_rows, pages_per_row), -1, device=self.device, dtype=torch.int32)
         self._free = list(range(n_pages))
         self._rows: dict[int, list[int]] = {}
+        self._holders = [0] * n_pages          # rows that hold each page
 
     @property
     def capacity(self) -> int:
@@ -85,18 +97,111 @@ class PagedKvCache:
             raise RuntimeError(f"page pool exhausted: need {need - len(pages)}, {len(self._free)} free")
         first = len(pages)
         while len(pages) < need:
-            pages.append(self._free.pop(0))
+            pages.append(self._take())
         if len(pages) > first:
             ids = torch.tensor(pages[first:], dtype=torch.int32)
             self.table[row, first:len(pages)].copy_(ids)
         return list(pages)
 
+    def _take(self) -> int:
+        page = self._free.pop(0)
+        self._holders[page] = 1
+        return page
+
     def release_row(self, row: int) -> None:
-        """Return the row's pages to the free list and unmap it."""
+        """Unmap the row and return the pages that no other row holds to the
+        free list."""
         pages = self._rows.pop(row, [])
-        self._free.extend(pages)
+        for page in pages:
+            self._holders[page] -= 1
+            if self._holders[page] == 0:
+                self._free.append(page)
         self._free.sort()
         self.table[row].fill_(-1)
+
+    def shared_pages(self, row: int) -> int:
+        """Pages of ``row`` that another row holds too."""
+        return sum(self._holders[p] > 1 for p in self._rows.get(row, []))
+
+    def fork_rows(self, src: int, rows, n_slots: int) -> None:
+        """Makes slots ``[0, n_slots)`` of row ``src`` those of every row of
+        ``rows`` (unmapped before): whole pages are shared, a partly filled last
+        page is copied into a page of the row's own, for all rows and layers in
+        one launch.  ``map_row`` then grows the rows as usual."""
+        rows = [int(r) for r in rows]
+        pages = self._rows.get(src, [])
+        if not 0 <= n_slots <= len(pages) * self.page_size:
+            raise ValueError(f"row {src} has {len(pages) * self.page_size} slots mapped, not {n_slots}")
+        if len(set(rows)) != len(rows) or any(
+                not 0 <= r < self.table.shape[0] or self._rows.get(r) for r in rows):
+            raise ValueError("rows to fork into must be distinct rows of the table with nothing mapped")
+        whole, rest = divmod(n_slots, self.page_size)
+        if rest and len(rows) > len(self._free):
+            raise RuntimeError(f"page pool exhausted: need {len(rows)}, {len(self._free)} free")
+        own = self._free[:len(rows)] if rest else []
+        if own:
+            copy_pages(self.store, [pages[whole]] * len(rows), own, slots=[rest] * len(rows))
+        for i, row in enumerate(rows):
+            if rest:
+                self._take()
+            for page in pages[:whole]:
+                self._holders[page] += 1
+            self._rows[row] = pages[:whole] + own[i:i + 1]
+        self._upload(rows)
+
+    def fork_row(self, src: int, row: int, n_slots: int) -> None:
+        """``fork_rows`` into one row."""
+        self.fork_rows(src, [row], n_slots)
+
+    def own_slots(self, row: int, first: int, n_slots: int) -> int:
+        """Gives ``row`` pages of its own for slots ``[first, first + n_slots)``,
+        copied from the shared ones it held there, so that it may write to them;
+        returns how many pages were copied."""
+        pages = self._rows.get(row, [])
+        if first < 0 or n_slots < 0 or first + n_slots > len(pages) * self.page_size:
+            raise ValueError(f"slots [{first}, {first + n_slots}) are not all mapped in row {row}")
+        if n_slots == 0:
+            return 0
+        at = [j for j in range(first // self.page_size, (first + n_slots - 1) // self.page_size + 1)
+              if self._holders[pages[j]] > 1]
+        if len(at) > len(self._free):
+            raise RuntimeError(f"page pool exhausted: need {len(at)}, {len(self._free)} free")
+        if at:
+            copy_pages(self.store, [pages[j] for j in at], self._free[:len(at)])
+            for j in at:
+                self._holders[pages[j]] -= 1
+                pages[j] = self._take()
+            self._upload([row])
+        return len(at)
+
+    def compact(self) -> int:
+        """Moves the pages in use to the lowest ids, so that the free ones are
+        the pool's end; returns how many moved.  Tables follow, shared pages
+        stay shared."""
+        used = [p for p, n in enumerate(self._holders) if n]
+        src = [p for p in used if p >= len(used)]
+        dst = [p for p in self._free if p < len(used)]
+        if not src:
+            return 0
+        copy_pages(self.store, src, dst)
+        to = dict(zip(src, dst))
+        for pages in self._rows.values():
+            pages[:] = [to.get(p, p) for p in pages]
+        for a, b in to.items():
+            self._holders[b], self._holders[a] = self._holders[a], 0
+        self._free = list(range(len(used), self.n_pages))
+        self._upload(self._rows)
+        return len(src)
+
+    def _upload(self, rows) -> None:
+        """The device table's entries of ``rows``, from the host lists, in one copy."""
+        rows = list(rows)
+        if not rows:
+            return
+        host = torch.full((len(rows), self.pages_per_row), -1, dtype=torch.int32)
+        for i, r in enumerate(rows):
+            host[i, :len(self._rows[r])] = torch.tensor(self._rows[r], dtype=torch.int32)
+        self.table.index_copy_(0, torch.tensor(rows, device=self.device), host.to(self.device))
 
     def gather(self, layer: int, row: int, length: int):
         """Slots ``[0, length)`` of ``row`` as dense ``(KVH, length, 64)`` K and V
@@ -140,6 +245,79 @@ def _slot_args(slots: torch.Tensor, batch: int, device):
     if slots.dim() != 1 or slots.numel() != batch:
         raise ValueError(f"slots must hold one slot per row ({batch})")
     return slots.data_ptr(), slots.stride(0)
+
+
+# --------------------------------------------------------------------------
+# page copies
+# --------------------------------------------------------------------------
+
+def _page_list(name: str, pages, n: int, low: int, high: int) -> list:
+    pages = [int(p) for p in pages]
+    if len(pages) != n or any(not low <= p < high for p in pages):
+        raise ValueError(f"{name} must be {n} whole numbers in [{low}, {high})")
+    return pages
+
+
+def copy_pages(pools, src, dst, slots=None) -> None:
+    """Page ``dst[i]`` becomes page ``src[i]`` -- its first ``slots[i]`` slots, all
+    of them without ``slots`` -- in every pool, in one launch.
+
+    ``pools``: a contiguous tensor (..., n_pages, KVH, P, 64) fp16 such as
+    ``PagedKvCache.store``, or a list of pools (n_pages, KVH, P, 64) of one
+    layout.  ``src``, ``dst`` and ``slots`` are all int32 device tensors (n,),
+    read when the kernel runs, or all sequences of ints.  Sequences are checked;
+    with device tensors a pair with a page outside the pool copies nothing, a
+    slot count is clamped to the page, and the caller sees to it that no page is
+    written twice or both written and read.
+    """
+    if isinstance(pools, torch.Tensor):
+        if pools.dim() < 4 or not pools.is_contiguous():
+            raise ValueError("pools must be a contiguous (..., n_pages, KVH, P, 64) tensor, or a list")
+        _require_cuda_fp16("pools", pools)
+        first, shape, stride = pools, pools.shape[-4:], pools.stride()[-4:]
+        count = pools.numel() // max(1, shape.numel())
+        step = 2 * shape.numel()
+        ptrs = range(pools.data_ptr(), pools.data_ptr() + count * step, step) if step else ()
+    else:
+        pools = list(pools)
+        if not pools:
+            raise ValueError("copy_pages needs at least one pool")
+        first = pools[0]
+        for t in pools:
+            _require_cuda_fp16("pool", t, 4)
+            if t.shape != first.shape or t.stride() != first.stride() or t.device != first.device:
+                raise ValueError("pools must have one shape, layout and device")
+        shape, stride = first.shape, first.stride()
+        count, ptrs = len(pools), [t.data_ptr() for t in pools]
+    n_pages, kvh, page, _ = shape
+    _check_page_size(page)
+    if count < 1 or n_pages < 1 or kvh < 1:
+        raise ValueError("copy_pages needs at least one pool, page and head")
+    given = [("src", src), ("dst", dst)] + ([("slots", slots)] if slots is not None else [])
+    if isinstance(src, torch.Tensor) and src.is_cuda:
+        n = src.numel()
+        for name, t in given:
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != first.device:
+                raise TypeError(f"{name} must be an int32 tensor on the pools' device, as src is")
+            if t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous ({n},)")
+        held = src, dst, slots
+    else:
+        if any(isinstance(t, torch.Tensor) and t.is_cuda for _, t in given):
+            raise TypeError("src, dst and slots must all be device tensors or all sequences of ints")
+        n = len(src)
+        a, b = _page_list("src", src, n, 0, n_pages), _page_list("dst", dst, n, 0, n_pages)
+        if len(set(b)) != n or set(a) & set(b):
+            raise ValueError("no page may be written twice, or both written and read")
+        rows = [a, b] + ([_page_list("slots", slots, n, 0, page + 1)] if slots is not None else [])
+        up = torch.tensor(rows, dtype=torch.int32).to(first.device)
+        held = up[0], up[1], up[2] if slots is not None else None
+    with torch.cuda.device(first.device):
+        rc = _lib.load().qf_copy_pages(
+            (C.c_void_p * count)(*ptrs), count, stride[0], stride[1], stride[2],
+            held[0].data_ptr(), held[1].data_ptr(), _ptr(held[2]), n, n_pages, kvh, page, HEAD_DIM,
+            _stream(first.device))
+    _lib.check(rc, "qf_copy_pages")
 
 
 # --------------------------------------------------------------------------
