@@ -273,6 +273,35 @@ SIGNATURES = {
         _vp, _vp, _vp, _i32,            # src, dst, slots, n_pairs
         _i32, _i32, _i32, _i32, _vp,    # n_pages, KVH, page_size, D, stream
     ],
+    "qf_decode_attn_prefix_workspace": [_i32, _i32, _i32, _i32, _i32],  # B, KVH, G, n_groups, cap
+    "qf_decode_attn_prefix_paged": [
+        _vp, _i64, _i64, _i64,          # q, q_sb, q_sh, q_sg
+        _vp, _i64, _i64, _i64,          # k_pool, kp_sp, kp_sh, kp_sn
+        _vp, _i64, _i64, _i64,          # v_pool, vp_sp, vp_sh, vp_sn
+        _vp, _i64, _i32, _i32, _i32,    # block_table, bt_sb, pages_per_row, n_pages, page_size
+        _vp, _vp, _i32,                 # prefix_rows, prefix_len, n_groups
+        _vp, _i64,                      # kv_last, kv_last_sb
+        _vp, _i64,                      # ws, ws_bytes
+        _vp, _i64, _i64, _i64,          # out, o_sb, o_sh, o_sg
+        _i32, _i32, _i32, _i32,         # B, KVH, G, D
+        _f32, _vp,                      # scale, stream
+    ],
+    "qf_prefill_extend_workspace": [_i32, _i32, _i32, _i32, _i32],      # B, QH, KVH, total, cap
+    "qf_prefill_extend_paged": [
+        _vp, _i64, _i64,                # q, q_sh, q_sn
+        _vp, _i64, _i64,                # k
+        _vp, _i64, _i64,                # v
+        _vp, _i32,                      # cu_seqlens, total
+        _vp, _i64,                      # context, ctx_sb
+        _vp, _vp, _i64,                 # cos, sin, cs_sn
+        _vp, _i64, _i64, _i64,          # k_pool
+        _vp, _i64, _i64, _i64,          # v_pool
+        _vp, _i64, _i32, _i32, _i32,    # block_table, bt_sb, pages_per_row, n_pages, page_size
+        _i32, _vp, _i64,                # cap, ws, ws_bytes
+        _vp, _i64, _i64,                # out, o_sh, o_sn
+        _i32, _i32, _i32, _i32,         # B, QH, KVH, D
+        _f32, _vp,                      # scale, stream
+    ],
     # include/qf_probe.h
     "qf_stream_read": [_vp, _i64, _vp, _i32, _vp],   # src, bytes, sink, workgroups, stream
     "qf_launch_probe": [_vp, _i64, _vp, _vp,          # src, bytes, index, sink
@@ -295,7 +324,8 @@ for _name in ("qf_decode_attn", "qf_decode_attn_paged"):
     SIGNATURES[_name + "_shared"] = SIGNATURES[_name]
 
 # Entry points that do not return an int status.
-RESTYPES = {"qf_error_string": C.c_char_p, "qf_prefill_layers_workspace": _i64}
+RESTYPES = {"qf_error_string": C.c_char_p, "qf_prefill_layers_workspace": _i64,
+            "qf_decode_attn_prefix_workspace": _i64, "qf_prefill_extend_workspace": _i64}
 
 _lock = threading.Lock()
 _lib: C.CDLL | None = None

@@ -1,0 +1,900 @@
+// Attention over spans of paged caches for gfx950: decode of a batch whose rows
+// share long prefixes, and new tokens behind cached ones.
+//
+// Both are softmax(q K^T) V over slots [0, lim) of a row's pages with a lim for
+// every query, and both are cut into units: up to kQB * 64 query rows (token,
+// query head of one kv head; the heads of a token are neighbours) times a range
+// of slots.  A unit leaves (sum p v, max, sum p), and span_merge_kernel joins
+// the ranges of each query:
+//   softmax over a union = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i.
+// Decode has two kinds of unit.  The shared slots of a group of rows are read
+// once per query tile of the whole group, the rows of a tile being the matrix
+// cores' columns; the slots behind them belong to one row, whose at most 16
+// queries are one column block, and the four waves of the workgroup take the
+// key tiles in turn.  New tokens are units of the first kind whose lim grows
+// with the token.
+//
+// Tiles of 64 keys go HBM -> LDS with direct-to-LDS loads and are read as in
+// lds_tile.h; scores and output are computed transposed (qf_common.h).  Slots
+// past a unit's last one read as zero, and masked slots count for nothing
+// whatever K and V hold there (masked_values).
+#include <algorithm>
+
+#include "lds_tile.h"
+#include "../../include/qf_prefix.h"
+
+namespace qf {
+namespace span {
+
+constexpr int kD = 64;
+constexpr int kBN = 64;                      // keys per tile
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+constexpr int kTileBytes = kBN * kRowBytes;  // of K or V
+constexpr int kMaxSplits = 64;               // of either kind of unit
+constexpr int kMinKeys = 128;                // least keys of a split
+
+struct Args {
+  const f16* q;
+  int64_t q_st, q_sh, q_sg;                  // token, kv head, query head of the kv head
+  const f16* k;
+  int64_t k_sp, k_sh, k_sn;
+  const f16* v;
+  int64_t v_sp, v_sh, v_sn;
+  const int32_t* table;
+  int64_t t_sb;
+  int log2p, n_pages, ppr;
+  // Segments: tokens [bounds[i], bounds[i + 1]) share their tiles.  Decode: a
+  // group of rows (a token is a row) with plen[i] shared slots, read from the
+  // pages of its first row; last[token] is the row's last slot.  Extension: the
+  // new tokens of row i behind last[i] cached slots.
+  const int32_t* bounds;
+  const int32_t* plen;
+  const int64_t* last;
+  int64_t last_sb;
+  int n_seg, tokens, KVH, G, cap;
+  int n_tiles, splits;                       // query tiles and splits of the grid's first units
+  int own_splits;                            // splits of each row's own slots (decode)
+  float* acc;                                // (token, kv head, split, query head, 64)
+  float2* ml;                                // (token, kv head, split, query head): max, sum
+  f16* out;
+  int64_t o_st, o_sh, o_sg;
+  float scale_log2;
+  const f16* cos;                            // per token: Q is rotated on its way in
+  const f16* sin;
+  int64_t cs_sn;
+};
+
+__device__ __forceinline__ int clampi(int64_t x, int lo, int hi) {
+  return (int)(x < lo ? lo : x > hi ? hi : x);
+}
+
+__device__ __forceinline__ int scan_max(int x, int n) {
+  const int lane = threadIdx.x & 63;
+  for (int d = 1; d < n; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x = max(x, y);
+  }
+  return x;
+}
+
+__device__ __forceinline__ int scan_sum(int x, int n) {
+  const int lane = threadIdx.x & 63;
+  for (int d = 1; d < n; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+// One segment: its tokens [lo, hi) and its index, -1 if there is none.
+struct Segment {
+  int index, lo, hi;
+};
+
+// Walks the segments 64 at a time and takes the first one for which `pick(lo,
+// hi, tiles ahead, its tiles)` is true, tiles holding tr query rows; `before`
+// becomes the tiles ahead of it.  Any contents of bounds give segments that ascend, do not
+// overlap and stay within the tokens.
+template <typename Pick>
+__device__ __forceinline__ Segment find_segment(const Args& a, int tr, int& before, Pick&& pick) {
+  const int lane = threadIdx.x & 63;
+  int top = 0;
+  before = 0;
+  for (int i0 = 0; i0 < a.n_seg; i0 += 64) {
+    const int n = min(a.n_seg - i0, 64);
+    const int i = i0 + min(lane, n - 1);
+    const int hi = scan_max(max(top, clampi(a.bounds[i + 1], 0, a.tokens)), n);
+    int lo = clampi(a.bounds[i], 0, a.tokens);
+    lo = max(max(top, scan_max(lo, n)), 0);
+    const int end = max(lo, hi);
+    const int tiles = lane < n ? ((end - lo) * a.G + tr - 1) / tr : 0;
+    const int upto = scan_sum(tiles, n);
+    const uint64_t hit = __ballot(lane < n && pick(lo, end, before + upto - tiles, tiles));
+    if (hit != 0) {
+      const int j = __builtin_ctzll(hit);
+      before += __builtin_amdgcn_readlane(upto - tiles, j);
+      return {i0 + j, __builtin_amdgcn_readlane(lo, j), __builtin_amdgcn_readlane(end, j)};
+    }
+    before += __builtin_amdgcn_readlane(upto, n - 1);
+    top = __builtin_amdgcn_readlane(end, n - 1);
+  }
+  return {-1, 0, 0};
+}
+
+// A range of slots of a row's pages, read tile by tile.
+struct Source {
+  const unsigned char* k;  // pool + kv head
+  const unsigned char* v;
+  const int32_t* row;      // block table row
+  int64_t k_sp, k_sn, v_sp, v_sn;  // bytes
+  int pid, pwin;           // lane j: page of logical page pwin + j
+  int log2p, ppr, n_pages;
+  int end;                 // slots from here on read as zero
+};
+
+__device__ __forceinline__ void load_pids(Source& s, int win) {
+  const int j = min(win + (int)(threadIdx.x & 63), s.ppr - 1);
+  s.pid = min(max(s.row[j], 0), s.n_pages - 1);
+  s.pwin = win;
+}
+
+// Async loads of kRows rows from row r0 of the tile at slot0 (a multiple of 64,
+// below s.end) into the K and V tiles at Kd and Vd; a lane's byte offsets within
+// 8 rows are ko, vo for even and odd groups of 8 (the swizzle differs).
+template <int kRows>
+__device__ __forceinline__ void issue(Source& s, int slot0, int r0, unsigned char* Kd,
+                                      unsigned char* Vd) {
+  const int lane = threadIdx.x & 63;
+  const int lp = slot0 >> s.log2p;
+  if (lp < s.pwin || lp - s.pwin >= 64) load_pids(s, lp);
+  const int page = __builtin_amdgcn_readlane(s.pid, lp - s.pwin);
+  const int in_page = slot0 & ((1 << s.log2p) - 1);
+  const int64_t rows = s.end - slot0;
+  const __amdgpu_buffer_rsrc_t rk =
+      tile_rsrc(s.k + (int64_t)page * s.k_sp + in_page * s.k_sn, rows * s.k_sn);
+  const __amdgpu_buffer_rsrc_t rv =
+      tile_rsrc(s.v + (int64_t)page * s.v_sp + in_page * s.v_sn, rows * s.v_sn);
+#pragma unroll
+  for (int i = 0; i < kRows / 8; ++i) {
+    const int r = r0 + 8 * i + (lane >> 3);
+    const int c = 16 * ((lane & 7) ^ swz(r));
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(Kd + (r0 + 8 * i) * kRowBytes), 16,
+                                             r * (int)s.k_sn + c, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(Vd + (r0 + 8 * i) * kRowBytes), 16,
+                                             r * (int)s.v_sn + c, 0, 0, 0);
+  }
+}
+
+// The softmax state of kQB blocks of 16 query columns of one wave.
+template <int kQB>
+struct State {
+  f16x8 q[kQB][2];
+  int lim[kQB];     // the column sees slots [lo, lim)
+  int lo;
+  float m[kQB];     // running reference, log2 units
+  f32x4 l[kQB];     // running sum of p, in every row of the column
+  f32x4 o[kQB][4];
+  float ks2;
+  int koff[2], voff[4];  // operand addresses within a tile
+};
+
+template <int kQB>
+__device__ __forceinline__ void init_state(State<kQB>& s, int lo, float scale_log2) {
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  s.lo = lo;
+  s.ks2 = scale_log2;
+  const int rk = 8 * (col >> 2) + (col & 3);
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) s.koff[kk] = rk * kRowBytes + 16 * ((grp + 4 * kk) ^ swz(rk));
+  const int rv = 8 * grp + (col >> 2);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int d = 16 * t + 4 * (col & 3);
+    s.voff[t] = rv * kRowBytes + 16 * ((d >> 3) ^ swz(rv)) + 2 * (d & 7);
+  }
+#pragma unroll
+  for (int b = 0; b < kQB; ++b) {
+    s.m[b] = kNegInf;
+    s.l[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) s.o[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+__device__ __forceinline__ bool special2(unsigned w) {  // either half an infinity or NaN
+  return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+}
+
+// The infinities and NaNs of a masked tile's V: out of the operands, so that a
+// masked slot's zero probability meets zeros, and into the output only where
+// the column sees the slot.  p of key 32 ch + 8 g + e of the tile is element e
+// of pb[ch] in the column's lane of group g.
+template <int kQB>
+__device__ __forceinline__ void masked_values(u32x2 (&vr)[2][4][2], const State<kQB>& s,
+                                              const f16x8 (&pb)[kQB][2], int key0, f32x4 (&o)[kQB][4],
+                                              const unsigned char* Vs) {
+#pragma unroll
+  for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          unsigned w = vr[ch][t][h][x];
+          if ((w & 0x7C00u) == 0x7C00u) w &= 0xFFFF0000u;
+          if ((w & 0x7C000000u) == 0x7C000000u) w &= 0xFFFFu;
+          vr[ch][t][h][x] = w;
+        }
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+#pragma unroll
+  for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      for (int g = 0; g < 4; ++g) {
+        const int j = 32 * ch + 8 * g + e;
+#pragma unroll
+        for (int b = 0; b < kQB; ++b) {
+          const float p = __shfl((float)pb[b][ch][e], col + 16 * g);
+          if (key0 + j < s.lo || key0 + j >= s.lim[b]) continue;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int d = 16 * t + 4 * grp + i;
+              const f16 v = *reinterpret_cast<const f16*>(Vs + j * kRowBytes +
+                                                          16 * ((d >> 3) ^ swz(j)) + 2 * (d & 7));
+              const float x = (float)v;
+              if (!(__builtin_fabsf(x) < __builtin_huge_valf())) o[b][t][i] += p * x;
+            }
+        }
+      }
+}
+
+// Scores, online softmax and PV product of the tile of keys [key0, key0 + 64)
+// in (Ks, Vs), whose loads have landed; `refill` runs once the K operands are
+// in registers.  p is rounded to fp16 for the matrix cores (relative error
+// 2^-11, as large as that of the fp16 V it meets), and the sum l adds the
+// rounded p, so that the weights add to one.
+template <int kQB, typename Refill>
+__device__ __forceinline__ void tile_step(State<kQB>& s, int key0, const unsigned char* Ks,
+                                          const unsigned char* Vs, Refill&& refill) {
+  const int grp = (threadIdx.x & 63) >> 4;
+  const unsigned ks = lds_addr(Ks), vs = lds_addr(Vs);
+  u32x4 kr[2][2][2];
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    const unsigned ka0 = ks + s.koff[kk];
+    kr[0][0][kk] = lds_read_b128<0>(ka0);
+    kr[0][1][kk] = lds_read_b128<4 * kRowBytes>(ka0);
+    kr[1][0][kk] = lds_read_b128<32 * kRowBytes>(ka0);
+    kr[1][1][kk] = lds_read_b128<36 * kRowBytes>(ka0);
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)"
+               : "+v"(kr[0][0][0]), "+v"(kr[0][0][1]), "+v"(kr[0][1][0]), "+v"(kr[0][1][1]),
+                 "+v"(kr[1][0][0]), "+v"(kr[1][0][1]), "+v"(kr[1][1][0]), "+v"(kr[1][1][1]));
+  u32x2 vr[2][4][2];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const unsigned va0 = vs + s.voff[t];
+    vr[0][t][0] = lds_read_tr_b64<0>(va0);
+    vr[0][t][1] = lds_read_tr_b64<4 * kRowBytes>(va0);
+    vr[1][t][0] = lds_read_tr_b64<32 * kRowBytes>(va0);
+    vr[1][t][1] = lds_read_tr_b64<36 * kRowBytes>(va0);
+  }
+  refill();
+  bool masked = key0 < s.lo;
+#pragma unroll
+  for (int b = 0; b < kQB; ++b) masked = masked || __any(s.lim[b] < key0 + kBN);
+  f16x8 pb[kQB][2];
+#pragma unroll
+  for (int b = 0; b < kQB; ++b) {
+    f32x4 sc[4];
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        acc = mfma16x16x32(__builtin_bit_cast(f16x8, kr[ch][j][0]), s.q[b][0], acc);
+        sc[2 * ch + j] = mfma16x16x32(__builtin_bit_cast(f16x8, kr[ch][j][1]), s.q[b][1], acc);
+      }
+    if (masked) {
+#pragma unroll
+      for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + 32 * (blk >> 1) + 8 * grp + 4 * (blk & 1) + i;
+          if (key < s.lo || key >= s.lim[b]) sc[blk][i] = kNegInf;
+        }
+    }
+    const float mx = max16(sc) * s.ks2;
+    if (__any(mx > s.m[b] + kRescaleSlack)) {
+      const float m_new = fmaxf(s.m[b], col_max(mx));
+      const float r = m_new == kNegInf ? 1.f : fast_exp2(s.m[b] - m_new);
+      s.l[b] *= r;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) s.o[b][t] *= r;
+      s.m[b] = m_new;
+    }
+    const float neg_m = s.m[b] == kNegInf ? 0.f : -s.m[b];
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = fast_exp2(__builtin_fmaf(sc[blk][i], s.ks2, neg_m));
+        pb[b][blk >> 1][4 * (blk & 1) + i] = (f16)p;
+      }
+    const f16x8 ones = {(f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f};
+    s.l[b] = mfma16x16x32(ones, pb[b][0], s.l[b]);
+    s.l[b] = mfma16x16x32(ones, pb[b][1], s.l[b]);
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)"
+               : "+v"(vr[0][0][0]), "+v"(vr[0][0][1]), "+v"(vr[0][1][0]), "+v"(vr[0][1][1]),
+                 "+v"(vr[0][2][0]), "+v"(vr[0][2][1]), "+v"(vr[0][3][0]), "+v"(vr[0][3][1]),
+                 "+v"(vr[1][0][0]), "+v"(vr[1][0][1]), "+v"(vr[1][1][0]), "+v"(vr[1][1][1]),
+                 "+v"(vr[1][2][0]), "+v"(vr[1][2][1]), "+v"(vr[1][3][0]), "+v"(vr[1][3][1]));
+  if (masked) {
+    bool bad = false;
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) bad = bad || special2(vr[ch][t][h][0]) || special2(vr[ch][t][h][1]);
+    if (__any(bad)) masked_values<kQB>(vr, s, pb, key0, s.o, Vs);
+  }
+#pragma unroll
+  for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const u32x4 w = {vr[ch][t][0][0], vr[ch][t][0][1], vr[ch][t][1][0], vr[ch][t][1][1]};
+      const f16x8 va = __builtin_bit_cast(f16x8, w);
+#pragma unroll
+      for (int b = 0; b < kQB; ++b) s.o[b][t] = mfma16x16x32(va, pb[b][ch], s.o[b][t]);
+    }
+}
+
+// This wave's loads have landed, and after the barrier every wave's.
+__device__ __forceinline__ void stage_ready() {
+  s_waitcnt_vm(0);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_barrier();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// One unit: query rows r0 .. of a segment's (token, query head) rows against
+// slots [k0, k1) of table row trow.
+struct Unit {
+  int tok0, rows;     // the segment's first token, its query rows
+  int r0, hk, trow;
+  int k0, k1;
+  int ctx;            // extension: cached slots of the row; decode: -1
+  int split, n_split; // place among each query's partials; n_split = 0: the output itself
+};
+
+__device__ __forceinline__ Source make_source(const Args& a, const Unit& u) {
+  Source s;
+  s.k = reinterpret_cast<const unsigned char*>(a.k + u.hk * a.k_sh);
+  s.v = reinterpret_cast<const unsigned char*>(a.v + u.hk * a.v_sh);
+  s.row = a.table + (int64_t)u.trow * a.t_sb;
+  s.k_sp = a.k_sp * 2; s.k_sn = a.k_sn * 2;
+  s.v_sp = a.v_sp * 2; s.v_sn = a.v_sn * 2;
+  s.log2p = a.log2p; s.ppr = a.ppr; s.n_pages = a.n_pages;
+  s.end = u.k1;
+  return s;
+}
+
+// Query row r of the unit's segment: its token, query head, and bound.
+__device__ __forceinline__ int row_limit(const Args& a, const Unit& u, int token) {
+  if (u.ctx >= 0) return min(u.ctx + (token - u.tok0) + 1, u.k1);
+  return min(clampi(a.last[token * a.last_sb], -1, a.cap - 1) + 1, u.k1);
+}
+
+__device__ __forceinline__ int64_t part_index(const Args& a, const Unit& u, int token, int g) {
+  return (((int64_t)token * a.KVH + u.hk) * u.n_split + u.split) * a.G + g;
+}
+
+template <int kQB>
+__device__ __forceinline__ void load_queries(State<kQB>& s, const Args& a, const Unit& u, int first) {
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+#pragma unroll
+  for (int b = 0; b < kQB; ++b) {
+    const int r = first + 16 * b + col;
+    const int rr = min(r, u.rows - 1);
+    const int token = u.tok0 + rr / a.G, g = rr % a.G;
+    const f16* qp = a.q + token * a.q_st + u.hk * a.q_sh + g * a.q_sg + 8 * grp;
+    s.q[b][0] = load16(qp);
+    s.q[b][1] = load16(qp + 32);
+    if (a.cos != nullptr) {
+      const int64_t co = token * a.cs_sn + 8 * grp;
+      rope_pair(s.q[b][0], s.q[b][1], load16(a.cos + co), load16(a.sin + co),
+                load16(a.cos + co + 32), load16(a.sin + co + 32));
+    }
+    s.lim[b] = r < u.rows ? row_limit(a, u, token) : u.k1;
+  }
+}
+
+// o / l of a column, zero where nothing was seen.
+__device__ __forceinline__ void store_out(const Args& a, int token, int hk, int g, int d, f32x4 o,
+                                          float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const f16x4 r = {(f16)(o[0] * inv), (f16)(o[1] * inv), (f16)(o[2] * inv), (f16)(o[3] * inv)};
+  *reinterpret_cast<f16x4*>(a.out + token * a.o_st + hk * a.o_sh + g * a.o_sg + d) = r;
+}
+
+__device__ __forceinline__ void store_part(const Args& a, const Unit& u, int r, int t, f32x4 o,
+                                           float m, float l, bool stats) {
+  const int grp = (threadIdx.x & 63) >> 4;
+  if (r >= u.rows) return;
+  const int token = u.tok0 + r / a.G, g = r % a.G;
+  if (u.n_split == 0) {
+    store_out(a, token, u.hk, g, 16 * t + 4 * grp, o, l);
+    return;
+  }
+  const int64_t p = part_index(a, u, token, g);
+  *reinterpret_cast<f32x4*>(a.acc + p * kD + 16 * t + 4 * grp) = o;
+  if (stats && grp == 0) a.ml[p] = float2{m, l};
+}
+
+// A unit with no slot: every query's partial is absent (l = 0), the output zero.
+__device__ __forceinline__ void empty_unit(const Args& a, const Unit& u, int n_rows) {
+  for (int i = threadIdx.x; i < n_rows * 16; i += kThreads) {
+    const int r = u.r0 + (i >> 4), d = 4 * (i & 15);
+    if (r >= u.rows) break;
+    const int token = u.tok0 + r / a.G, g = r % a.G;
+    if (u.n_split == 0) store_out(a, token, u.hk, g, d, f32x4{0.f, 0.f, 0.f, 0.f}, 0.f);
+    else if (d == 0) a.ml[part_index(a, u, token, g)] = float2{kNegInf, 0.f};
+  }
+}
+
+// kQB * 64 query rows, kQB * 16 per wave; the waves share the key tiles, which
+// are double-buffered.
+template <int kQB>
+__device__ __forceinline__ void wide_unit(const Args& a, const Unit& u, unsigned char* lds) {
+  if (u.k1 <= u.k0) {
+    empty_unit(a, u, kQB * 64);
+    return;
+  }
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const auto stage = [&](int i, int kv) { return lds + ((i & 1) * 2 + kv) * kTileBytes; };
+  Source src = make_source(a, u);
+  const int first = u.k0 & ~(kBN - 1);
+  const int n = (u.k1 - first + kBN - 1) / kBN;
+  load_pids(src, first >> a.log2p);
+  issue<16>(src, first, 16 * w, stage(0, 0), stage(0, 1));
+  State<kQB> s;
+  init_state(s, u.k0, a.scale_log2);
+  const int row0 = u.r0 + w * kQB * 16;
+  load_queries(s, a, u, row0);
+  for (int i = 0; i < n; ++i) {
+    // Every wave is past tile i - 1, whose stage takes tile i + 1.
+    stage_ready();
+    tile_step(s, first + i * kBN, stage(i, 0), stage(i, 1), [&] {
+      if (i + 1 < n)
+        issue<16>(src, first + (i + 1) * kBN, 16 * w, stage(i + 1, 0), stage(i + 1, 1));
+    });
+  }
+  const int col = threadIdx.x & 15;
+#pragma unroll
+  for (int b = 0; b < kQB; ++b)
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      store_part(a, u, row0 + 16 * b + col, t, s.o[b][t], s.m[b], s.l[b][0], t == 0);
+}
+
+// At most 16 query rows; the waves take the key tiles in turn and join their
+// states in LDS.
+__device__ __forceinline__ void narrow_unit(const Args& a, const Unit& u, unsigned char* lds) {
+  if (u.k1 <= u.k0) {
+    empty_unit(a, u, 16);
+    return;
+  }
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  unsigned char* Ks = lds + w * 2 * kTileBytes;
+  unsigned char* Vs = Ks + kTileBytes;
+  Source src = make_source(a, u);
+  const int first = u.k0 & ~(kBN - 1);
+  const int n = (u.k1 - first + kBN - 1) / kBN;
+  if (w < n) {
+    load_pids(src, (first + w * kBN) >> a.log2p);
+    issue<64>(src, first + w * kBN, 0, Ks, Vs);
+  }
+  State<1> s;
+  init_state(s, u.k0, a.scale_log2);
+  load_queries(s, a, u, u.r0);
+  for (int i = w; i < n; i += kWaves) {
+    s_waitcnt_vm(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    tile_step(s, first + i * kBN, Ks, Vs, [] {});
+    // The tile's reads are done: its LDS takes the wave's next one.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (i + kWaves < n) issue<64>(src, first + (i + kWaves) * kBN, 0, Ks, Vs);
+  }
+  __syncthreads();
+  f32x4* so = reinterpret_cast<f32x4*>(lds);                              // [wave][d tile][lane]
+  float2* sml = reinterpret_cast<float2*>(lds + kWaves * 4 * 64 * 16);    // [wave][lane]
+#pragma unroll
+  for (int t = 0; t < 4; ++t) so[(w * 4 + t) * 64 + lane] = s.o[0][t];
+  sml[w * 64 + lane] = float2{s.m[0], s.l[0][0]};
+  __syncthreads();
+  // Wave w joins dims 16 w .. 16 w + 15.
+  float m[kWaves], l[kWaves], top = kNegInf;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const float2 x = sml[i * 64 + lane];
+    m[i] = x.x;
+    l[i] = x.y;
+    top = fmaxf(top, x.x);
+  }
+  float sum = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (l[i] == 0.f) continue;
+    const float r = m[i] == top ? 1.f : fast_exp2(m[i] - top);
+    sum += l[i] * r;
+    o += so[(i * 4 + w) * 64 + lane] * r;
+  }
+  store_part(a, u, u.r0 + (lane & 15), w, o, top, sum, w == 0);
+}
+
+// Slots [k0, k1) of split s of `n` splits over [lo, hi), cut at multiples of 64.
+__device__ __forceinline__ void cut(int lo, int hi, int s, int n, int& k0, int& k1) {
+  const int first = lo & ~(kBN - 1);
+  const int len = max((int)(((int64_t)hi - first + n * kBN - 1) / (n * kBN)) * kBN, kMinKeys);
+  const int64_t at = first + (int64_t)s * len;
+  k0 = (int)(at < hi ? (s == 0 ? lo : at) : hi);
+  k1 = (int)(at + len < hi ? at + len : hi);
+}
+
+// kForm: 0 narrow units, 1 and 2 wide ones of 64 kForm query rows.  Decode: the
+// grid's first n_tiles * KVH * splits workgroups take the shared slots, the
+// others one row's own slots each.
+template <int kForm, bool kDecode>
+__global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kWaves * 2 * kTileBytes];
+  constexpr int kTr = kForm == 0 ? 16 : 64 * kForm;
+  const int n_first = a.n_tiles * a.KVH * a.splits;
+  Unit u;
+  u.ctx = -1;
+  u.n_split = kDecode ? a.splits + a.own_splits : a.splits > 1 ? a.splits : 0;
+  int before;
+  if (!kDecode || (int)blockIdx.x < n_first) {
+    const int tile = blockIdx.x % a.n_tiles, rest = blockIdx.x / a.n_tiles;
+    u.hk = rest % a.KVH;
+    u.split = rest / a.KVH;
+    const Segment g = find_segment(a, kTr, before, [&](int, int, int ahead, int tiles) {
+      return tile < ahead + tiles;
+    });
+    if (g.index < 0) return;
+    u.tok0 = g.lo;
+    u.rows = (g.hi - g.lo) * a.G;
+    u.r0 = (tile - before) * kTr;
+    int end;
+    if (kDecode) {
+      u.trow = g.lo;
+      end = clampi(a.plen[g.index], 0, a.cap);
+    } else {
+      u.trow = g.index;
+      u.ctx = clampi(a.last[g.index * a.last_sb], -1, a.cap);
+      const int newest = (min(u.r0 + kTr, u.rows) - 1) / a.G;   // last token of the tile
+      end = u.ctx < 0 ? 0 : min(u.ctx + newest + 1, a.cap);
+    }
+    cut(0, end, u.split, a.splits, u.k0, u.k1);
+    if constexpr (kForm == 0) narrow_unit(a, u, lds);
+    else wide_unit<kForm>(a, u, lds);
+  } else {
+    const int id = blockIdx.x - n_first;
+    const int s = id % a.own_splits, rest = id / a.own_splits;
+    u.hk = rest % a.KVH;
+    const int token = rest / a.KVH;
+    const Segment g = find_segment(a, kTr, before, [&](int lo, int hi, int, int) {
+      return lo <= token && token < hi;
+    });
+    const int end = clampi(a.last[token * a.last_sb], -1, a.cap - 1) + 1;
+    const int lo = min(g.index < 0 ? 0 : clampi(a.plen[g.index], 0, a.cap), end);
+    u.tok0 = u.trow = token;
+    u.rows = a.G;
+    u.r0 = 0;
+    if (g.index < 0) {  // in no group: no workgroup reports on its shared slots
+      u.k0 = u.k1 = 0;
+      for (u.split = s; u.split < a.splits; u.split += a.own_splits) empty_unit(a, u, 16);
+    }
+    u.split = a.splits + s;
+    cut(lo, end, s, a.own_splits, u.k0, u.k1);
+    narrow_unit(a, u, lds);
+  }
+}
+
+// Joins the `n` partials of each (token, kv head, query head): one wave each,
+// lane j holding the weights of partials j and j + 64, then 16 lanes of 4 dims
+// for each of four partials at a time.
+__global__ __launch_bounds__(256) void span_merge_kernel(Args a, int n) {
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= (int64_t)a.tokens * a.KVH * a.G) return;
+  const int g = (int)(id % a.G);
+  const int64_t th = id / a.G;
+  const int hk = (int)(th % a.KVH), token = (int)(th / a.KVH);
+  const int64_t p0 = th * n * a.G + g;
+  float2 x[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    x[h] = lane + 64 * h < n ? a.ml[p0 + (int64_t)(lane + 64 * h) * a.G] : float2{kNegInf, 0.f};
+  float top = fmaxf(x[0].x, x[1].x);
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  float wt[2], sum = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    wt[h] = x[h].y == 0.f ? 0.f : x[h].x == top ? 1.f : fast_exp2(x[h].x - top);
+    sum += x[h].y == 0.f ? 0.f : wt[h] * x[h].y;
+  }
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  uint64_t there[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) there[h] = __ballot(x[h].y != 0.f);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  const int sub = lane >> 4, d = 4 * (lane & 15);
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    for (int j0 = 0; j0 < 64 && 64 * h + j0 < n; j0 += 4) {
+      const int j = j0 + sub;
+      const float w = __shfl(wt[h], j);
+      if (there[h] >> j & 1)
+        o += *reinterpret_cast<const f32x4*>(a.acc + (p0 + (int64_t)(64 * h + j) * a.G) * kD + d) * w;
+    }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) o[c] = col_sum(o[c]);
+  if (sub == 0) store_out(a, token, hk, g, d, o, sum);
+}
+
+// K (rotated with cos / sin if given) and V of every new token into its slot:
+// 16 tokens of one kv head per workgroup, 16 threads a token, four for K's
+// rotate-half chunk pairs and eight for V's chunks.
+struct AppendArgs {
+  const f16* k;
+  int64_t k_sh, k_sn;
+  const f16* v;
+  int64_t v_sh, v_sn;
+  f16* kp;
+  f16* vp;
+};
+
+__global__ __launch_bounds__(256) void extend_append_kernel(Args a, AppendArgs p) {
+  const int token = blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int sub = threadIdx.x & 15, h = blockIdx.y;
+  if (token >= a.tokens || sub >= 12) return;
+  int lo = 0, hi = a.n_seg;  // the token's row: the last one that starts at or before it
+  while (lo + 1 < hi) {
+    const int mid = (lo + hi) / 2;
+    if (a.bounds[mid] <= token) lo = mid;
+    else hi = mid;
+  }
+  const int start = a.bounds[lo];
+  if (start < 0 || start > token || a.bounds[lo + 1] <= token) return;
+  const int64_t ctx = a.last[lo * a.last_sb];
+  if (ctx < 0 || ctx > a.cap) return;
+  const int slot = (int)ctx + token - start;
+  if (slot >= a.cap) return;
+  const int page = a.table[(int64_t)lo * a.t_sb + (slot >> a.log2p)];
+  if (page < 0 || page >= a.n_pages) return;
+  const int in_page = slot & ((1 << a.log2p) - 1);
+  if (sub < 4) {
+    const f16* src = p.k + h * p.k_sh + token * p.k_sn + 8 * sub;
+    f16x8 x = load16(src), y = load16(src + 32);
+    if (a.cos != nullptr) {
+      const int64_t co = token * a.cs_sn + 8 * sub;
+      rope_pair(x, y, load16(a.cos + co), load16(a.sin + co), load16(a.cos + co + 32),
+                load16(a.sin + co + 32));
+    }
+    f16* dst = p.kp + page * a.k_sp + h * a.k_sh + in_page * a.k_sn + 8 * sub;
+    store16(dst, x);
+    store16(dst + 32, y);
+  } else {
+    const int c = 8 * (sub - 4);
+    store16(p.vp + page * a.v_sp + h * a.v_sh + in_page * a.v_sn + c,
+            load16(p.v + h * p.v_sh + token * p.v_sn + c));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+
+constexpr int kCus = 256;
+
+struct Plan {
+  int form, n_tiles, splits, own_splits;
+};
+
+int64_t part_bytes(int64_t queries, int n) { return queries * n * (kD * 4 + (int64_t)sizeof(float2)); }
+
+// Units of the larger forms read a tile's K and V for more query rows, those of
+// the smaller ones leave fewer columns empty and make more workgroups.
+int pick_form(int64_t rows_per_segment) {
+  return rows_per_segment <= 16 ? 0 : rows_per_segment <= 64 ? 1 : 2;
+}
+
+// Splits so that the units fill the CUs twice, none for less than kMinKeys.
+int pick_splits(int64_t units, int cap, int fill) {
+  const int by_len = (int)std::min<int64_t>(kMaxSplits, ((int64_t)cap + kMinKeys - 1) / kMinKeys);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(by_len, fill / std::max<int64_t>(1, units)));
+}
+
+Plan decode_plan(int B, int KVH, int G, int n_groups, int cap) {
+  Plan p;
+  const int64_t rows = (int64_t)B * G;
+  p.form = pick_form((rows + n_groups - 1) / n_groups);
+  const int tr = p.form == 0 ? 16 : 64 * p.form;
+  p.n_tiles = (int)(rows / tr) + n_groups;
+  p.splits = pick_splits((int64_t)p.n_tiles * KVH, cap, 2 * kCus);
+  p.own_splits = pick_splits((int64_t)B * KVH, cap, 2 * kCus);
+  return p;
+}
+
+Plan extend_plan(int B, int KVH, int G, int total, int cap) {
+  Plan p;
+  const int64_t rows = (int64_t)total * G;
+  p.form = pick_form((rows + B - 1) / B);
+  const int tr = p.form == 0 ? 16 : 64 * p.form;
+  p.n_tiles = (int)(rows / tr) + B;
+  p.splits = pick_splits((int64_t)p.n_tiles * KVH, cap, 2 * kCus);
+  p.own_splits = 0;
+  return p;
+}
+
+template <bool kDecode>
+int launch(const Args& a, const Plan& p, hipStream_t st) {
+  const int64_t grid = (int64_t)a.n_tiles * a.KVH * a.splits +
+                       (kDecode ? (int64_t)a.tokens * a.KVH * a.own_splits : 0);
+  if (grid > 0x7fffffff) return QF_ERR_UNSUPPORTED;
+  const dim3 g((unsigned)grid), b(kThreads);
+  if (p.form == 0) hipLaunchKernelGGL((span_kernel<0, kDecode>), g, b, 0, st, a);
+  else if (p.form == 1) hipLaunchKernelGGL((span_kernel<1, kDecode>), g, b, 0, st, a);
+  else hipLaunchKernelGGL((span_kernel<2, kDecode>), g, b, 0, st, a);
+  int rc = (int)hipGetLastError();
+  const int n = kDecode ? a.splits + a.own_splits : a.splits;
+  if (rc == 0 && (kDecode || n > 1)) {
+    const int64_t queries = (int64_t)a.tokens * a.KVH * a.G;
+    hipLaunchKernelGGL(span_merge_kernel, dim3((unsigned)((queries + 3) / 4)), dim3(256), 0, st, a, n);
+    rc = (int)hipGetLastError();
+  }
+  return rc;
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Checks and fills what both entry points share; the query rows' strides and
+// the segments are the caller's.
+int fill(Args& a, const void* q, const void* k_pool, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn,
+         const void* v_pool, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn,
+         const int32_t* block_table, int64_t bt_sb, int pages_per_row, int n_pages, int page_size,
+         const int32_t* bounds, const int64_t* last, int64_t last_sb, void* ws, void* out, int n_seg,
+         int tokens, int KVH, int G, int D, int cap, float scale) {
+  const int l2 = page_log2(page_size, pages_per_row, n_pages);
+  if (D != kD || G < 1 || G > 16 || l2 < 0) return QF_ERR_UNSUPPORTED;
+  if (!q || !k_pool || !v_pool || !block_table || !bounds || !last || !ws || !out)
+    return QF_ERR_INVALID_ARG;
+  if (n_seg < 1 || tokens < 1 || KVH < 1 || bt_sb < pages_per_row || cap < 1 ||
+      cap > pages_per_row * page_size || !(scale > 0.f) || !(scale < 1e30f))
+    return QF_ERR_INVALID_ARG;
+  if (!al16(q) || !al16(k_pool) || !al16(v_pool) || !al16(ws) ||
+      (reinterpret_cast<uintptr_t>(out) & 7u) != 0 ||
+      ((kp_sp | kp_sh | kp_sn | vp_sp | vp_sh | vp_sn) & 7) != 0)
+    return QF_ERR_INVALID_ARG;
+  // A tile's rows are addressed with 32-bit byte offsets below a record count.
+  if (kp_sn < kD || vp_sn < kD || kp_sn * 2 * kBN > 0x7fffffff || vp_sn * 2 * kBN > 0x7fffffff)
+    return QF_ERR_UNSUPPORTED;
+  if ((int64_t)tokens * G > 0x3fffffff || (int64_t)tokens * KVH * G > 0x7fffffff ||
+      (int64_t)cap + tokens > 0x7fffffff)
+    return QF_ERR_UNSUPPORTED;
+  a = Args{};
+  a.q = static_cast<const f16*>(q);
+  a.k = static_cast<const f16*>(k_pool);
+  a.k_sp = kp_sp; a.k_sh = kp_sh; a.k_sn = kp_sn;
+  a.v = static_cast<const f16*>(v_pool);
+  a.v_sp = vp_sp; a.v_sh = vp_sh; a.v_sn = vp_sn;
+  a.table = block_table;
+  a.t_sb = bt_sb;
+  a.log2p = l2; a.n_pages = n_pages; a.ppr = pages_per_row;
+  a.bounds = bounds;
+  a.last = last;
+  a.last_sb = last_sb;
+  a.n_seg = n_seg; a.tokens = tokens; a.KVH = KVH; a.G = G; a.cap = cap;
+  a.out = static_cast<f16*>(out);
+  a.scale_log2 = scale * kLog2e;
+  return QF_OK;
+}
+
+void set_parts(Args& a, const Plan& p, void* ws) {
+  a.n_tiles = p.n_tiles;
+  a.splits = p.splits;
+  a.own_splits = p.own_splits;
+  a.acc = static_cast<float*>(ws);
+  a.ml = reinterpret_cast<float2*>(a.acc + (int64_t)a.tokens * a.KVH * a.G *
+                                               (p.splits + p.own_splits) * kD);
+}
+
+}  // namespace span
+}  // namespace qf
+
+extern "C" int64_t qf_decode_attn_prefix_workspace(int B, int KVH, int G, int n_groups, int cap) {
+  using namespace qf::span;
+  if (B < 1 || KVH < 1 || n_groups < 1 || cap < 1) return QF_ERR_INVALID_ARG;
+  if (G < 1 || G > 16 || (int64_t)B * KVH * G > 0x7fffffff) return QF_ERR_UNSUPPORTED;
+  const Plan p = decode_plan(B, KVH, G, n_groups, cap);
+  return part_bytes((int64_t)B * KVH * G, p.splits + p.own_splits);
+}
+
+extern "C" int qf_decode_attn_prefix_paged(
+    const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sg, const void* k_pool, int64_t kp_sp,
+    int64_t kp_sh, int64_t kp_sn, const void* v_pool, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn,
+    const int32_t* block_table, int64_t bt_sb, int pages_per_row, int n_pages, int page_size,
+    const int32_t* prefix_rows, const int32_t* prefix_len, int n_groups, const int64_t* kv_last,
+    int64_t kv_last_sb, void* ws, int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh,
+    int64_t o_sg, int B, int KVH, int G, int D, float scale, void* stream) {
+  using namespace qf;
+  using namespace qf::span;
+  Args a;
+  const int cap = page_log2(page_size, pages_per_row, n_pages) < 0 ? 0 : pages_per_row * page_size;
+  const int rc = fill(a, q, k_pool, kp_sp, kp_sh, kp_sn, v_pool, vp_sp, vp_sh, vp_sn, block_table,
+                      bt_sb, pages_per_row, n_pages, page_size, prefix_rows, kv_last, kv_last_sb, ws,
+                      out, n_groups, B, KVH, G, D, cap, scale);
+  if (rc != QF_OK) return rc;
+  if (!prefix_len || ((q_sb | q_sh | q_sg) & 7) != 0 || ((o_sb | o_sh | o_sg) & 3) != 0)
+    return QF_ERR_INVALID_ARG;
+  a.q_st = q_sb; a.q_sh = q_sh; a.q_sg = q_sg;
+  a.o_st = o_sb; a.o_sh = o_sh; a.o_sg = o_sg;
+  a.plen = prefix_len;
+  const Plan p = decode_plan(B, KVH, G, n_groups, cap);
+  if (ws_bytes < part_bytes((int64_t)B * KVH * G, p.splits + p.own_splits)) return QF_ERR_SCRATCH_LIMIT;
+  set_parts(a, p, ws);
+  return launch<true>(a, p, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int64_t qf_prefill_extend_workspace(int B, int QH, int KVH, int total, int cap) {
+  using namespace qf::span;
+  if (B < 1 || KVH < 1 || QH < KVH || QH % KVH != 0 || total < 1 || cap < 1) return QF_ERR_INVALID_ARG;
+  if (QH / KVH > 16 || (int64_t)total * QH > 0x7fffffff) return QF_ERR_UNSUPPORTED;
+  const Plan p = extend_plan(B, KVH, QH / KVH, total, cap);
+  return p.splits > 1 ? part_bytes((int64_t)total * QH, p.splits) : 0;
+}
+
+extern "C" int qf_prefill_extend_paged(
+    const void* q, int64_t q_sh, int64_t q_sn, const void* k, int64_t k_sh, int64_t k_sn,
+    const void* v, int64_t v_sh, int64_t v_sn, const int32_t* cu_seqlens, int total,
+    const int64_t* context, int64_t ctx_sb, const void* cos, const void* sin, int64_t cs_sn,
+    void* k_pool, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn, void* v_pool, int64_t vp_sp,
+    int64_t vp_sh, int64_t vp_sn, const int32_t* block_table, int64_t bt_sb, int pages_per_row,
+    int n_pages, int page_size, int cap, void* ws, int64_t ws_bytes, void* out, int64_t o_sh,
+    int64_t o_sn, int B, int QH, int KVH, int D, float scale, void* stream) {
+  using namespace qf;
+  using namespace qf::span;
+  if (KVH < 1 || QH < KVH || QH % KVH != 0) return QF_ERR_INVALID_ARG;
+  const int G = QH / KVH;
+  Args a;
+  const int rc = fill(a, q, k_pool, kp_sp, kp_sh, kp_sn, v_pool, vp_sp, vp_sh, vp_sn, block_table,
+                      bt_sb, pages_per_row, n_pages, page_size, cu_seqlens, context, ctx_sb, ws, out,
+                      B, total, KVH, G, D, cap, scale);
+  if (rc != QF_OK) return rc;
+  if (!k || !v || !al16(k) || !al16(v) || ((q_sh | q_sn | k_sh | k_sn | v_sh | v_sn) & 7) != 0 ||
+      ((o_sh | o_sn) & 3) != 0 || (cos == nullptr) != (sin == nullptr) || !al16(cos) || !al16(sin) ||
+      (cos != nullptr && (cs_sn & 7) != 0))
+    return QF_ERR_INVALID_ARG;
+  if (KVH > 65535) return QF_ERR_UNSUPPORTED;
+  a.q_st = q_sn; a.q_sh = G * q_sh; a.q_sg = q_sh;
+  a.o_st = o_sn; a.o_sh = G * o_sh; a.o_sg = o_sh;
+  a.cos = static_cast<const f16*>(cos);
+  a.sin = static_cast<const f16*>(sin);
+  a.cs_sn = cs_sn;
+  const Plan p = extend_plan(B, KVH, G, total, cap);
+  if (p.splits > 1 && ws_bytes < part_bytes((int64_t)total * QH, p.splits)) return QF_ERR_SCRATCH_LIMIT;
+  set_parts(a, p, ws);
+  const AppendArgs ap = {static_cast<const f16*>(k), k_sh, k_sn, static_cast<const f16*>(v), v_sh, v_sn,
+                         static_cast<f16*>(k_pool), static_cast<f16*>(v_pool)};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(extend_append_kernel, dim3((total + 15) / 16, KVH), dim3(256), 0, st, a, ap);
+  const int err = (int)hipGetLastError();
+  return err != 0 ? err : launch<false>(a, p, st);
+}

@@ -14,8 +14,11 @@ and can be admitted and retired independently.  The ops call the C ABI in
 * ``copy_pages`` -- pages of every layer copied to other pages in one launch.
 * ``flash_decode_attention_paged`` / ``flash_decode_split_paged`` -- split-K
   decode (SE:834-874 semantics) through the block table.
+* ``flash_decode_attention_prefix_paged`` -- decode of a batch whose rows share
+  prefixes, which are read once.
 * ``rope_append_paged`` -- one-token RoPE + append at a per-row slot.
 * ``prefill_varlen_paged`` -- packed ragged prefill appending into pages.
+* ``prefill_extend_paged`` -- packed new tokens of rows that hold slots already.
 * ``rms_qkv_rope_append_paged`` -- the fused decode-step QKV kernel appending
   into pages.
 """
@@ -379,6 +382,68 @@ def flash_decode_split_paged(grouped, k_pool, v_pool, block_table, attn_bias, fl
     return acc, m, l
 
 
+def _int_rows(name: str, t: torch.Tensor, n: int, dtype, device) -> int:
+    """Element stride of an ``(n,)`` device tensor of ``dtype``, or raises."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
+        raise TypeError(f"{name} must be an {str(dtype)[6:]} tensor on {device}")
+    if t.dim() != 1 or t.numel() != n:
+        raise ValueError(f"{name} must be ({n},) (got {tuple(t.shape)})")
+    return t.stride(0)
+
+
+def _workspace(need: int, name: str, device) -> torch.Tensor:
+    _lib.check(min(need, 0), name)
+    return torch.empty(max(need, 16), device=device, dtype=torch.uint8)
+
+
+def flash_decode_attention_prefix_paged(grouped: torch.Tensor, k_pool: torch.Tensor,
+                                        v_pool: torch.Tensor, block_table: torch.Tensor,
+                                        prefix_rows: torch.Tensor, prefix_len: torch.Tensor,
+                                        kv_last: torch.Tensor, scale: float | None = None,
+                                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention of a batch whose rows share prefixes, each read once.
+
+    grouped (B, KVH, G, 64), pools and block_table as in
+    ``flash_decode_attention_paged``; ``prefix_rows`` (N + 1,) int32: rows
+    [prefix_rows[g], prefix_rows[g + 1]) are group g, whose slots
+    [0, prefix_len[g]) hold the same K and V in every row (forked rows'); they
+    are read from the pages of the group's first row.  Rows outside the groups
+    share nothing.  ``kv_last`` (B,) int64 is each row's last slot; a row with a
+    negative one (parked) gets zeros.  The three are read on the device when the
+    kernels run.  Returns (B, KVH, G, 64), written to ``out`` if given.
+    """
+    _require_cuda_fp16("grouped", grouped, 4)
+    b, kvh, g, d = grouped.shape
+    pool, cap = _pool_args(k_pool, v_pool, block_table, b)
+    dev = grouped.device
+    if k_pool.shape[1] != kvh or k_pool.device != dev:
+        raise ValueError(f"pools must hold {kvh} kv heads on {dev}")
+    groups = prefix_len.numel() if isinstance(prefix_len, torch.Tensor) else 0
+    if groups < 1:
+        raise ValueError("prefix_len must hold at least one group")
+    if (_int_rows("prefix_rows", prefix_rows, groups + 1, torch.int32, dev) != 1
+            or (_int_rows("prefix_len", prefix_len, groups, torch.int32, dev) != 1 and groups > 1)):
+        raise ValueError("prefix_rows and prefix_len must be contiguous")
+    last_sb = _int_rows("kv_last", kv_last, b, torch.int64, dev)
+    if out is None:
+        out = torch.empty((b, kvh, g, d), device=dev, dtype=torch.float16)
+    else:
+        _require_cuda_fp16("out", out, 4)
+        if out.shape != grouped.shape or out.device != dev:
+            raise ValueError(f"out must be {tuple(grouped.shape)} on {dev}")
+    lib = _lib.load()
+    ws = _workspace(lib.qf_decode_attn_prefix_workspace(b, kvh, g, groups, cap),
+                    "qf_decode_attn_prefix_workspace", dev)
+    with torch.cuda.device(dev):
+        rc = lib.qf_decode_attn_prefix_paged(
+            grouped.data_ptr(), grouped.stride(0), grouped.stride(1), grouped.stride(2), *pool,
+            prefix_rows.data_ptr(), prefix_len.data_ptr(), groups, kv_last.data_ptr(), last_sb,
+            ws.data_ptr(), ws.numel(), out.data_ptr(), out.stride(0), out.stride(1), out.stride(2),
+            b, kvh, g, d, float(d ** -0.5 if scale is None else scale), _stream(dev))
+    _lib.check(rc, "qf_decode_attn_prefix_paged")
+    return out
+
+
 # --------------------------------------------------------------------------
 # appends and prefill
 # --------------------------------------------------------------------------
@@ -477,6 +542,72 @@ def prefill_varlen_paged(query: torch.Tensor, key: torch.Tensor, value: torch.Te
             out.data_ptr(), out.stride(1), out.stride(0),
             b, qh, kvh, d, float(d ** -0.5), _stream(query.device))
     _lib.check(rc, "qf_prefill_varlen_paged")
+    return out
+
+
+def prefill_extend_paged(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                         cu_seqlens: torch.Tensor, max_seqlen: int, context: torch.Tensor,
+                         cos: torch.Tensor | None, sin: torch.Tensor | None, k_pool: torch.Tensor,
+                         v_pool: torch.Tensor, block_table: torch.Tensor, lengths=None,
+                         max_slots: int | None = None, scale: float | None = None) -> torch.Tensor:
+    """``prefill_varlen_paged`` for rows that hold slots already.
+
+    Packed query (T, QH, 64), key/value (T, KVH, 64) of the rows' new tokens;
+    row b's token i goes to its slot context[b] + i and attends to slots
+    [0, context[b] + i].  ``cu_seqlens``, ``max_seqlen`` and ``lengths`` as
+    there, but a row may have no tokens.  ``context`` (B,) int64 is read on the
+    device; a row with a negative one appends nothing and gets zeros.
+    ``cos``/``sin`` (T, 64) are the tokens' own tables, or None for q and k that
+    are rotated already.  ``max_slots`` bounds every row's context + tokens
+    (default: the table's): the work is split by it, and slots past it are
+    neither written nor read.  Pages that hold the new slots must be the row's
+    own (``PagedKvCache.own_slots``).  Returns (T, QH, 64).
+    """
+    for n, t in (("query", query), ("key", key), ("value", value)):
+        _require_cuda_fp16(n, t, 3)
+    t_, qh, d = query.shape
+    kvh = key.shape[1]
+    if key.shape != (t_, kvh, d) or value.shape != key.shape or kvh < 1 or qh % kvh != 0:
+        raise ValueError("packed extension shapes: query (T, QH, D), key/value (T, KVH, D)")
+    dev = query.device
+    b = cu_seqlens.numel() - 1 if isinstance(cu_seqlens, torch.Tensor) else 0
+    if b < 1 or not 1 <= max_seqlen <= t_:
+        raise ValueError(f"need B >= 1 rows and 1 <= max_seqlen <= T (got {b}, {max_seqlen})")
+    if _int_rows("cu_seqlens", cu_seqlens, b + 1, torch.int32, dev) != 1:
+        raise ValueError("cu_seqlens must be contiguous")
+    ctx_sb = _int_rows("context", context, b, torch.int64, dev)
+    check_cu_seqlens(cu_seqlens, t_, max_seqlen, lengths)
+    pool, cap = _pool_args(k_pool, v_pool, block_table, b)
+    if k_pool.shape[1] != kvh or k_pool.device != dev or key.device != dev or value.device != dev:
+        raise ValueError(f"pools must hold {kvh} kv heads, and all tensors be on {dev}")
+    if max_slots is not None:
+        if not max_seqlen <= max_slots <= cap:
+            raise ValueError(f"max_slots must be in [{max_seqlen}, {cap}] (got {max_slots})")
+        cap = int(max_slots)
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    cs_sn = 0
+    if cos is not None:
+        for n, t in (("cos", cos), ("sin", sin)):
+            _require_cuda_fp16(n, t, 2)
+            if t.shape[0] != t_ or t.device != dev:
+                raise ValueError(f"{n} must be (T, 64) on {dev}")
+        if cos.stride(0) != sin.stride(0):
+            cos, sin = cos.contiguous(), sin.contiguous()
+        cs_sn = cos.stride(0)
+    out = torch.empty((t_, qh, d), device=dev, dtype=torch.float16)
+    lib = _lib.load()
+    ws = _workspace(lib.qf_prefill_extend_workspace(b, qh, kvh, t_, cap),
+                    "qf_prefill_extend_workspace", dev)
+    with torch.cuda.device(dev):
+        rc = lib.qf_prefill_extend_paged(
+            query.data_ptr(), query.stride(1), query.stride(0),
+            key.data_ptr(), key.stride(1), key.stride(0),
+            value.data_ptr(), value.stride(1), value.stride(0),
+            cu_seqlens.data_ptr(), t_, context.data_ptr(), ctx_sb, _ptr(cos), _ptr(sin), cs_sn,
+            *pool, cap, ws.data_ptr(), ws.numel(), out.data_ptr(), out.stride(1), out.stride(0),
+            b, qh, kvh, d, float(d ** -0.5 if scale is None else scale), _stream(dev))
+    _lib.check(rc, "qf_prefill_extend_paged")
     return out
 
 
