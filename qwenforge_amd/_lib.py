@@ -1,6 +1,6 @@
 """ctypes binding of the C ABI in ``include/qf_attn.h``, ``include/qf_step.h``,
 ``include/qf_wide.h``, ``include/qf_prefill.h``, ``include/qf_paged.h``,
-``include/qf_prefix.h`` and ``include/qf_probe.h``.
+``include/qf_prefix.h``, ``include/qf_verify.h`` and ``include/qf_probe.h``.
 
 The shared object is built in-tree by ``qwenforge_amd.build``.  There is no
 fallback: if it is missing or does not load, every op raises.
@@ -302,6 +302,14 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32,         # B, QH, KVH, D
         _f32, _vp,                      # scale, stream
     ],
+    # include/qf_verify.h
+    "qf_verify_workspace": [_i32, _i32, _i32],                          # T, B, V
+    "qf_verify_drafts": [
+        _vp, _i32, _i64, _vp, _vp,      # logits, dtype, lg_sn, tokens, cu_seqlens
+        _vp, _vp, _vp, _i64, C.c_double,  # accept_u, sample_u, draft_probs, dp_sn, temperature
+        _vp, _i32, _vp, _vp, _i64,      # out, width, count, ws, ws_bytes
+        _i32, _i32, _i32, _vp,          # T, B, V, stream
+    ],
     # include/qf_probe.h
     "qf_stream_read": [_vp, _i64, _vp, _i32, _vp],   # src, bytes, sink, workgroups, stream
     "qf_launch_probe": [_vp, _i64, _vp, _vp,          # src, bytes, index, sink
@@ -325,7 +333,8 @@ for _name in ("qf_decode_attn", "qf_decode_attn_paged"):
 
 # Entry points that do not return an int status.
 RESTYPES = {"qf_error_string": C.c_char_p, "qf_prefill_layers_workspace": _i64,
-            "qf_decode_attn_prefix_workspace": _i64, "qf_prefill_extend_workspace": _i64}
+            "qf_decode_attn_prefix_workspace": _i64, "qf_prefill_extend_workspace": _i64,
+            "qf_verify_workspace": _i64}
 
 _lock = threading.Lock()
 _lib: C.CDLL | None = None

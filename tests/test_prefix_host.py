@@ -83,3 +83,60 @@ def test_copy_pages_refusals():
     assert call(d=128) == -2 and call(page=96) == -2 and call(pages=0) == -2
     assert call(pools=None) == -1 and call(pools=(16, None)) == -1 and call(pools=(16, 8)) == -1
     assert call(sp=8188) == -1 and call(src=None) == -1 and call(n=-1) == -1 and call(kvh=0) == -1
+
+
+def test_verify_refusals_without_a_gpu():
+    from qwenforge_amd import verify
+
+    lib = _lib.load()
+
+    def call(logits=16, dtype=0, sn=100, tokens=16, au=16, su=16, q=None, qsn=100, temp=1.0, width=2, ws=16,
+             bytes_=1 << 20, t=4, b=2, v=100):
+        return lib.qf_verify_drafts(logits, dtype, sn, tokens, 16, au, su, q, qsn, temp, 16, width, 16, ws,
+                                    bytes_, t, b, v, None)
+
+    assert call(dtype=2) == -2 and call(t=0) == -1 and call(v=0) == -1 and call(b=0) == -1
+    assert call(v=2**31 - 1, sn=2**31) == -2
+    assert call(logits=None) == -1 and call(logits=17) == -1 and call(logits=18, dtype=1) == -1
+    assert call(sn=99) == -1 and call(tokens=None) == -1 and call(au=None) == -1 and call(su=None) == -1
+    assert call(q=16, qsn=99) == -1 and call(width=0) == -1 and call(ws=8) == -1
+    assert call(temp=-0.5) == -1 and call(temp=float("nan")) == -1 and call(temp=float("inf")) == -1
+    assert call(temp=1e-320) == -1
+    assert call(bytes_=8) == -3
+    assert lib.qf_verify_workspace(4, 2, 100) > 0
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        verify.verify_drafts(torch.zeros(2, 8), None, None, 1, None, None)
+
+
+def test_span_attention_refusals_without_a_gpu():
+    lib = _lib.load()
+
+    def prefix(q=16, page=64, rows=16, plen=16, last=16, ws=16, bytes_=1 << 30, out=16, b=2, kvh=2, g=7, d=64,
+               scale=0.125, q_sb=896, sn=64, groups=1, bt_sb=4, ppr=4):
+        return lib.qf_decode_attn_prefix_paged(q, q_sb, 448, 64, 16, 8192, 4096, sn, 16, 8192, 4096, 64, 16, bt_sb,
+                                               ppr, 8, page, rows, plen, groups, last, 1, ws, bytes_, out, 896,
+                                               448, 64, b, kvh, g, d, scale, None)
+
+    assert prefix(d=128) == -2 and prefix(g=17) == -2 and prefix(page=32) == -2 and prefix(sn=56) == -2
+    for bad in (dict(q=None), dict(q=8), dict(rows=None), dict(plen=None), dict(last=None), dict(ws=None),
+                dict(ws=8), dict(out=None), dict(out=4), dict(b=0), dict(kvh=0), dict(groups=0), dict(q_sb=4),
+                dict(bt_sb=3), dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")),
+                dict(scale=float("inf"))):
+        assert prefix(**bad) == -1, bad
+    assert prefix(bytes_=100) == -3
+    assert lib.qf_decode_attn_prefix_workspace(0, 2, 7, 1, 64) == -1
+    assert lib.qf_decode_attn_prefix_workspace(1, 2, 17, 1, 64) == -2
+
+    def extend(q=16, cu=16, total=8, ctx=16, cos=None, sin=None, cap=256, ws=16, bytes_=1 << 30, out=16, b=2,
+               qh=14, kvh=2, d=64, k_sn=1152, ppr=4):
+        return lib.qf_prefill_extend_paged(q, 64, 1152, 16, 64, k_sn, 16, 64, 1152, cu, total, ctx, 1, cos, sin, 64,
+                                           16, 8192, 4096, 64, 16, 8192, 4096, 64, 16, 4, ppr, 8, 64, cap, ws,
+                                           bytes_, out, 64, 896, b, qh, kvh, d, 0.125, None)
+
+    assert extend(d=32) == -2 and extend(qh=34) == -2 and extend(ppr=0) == -2
+    for bad in (dict(q=None), dict(cu=None), dict(total=0), dict(ctx=None), dict(cos=16), dict(sin=16),
+                dict(cos=8, sin=16), dict(cap=0), dict(cap=257), dict(ws=None), dict(out=None), dict(b=0),
+                dict(qh=13), dict(kvh=0), dict(k_sn=1150)):
+        assert extend(**bad) == -1, bad
+    assert extend(bytes_=16) == -3
+    assert lib.qf_prefill_extend_workspace(2, 14, 2, 0, 256) == -1
