@@ -56,6 +56,19 @@ int qf_prefill_layers(const QfPrefillLayer* layers, int n_layers, void* hidden, 
                       int64_t ws_bytes, float eps, int hidden_size, int QH, int KVH, int D, int I,
                       void* stream);
 
+/* qf_prefill_layers for packed new tokens of rows that hold slots already, over
+ * paged caches (qf_prefill_extend_paged in qf_prefix.h: cu, context, ctx_sb and
+ * cap as there): token i of row b has position and slot context[b] + i and
+ * attends to slots [0, context[b] + i].  ws as above, of at least
+ * qf_extend_layers_workspace bytes. */
+int64_t qf_extend_layers_workspace(int T, int hidden, int QH, int KVH, int D, int I, int B, int cap);
+
+int qf_extend_layers(const QfPrefillLayer* layers, int n_layers, void* hidden, int T, int B,
+                     const int32_t* cu, const int64_t* context, int64_t ctx_sb, int cap,
+                     const float* inv_freq, const int32_t* block_table, int64_t bt_sb,
+                     int pages_per_row, int n_pages, int page_size, void* ws, int64_t ws_bytes,
+                     float eps, int hidden_size, int QH, int KVH, int D, int I, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

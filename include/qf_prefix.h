@@ -50,8 +50,11 @@ int qf_copy_pages(const void* const* pools, int n_pools, int64_t sp, int64_t sh,
  *                every group share nothing
  *   prefix_len   int32[n_groups] on the device: slots [0, prefix_len[g]) hold
  *                the same K and V in every row of group g.  They are read from
- *                the pages of its first row, for each row up to its own kv_last;
- *                the slots behind from the row's own pages
+ *                the group's pages, for each row up to its own kv_last; the slots
+ *                behind from the row's own pages
+ *   prefix_table NULL: a group's pages are those of its first row.  Else int32
+ *                (n_groups, prefix_pages) on the device, row stride pt_sb: group
+ *                g's pages (its first row may then have none mapped)
  *   kv_last      int64 on the device, row b reads kv_last[b * kv_last_sb]: its
  *                last slot (inclusive).  A row with kv_last < 0 has none, and
  *                its output is zero
@@ -74,6 +77,7 @@ int qf_decode_attn_prefix_paged(const void* q, int64_t q_sb, int64_t q_sh, int64
                                 const int32_t* block_table, int64_t bt_sb, int pages_per_row,
                                 int n_pages, int page_size,
                                 const int32_t* prefix_rows, const int32_t* prefix_len, int n_groups,
+                                const int32_t* prefix_table, int64_t pt_sb, int prefix_pages,
                                 const int64_t* kv_last, int64_t kv_last_sb,
                                 void* ws, int64_t ws_bytes,
                                 void* out, int64_t o_sb, int64_t o_sh, int64_t o_sg,

@@ -259,6 +259,15 @@ SIGNATURES = {
     ],
     # include/qf_prefill.h
     "qf_prefill_layers_workspace": [_i32, _i32, _i32, _i32, _i32, _i32],  # T, hidden, QH, KVH, D, I
+    "qf_extend_layers_workspace": [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32],  # ..., B, cap
+    "qf_extend_layers": [
+        _vp, _i32, _vp, _i32, _i32,     # layers, n_layers, hidden, T, B
+        _vp, _vp, _i64, _i32, _vp,      # cu, context, ctx_sb, cap, inv_freq
+        _vp, _i64, _i32, _i32, _i32,    # block_table, bt_sb, pages_per_row, n_pages, page_size
+        _vp, _i64, _f32,                # ws, ws_bytes, eps
+        _i32, _i32, _i32, _i32, _i32,   # hidden_size, QH, KVH, D, I
+        _vp,                            # stream
+    ],
     "qf_prefill_layers": [
         _vp, _i32, _vp, _i32, _i32, _i32,  # layers, n_layers, hidden, T, B, S
         _vp, _vp,                       # cu, inv_freq
@@ -280,6 +289,7 @@ SIGNATURES = {
         _vp, _i64, _i64, _i64,          # v_pool, vp_sp, vp_sh, vp_sn
         _vp, _i64, _i32, _i32, _i32,    # block_table, bt_sb, pages_per_row, n_pages, page_size
         _vp, _vp, _i32,                 # prefix_rows, prefix_len, n_groups
+        _vp, _i64, _i32,                # prefix_table, pt_sb, prefix_pages
         _vp, _i64,                      # kv_last, kv_last_sb
         _vp, _i64,                      # ws, ws_bytes
         _vp, _i64, _i64, _i64,          # out, o_sb, o_sh, o_sg
@@ -333,7 +343,7 @@ for _name in ("qf_decode_attn", "qf_decode_attn_paged"):
 
 # Entry points that do not return an int status.
 RESTYPES = {"qf_error_string": C.c_char_p, "qf_prefill_layers_workspace": _i64,
-            "qf_decode_attn_prefix_workspace": _i64, "qf_prefill_extend_workspace": _i64,
+            "qf_decode_attn_prefix_workspace": _i64, "qf_prefill_extend_workspace": _i64, "qf_extend_layers_workspace": _i64,
             "qf_verify_workspace": _i64}
 
 _lock = threading.Lock()

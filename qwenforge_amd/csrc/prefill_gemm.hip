@@ -20,6 +20,7 @@
 
 #include "step_common.h"
 #include "../../include/qf_prefill.h"
+#include "../../include/qf_prefix.h"
 
 namespace qf {
 namespace pgemm {
@@ -452,7 +453,8 @@ __global__ __launch_bounds__(256) void prefill_tokens_kernel(const int* cu, int 
                                                              const float* inv_freq,
                                                              const int32_t* table, int64_t t_sb,
                                                              int log2p, int ppr, int n_pages,
-                                                             f16* cs, int2* info) {
+                                                             const int64_t* context, int64_t ctx_sb,
+                                                             int cap, f16* cs, int2* info) {
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5), i = threadIdx.x & 31;
   if (t >= T) return;
   int b, pos;
@@ -465,6 +467,11 @@ __global__ __launch_bounds__(256) void prefill_tokens_kernel(const int* cu, int 
     }
     b = lo;
     pos = t - cu[b];
+    if (context != nullptr) {  // behind the row's cached slots; a parked row appends nothing
+      const int64_t c = context[b * ctx_sb];
+      S = c < 0 || c > cap ? 0 : cap;
+      pos += (int)(c < 0 ? 0 : c > cap ? cap : c);
+    }
   } else {
     b = t / S;
     pos = t - b * S;
@@ -652,11 +659,13 @@ extern "C" int64_t qf_prefill_layers_workspace(int T, int hidden, int QH, int KV
   return workspace(T, hidden, QH, KVH, I).bytes;
 }
 
-extern "C" int qf_prefill_layers(const QfPrefillLayer* layers, int n_layers, void* hidden_p, int T,
-                                 int B, int S, const int32_t* cu, const float* inv_freq,
-                                 const int32_t* block_table, int64_t bt_sb, int pages_per_row,
-                                 int n_pages, int page_size, void* ws, int64_t ws_bytes, float eps,
-                                 int H, int QH, int KVH, int D, int I, void* stream) {
+// Every layer of a prompt pass, or with `context` of an extension (then with cu
+// and block_table; `cap` as there).
+static int run_layers(const QfPrefillLayer* layers, int n_layers, void* hidden_p, int T, int B, int S,
+                      const int32_t* cu, const int64_t* context, int64_t ctx_sb, int cap,
+                      const float* inv_freq, const int32_t* block_table, int64_t bt_sb,
+                      int pages_per_row, int n_pages, int page_size, void* ws, int64_t ws_bytes,
+                      float eps, int H, int QH, int KVH, int D, int I, void* stream) {
   if (!shapes_ok(T, H, QH, KVH, D, I)) return QF_ERR_UNSUPPORTED;
   if (!layers || n_layers < 1 || !hidden_p || !inv_freq || !ws || B < 1 || S < 1)
     return QF_ERR_INVALID_ARG;
@@ -665,7 +674,12 @@ extern "C" int qf_prefill_layers(const QfPrefillLayer* layers, int n_layers, voi
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int found = stream_cus(st), cus = found > 0 && found < kMaxCus ? found : kMaxCus;
   const Workspace w = workspace(T, H, QH, KVH, I);
-  if (ws_bytes < w.bytes) return QF_ERR_SCRATCH_LIMIT;
+  int64_t spans = 0;  // the extension's attention scratch, behind the rest
+  if (context != nullptr) {
+    spans = qf_prefill_extend_workspace(B, QH, KVH, T, cap);
+    if (spans < 0) return (int)spans;
+  }
+  if (ws_bytes < w.bytes + spans) return QF_ERR_SCRATCH_LIMIT;
   int l2 = 0;
   if (block_table != nullptr) {
     l2 = page_log2(page_size, pages_per_row, n_pages);
@@ -704,7 +718,8 @@ extern "C" int qf_prefill_layers(const QfPrefillLayer* layers, int n_layers, voi
                          0, T, H, eps);
   };
   hipLaunchKernelGGL(prefill_tokens_kernel, dim3((T + 7) / 8), dim3(256), 0, st, cu, B, S, T,
-                     inv_freq, block_table, bt_sb, l2, pages_per_row, n_pages, cs, info);
+                     inv_freq, block_table, bt_sb, l2, pages_per_row, n_pages, context, ctx_sb, cap, cs,
+                     info);
   int rc = (int)hipGetLastError();
   for (int i = 0; i < n_layers && rc == 0; ++i) {
     const QfPrefillLayer& y = layers[i];
@@ -729,7 +744,12 @@ extern "C" int qf_prefill_layers(const QfPrefillLayer* layers, int n_layers, voi
     gq.N = W; gq.K = H;
     rc = launch<kEpiQkv>(gq, cus, st);
     if (rc) break;
-    if (cu == nullptr)
+    if (context != nullptr) {
+      const ExtendCall c = {cu, context, ctx_sb, block_table, bt_sb, pages_per_row, n_pages, page_size,
+                            cap, B, T, QH, KVH};
+      rc = extend_attention(c, qkv, 64, W, att, 64, A, y.k_cache, y.kc_sb, y.kc_sh, y.kc_sn, y.v_cache,
+                            y.vc_sb, y.vc_sh, y.vc_sn, base + w.bytes, spans, 0.125f, st);
+    } else if (cu == nullptr)
       rc = qf_prefill_attn(qkv, (int64_t)S * W, 64, W, qkv + A, (int64_t)S * W, 64, W,
                            qkv + A + KVH * 64, (int64_t)S * W, 64, W, nullptr, nullptr, 0, 0,
                            nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0, att, (int64_t)S * A, 64, A, B,
@@ -761,4 +781,35 @@ extern "C" int qf_prefill_layers(const QfPrefillLayer* layers, int n_layers, voi
     rc = (int)hipGetLastError();
   }
   return rc;
+}
+
+extern "C" int qf_prefill_layers(const QfPrefillLayer* layers, int n_layers, void* hidden_p, int T,
+                                 int B, int S, const int32_t* cu, const float* inv_freq,
+                                 const int32_t* block_table, int64_t bt_sb, int pages_per_row,
+                                 int n_pages, int page_size, void* ws, int64_t ws_bytes, float eps,
+                                 int H, int QH, int KVH, int D, int I, void* stream) {
+  return run_layers(layers, n_layers, hidden_p, T, B, S, cu, nullptr, 0, 0, inv_freq, block_table,
+                    bt_sb, pages_per_row, n_pages, page_size, ws, ws_bytes, eps, H, QH, KVH, D, I,
+                    stream);
+}
+
+extern "C" int64_t qf_extend_layers_workspace(int T, int hidden, int QH, int KVH, int D, int I, int B,
+                                              int cap) {
+  const int64_t bytes = qf_prefill_layers_workspace(T, hidden, QH, KVH, D, I);
+  const int64_t spans = bytes < 0 ? bytes : qf_prefill_extend_workspace(B, QH, KVH, T, cap);
+  return spans < 0 ? spans : bytes + spans;
+}
+
+extern "C" int qf_extend_layers(const QfPrefillLayer* layers, int n_layers, void* hidden_p, int T,
+                                int B, const int32_t* cu, const int64_t* context, int64_t ctx_sb,
+                                int cap, const float* inv_freq, const int32_t* block_table,
+                                int64_t bt_sb, int pages_per_row, int n_pages, int page_size, void* ws,
+                                int64_t ws_bytes, float eps, int H, int QH, int KVH, int D, int I,
+                                void* stream) {
+  if (!cu || !context || !block_table || B < 1 || cap < 1) return QF_ERR_INVALID_ARG;
+  if (page_log2(page_size, pages_per_row, n_pages) < 0) return QF_ERR_UNSUPPORTED;
+  if (cap > pages_per_row * page_size) return QF_ERR_INVALID_ARG;
+  return run_layers(layers, n_layers, hidden_p, T, B, 1, cu, context, ctx_sb, cap, inv_freq,
+                    block_table, bt_sb, pages_per_row, n_pages, page_size, ws, ws_bytes, eps, H, QH,
+                    KVH, D, I, stream);
 }

@@ -45,11 +45,15 @@ struct Args {
   int64_t t_sb;
   int log2p, n_pages, ppr;
   // Segments: tokens [bounds[i], bounds[i + 1]) share their tiles.  Decode: a
-  // group of rows (a token is a row) with plen[i] shared slots, read from the
-  // pages of its first row; last[token] is the row's last slot.  Extension: the
-  // new tokens of row i behind last[i] cached slots.
+  // group of rows (a token is a row) with plen[i] shared slots, at most pcap, in
+  // the pages of ptable's row i, or without it of the group's first row;
+  // last[token] is the row's last slot.  Extension: the new tokens of row i
+  // behind last[i] cached slots.
   const int32_t* bounds;
   const int32_t* plen;
+  const int32_t* ptable;
+  int64_t pt_sb;
+  int pcap, pppr;
   const int64_t* last;
   int64_t last_sb;
   int n_seg, tokens, KVH, G, cap;
@@ -308,10 +312,13 @@ __device__ __forceinline__ void tile_step(State<kQB>& s, int key0, const unsigne
           if (key < s.lo || key >= s.lim[b]) sc[blk][i] = kNegInf;
         }
     }
-    const float mx = max16(sc) * s.ks2;
+    // A column moves its reference only for scores of its own, so that a query's
+    // result does not depend on the others of its wave.
+    float mx = max16(sc) * s.ks2;
     if (__any(mx > s.m[b] + kRescaleSlack)) {
-      const float m_new = fmaxf(s.m[b], col_max(mx));
-      const float r = m_new == kNegInf ? 1.f : fast_exp2(s.m[b] - m_new);
+      mx = col_max(mx);
+      const float m_new = mx > s.m[b] + kRescaleSlack ? mx : s.m[b];
+      const float r = m_new == s.m[b] ? 1.f : fast_exp2(s.m[b] - m_new);
       s.l[b] *= r;
 #pragma unroll
       for (int t = 0; t < 4; ++t) s.o[b][t] *= r;
@@ -364,10 +371,12 @@ __device__ __forceinline__ void stage_ready() {
 }
 
 // One unit: query rows r0 .. of a segment's (token, query head) rows against
-// slots [k0, k1) of table row trow.
+// slots [k0, k1) of a block table row.
 struct Unit {
   int tok0, rows;     // the segment's first token, its query rows
-  int r0, hk, trow;
+  int r0, hk;
+  const int32_t* pages;
+  int n_pages;        // entries of `pages`
   int k0, k1;
   int ctx;            // extension: cached slots of the row; decode: -1
   int split, n_split; // place among each query's partials; n_split = 0: the output itself
@@ -377,10 +386,10 @@ __device__ __forceinline__ Source make_source(const Args& a, const Unit& u) {
   Source s;
   s.k = reinterpret_cast<const unsigned char*>(a.k + u.hk * a.k_sh);
   s.v = reinterpret_cast<const unsigned char*>(a.v + u.hk * a.v_sh);
-  s.row = a.table + (int64_t)u.trow * a.t_sb;
+  s.row = u.pages;
   s.k_sp = a.k_sp * 2; s.k_sn = a.k_sn * 2;
   s.v_sp = a.v_sp * 2; s.v_sn = a.v_sn * 2;
-  s.log2p = a.log2p; s.ppr = a.ppr; s.n_pages = a.n_pages;
+  s.log2p = a.log2p; s.ppr = u.n_pages; s.n_pages = a.n_pages;
   s.end = u.k1;
   return s;
 }
@@ -574,10 +583,13 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
     u.r0 = (tile - before) * kTr;
     int end;
     if (kDecode) {
-      u.trow = g.lo;
-      end = clampi(a.plen[g.index], 0, a.cap);
+      const bool given = a.ptable != nullptr;
+      u.pages = given ? a.ptable + (int64_t)g.index * a.pt_sb : a.table + (int64_t)g.lo * a.t_sb;
+      u.n_pages = given ? a.pppr : a.ppr;
+      end = clampi(a.plen[g.index], 0, a.pcap);
     } else {
-      u.trow = g.index;
+      u.pages = a.table + (int64_t)g.index * a.t_sb;
+      u.n_pages = a.ppr;
       u.ctx = clampi(a.last[g.index * a.last_sb], -1, a.cap);
       const int newest = (min(u.r0 + kTr, u.rows) - 1) / a.G;   // last token of the tile
       end = u.ctx < 0 ? 0 : min(u.ctx + newest + 1, a.cap);
@@ -594,8 +606,10 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
       return lo <= token && token < hi;
     });
     const int end = clampi(a.last[token * a.last_sb], -1, a.cap - 1) + 1;
-    const int lo = min(g.index < 0 ? 0 : clampi(a.plen[g.index], 0, a.cap), end);
-    u.tok0 = u.trow = token;
+    const int lo = min(g.index < 0 ? 0 : clampi(a.plen[g.index], 0, a.pcap), end);
+    u.tok0 = token;
+    u.pages = a.table + (int64_t)token * a.t_sb;
+    u.n_pages = a.ppr;
     u.rows = a.G;
     u.r0 = 0;
     if (g.index < 0) {  // in no group: no workgroup reports on its shared slots
@@ -831,8 +845,8 @@ extern "C" int qf_decode_attn_prefix_paged(
     const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sg, const void* k_pool, int64_t kp_sp,
     int64_t kp_sh, int64_t kp_sn, const void* v_pool, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn,
     const int32_t* block_table, int64_t bt_sb, int pages_per_row, int n_pages, int page_size,
-    const int32_t* prefix_rows, const int32_t* prefix_len, int n_groups, const int64_t* kv_last,
-    int64_t kv_last_sb, void* ws, int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh,
+    const int32_t* prefix_rows, const int32_t* prefix_len, int n_groups, const int32_t* prefix_table,
+    int64_t pt_sb, int prefix_pages, const int64_t* kv_last, int64_t kv_last_sb, void* ws, int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh,
     int64_t o_sg, int B, int KVH, int G, int D, float scale, void* stream) {
   using namespace qf;
   using namespace qf::span;
@@ -842,11 +856,18 @@ extern "C" int qf_decode_attn_prefix_paged(
                       bt_sb, pages_per_row, n_pages, page_size, prefix_rows, kv_last, kv_last_sb, ws,
                       out, n_groups, B, KVH, G, D, cap, scale);
   if (rc != QF_OK) return rc;
+  if (prefix_table != nullptr &&
+      (prefix_pages < 1 || pt_sb < prefix_pages || (int64_t)prefix_pages * page_size > 0x7fffffff - B))
+    return QF_ERR_INVALID_ARG;
   if (!prefix_len || ((q_sb | q_sh | q_sg) & 7) != 0 || ((o_sb | o_sh | o_sg) & 3) != 0)
     return QF_ERR_INVALID_ARG;
   a.q_st = q_sb; a.q_sh = q_sh; a.q_sg = q_sg;
   a.o_st = o_sb; a.o_sh = o_sh; a.o_sg = o_sg;
   a.plen = prefix_len;
+  a.ptable = prefix_table;
+  a.pt_sb = pt_sb;
+  a.pppr = prefix_pages;
+  a.pcap = prefix_table == nullptr ? cap : std::min(cap, prefix_pages * page_size);
   const Plan p = decode_plan(B, KVH, G, n_groups, cap);
   if (ws_bytes < part_bytes((int64_t)B * KVH * G, p.splits + p.own_splits)) return QF_ERR_SCRATCH_LIMIT;
   set_parts(a, p, ws);
@@ -859,6 +880,25 @@ extern "C" int64_t qf_prefill_extend_workspace(int B, int QH, int KVH, int total
   if (QH / KVH > 16 || (int64_t)total * QH > 0x7fffffff) return QF_ERR_UNSUPPORTED;
   const Plan p = extend_plan(B, KVH, QH / KVH, total, cap);
   return p.splits > 1 ? part_bytes((int64_t)total * QH, p.splits) : 0;
+}
+
+int qf::extend_attention(const ExtendCall& c, const void* q, int64_t q_sh, int64_t q_sn, void* out,
+                         int64_t o_sh, int64_t o_sn, const void* k_pool, int64_t kp_sp, int64_t kp_sh,
+                         int64_t kp_sn, const void* v_pool, int64_t vp_sp, int64_t vp_sh,
+                         int64_t vp_sn, void* ws, int64_t ws_bytes, float scale, hipStream_t st) {
+  using namespace qf::span;
+  const int G = c.QH / c.KVH;
+  Args a;
+  const int rc = fill(a, q, k_pool, kp_sp, kp_sh, kp_sn, v_pool, vp_sp, vp_sh, vp_sn, c.table, c.t_sb,
+                      c.ppr, c.n_pages, c.page_size, c.cu, c.context, c.ctx_sb, ws, out, c.B, c.T, c.KVH,
+                      G, kD, c.cap, scale);
+  if (rc != QF_OK) return rc;
+  a.q_st = q_sn; a.q_sh = G * q_sh; a.q_sg = q_sh;
+  a.o_st = o_sn; a.o_sh = G * o_sh; a.o_sg = o_sh;
+  const Plan p = extend_plan(c.B, c.KVH, G, c.T, c.cap);
+  if (p.splits > 1 && ws_bytes < part_bytes((int64_t)c.T * c.QH, p.splits)) return QF_ERR_SCRATCH_LIMIT;
+  set_parts(a, p, ws);
+  return launch<false>(a, p, st);
 }
 
 extern "C" int qf_prefill_extend_paged(

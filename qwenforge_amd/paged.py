@@ -400,15 +400,17 @@ def flash_decode_attention_prefix_paged(grouped: torch.Tensor, k_pool: torch.Ten
                                         v_pool: torch.Tensor, block_table: torch.Tensor,
                                         prefix_rows: torch.Tensor, prefix_len: torch.Tensor,
                                         kv_last: torch.Tensor, scale: float | None = None,
-                                        out: torch.Tensor | None = None) -> torch.Tensor:
+                                        out: torch.Tensor | None = None,
+                                        prefix_table: torch.Tensor | None = None) -> torch.Tensor:
     """Decode attention of a batch whose rows share prefixes, each read once.
 
     grouped (B, KVH, G, 64), pools and block_table as in
     ``flash_decode_attention_paged``; ``prefix_rows`` (N + 1,) int32: rows
     [prefix_rows[g], prefix_rows[g + 1]) are group g, whose slots
     [0, prefix_len[g]) hold the same K and V in every row (forked rows'); they
-    are read from the pages of the group's first row.  Rows outside the groups
-    share nothing.  ``kv_last`` (B,) int64 is each row's last slot; a row with a
+    are read from the pages of the group's first row, or of row g of
+    ``prefix_table`` (N, pages) int32 -- needed where the first row may have
+    nothing mapped.  Rows outside the groups share nothing.  ``kv_last`` (B,) int64 is each row's last slot; a row with a
     negative one (parked) gets zeros.  The three are read on the device when the
     kernels run.  Returns (B, KVH, G, 64), written to ``out`` if given.
     """
@@ -425,6 +427,14 @@ def flash_decode_attention_prefix_paged(grouped: torch.Tensor, k_pool: torch.Ten
             or (_int_rows("prefix_len", prefix_len, groups, torch.int32, dev) != 1 and groups > 1)):
         raise ValueError("prefix_rows and prefix_len must be contiguous")
     last_sb = _int_rows("kv_last", kv_last, b, torch.int64, dev)
+    shared = (None, 0, 0)
+    if prefix_table is not None:
+        if prefix_table.dtype != torch.int32 or prefix_table.device != dev:
+            raise TypeError(f"prefix_table must be an int32 tensor on {dev}")
+        if (prefix_table.dim() != 2 or prefix_table.shape[0] != groups or prefix_table.shape[1] < 1
+                or prefix_table.stride(1) != 1):
+            raise ValueError(f"prefix_table must be ({groups}, pages >= 1) with unit inner stride")
+        shared = (prefix_table.data_ptr(), prefix_table.stride(0), prefix_table.shape[1])
     if out is None:
         out = torch.empty((b, kvh, g, d), device=dev, dtype=torch.float16)
     else:
@@ -437,7 +447,7 @@ def flash_decode_attention_prefix_paged(grouped: torch.Tensor, k_pool: torch.Ten
     with torch.cuda.device(dev):
         rc = lib.qf_decode_attn_prefix_paged(
             grouped.data_ptr(), grouped.stride(0), grouped.stride(1), grouped.stride(2), *pool,
-            prefix_rows.data_ptr(), prefix_len.data_ptr(), groups, kv_last.data_ptr(), last_sb,
+            prefix_rows.data_ptr(), prefix_len.data_ptr(), groups, *shared, kv_last.data_ptr(), last_sb,
             ws.data_ptr(), ws.numel(), out.data_ptr(), out.stride(0), out.stride(1), out.stride(2),
             b, kvh, g, d, float(d ** -0.5 if scale is None else scale), _stream(dev))
     _lib.check(rc, "qf_decode_attn_prefix_paged")

@@ -12,7 +12,11 @@ pools (``paged.PagedKvCache``):
 * ``serve`` admits a waiting request into a row as soon as that row's request
   finishes: the row's pages go back to the pool, the new prompt is prefilled
   into fresh pages of the same row, and the captured step keeps replaying
-  for all rows (first come, first served).
+  for all rows (first come, first served).  Requests with a common prefix fork
+  its pages, extend them by their own prompts, and each step's attention reads
+  the prefix once for all rows;
+* ``generate_drafted`` runs a row's last token and drafted ones in one pass and
+  keeps those that the model would have drawn.
 
 The captured step is the dense engine's step with the paged kernels: for 1..4
 rows the fused weight-streaming kernels (QKV + RoPE + paged append, paged
@@ -29,9 +33,21 @@ from collections import deque
 import torch
 import torch.nn.functional as F
 
-from . import ops, paged, step_ops, wide_ops
+from . import ops, paged, prefill_ops, step_ops, verify, wide_ops
 from .engine import DecodeEngine
 from .rope import cos_sin
+
+
+def lookup_drafts(tokens, n: int, longest: int = 3) -> list:
+    """Up to ``n`` tokens that followed the last earlier occurrence of the
+    sequence's end (its last ``longest`` tokens, else fewer)."""
+    tokens = list(tokens)
+    for k in range(min(longest, len(tokens) - 1), 0, -1):
+        end = tokens[-k:]
+        for i in range(len(tokens) - k - 1, -1, -1):
+            if tokens[i:i + k] == end:
+                return tokens[i + k:i + k + n]
+    return []
 
 
 class PagedDecodeEngine(DecodeEngine):
@@ -54,10 +70,7 @@ class PagedDecodeEngine(DecodeEngine):
         rows = list(rows)
         if len(rows) != len(prompts):
             raise ValueError("one row per prompt")
-        if rows == list(range(rows[0], rows[0] + len(rows))):
-            table = kv.table[rows[0]:rows[0] + len(rows)]
-        else:
-            table = kv.table[torch.tensor(rows, device=self.device)]
+        table = self._table_rows(kv, rows)
         return self._prefill_packed(
             prompts, lambda i, q, k, v, cu, n, cos, sin, lengths: paged.prefill_varlen_paged(
                 q, k, v, cu, n, cos, sin, kv.pools[i][0], kv.pools[i][1], table, 0,
@@ -67,16 +80,79 @@ class PagedDecodeEngine(DecodeEngine):
                 len(prompts), longest, cu=cu, block_table=table, n_pages=kv.n_pages,
                 page_size=kv.page_size))
 
+    def _table_rows(self, kv: paged.PagedKvCache, rows):
+        if rows == list(range(rows[0], rows[0] + len(rows))):
+            return kv.table[rows[0]:rows[0] + len(rows)]
+        return kv.table[torch.tensor(rows, device=self.device)]
+
+    @torch.no_grad()
+    def extend_paged(self, chunks, kv: paged.PagedKvCache, rows, contexts, last_only: bool = True):
+        """New tokens (list of 1-D id tensors, one or more each) of rows that hold
+        ``contexts`` (ints) slots already: appended behind them and run in one
+        packed pass -> logits after each row's last token (len(rows), vocab), or
+        after every token (packed) without ``last_only``.
+
+        The slots must be mapped; pages of theirs that another row holds too are
+        copied first (``PagedKvCache.own_slots``)."""
+        cfg, dev = self.cfg, self.device
+        rows, contexts = list(rows), [int(c) for c in contexts]
+        lengths = [int(c.numel()) for c in chunks]
+        if not rows or not len(rows) == len(chunks) == len(contexts) == len(set(rows)):
+            raise ValueError("one chunk and one context for each of distinct rows")
+        if min(lengths) < 1:
+            raise ValueError("a chunk needs at least one token")
+        for r, c, n in zip(rows, contexts, lengths):
+            kv.own_slots(r, c, n)
+        table = self._table_rows(kv, rows)
+        starts = [0]
+        for n in lengths:
+            starts.append(starts[-1] + n)
+        total, most = starts[-1], max(c + n for c, n in zip(contexts, lengths))
+        ids = torch.cat([c.reshape(-1).to(dev) for c in chunks])
+        cu = torch.tensor(starts, dtype=torch.int32, device=dev)
+        ctx = torch.tensor(contexts, dtype=torch.int64, device=dev)
+        hidden = F.embedding(ids, self.w["embed"])
+        if not self._native_extension(hidden, kv, cu, ctx, most, table):
+            pos = torch.cat([torch.arange(c, c + n, device=dev) for c, n in zip(contexts, lengths)])
+            cos, sin = cos_sin(pos, self.inv_freq)
+            qh, kvh, d = cfg.heads, cfg.kv_heads, cfg.head_dim
+            for layer, (kp, vp) in zip(self.w["layers"], kv.pools):
+                proj = F.linear(self._rms(hidden, layer["input_norm"]), layer["qkv_weight"],
+                                layer["qkv_bias"]).view(total, qh + 2 * kvh, d)
+                att = paged.prefill_extend_paged(proj[:, :qh], proj[:, qh:qh + kvh], proj[:, qh + kvh:],
+                                                 cu, max(lengths), ctx, cos, sin, kp, vp, table,
+                                                 lengths=lengths, max_slots=most, scale=self.scale)
+                hidden = hidden + F.linear(att.reshape(total, qh * d), layer["o_weight"])
+                hidden = hidden + self._mlp(self._rms(hidden, layer["post_norm"]), layer)
+        return self._last_logits(hidden[cu[1:].long() - 1] if last_only else hidden)
+
+    def _native_extension(self, hidden, kv, cu, ctx, most: int, table) -> bool:
+        """Every layer of an extension in one native call, or False where the
+        model's or the caches' layout is one it does not take."""
+        cfg = self.cfg
+        if (hidden.dtype != torch.float16 or not hidden.is_cuda
+                or prefill_ops.workspace_bytes(cfg, hidden.shape[0]) < 0):
+            return False
+        layers = prefill_ops.layer_table(cfg, self.w["layers"], kv.pools, hidden.device,
+                                         (kv.n_pages, kv.kv_heads, kv.page_size, cfg.head_dim))
+        if layers is None:
+            return False
+        prefill_ops.extend_layers(cfg, layers, hidden, cu, ctx, most, self.inv_freq, table, kv.n_pages,
+                                  kv.page_size)
+        return True
+
     # ------------------------------------------------------------------ decode
     def make_paged_context(self, kv: paged.PagedKvCache, batch: int, n_cols: int,
-                           share_rows: bool = False):
+                           share_rows: bool = False, prefix=None):
         """Static buffers of the paged graph step over rows [0, batch) of ``kv``.
 
         ``pos[b]`` is row b's next slot (= its length so far) and its position;
         ``rows[:, step]`` receives each replay's tokens (``n_cols`` columns).
         ``share_rows``: attention may share its workgroups out by the rows'
         lengths (``ops.flash_decode_attention``); without it a row's results do
-        not depend on the other rows."""
+        not depend on the other rows.  ``prefix`` = (prefix_rows, prefix_len,
+        prefix_table) of ``paged.flash_decode_attention_prefix_paged``: the step
+        attends with it, the shared slots read once."""
         cfg = self.cfg
         dev = self.device
         fused = self.uses_fused_step(batch)
@@ -99,9 +175,19 @@ class PagedDecodeEngine(DecodeEngine):
             "fused": fused,
             "wide": self.uses_wide_step(batch),
             "share_rows": share_rows,
+            "prefix": prefix,
         }
         self._step_buffers(ctx, batch)
+        if prefix is not None:
+            ctx["att"] = torch.zeros(batch, cfg.kv_heads, cfg.groups, cfg.head_dim, device=dev,
+                                     dtype=torch.float16)
         return ctx
+
+    def _attend_prefix(self, ctx, grouped, kp, vp):
+        rows, length, table = ctx["prefix"]
+        return paged.flash_decode_attention_prefix_paged(grouped, kp, vp, ctx["table"], rows, length,
+                                                         ctx["pos"], scale=self.scale, out=ctx["att"],
+                                                         prefix_table=table)
 
     def _step(self, ctx):
         if "kv" not in ctx:
@@ -133,9 +219,13 @@ class PagedDecodeEngine(DecodeEngine):
                                                 kp, vp, table, pos, q_rot, positions=rope)
             grouped = q_rot.view(b, cfg.kv_heads, cfg.groups, cfg.head_dim)
             # The slot just written is the row's last valid one.
-            paged.flash_decode_split_paged(grouped, kp, vp, table, None, ctx["flash"], kv_last=pos,
-                                           scale=self.scale)
-            step_ops.attn_merge_o_proj(ctx["flash"], self.o_proj_weight(i, b), hidden)
+            if ctx["prefix"] is not None:
+                att = self._attend_prefix(ctx, grouped, kp, vp)
+                step_ops.gemv_residual(att.view(b, -1), layer["o_weight"], hidden)
+            else:
+                paged.flash_decode_split_paged(grouped, kp, vp, table, None, ctx["flash"], kv_last=pos,
+                                               scale=self.scale)
+                step_ops.attn_merge_o_proj(ctx["flash"], self.o_proj_weight(i, b), hidden)
             step_ops.rms_gate_up_swiglu(hidden, layer["post_norm"], eps, w_gate_up, h)
             step_ops.gemv_residual(h, layer["down_weight"], hidden)
         step_ops.rms_lm_head(hidden, self.w["final_norm"], eps, self.lm_head_weight(b), ctx["logits"],
@@ -151,6 +241,8 @@ class PagedDecodeEngine(DecodeEngine):
                                                *kv.pools[i], table, pos, ctx["q_rot"])
 
         def attend(i, grouped):
+            if ctx["prefix"] is not None:
+                return self._attend_prefix(ctx, grouped, *kv.pools[i])
             return paged.flash_decode_attention_paged(grouped, *kv.pools[i], table, None,
                                                       ctx["flash"], kv_last=pos, scale=self.scale,
                                                       share_rows=ctx["share_rows"])
@@ -168,9 +260,12 @@ class PagedDecodeEngine(DecodeEngine):
             q, k, v = self._qkv(self._rms(hidden, layer["input_norm"]), layer)
             q_rot = paged.rope_append_paged(q, k, v, cos, sin, kp, vp, table, pos)
             grouped = q_rot.view(b, cfg.kv_heads, cfg.groups, cfg.head_dim)
-            att = paged.flash_decode_attention_paged(grouped, kp, vp, table, None, ctx["flash"],
-                                                     kv_last=pos, scale=self.scale,
-                                                     share_rows=ctx["share_rows"])
+            if ctx["prefix"] is not None:
+                att = self._attend_prefix(ctx, grouped, kp, vp)
+            else:
+                att = paged.flash_decode_attention_paged(grouped, kp, vp, table, None, ctx["flash"],
+                                                         kv_last=pos, scale=self.scale,
+                                                         share_rows=ctx["share_rows"])
             hidden = residual + F.linear(att.reshape(b, 1, cfg.hidden), layer["o_weight"])
             residual = hidden
             hidden = residual + self._mlp(self._rms(hidden, layer["post_norm"]), layer)
@@ -244,8 +339,71 @@ class PagedDecodeEngine(DecodeEngine):
         return ctx["rows"].clone()
 
     @torch.no_grad()
+    def generate_drafted(self, prompts, max_new_tokens: int, draft_len: int = 4,
+                         temperature: float = 0.0, seed: int = 0, drafter=lookup_drafts,
+                         page_size: int = 64, stats: dict | None = None):
+        """``max_new_tokens`` ids for each of variable-length prompts (B, new), up
+        to ``draft_len`` + 1 of them per pass.
+
+        ``drafter(tokens, n)`` proposes up to n tokens after a row's tokens (a
+        list of ints); the default looks them up in the row's own text.  A pass
+        runs every unfinished row's last token and its drafts together
+        (``extend_paged``), and ``verify.verify_drafts`` keeps what the model
+        would have said: the argmax at ``temperature`` 0, else tokens distributed
+        as softmax(logits / temperature) whatever the drafter proposes, from
+        random numbers of a generator seeded with ``seed``.  ``stats`` (optional
+        dict) receives the passes, drafts and accepted drafts."""
+        b, dev = len(prompts), self.device
+        if b < 1 or max_new_tokens < 1 or draft_len < 0 or min(int(p.numel()) for p in prompts) < 1:
+            raise ValueError("need prompts of one token or more, max_new_tokens >= 1 and draft_len >= 0")
+        gen = torch.Generator(dev).manual_seed(seed)
+        text = [p.reshape(-1).tolist() for p in prompts]
+        ends = [len(t) + max_new_tokens for t in text]
+        ppr = -(-max(ends) // page_size)
+        kv = self.new_paged_cache(b, sum(-(-n // page_size) for n in ends), page_size, ppr)
+        for r, n in enumerate(ends):
+            kv.map_row(r, n)
+
+        def draw(logits, chunks):
+            lengths = [len(c) for c in chunks]
+            cu = torch.tensor([sum(lengths[:i]) for i in range(len(chunks) + 1)], dtype=torch.int32,
+                              device=dev)
+            u, r = (torch.rand(n, generator=gen, device=dev) for n in (sum(lengths), len(chunks)))
+            count, out = verify.verify_drafts(
+                logits, torch.tensor([t for c in chunks for t in c], device=dev), cu, max(lengths), u, r,
+                temperature=temperature, lengths=lengths)
+            return [row[:n] for n, row in zip(count.tolist(), out.tolist())]
+
+        passes = drafted = accepted = 0
+        new = dict(enumerate(draw(self.prefill_paged(prompts, kv, range(b)), [t[-1:] for t in text])))
+        while True:
+            for r, ids in new.items():
+                if not ids:
+                    raise RuntimeError("the logits give no distribution to draw from")
+                text[r] += ids
+            open_rows = [r for r in range(b) if len(text[r]) < ends[r]]
+            if not open_rows:
+                break
+            chunks = []
+            for r in open_rows:
+                n = min(draft_len, ends[r] - len(text[r]) - 1)
+                ids = [int(t) for t in drafter(text[r], n)][:n] if n > 0 else []
+                if any(not 0 <= t < self.cfg.vocab for t in ids):
+                    raise ValueError("drafted tokens must be in the vocabulary")
+                chunks.append(text[r][-1:] + ids)
+            logits = self.extend_paged([torch.tensor(c) for c in chunks], kv, open_rows,
+                                       [len(text[r]) - 1 for r in open_rows], last_only=False)
+            new = dict(zip(open_rows, draw(logits, chunks)))
+            passes += 1
+            drafted += sum(len(c) - 1 for c in chunks)
+            accepted += sum(max(0, len(ids) - 1) for ids in new.values())
+        if stats is not None:
+            stats.update(passes=passes, drafted=drafted, accepted=accepted)
+        return torch.tensor([t[-max_new_tokens:] for t in text], device=dev)
+
+    @torch.no_grad()
     def serve(self, prompts, max_new_tokens, max_batch: int = 4, page_size: int = 64,
-              n_pages: int | None = None, stats: dict | None = None):
+              n_pages: int | None = None, stats: dict | None = None, prefix=None):
         """Continuous batching: greedy ids for every prompt (list of 1-D tensors),
         ``max_new_tokens`` an int or one per prompt.
 
@@ -257,18 +415,35 @@ class PagedDecodeEngine(DecodeEngine):
         the step: ``max_batch`` rows of the pages that the longest request
         needs.  A row with no request is parked at slot -1: it appends nothing and its output is
         ignored.  Returns a list of 1-D id tensors, one per prompt.
+
+        ``prefix`` (1-D ids): every request is the prefix followed by its prompt.
+        The prefix is prefilled once, each request's row forks its pages and
+        extends them by the prompt, and the steps read the shared pages once for
+        all rows.
         """
         n_req = len(prompts)
         news = [max_new_tokens] * n_req if isinstance(max_new_tokens, int) else list(max_new_tokens)
         if len(news) != n_req or min(news) < 1:
             raise ValueError("one max_new_tokens >= 1 per prompt")
-        need = [int(p.numel()) + n - 1 for p, n in zip(prompts, news)]
+        common = 0 if prefix is None else int(prefix.numel())
+        if prefix is not None and (common < 1 or min(int(p.numel()) for p in prompts) < 1):
+            raise ValueError("a prefix and the prompts behind it need at least one token each")
+        need = [common + int(p.numel()) + n - 1 for p, n in zip(prompts, news)]
         ppr = -(-max(need) // page_size)
+        whole = common // page_size       # pages that rows share
         if n_pages is None:
-            n_pages = max_batch * ppr
-        kv = self.new_paged_cache(max_batch, n_pages, page_size, ppr)
+            n_pages = max_batch * (ppr - whole) + -(-common // page_size)
+        kv = self.new_paged_cache(max_batch + (common > 0), n_pages, page_size, ppr)
+        shared = None
+        if common:
+            # The row behind the batch holds the prefix for as long as the call runs.
+            kv.map_row(max_batch, common)
+            self.prefill_paged([prefix], kv, [max_batch])
+            i32 = dict(device=self.device, dtype=torch.int32)
+            shared = (torch.tensor([0, max_batch], **i32), torch.tensor([common], **i32),
+                      kv.table[max_batch:])
         # Upper bound on replays: every request decoded back to back.
-        ctx = self.make_paged_context(kv, max_batch, sum(n - 1 for n in news) + 1)
+        ctx = self.make_paged_context(kv, max_batch, sum(n - 1 for n in news) + 1, prefix=shared)
         self.capture_paged(ctx)
         ctx["step"].fill_(0)
         queue = deque(range(n_req))
@@ -290,8 +465,10 @@ class PagedDecodeEngine(DecodeEngine):
             nonlocal admitted
             free = [r for r in range(max_batch) if r not in active]
             batch = []
-            while free and queue and kv.free_pages() >= -(-need[queue[0]] // page_size):
+            while free and queue and kv.free_pages() >= -(-need[queue[0]] // page_size) - whole:
                 r, i = free.pop(0), queue.popleft()
+                if common:
+                    kv.fork_row(max_batch, r, common)
                 kv.map_row(r, need[i])
                 batch.append((r, i))
             if not batch:
@@ -301,11 +478,12 @@ class PagedDecodeEngine(DecodeEngine):
             # shapes whatever it is admitted with, so its tokens do not depend
             # on the other rows (the decode step is row-independent too: its
             # context shares no workgroups between rows).
-            first = torch.cat([torch.argmax(self.prefill_paged([prompts[i]], kv, [r]), dim=-1)
-                               for r, i in batch])
+            first = torch.cat([torch.argmax(
+                self.extend_paged([prompts[i]], kv, [r], [common]) if common
+                else self.prefill_paged([prompts[i]], kv, [r]), dim=-1) for r, i in batch])
             idx = torch.tensor(rows, device=self.device)
             ctx["token"].index_copy_(0, idx, first)
-            lens = torch.tensor([int(prompts[i].numel()) for _, i in batch], device=self.device)
+            lens = torch.tensor([common + int(prompts[i].numel()) for _, i in batch], device=self.device)
             ctx["pos"].index_copy_(0, idx, lens)
             for j, (r, i) in enumerate(batch):
                 if news[i] == 1:
@@ -337,6 +515,8 @@ class PagedDecodeEngine(DecodeEngine):
                 else:
                     active[r] = (i, t0, left - n, first)
             admit()
+        if common:
+            kv.release_row(max_batch)
         torch.cuda.synchronize(self.device)
         if stats is not None:
             stats["replays"] = replays

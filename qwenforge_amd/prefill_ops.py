@@ -4,7 +4,8 @@
 o_proj + residual, rms_norm, gate/up + SwiGLU and down_proj + residual of all
 layers (SE:679-737, SE:1162-1204).  ``layer_table`` says whether a model and its
 caches have the layouts it takes; the engine keeps the torch projections
-otherwise.
+otherwise.  ``extend_layers`` is the same pass for new tokens of rows that hold
+cached slots already.
 """
 
 from __future__ import annotations
@@ -115,3 +116,38 @@ def prefill_layers(cfg, table, hidden: torch.Tensor, rows: int, longest: int,
             need, float(cfg.rms_eps), cfg.hidden, cfg.heads, cfg.kv_heads, cfg.head_dim,
             cfg.intermediate, _stream(hidden.device))
     _lib.check(rc, "qf_prefill_layers")
+
+
+def extend_layers(cfg, table, hidden: torch.Tensor, cu: torch.Tensor, context: torch.Tensor,
+                  max_slots: int, inv_freq: torch.Tensor, block_table: torch.Tensor, n_pages: int,
+                  page_size: int) -> None:
+    """Runs the layers of ``table`` over ``hidden`` (tokens, cfg.hidden), new tokens
+    of rows that hold ``context`` (rows,) int64 slots already, in place: packed by
+    ``cu`` (rows + 1) int32 as in ``prefill_layers``, over paged caches.  No row's
+    context + tokens exceeds ``max_slots``."""
+    rows, tokens = context.numel(), hidden.numel() // cfg.hidden
+    dev = hidden.device
+    if hidden.dtype != torch.float16 or dev.type != "cuda" or not hidden.is_contiguous():
+        raise ValueError("hidden must be a contiguous fp16 device tensor")
+    if (n_pages, page_size) != (table.rows, table.slots):
+        raise ValueError("n_pages and page_size must be the pools'")
+    for name, t, dtype, shape in (("cu", cu, torch.int32, (rows + 1,)),
+                                  ("context", context, torch.int64, (rows,)),
+                                  ("inv_freq", inv_freq, torch.float32, (cfg.head_dim // 2,))):
+        if t.dtype != dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {shape} {str(dtype)[6:]} on hidden's device")
+    if (block_table.dtype != torch.int32 or block_table.device != dev or block_table.dim() != 2
+            or block_table.shape[0] != rows or block_table.stride(1) != 1):
+        raise ValueError("block_table must be (rows, pages) int32 with unit inner stride")
+    lib = _lib.load()
+    need = lib.qf_extend_layers_workspace(tokens, cfg.hidden, cfg.heads, cfg.kv_heads, cfg.head_dim,
+                                          cfg.intermediate, rows, max_slots)
+    _lib.check(min(need, 0), "qf_extend_layers_workspace")
+    with torch.cuda.device(dev):
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        rc = lib.qf_extend_layers(
+            table, len(table), hidden.data_ptr(), tokens, rows, cu.data_ptr(), context.data_ptr(), 1,
+            int(max_slots), inv_freq.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], n_pages, page_size, ws.data_ptr(), need, float(cfg.rms_eps),
+            cfg.hidden, cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.intermediate, _stream(dev))
+    _lib.check(rc, "qf_extend_layers")

@@ -242,6 +242,49 @@ def test_captured_prefix_decode_follows_lengths_groups_and_tables(dev):
         assert (got.cpu().double() - ref).abs().max().item() <= TOL * vp.abs().max().item()
 
 
+def test_prefix_pages_of_their_own_table(dev):
+    """Groups whose first rows have nothing mapped: the prefix comes from
+    ``prefix_table``; a prefix length past its pages is clamped to them."""
+    gen = torch.Generator().manual_seed(12)
+    lens = [0, 300, 280, 0, 0, 150]
+    kp, vp, table = _prefix_case(gen, dev, [3, 3], lens, [256, 128], 2, 64)
+    own = torch.stack([table[1].clone(), table[5].clone()])[:, :4].contiguous()
+    own[1, 2:] = -7                                      # group 1's pages end at slot 128
+    gone = table.clone()
+    gone[0], gone[3] = -1, -1
+    q = torch.randn(6, 2, 7, D, generator=gen).half().to(dev)
+    ref = _prefix_ref(q, kp, vp, table, lens)
+    rows = torch.tensor([0, 3, 6], dtype=torch.int32, device=dev)
+    last = torch.tensor([n - 1 for n in lens], device=dev)
+    for pages, plen in ((own, [256, 128]), (own[:, :2].contiguous(), [1000, 128])):
+        got = paged.flash_decode_attention_prefix_paged(
+            q, kp, vp, gone.to(dev), rows, torch.tensor(plen, dtype=torch.int32, device=dev), last,
+            prefix_table=pages.to(dev))
+        assert (got.cpu().double() - ref).abs().max().item() <= TOL * vp.abs().max().item()
+    for bad, kind in ((own[:1], ValueError), (own.long(), TypeError), (own[:, :0], ValueError)):
+        with pytest.raises(kind):
+            paged.flash_decode_attention_prefix_paged(
+                q, kp, vp, gone.to(dev), rows, torch.tensor([256, 128], dtype=torch.int32, device=dev), last,
+                prefix_table=bad.to(dev))
+
+
+def test_a_row_keeps_its_bits_in_any_company(dev):
+    gen = torch.Generator().manual_seed(13)
+    b = 20
+    kp, vp, table = _prefix_case(gen, dev, [b], [1000] * b, [640], 2, 64)
+    q = torch.randn(b, 2, 7, D, generator=gen).half().to(dev)
+    rows = torch.tensor([0, b], dtype=torch.int32, device=dev)
+    plen = torch.tensor([640], dtype=torch.int32, device=dev)
+    seen = []
+    for others, scale in ((999, 1.0), (-1, 1.0), (641, 30.0)):
+        last = torch.full((b,), others, dtype=torch.int64, device=dev)
+        last[9] = 800
+        qs = q * scale
+        qs[9] = q[9]
+        seen.append(paged.flash_decode_attention_prefix_paged(qs, kp, vp, table.to(dev), rows, plen, last)[9].clone())
+    assert torch.equal(seen[0], seen[1]) and torch.equal(seen[0], seen[2])
+
+
 def test_prefix_decode_refusals(dev):
     gen = torch.Generator().manual_seed(10)
     kp, vp, table = _prefix_case(gen, dev, [2], [70, 80], [64], 2, 64)

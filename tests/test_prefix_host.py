@@ -112,15 +112,15 @@ def test_span_attention_refusals_without_a_gpu():
     lib = _lib.load()
 
     def prefix(q=16, page=64, rows=16, plen=16, last=16, ws=16, bytes_=1 << 30, out=16, b=2, kvh=2, g=7, d=64,
-               scale=0.125, q_sb=896, sn=64, groups=1, bt_sb=4, ppr=4):
+               scale=0.125, q_sb=896, sn=64, groups=1, bt_sb=4, ppr=4, pt=None, pt_sb=4, ppp=4):
         return lib.qf_decode_attn_prefix_paged(q, q_sb, 448, 64, 16, 8192, 4096, sn, 16, 8192, 4096, 64, 16, bt_sb,
-                                               ppr, 8, page, rows, plen, groups, last, 1, ws, bytes_, out, 896,
-                                               448, 64, b, kvh, g, d, scale, None)
+                                               ppr, 8, page, rows, plen, groups, pt, pt_sb, ppp, last, 1, ws,
+                                               bytes_, out, 896, 448, 64, b, kvh, g, d, scale, None)
 
     assert prefix(d=128) == -2 and prefix(g=17) == -2 and prefix(page=32) == -2 and prefix(sn=56) == -2
     for bad in (dict(q=None), dict(q=8), dict(rows=None), dict(plen=None), dict(last=None), dict(ws=None),
                 dict(ws=8), dict(out=None), dict(out=4), dict(b=0), dict(kvh=0), dict(groups=0), dict(q_sb=4),
-                dict(bt_sb=3), dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")),
+                dict(bt_sb=3), dict(pt=16, ppp=0), dict(pt=16, pt_sb=3), dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")),
                 dict(scale=float("inf"))):
         assert prefix(**bad) == -1, bad
     assert prefix(bytes_=100) == -3
