@@ -31,6 +31,7 @@ constexpr int kBN = 64;                      // keys per tile
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kTileBytes = kBN * kRowBytes;  // of K or V
+constexpr int kStages = 5;                   // ring of the wide units: two workgroups fill a CU's LDS
 constexpr int kMaxSplits = 64;               // of either kind of unit
 constexpr int kMinKeys = 128;                // least keys of a split
 
@@ -68,6 +69,15 @@ struct Args {
   const f16* sin;
   int64_t cs_sn;
 };
+
+// The kernel's arguments read anew from the argument block.  What only the end
+// of a unit needs would otherwise stay in scalar registers through its loop,
+// which has none to spare (the compiler then parks them in vector registers).
+__device__ __forceinline__ const Args& late_args() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Args*)p;
+}
 
 __device__ __forceinline__ int clampi(int64_t x, int lo, int hi) {
   return (int)(x < lo ? lo : x > hi ? hi : x);
@@ -126,12 +136,15 @@ __device__ __forceinline__ Segment find_segment(const Args& a, int tr, int& befo
   return {-1, 0, 0};
 }
 
-// A range of slots of a row's pages, read tile by tile.
+// A range of slots of a row's pages, read tile by tile.  A tile's address takes a
+// dozen scalar instructions per wave, so they are 32-bit ones (the host refuses
+// strides past them); tiles come in ascending order.
 struct Source {
   const unsigned char* k;  // pool + kv head
   const unsigned char* v;
   const int32_t* row;      // block table row
-  int64_t k_sp, k_sn, v_sp, v_sn;  // bytes
+  unsigned k_sp, v_sp;     // page strides, 16 bytes
+  int k_sn, v_sn;          // slot strides, bytes
   int pid, pwin;           // lane j: page of logical page pwin + j
   int log2p, ppr, n_pages;
   int end;                 // slots from here on read as zero
@@ -144,29 +157,29 @@ __device__ __forceinline__ void load_pids(Source& s, int win) {
 }
 
 // Async loads of kRows rows from row r0 of the tile at slot0 (a multiple of 64,
-// below s.end) into the K and V tiles at Kd and Vd; a lane's byte offsets within
-// 8 rows are ko, vo for even and odd groups of 8 (the swizzle differs).
+// below s.end) into the K and V tiles at Kd and Vd.
 template <int kRows>
 __device__ __forceinline__ void issue(Source& s, int slot0, int r0, unsigned char* Kd,
                                       unsigned char* Vd) {
   const int lane = threadIdx.x & 63;
   const int lp = slot0 >> s.log2p;
-  if (lp < s.pwin || lp - s.pwin >= 64) load_pids(s, lp);
-  const int page = __builtin_amdgcn_readlane(s.pid, lp - s.pwin);
-  const int in_page = slot0 & ((1 << s.log2p) - 1);
-  const int64_t rows = s.end - slot0;
-  const __amdgpu_buffer_rsrc_t rk =
-      tile_rsrc(s.k + (int64_t)page * s.k_sp + in_page * s.k_sn, rows * s.k_sn);
-  const __amdgpu_buffer_rsrc_t rv =
-      tile_rsrc(s.v + (int64_t)page * s.v_sp + in_page * s.v_sn, rows * s.v_sn);
+  if (lp - s.pwin >= 64) load_pids(s, lp);
+  const unsigned page = __builtin_amdgcn_readlane(s.pid, lp - s.pwin);
+  const int in_page = slot0 & ((1 << s.log2p) - 1), rows = min(s.end - slot0, kBN);
+  const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<unsigned char*>(s.k + ((uint64_t)page * s.k_sp << 4) + in_page * s.k_sn), (short)0,
+      rows * s.k_sn, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<unsigned char*>(s.v + ((uint64_t)page * s.v_sp << 4) + in_page * s.v_sn), (short)0,
+      rows * s.v_sn, 0x00020000);
 #pragma unroll
   for (int i = 0; i < kRows / 8; ++i) {
     const int r = r0 + 8 * i + (lane >> 3);
     const int c = 16 * ((lane & 7) ^ swz(r));
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(Kd + (r0 + 8 * i) * kRowBytes), 16,
-                                             r * (int)s.k_sn + c, 0, 0, 0);
+                                             r * s.k_sn + c, 0, 0, 0);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(Vd + (r0 + 8 * i) * kRowBytes), 16,
-                                             r * (int)s.v_sn + c, 0, 0, 0);
+                                             r * s.v_sn + c, 0, 0, 0);
   }
 }
 
@@ -256,115 +269,210 @@ __device__ __forceinline__ void masked_values(u32x2 (&vr)[2][4][2], const State<
       }
 }
 
-// Scores, online softmax and PV product of the tile of keys [key0, key0 + 64)
-// in (Ks, Vs), whose loads have landed; `refill` runs once the K operands are
-// in registers.  p is rounded to fp16 for the matrix cores (relative error
-// 2^-11, as large as that of the fp16 V it meets), and the sum l adds the
-// rounded p, so that the weights add to one.
-template <int kQB, typename Refill>
-__device__ __forceinline__ void tile_step(State<kQB>& s, int key0, const unsigned char* Ks,
-                                          const unsigned char* Vs, Refill&& refill) {
-  const int grp = (threadIdx.x & 63) >> 4;
-  const unsigned ks = lds_addr(Ks), vs = lds_addr(Vs);
-  u32x4 kr[2][2][2];
+// The K operands of a tile, waited for.
+struct KTile {
+  u32x4 r[2][2][2];  // [32 keys][4-key half][32 dims]
+};
+
+__device__ __forceinline__ void read_k(KTile& k, const int (&koff)[2], const unsigned char* Ks) {
+  const unsigned ks = lds_addr(Ks);
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
-    const unsigned ka0 = ks + s.koff[kk];
-    kr[0][0][kk] = lds_read_b128<0>(ka0);
-    kr[0][1][kk] = lds_read_b128<4 * kRowBytes>(ka0);
-    kr[1][0][kk] = lds_read_b128<32 * kRowBytes>(ka0);
-    kr[1][1][kk] = lds_read_b128<36 * kRowBytes>(ka0);
+    const unsigned at = ks + koff[kk];
+    k.r[0][0][kk] = lds_read_b128<0>(at);
+    k.r[0][1][kk] = lds_read_b128<4 * kRowBytes>(at);
+    k.r[1][0][kk] = lds_read_b128<32 * kRowBytes>(at);
+    k.r[1][1][kk] = lds_read_b128<36 * kRowBytes>(at);
   }
+}
+
+__device__ __forceinline__ void wait_k(KTile& k) {
   asm volatile("s_waitcnt lgkmcnt(0)"
-               : "+v"(kr[0][0][0]), "+v"(kr[0][0][1]), "+v"(kr[0][1][0]), "+v"(kr[0][1][1]),
-                 "+v"(kr[1][0][0]), "+v"(kr[1][0][1]), "+v"(kr[1][1][0]), "+v"(kr[1][1][1]));
-  u32x2 vr[2][4][2];
+               : "+v"(k.r[0][0][0]), "+v"(k.r[0][0][1]), "+v"(k.r[0][1][0]), "+v"(k.r[0][1][1]),
+                 "+v"(k.r[1][0][0]), "+v"(k.r[1][0][1]), "+v"(k.r[1][1][0]), "+v"(k.r[1][1][1]));
+}
+
+// The V^T operands of a tile: [32 keys][16 dims][4-key half].
+struct VTile {
+  u32x2 r[2][4][2];
+};
+
+__device__ __forceinline__ void read_v(VTile& v, const int (&voff)[4], const unsigned char* Vs) {
+  const unsigned vs = lds_addr(Vs);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    const unsigned va0 = vs + s.voff[t];
-    vr[0][t][0] = lds_read_tr_b64<0>(va0);
-    vr[0][t][1] = lds_read_tr_b64<4 * kRowBytes>(va0);
-    vr[1][t][0] = lds_read_tr_b64<32 * kRowBytes>(va0);
-    vr[1][t][1] = lds_read_tr_b64<36 * kRowBytes>(va0);
+    const unsigned at = vs + voff[t];
+    v.r[0][t][0] = lds_read_tr_b64<0>(at);
+    v.r[0][t][1] = lds_read_tr_b64<4 * kRowBytes>(at);
+    v.r[1][t][0] = lds_read_tr_b64<32 * kRowBytes>(at);
+    v.r[1][t][1] = lds_read_tr_b64<36 * kRowBytes>(at);
   }
-  refill();
+}
+
+__device__ __forceinline__ void wait_v(VTile& v) {
+  asm volatile("s_waitcnt lgkmcnt(0)"
+               : "+v"(v.r[0][0][0]), "+v"(v.r[0][0][1]), "+v"(v.r[0][1][0]), "+v"(v.r[0][1][1]),
+                 "+v"(v.r[0][2][0]), "+v"(v.r[0][2][1]), "+v"(v.r[0][3][0]), "+v"(v.r[0][3][1]),
+                 "+v"(v.r[1][0][0]), "+v"(v.r[1][0][1]), "+v"(v.r[1][1][0]), "+v"(v.r[1][1][1]),
+                 "+v"(v.r[1][2][0]), "+v"(v.r[1][2][1]), "+v"(v.r[1][3][0]), "+v"(v.r[1][3][1]));
+}
+
+// S^T of a tile: block 2 ch + j holds keys 32 ch + 8 grp + 4 j + i in element i.
+template <int kQB>
+__device__ __forceinline__ void scores(f32x4 (&sc)[kQB][4], const KTile& k, const State<kQB>& s) {
+  // All of the first 32 dims before the second: no product waits for the last.
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+    for (int b = 0; b < kQB; ++b)
+#pragma unroll
+      for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const f32x4 acc = kk == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[b][2 * ch + j];
+          sc[b][2 * ch + j] = mfma16x16x32(__builtin_bit_cast(f16x8, k.r[ch][j][kk]), s.q[b][kk], acc);
+        }
+}
+
+// Whether a query of the wave does not see all of the tile at key0.
+template <int kQB>
+__device__ __forceinline__ bool is_masked(const State<kQB>& s, int key0) {
   bool masked = key0 < s.lo;
 #pragma unroll
   for (int b = 0; b < kQB; ++b) masked = masked || __any(s.lim[b] < key0 + kBN);
-  f16x8 pb[kQB][2];
+  return masked;
+}
+
+template <int kQB>
+__device__ __forceinline__ void mask(f32x4 (&sc)[kQB][4], const State<kQB>& s, int key0) {
+  const int grp = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int b = 0; b < kQB; ++b)
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = key0 + 32 * (blk >> 1) + 8 * grp + 4 * (blk & 1) + i;
+        if (key < s.lo || key >= s.lim[b]) sc[b][blk][i] = kNegInf;
+      }
+}
+
+// Largest score of each lane, log2 units.
+template <int kQB>
+__device__ __forceinline__ void tops(float (&mx)[kQB], const f32x4 (&sc)[kQB][4], float ks2) {
 #pragma unroll
   for (int b = 0; b < kQB; ++b) {
-    f32x4 sc[4];
+    float t[4];
 #pragma unroll
-    for (int ch = 0; ch < 2; ++ch)
+    for (int blk = 0; blk < 4; ++blk)
+      t[blk] = fmaxf(fmaxf(sc[b][blk][0], sc[b][blk][1]), fmaxf(sc[b][blk][2], sc[b][blk][3]));
+    mx[b] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * ks2;
+  }
+}
+
+// Moves the references of the columns whose scores grew past them.  A column
+// moves only for scores of its own, so that a query's result does not depend on
+// the others of its wave.
+template <int kQB>
+__device__ __forceinline__ void raise(State<kQB>& s, const float (&mx)[kQB]) {
+  bool grew = false;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        acc = mfma16x16x32(__builtin_bit_cast(f16x8, kr[ch][j][0]), s.q[b][0], acc);
-        sc[2 * ch + j] = mfma16x16x32(__builtin_bit_cast(f16x8, kr[ch][j][1]), s.q[b][1], acc);
-      }
-    if (masked) {
+  for (int b = 0; b < kQB; ++b) grew = grew || mx[b] > s.m[b] + kRescaleSlack;
+  if (__any(grew)) {
 #pragma unroll
-      for (int blk = 0; blk < 4; ++blk)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = key0 + 32 * (blk >> 1) + 8 * grp + 4 * (blk & 1) + i;
-          if (key < s.lo || key >= s.lim[b]) sc[blk][i] = kNegInf;
-        }
-    }
-    // A column moves its reference only for scores of its own, so that a query's
-    // result does not depend on the others of its wave.
-    float mx = max16(sc) * s.ks2;
-    if (__any(mx > s.m[b] + kRescaleSlack)) {
-      mx = col_max(mx);
-      const float m_new = mx > s.m[b] + kRescaleSlack ? mx : s.m[b];
+    for (int b = 0; b < kQB; ++b) {
+      const float top = col_max(mx[b]);
+      const float m_new = top > s.m[b] + kRescaleSlack ? top : s.m[b];
       const float r = m_new == s.m[b] ? 1.f : fast_exp2(s.m[b] - m_new);
       s.l[b] *= r;
 #pragma unroll
       for (int t = 0; t < 4; ++t) s.o[b][t] *= r;
       s.m[b] = m_new;
     }
-    const float neg_m = s.m[b] == kNegInf ? 0.f : -s.m[b];
-#pragma unroll
-    for (int blk = 0; blk < 4; ++blk)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = fast_exp2(__builtin_fmaf(sc[blk][i], s.ks2, neg_m));
-        pb[b][blk >> 1][4 * (blk & 1) + i] = (f16)p;
-      }
-    const f16x8 ones = {(f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f};
-    s.l[b] = mfma16x16x32(ones, pb[b][0], s.l[b]);
-    s.l[b] = mfma16x16x32(ones, pb[b][1], s.l[b]);
   }
-  asm volatile("s_waitcnt lgkmcnt(0)"
-               : "+v"(vr[0][0][0]), "+v"(vr[0][0][1]), "+v"(vr[0][1][0]), "+v"(vr[0][1][1]),
-                 "+v"(vr[0][2][0]), "+v"(vr[0][2][1]), "+v"(vr[0][3][0]), "+v"(vr[0][3][1]),
-                 "+v"(vr[1][0][0]), "+v"(vr[1][0][1]), "+v"(vr[1][1][0]), "+v"(vr[1][1][1]),
-                 "+v"(vr[1][2][0]), "+v"(vr[1][2][1]), "+v"(vr[1][3][0]), "+v"(vr[1][3][1]));
-  if (masked) {
-    bool bad = false;
+}
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// p of block b, rounded to fp16 for the matrix cores (relative error 2^-11, as
+// large as that of the fp16 V it meets).
+template <int kQB>
+__device__ __forceinline__ void weights(f16x8 (&pb)[kQB][2], const f32x4 (&sc)[kQB][4],
+                                        const State<kQB>& s, int b) {
+  const float neg_m = s.m[b] == kNegInf ? 0.f : -s.m[b];
 #pragma unroll
-    for (int ch = 0; ch < 2; ++ch)
+  for (int ch = 0; ch < 2; ++ch) {
+    f32x8 p;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) bad = bad || special2(vr[ch][t][h][0]) || special2(vr[ch][t][h][1]);
-    if (__any(bad)) masked_values<kQB>(vr, s, pb, key0, s.o, Vs);
+    for (int e = 0; e < 8; ++e)
+      p[e] = fast_exp2(__builtin_fmaf(sc[b][2 * ch + e / 4][e % 4], s.ks2, neg_m));
+    pb[b][ch] = __builtin_convertvector(p, f16x8);
   }
+}
+
+// o += V^T P^T, l += ones P^T: the sum adds the rounded p, so that the weights
+// add to one.
+template <int kQB>
+__device__ __forceinline__ void add_values(State<kQB>& s, const f16x8 (&pb)[kQB][2], const VTile& v) {
+  const f16x8 ones = {(f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f};
 #pragma unroll
-  for (int ch = 0; ch < 2; ++ch)
+  for (int ch = 0; ch < 2; ++ch) {
+#pragma unroll
+    for (int b = 0; b < kQB; ++b) s.l[b] = mfma16x16x32(ones, pb[b][ch], s.l[b]);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const u32x4 w = {vr[ch][t][0][0], vr[ch][t][0][1], vr[ch][t][1][0], vr[ch][t][1][1]};
+      const u32x4 w = {v.r[ch][t][0][0], v.r[ch][t][0][1], v.r[ch][t][1][0], v.r[ch][t][1][1]};
       const f16x8 va = __builtin_bit_cast(f16x8, w);
 #pragma unroll
       for (int b = 0; b < kQB; ++b) s.o[b][t] = mfma16x16x32(va, pb[b][ch], s.o[b][t]);
     }
+  }
 }
 
-// This wave's loads have landed, and after the barrier every wave's.
-__device__ __forceinline__ void stage_ready() {
-  s_waitcnt_vm(0);
+template <int kQB>
+__device__ __forceinline__ void check_values(VTile& v, State<kQB>& s, const f16x8 (&pb)[kQB][2],
+                                             int key0, const unsigned char* Vs) {
+  bool bad = false;
+#pragma unroll
+  for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) bad = bad || special2(v.r[ch][t][h][0]) || special2(v.r[ch][t][h][1]);
+  if (__any(bad)) masked_values<kQB>(v.r, s, pb, key0, s.o, Vs);
+}
+
+// Scores, online softmax and PV product of the tile of keys [key0, key0 + 64)
+// in (Ks, Vs), whose loads have landed.
+template <int kQB>
+__device__ __forceinline__ void tile_step(State<kQB>& s, int key0, const unsigned char* Ks,
+                                          const unsigned char* Vs) {
+  KTile k;
+  read_k(k, s.koff, Ks);
+  wait_k(k);
+  f32x4 sc[kQB][4];
+  scores(sc, k, s);
+  const bool masked = is_masked(s, key0);
+  if (masked) mask(sc, s, key0);
+  float mx[kQB];
+  tops(mx, sc, s.ks2);
+  raise(s, mx);
+  VTile v;
+  read_v(v, s.voff, Vs);
+  f16x8 pb[kQB][2];
+#pragma unroll
+  for (int b = 0; b < kQB; ++b) weights(pb, sc, s, b);
+  wait_v(v);
+  if (masked) check_values(v, s, pb, key0, Vs);
+  add_values(s, pb, v);
+}
+
+// All but this wave's newest `ahead` tiles of loads (four each) have landed, and
+// after the barrier that holds for every wave.
+__device__ __forceinline__ void stage_ready(int ahead) {
+  if (ahead >= 2) __builtin_amdgcn_s_waitcnt(0x0F78);       // vmcnt(8)
+  else if (ahead == 1) __builtin_amdgcn_s_waitcnt(0x0F74);  // vmcnt(4)
+  else __builtin_amdgcn_s_waitcnt(0x0F70);
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __builtin_amdgcn_s_barrier();
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -387,8 +495,8 @@ __device__ __forceinline__ Source make_source(const Args& a, const Unit& u) {
   s.k = reinterpret_cast<const unsigned char*>(a.k + u.hk * a.k_sh);
   s.v = reinterpret_cast<const unsigned char*>(a.v + u.hk * a.v_sh);
   s.row = u.pages;
-  s.k_sp = a.k_sp * 2; s.k_sn = a.k_sn * 2;
-  s.v_sp = a.v_sp * 2; s.v_sn = a.v_sn * 2;
+  s.k_sp = (unsigned)(a.k_sp >> 3); s.k_sn = (int)a.k_sn * 2;
+  s.v_sp = (unsigned)(a.v_sp >> 3); s.v_sn = (int)a.v_sn * 2;
   s.log2p = a.log2p; s.ppr = u.n_pages; s.n_pages = a.n_pages;
   s.end = u.k1;
   return s;
@@ -457,8 +565,11 @@ __device__ __forceinline__ void empty_unit(const Args& a, const Unit& u, int n_r
   }
 }
 
-// kQB * 64 query rows, kQB * 16 per wave; the waves share the key tiles, which
-// are double-buffered.
+// kQB * 64 query rows, kQB * 16 per wave; the waves share the key tiles, on a
+// ring of kStages.  A step takes tile i's probabilities while the matrix cores
+// form tile i + 1's scores (its K came into registers during the step before),
+// then reads tile i + 2's K behind tile i's output product; tiles i + 3 and
+// i + 4 are on their way.
 template <int kQB>
 __device__ __forceinline__ void wide_unit(const Args& a, const Unit& u, unsigned char* lds) {
   if (u.k1 <= u.k0) {
@@ -466,30 +577,85 @@ __device__ __forceinline__ void wide_unit(const Args& a, const Unit& u, unsigned
     return;
   }
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const auto stage = [&](int i, int kv) { return lds + ((i & 1) * 2 + kv) * kTileBytes; };
+  const auto stage = [&](int st, int kv) { return lds + (st * 2 + kv) * kTileBytes; };
+  const auto after = [](int st, int d) { return st + d < kStages ? st + d : st + d - kStages; };
   Source src = make_source(a, u);
   const int first = u.k0 & ~(kBN - 1);
   const int n = (u.k1 - first + kBN - 1) / kBN;
+  const auto load = [&](int i, int st) {
+    if (i < n) issue<16>(src, first + i * kBN, 16 * w, stage(st, 0), stage(st, 1));
+  };
   load_pids(src, first >> a.log2p);
-  issue<16>(src, first, 16 * w, stage(0, 0), stage(0, 1));
+  load(0, 0);
   State<kQB> s;
   init_state(s, u.k0, a.scale_log2);
   const int row0 = u.r0 + w * kQB * 16;
   load_queries(s, a, u, row0);
-  for (int i = 0; i < n; ++i) {
-    // Every wave is past tile i - 1, whose stage takes tile i + 1.
-    stage_ready();
-    tile_step(s, first + i * kBN, stage(i, 0), stage(i, 1), [&] {
-      if (i + 1 < n)
-        issue<16>(src, first + (i + 1) * kBN, 16 * w, stage(i + 1, 0), stage(i + 1, 1));
-    });
+  load(1, 1);
+  load(2, 2);
+  load(3, 3);
+  f32x4 sc[kQB][4];
+  float mx[kQB];
+  KTile k;
+  stage_ready(n - 2);  // tiles 0 and, if there is one, 1
+  read_k(k, s.koff, stage(0, 0));
+  wait_k(k);
+  scores(sc, k, s);
+  tops(mx, sc, s.ks2);
+  if (n > 1) {
+    read_k(k, s.koff, stage(1, 0));
+    wait_k(k);
+  }
+  for (int i = 0, st = 0; i < n; ++i, st = after(st, 1)) {
+    const int key0 = first + i * kBN;
+    const bool masked = is_masked(s, key0);
+    if (masked) {
+      mask(sc, s, key0);
+      tops(mx, sc, s.ks2);
+    }
+    raise(s, mx);
+    // From here to wait_v, and from read_k to wait_k, nothing may branch: the
+    // reads in flight are not the compiler's.
+    VTile v;
+    read_v(v, s.voff, stage(st, 1));
+    f32x4 next[kQB][4];  // past the last tile: of its K again, unused
+    f16x8 pb[kQB][2];
+    scores(next, k, s);
+#pragma unroll
+    for (int b = 0; b < kQB; ++b) weights(pb, sc, s, b);
+    // One matrix product, then vector work for the 16 cycles that it takes.
+#pragma unroll
+    for (int j = 0; j < 8 * kQB; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+      __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);  // fma, conversion
+      __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);  // exp
+    }
+    // Keeps the exponentials here, with the matrix products (left alone, they
+    // sink behind the branches to their use).
+#pragma unroll
+    for (int b = 0; b < kQB; ++b) asm volatile("" : "+v"(pb[b][0]), "+v"(pb[b][1]));
+    wait_v(v);
+    // Tile i + 2 is there, and every wave is past tile i - 1, whose stage takes
+    // tile i + 4.
+    stage_ready(min(n - 3 - i, 1));
+    load(i + 4, after(st, 4));
+    if (masked) check_values(v, s, pb, key0, stage(st, 1));
+    read_k(k, s.koff, stage(i + 2 < n ? after(st, 2) : st, 0));
+    add_values(s, pb, v);
+    tops(mx, next, s.ks2);
+    wait_k(k);
+#pragma unroll
+    for (int b = 0; b < kQB; ++b)
+#pragma unroll
+      for (int blk = 0; blk < 4; ++blk) sc[b][blk] = next[b][blk];
   }
   const int col = threadIdx.x & 15;
+  const Args& late = late_args();
 #pragma unroll
   for (int b = 0; b < kQB; ++b)
 #pragma unroll
     for (int t = 0; t < 4; ++t)
-      store_part(a, u, row0 + 16 * b + col, t, s.o[b][t], s.m[b], s.l[b][0], t == 0);
+      store_part(late, u, row0 + 16 * b + col, t, s.o[b][t], s.m[b], s.l[b][0], t == 0);
 }
 
 // At most 16 query rows; the waves take the key tiles in turn and join their
@@ -516,7 +682,7 @@ __device__ __forceinline__ void narrow_unit(const Args& a, const Unit& u, unsign
   for (int i = w; i < n; i += kWaves) {
     s_waitcnt_vm(0);
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    tile_step(s, first + i * kBN, Ks, Vs, [] {});
+    tile_step(s, first + i * kBN, Ks, Vs);
     // The tile's reads are done: its LDS takes the wave's next one.
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (i + kWaves < n) issue<64>(src, first + (i + kWaves) * kBN, 0, Ks, Vs);
@@ -546,7 +712,7 @@ __device__ __forceinline__ void narrow_unit(const Args& a, const Unit& u, unsign
     sum += l[i] * r;
     o += so[(i * 4 + w) * 64 + lane] * r;
   }
-  store_part(a, u, u.r0 + (lane & 15), w, o, top, sum, w == 0);
+  store_part(late_args(), u, u.r0 + (lane & 15), w, o, top, sum, w == 0);
 }
 
 // Slots [k0, k1) of split s of `n` splits over [lo, hi), cut at multiples of 64.
@@ -563,7 +729,8 @@ __device__ __forceinline__ void cut(int lo, int hi, int s, int n, int& k0, int& 
 // others one row's own slots each.
 template <int kForm, bool kDecode>
 __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[kWaves * 2 * kTileBytes];
+  static_assert(kStages >= kWaves, "the narrow units' four tiles fit too");
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kStages * 2 * kTileBytes];
   constexpr int kTr = kForm == 0 ? 16 : 64 * kForm;
   const int n_first = a.n_tiles * a.KVH * a.splits;
   Unit u;
@@ -797,8 +964,10 @@ int fill(Args& a, const void* q, const void* k_pool, int64_t kp_sp, int64_t kp_s
       (reinterpret_cast<uintptr_t>(out) & 7u) != 0 ||
       ((kp_sp | kp_sh | kp_sn | vp_sp | vp_sh | vp_sn) & 7) != 0)
     return QF_ERR_INVALID_ARG;
-  // A tile's rows are addressed with 32-bit byte offsets below a record count.
-  if (kp_sn < kD || vp_sn < kD || kp_sn * 2 * kBN > 0x7fffffff || vp_sn * 2 * kBN > 0x7fffffff)
+  // A page's rows are addressed with 32-bit byte offsets, pages with 32-bit
+  // strides of 16 bytes.
+  if (kp_sn < kD || vp_sn < kD || kp_sn > 0x3fffffff / page_size || vp_sn > 0x3fffffff / page_size ||
+      kp_sp < 0 || vp_sp < 0 || kp_sp >> 3 > 0x7fffffff || vp_sp >> 3 > 0x7fffffff)
     return QF_ERR_UNSUPPORTED;
   if ((int64_t)tokens * G > 0x3fffffff || (int64_t)tokens * KVH * G > 0x7fffffff ||
       (int64_t)cap + tokens > 0x7fffffff)

@@ -335,8 +335,13 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Args a) {
     double2* s = a.sums + (int64_t)b * a.chunks + chunk;
     __hip_atomic_store(&s->x, chunk_left, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __hip_atomic_store(&s->y, chunk_all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // Release: the sums are visible before the count; acquire: the last one sees all.
-    mine = __hip_atomic_fetch_add(&a.ticket[b], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+    // The sums go past the L2 (agent-scope accesses) and have arrived before the
+    // count; their readers use such accesses too.  No fence: releasing every
+    // workgroup's L2 took four times the rest of the kernel.
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    s_waitcnt_vm(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    mine = __hip_atomic_fetch_add(&a.ticket[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
            a.chunks - 1;
   }
   __syncthreads();
