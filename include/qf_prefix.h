@@ -22,11 +22,12 @@ extern "C" {
 #endif
 
 /*
- * Copies pages within every one of n_pools page pools: for each pair i, slots
- * [0, slots[i]) of all KVH heads of page dst[i] become those of page src[i].
+ * Copies pages within every one of n_pools * per page pools: for each pair i,
+ * slots [0, slots[i]) of all KVH heads of page dst[i] become those of src[i].
  *
- *   pools   HOST array of n_pools device pointers (read during the call), each
- *           a pool (n_pages, KVH, page_size, D) with the strides sp, sh, sn
+ *   pools   HOST array of n_pools device pointers (read during the call); at each
+ *           begin `per` pools (n_pages, KVH, page_size, D), `step` elements apart,
+ *           with the strides sp, sh, sn
  *   src, dst  int32[n_pairs] on the device; a pair with a page outside
  *           [0, n_pages) copies nothing
  *   slots   int32[n_pairs] on the device, clamped to [0, page_size]; NULL
@@ -35,8 +36,8 @@ extern "C" {
  * No page may be written twice, or written and read, by one call: what such a
  * page holds afterwards is unspecified.  n_pairs = 0 launches nothing.
  */
-int qf_copy_pages(const void* const* pools, int n_pools, int64_t sp, int64_t sh, int64_t sn,
-                  const int32_t* src, const int32_t* dst, const int32_t* slots, int n_pairs,
+int qf_copy_pages(const void* const* pools, int n_pools, int per, int64_t step,
+                  int64_t sp, int64_t sh, int64_t sn, const int32_t* src, const int32_t* dst, const int32_t* slots, int n_pairs,
                   int n_pages, int KVH, int page_size, int D, void* stream);
 
 /*

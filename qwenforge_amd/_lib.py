@@ -278,7 +278,8 @@ SIGNATURES = {
     ],
     # include/qf_prefix.h
     "qf_copy_pages": [
-        C.POINTER(_vp), _i32, _i64, _i64, _i64,  # pools, n_pools, sp, sh, sn
+        C.POINTER(_vp), _i32, _i32, _i64,  # pools, n_pools, per, step
+        _i64, _i64, _i64,               # sp, sh, sn
         _vp, _vp, _vp, _i32,            # src, dst, slots, n_pairs
         _i32, _i32, _i32, _i32, _vp,    # n_pages, KVH, page_size, D, stream
     ],

@@ -242,6 +242,65 @@ def _pool_args(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Te
             ppr * page_size)
 
 
+# The calls below serve single tokens, where a microsecond on the host counts:
+# checks read as few tensor properties as they can and explain themselves only
+# when they fail.
+
+def _half(name: str, t: torch.Tensor, ndim: int) -> None:
+    """``_require_cuda_fp16`` for a tensor that is expected to pass."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float16 and t.is_cuda and t.dim() == ndim
+            and t.shape[-1] == HEAD_DIM and t.stride(-1) == 1):
+        _require_cuda_fp16(name, t, ndim)
+
+
+def _int_rows(name: str, t: torch.Tensor, n: int, dtype, index: int) -> int:
+    """Element stride of an ``(n,)`` tensor of ``dtype`` on GPU ``index``, or raises."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index:
+        raise TypeError(f"{name} must be an {str(dtype)[6:]} tensor on cuda:{index}")
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must be ({n},) (got {tuple(t.shape)})")
+    return t.stride(0)
+
+
+def _pools(k_pool, v_pool, block_table, batch: int, kv_heads: int, index: int):
+    """``_pool_args`` for ``kv_heads`` heads on GPU ``index``."""
+    _half("k_pool", k_pool, 4)
+    _half("v_pool", v_pool, 4)
+    shape, ks, vs = k_pool.shape, k_pool.stride(), v_pool.stride()
+    n_pages, kvh, page, _ = shape
+    if v_pool.shape != shape or kvh != kv_heads or k_pool.get_device() != index \
+            or v_pool.get_device() != index:
+        raise ValueError(f"k_pool and v_pool must be alike and hold {kv_heads} kv heads on cuda:{index}")
+    _check_page_size(page)
+    if (not isinstance(block_table, torch.Tensor) or block_table.dtype is not torch.int32
+            or block_table.get_device() != index):
+        raise TypeError(f"block_table must be an int32 tensor on cuda:{index}")
+    if block_table.dim() != 2 or block_table.shape[0] != batch or block_table.stride(1) != 1:
+        raise ValueError(f"block_table must be (B={batch}, pages_per_row) with unit inner stride")
+    ppr = block_table.shape[1]
+    return ((k_pool.data_ptr(), *ks[:3], v_pool.data_ptr(), *vs[:3], block_table.data_ptr(),
+             block_table.stride(0), ppr, n_pages, page), ppr * page)
+
+
+def _call(name: str, index: int, *args) -> None:
+    """Entry point ``name`` on GPU ``index`` and its current stream."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+def _check_rows(cu_seqlens, total: int, max_seqlen: int, lengths) -> None:
+    """``check_cu_seqlens``; host lengths that are right are not walked through."""
+    if (lengths is None or len(lengths) != cu_seqlens.shape[0] - 1 or sum(lengths) != total
+            or min(lengths) < 0 or max(lengths) > max_seqlen):
+        check_cu_seqlens(cu_seqlens, total, max_seqlen, lengths)
+
+
 def _slot_args(slots: torch.Tensor, batch: int, device):
     if not isinstance(slots, torch.Tensor) or slots.dtype != torch.int64 or slots.device != device:
         raise TypeError("slots must be an int64 device tensor")
@@ -278,35 +337,32 @@ def copy_pages(pools, src, dst, slots=None) -> None:
             raise ValueError("pools must be a contiguous (..., n_pages, KVH, P, 64) tensor, or a list")
         _require_cuda_fp16("pools", pools)
         first, shape, stride = pools, pools.shape[-4:], pools.stride()[-4:]
-        count = pools.numel() // max(1, shape.numel())
-        step = 2 * shape.numel()
-        ptrs = range(pools.data_ptr(), pools.data_ptr() + count * step, step) if step else ()
+        step = shape.numel()
+        per = pools.numel() // step if step else 0
+        bases = (pools.data_ptr(),)
     else:
         pools = list(pools)
         if not pools:
             raise ValueError("copy_pages needs at least one pool")
-        first = pools[0]
+        first, per, step = pools[0], 1, 0
         for t in pools:
             _require_cuda_fp16("pool", t, 4)
             if t.shape != first.shape or t.stride() != first.stride() or t.device != first.device:
                 raise ValueError("pools must have one shape, layout and device")
-        shape, stride = first.shape, first.stride()
-        count, ptrs = len(pools), [t.data_ptr() for t in pools]
+        shape, stride, bases = first.shape, first.stride(), [t.data_ptr() for t in pools]
     n_pages, kvh, page, _ = shape
     _check_page_size(page)
-    if count < 1 or n_pages < 1 or kvh < 1:
+    if per < 1 or n_pages < 1 or kvh < 1:
         raise ValueError("copy_pages needs at least one pool, page and head")
-    given = [("src", src), ("dst", dst)] + ([("slots", slots)] if slots is not None else [])
+    index = first.get_device()
     if isinstance(src, torch.Tensor) and src.is_cuda:
         n = src.numel()
-        for name, t in given:
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != first.device:
-                raise TypeError(f"{name} must be an int32 tensor on the pools' device, as src is")
-            if t.dim() != 1 or t.numel() != n or not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous ({n},)")
-        held = src, dst, slots
+        for name, t in (("src", src), ("dst", dst), ("slots", slots)):
+            if t is not None or name != "slots":
+                if _int_rows(name, t, n, torch.int32, index) != 1 and n > 1:
+                    raise ValueError(f"{name} must be contiguous")
     else:
-        if any(isinstance(t, torch.Tensor) and t.is_cuda for _, t in given):
+        if any(isinstance(t, torch.Tensor) and t.is_cuda for t in (src, dst, slots)):
             raise TypeError("src, dst and slots must all be device tensors or all sequences of ints")
         n = len(src)
         a, b = _page_list("src", src, n, 0, n_pages), _page_list("dst", dst, n, 0, n_pages)
@@ -314,13 +370,9 @@ def copy_pages(pools, src, dst, slots=None) -> None:
             raise ValueError("no page may be written twice, or both written and read")
         rows = [a, b] + ([_page_list("slots", slots, n, 0, page + 1)] if slots is not None else [])
         up = torch.tensor(rows, dtype=torch.int32).to(first.device)
-        held = up[0], up[1], up[2] if slots is not None else None
-    with torch.cuda.device(first.device):
-        rc = _lib.load().qf_copy_pages(
-            (C.c_void_p * count)(*ptrs), count, stride[0], stride[1], stride[2],
-            held[0].data_ptr(), held[1].data_ptr(), _ptr(held[2]), n, n_pages, kvh, page, HEAD_DIM,
-            _stream(first.device))
-    _lib.check(rc, "qf_copy_pages")
+        src, dst, slots = up[0], up[1], up[2] if slots is not None else None
+    _call("qf_copy_pages", index, (C.c_void_p * len(bases))(*bases), len(bases), per, step, stride[0],
+          stride[1], stride[2], src.data_ptr(), dst.data_ptr(), _ptr(slots), n, n_pages, kvh, page, HEAD_DIM)
 
 
 # --------------------------------------------------------------------------
@@ -382,17 +434,9 @@ def flash_decode_split_paged(grouped, k_pool, v_pool, block_table, attn_bias, fl
     return acc, m, l
 
 
-def _int_rows(name: str, t: torch.Tensor, n: int, dtype, device) -> int:
-    """Element stride of an ``(n,)`` device tensor of ``dtype``, or raises."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
-        raise TypeError(f"{name} must be an {str(dtype)[6:]} tensor on {device}")
-    if t.dim() != 1 or t.numel() != n:
-        raise ValueError(f"{name} must be ({n},) (got {tuple(t.shape)})")
-    return t.stride(0)
-
-
 def _workspace(need: int, name: str, device) -> torch.Tensor:
-    _lib.check(min(need, 0), name)
+    if need < 0:
+        _lib.check(need, name)
     return torch.empty(max(need, 16), device=device, dtype=torch.uint8)
 
 
@@ -414,43 +458,38 @@ def flash_decode_attention_prefix_paged(grouped: torch.Tensor, k_pool: torch.Ten
     negative one (parked) gets zeros.  The three are read on the device when the
     kernels run.  Returns (B, KVH, G, 64), written to ``out`` if given.
     """
-    _require_cuda_fp16("grouped", grouped, 4)
+    _half("grouped", grouped, 4)
     b, kvh, g, d = grouped.shape
-    pool, cap = _pool_args(k_pool, v_pool, block_table, b)
-    dev = grouped.device
-    if k_pool.shape[1] != kvh or k_pool.device != dev:
-        raise ValueError(f"pools must hold {kvh} kv heads on {dev}")
-    groups = prefix_len.numel() if isinstance(prefix_len, torch.Tensor) else 0
+    index = grouped.get_device()
+    pool, cap = _pools(k_pool, v_pool, block_table, b, kvh, index)
+    groups = prefix_len.shape[0] if isinstance(prefix_len, torch.Tensor) and prefix_len.dim() == 1 else 0
     if groups < 1:
         raise ValueError("prefix_len must hold at least one group")
-    if (_int_rows("prefix_rows", prefix_rows, groups + 1, torch.int32, dev) != 1
-            or (_int_rows("prefix_len", prefix_len, groups, torch.int32, dev) != 1 and groups > 1)):
+    if (_int_rows("prefix_rows", prefix_rows, groups + 1, torch.int32, index) != 1
+            or (_int_rows("prefix_len", prefix_len, groups, torch.int32, index) != 1 and groups > 1)):
         raise ValueError("prefix_rows and prefix_len must be contiguous")
-    last_sb = _int_rows("kv_last", kv_last, b, torch.int64, dev)
+    last_sb = _int_rows("kv_last", kv_last, b, torch.int64, index)
     shared = (None, 0, 0)
     if prefix_table is not None:
-        if prefix_table.dtype != torch.int32 or prefix_table.device != dev:
-            raise TypeError(f"prefix_table must be an int32 tensor on {dev}")
+        if prefix_table.dtype is not torch.int32 or prefix_table.get_device() != index:
+            raise TypeError(f"prefix_table must be an int32 tensor on cuda:{index}")
         if (prefix_table.dim() != 2 or prefix_table.shape[0] != groups or prefix_table.shape[1] < 1
                 or prefix_table.stride(1) != 1):
             raise ValueError(f"prefix_table must be ({groups}, pages >= 1) with unit inner stride")
         shared = (prefix_table.data_ptr(), prefix_table.stride(0), prefix_table.shape[1])
+    dev = grouped.device
     if out is None:
         out = torch.empty((b, kvh, g, d), device=dev, dtype=torch.float16)
     else:
-        _require_cuda_fp16("out", out, 4)
-        if out.shape != grouped.shape or out.device != dev:
+        _half("out", out, 4)
+        if out.shape != grouped.shape or out.get_device() != index:
             raise ValueError(f"out must be {tuple(grouped.shape)} on {dev}")
-    lib = _lib.load()
-    ws = _workspace(lib.qf_decode_attn_prefix_workspace(b, kvh, g, groups, cap),
+    ws = _workspace(_lib.load().qf_decode_attn_prefix_workspace(b, kvh, g, groups, cap),
                     "qf_decode_attn_prefix_workspace", dev)
-    with torch.cuda.device(dev):
-        rc = lib.qf_decode_attn_prefix_paged(
-            grouped.data_ptr(), grouped.stride(0), grouped.stride(1), grouped.stride(2), *pool,
-            prefix_rows.data_ptr(), prefix_len.data_ptr(), groups, *shared, kv_last.data_ptr(), last_sb,
-            ws.data_ptr(), ws.numel(), out.data_ptr(), out.stride(0), out.stride(1), out.stride(2),
-            b, kvh, g, d, float(d ** -0.5 if scale is None else scale), _stream(dev))
-    _lib.check(rc, "qf_decode_attn_prefix_paged")
+    _call("qf_decode_attn_prefix_paged", index, grouped.data_ptr(), *grouped.stride()[:3], *pool,
+          prefix_rows.data_ptr(), prefix_len.data_ptr(), groups, *shared, kv_last.data_ptr(), last_sb,
+          ws.data_ptr(), ws.shape[0], out.data_ptr(), *out.stride()[:3], b, kvh, g, d,
+          d ** -0.5 if scale is None else scale)
     return out
 
 
@@ -573,23 +612,24 @@ def prefill_extend_paged(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     neither written nor read.  Pages that hold the new slots must be the row's
     own (``PagedKvCache.own_slots``).  Returns (T, QH, 64).
     """
-    for n, t in (("query", query), ("key", key), ("value", value)):
-        _require_cuda_fp16(n, t, 3)
+    _half("query", query, 3)
+    _half("key", key, 3)
+    _half("value", value, 3)
     t_, qh, d = query.shape
     kvh = key.shape[1]
-    if key.shape != (t_, kvh, d) or value.shape != key.shape or kvh < 1 or qh % kvh != 0:
+    if key.shape[0] != t_ or value.shape != key.shape or kvh < 1 or qh % kvh != 0:
         raise ValueError("packed extension shapes: query (T, QH, D), key/value (T, KVH, D)")
-    dev = query.device
-    b = cu_seqlens.numel() - 1 if isinstance(cu_seqlens, torch.Tensor) else 0
+    index, dev = query.get_device(), query.device
+    if key.get_device() != index or value.get_device() != index:
+        raise ValueError(f"query, key and value must be on one device ({dev})")
+    b = cu_seqlens.shape[0] - 1 if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.dim() == 1 else 0
     if b < 1 or not 1 <= max_seqlen <= t_:
         raise ValueError(f"need B >= 1 rows and 1 <= max_seqlen <= T (got {b}, {max_seqlen})")
-    if _int_rows("cu_seqlens", cu_seqlens, b + 1, torch.int32, dev) != 1:
+    if _int_rows("cu_seqlens", cu_seqlens, b + 1, torch.int32, index) != 1:
         raise ValueError("cu_seqlens must be contiguous")
-    ctx_sb = _int_rows("context", context, b, torch.int64, dev)
-    check_cu_seqlens(cu_seqlens, t_, max_seqlen, lengths)
-    pool, cap = _pool_args(k_pool, v_pool, block_table, b)
-    if k_pool.shape[1] != kvh or k_pool.device != dev or key.device != dev or value.device != dev:
-        raise ValueError(f"pools must hold {kvh} kv heads, and all tensors be on {dev}")
+    ctx_sb = _int_rows("context", context, b, torch.int64, index)
+    _check_rows(cu_seqlens, t_, max_seqlen, lengths)
+    pool, cap = _pools(k_pool, v_pool, block_table, b, kvh, index)
     if max_slots is not None:
         if not max_seqlen <= max_slots <= cap:
             raise ValueError(f"max_slots must be in [{max_seqlen}, {cap}] (got {max_slots})")
@@ -599,25 +639,20 @@ def prefill_extend_paged(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     cs_sn = 0
     if cos is not None:
         for n, t in (("cos", cos), ("sin", sin)):
-            _require_cuda_fp16(n, t, 2)
-            if t.shape[0] != t_ or t.device != dev:
+            _half(n, t, 2)
+            if t.shape[0] != t_ or t.get_device() != index:
                 raise ValueError(f"{n} must be (T, 64) on {dev}")
         if cos.stride(0) != sin.stride(0):
             cos, sin = cos.contiguous(), sin.contiguous()
         cs_sn = cos.stride(0)
     out = torch.empty((t_, qh, d), device=dev, dtype=torch.float16)
-    lib = _lib.load()
-    ws = _workspace(lib.qf_prefill_extend_workspace(b, qh, kvh, t_, cap),
+    ws = _workspace(_lib.load().qf_prefill_extend_workspace(b, qh, kvh, t_, cap),
                     "qf_prefill_extend_workspace", dev)
-    with torch.cuda.device(dev):
-        rc = lib.qf_prefill_extend_paged(
-            query.data_ptr(), query.stride(1), query.stride(0),
-            key.data_ptr(), key.stride(1), key.stride(0),
-            value.data_ptr(), value.stride(1), value.stride(0),
-            cu_seqlens.data_ptr(), t_, context.data_ptr(), ctx_sb, _ptr(cos), _ptr(sin), cs_sn,
-            *pool, cap, ws.data_ptr(), ws.numel(), out.data_ptr(), out.stride(1), out.stride(0),
-            b, qh, kvh, d, float(d ** -0.5 if scale is None else scale), _stream(dev))
-    _lib.check(rc, "qf_prefill_extend_paged")
+    qs, ks, vs = query.stride(), key.stride(), value.stride()
+    _call("qf_prefill_extend_paged", index, query.data_ptr(), qs[1], qs[0], key.data_ptr(), ks[1], ks[0],
+          value.data_ptr(), vs[1], vs[0], cu_seqlens.data_ptr(), t_, context.data_ptr(), ctx_sb, _ptr(cos),
+          _ptr(sin), cs_sn, *pool, cap, ws.data_ptr(), ws.shape[0], out.data_ptr(), d, qh * d, b, qh, kvh, d,
+          d ** -0.5 if scale is None else scale)
     return out
 
 

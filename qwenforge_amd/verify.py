@@ -12,15 +12,16 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _ptr, _stream, check_cu_seqlens
+from .ops import _ptr
+from .paged import _call, _check_rows, _workspace
 
 _DTYPES = {torch.float16: 0, torch.float32: 1}
 
 
-def _vector(name: str, t, n: int, dtype, device) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
-        raise TypeError(f"{name} must be a {str(dtype)[6:]} tensor on {device}")
-    if t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+def _vector(name: str, t, n: int, dtype, index: int) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index:
+        raise TypeError(f"{name} must be a {str(dtype)[6:]} tensor on cuda:{index}")
+    if t.dim() != 1 or t.shape[0] != n or (t.stride(0) != 1 and n > 1):
         raise ValueError(f"{name} must be contiguous ({n},) (got {tuple(t.shape)})")
 
 
@@ -48,45 +49,42 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     count[b] new tokens, then -1.  A position whose logits give no distribution
     (NaN and the like) draws nothing.
     """
-    if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda":
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise RuntimeError("logits must be a HIP device tensor; there is no CPU path")
-    if logits.dtype not in _DTYPES:
+    kind = _DTYPES.get(logits.dtype)
+    if kind is None:
         raise TypeError(f"logits must be float16 or float32 (got {logits.dtype})")
     if logits.dim() != 2 or logits.numel() == 0 or logits.stride(1) != 1:
         raise ValueError(f"logits must be (T, V) with unit last stride (got {tuple(logits.shape)})")
     total, vocab = logits.shape
-    dev = logits.device
-    b = cu_seqlens.numel() - 1 if isinstance(cu_seqlens, torch.Tensor) else 0
+    index, dev = logits.get_device(), logits.device
+    b = cu_seqlens.shape[0] - 1 if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.dim() == 1 else 0
     if b < 1 or not 1 <= max_seqlen <= total:
         raise ValueError(f"need B >= 1 rows and 1 <= max_seqlen <= T (got {b}, {max_seqlen})")
-    _vector("cu_seqlens", cu_seqlens, b + 1, torch.int32, dev)
-    _vector("tokens", tokens, total, torch.int64, dev)
+    _vector("cu_seqlens", cu_seqlens, b + 1, torch.int32, index)
+    _vector("tokens", tokens, total, torch.int64, index)
     temperature = float(temperature)
     if not 0.0 <= temperature < float("inf"):
         raise ValueError(f"temperature must be >= 0 and finite (got {temperature})")
+    probs_sn = 0
     if temperature > 0:
-        _vector("accept_u", accept_u, total, torch.float32, dev)
-        _vector("sample_u", sample_u, b, torch.float32, dev)
+        _vector("accept_u", accept_u, total, torch.float32, index)
+        _vector("sample_u", sample_u, b, torch.float32, index)
         if draft_probs is not None:
-            if draft_probs.dtype != torch.float32 or draft_probs.device != dev:
+            if draft_probs.dtype is not torch.float32 or draft_probs.get_device() != index:
                 raise TypeError(f"draft_probs must be a float32 tensor on {dev}")
             if draft_probs.shape != logits.shape or draft_probs.stride(1) != 1:
                 raise ValueError("draft_probs must have the logits' shape and unit last stride")
+            probs_sn = draft_probs.stride(0) if total > 1 else vocab
     else:
         accept_u = sample_u = draft_probs = None
-    check_cu_seqlens(cu_seqlens, total, max_seqlen, lengths)
-    lib = _lib.load()
-    need = lib.qf_verify_workspace(total, b, vocab)
-    _lib.check(min(need, 0), "qf_verify_workspace")
-    ws = torch.empty(need, device=dev, dtype=torch.uint8)
-    out = torch.empty((b, max_seqlen), device=dev, dtype=torch.int64)
-    count = torch.empty(b, device=dev, dtype=torch.int64)
-    with torch.cuda.device(dev):
-        rc = lib.qf_verify_drafts(
-            logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0) if total > 1 else vocab,
-            tokens.data_ptr(), cu_seqlens.data_ptr(), _ptr(accept_u), _ptr(sample_u),
-            _ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0) if total > 1 else vocab,
-            temperature, out.data_ptr(), int(max_seqlen), count.data_ptr(), ws.data_ptr(), need,
-            total, b, vocab, _stream(dev))
-    _lib.check(rc, "qf_verify_drafts")
+    _check_rows(cu_seqlens, total, max_seqlen, lengths)
+    # The counts lie behind the rows' tokens, in one allocation.
+    both = torch.empty(b * (max_seqlen + 1), device=dev, dtype=torch.int64)
+    out, count = both[:b * max_seqlen].view(b, max_seqlen), both[b * max_seqlen:]
+    ws = _workspace(_lib.load().qf_verify_workspace(total, b, vocab), "qf_verify_workspace", dev)
+    _call("qf_verify_drafts", index, logits.data_ptr(), kind, logits.stride(0) if total > 1 else vocab,
+          tokens.data_ptr(), cu_seqlens.data_ptr(), _ptr(accept_u), _ptr(sample_u), _ptr(draft_probs),
+          probs_sn, temperature, out.data_ptr(), max_seqlen, count.data_ptr(), ws.data_ptr(), ws.shape[0],
+          total, b, vocab)
     return count, out

@@ -73,16 +73,17 @@ def test_copy_pages_refusals():
         paged.copy_pages(pool.transpose(0, 1), [0], [1])
     lib = _lib.load()
 
-    def call(pools=(16, 32), sp=8192, src=16, dst=16, n=1, pages=4, kvh=2, page=64, d=64):
+    def call(pools=(16, 32), sp=8192, src=16, dst=16, n=1, pages=4, kvh=2, page=64, d=64, per=1, step=8):
         import ctypes as C
         arr = None if pools is None else (C.c_void_p * len(pools))(*pools)
-        return lib.qf_copy_pages(arr, 0 if pools is None else len(pools), sp, 4096, 64, src, dst, None,
+        return lib.qf_copy_pages(arr, 0 if pools is None else len(pools), per, step, sp, 4096, 64, src, dst, None,
                                  n, pages, kvh, page, d, None)
 
     assert call(n=0) == 0                                # nothing to do, nothing launched
     assert call(d=128) == -2 and call(page=96) == -2 and call(pages=0) == -2
     assert call(pools=None) == -1 and call(pools=(16, None)) == -1 and call(pools=(16, 8)) == -1
     assert call(sp=8188) == -1 and call(src=None) == -1 and call(n=-1) == -1 and call(kvh=0) == -1
+    assert call(per=0) == -1 and call(per=65536) == -1 and call(step=4) == -1
 
 
 def test_verify_refusals_without_a_gpu():
