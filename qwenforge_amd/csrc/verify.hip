@@ -4,14 +4,15 @@
 //
 // stats_kernel reads every logit once: maximum and sum of exponentials (or the
 // argmax) of each chunk of each position, fp32 within a thread's few values.
-// draw_kernel, a workgroup per row and chunk of 2048 tokens, finds the row's
-// first rejection from those and goes over the logits of that one position
-// again.  Its weights and sums are in 64 bits: the token drawn is where a
-// running sum over the vocabulary crosses a number, and a sum off by 2^-24 would
-// move that crossing past a token in some draws out of a hundred.  The workgroup
-// that completes a row adds up its chunks and searches the one of the crossing.
-// With draft probabilities the sum of exponentials has to be known in 64 bits
-// before max(p - q, 0) can be formed, so a first launch of the kernel takes it.
+// decide_kernel, a workgroup per row, finds the row's first rejection from
+// those.  draw_kernel, a workgroup per row and chunk of 2048 tokens, goes over the
+// logits of that one position again.  Its weights and sums are in 64 bits: the
+// token drawn is where a running sum over the vocabulary crosses a number, and a
+// sum off by 2^-24 would move that crossing past a token in some draws out of a
+// hundred.  The workgroup that completes a row adds up its chunks and searches
+// the one of the crossing.  With draft probabilities the sum of exponentials has
+// to be known in 64 bits before max(p - q, 0) can be formed, so a first launch of
+// the kernel takes it.
 #include <algorithm>
 #include <cmath>
 
@@ -26,6 +27,9 @@ constexpr int kGroup = 8;                  // consecutive logits of a thread
 constexpr int kChunk = kThreads * kGroup;  // tokens of a draw_kernel workgroup
 constexpr int kMaxParts = 64;              // chunks of a position in stats_kernel
 constexpr int kMinPart = 256;              // least groups of one
+// Counters of the rows, each on a 128-byte line of its own: counts of one line
+// are taken one after the other, 32 rows' 2400 of them in some 20 us.
+constexpr int kTicket = 32;
 
 struct Args {
   const void* logits;
@@ -43,7 +47,8 @@ struct Args {
   float2* stats;       // (T, parts): max, sum (argmax: max, index)
   double2* sums;       // (B, chunks): weights left after the draft, all weights
   double* total;       // (B, chunks): sums of exponentials (draft probabilities)
-  int32_t* ticket;     // (B), zeroed by stats_kernel
+  int4* rows;          // (B): first position, positions, accepted drafts, maximum there
+  int32_t* ticket;     // one in every kTicket, zeroed by decide_kernel
   int width, T, B, V, parts, chunks;
 };
 
@@ -90,9 +95,6 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(Args a) {
   __shared__ int si[4];
   const int part = blockIdx.x % a.parts, pos = blockIdx.x / a.parts;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  if (!kArgmax)
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < a.B; i += (int64_t)gridDim.x * kThreads)
-      a.ticket[i] = 0;
   const E* row = static_cast<const E*>(a.logits) + pos * a.lg_sn;
   const int before = lead(row);
   const int groups = (int)(((int64_t)a.V + before + kGroup - 1) / kGroup);
@@ -213,12 +215,22 @@ __device__ __forceinline__ double exp_of(const Args& a, float x, float top) {
   return exp(((double)x - (double)top) * a.inv_t);
 }
 
-// Drafts of the row that are accepted, by the whole workgroup: waves take the
-// positions in turn.
+// Drafts of the row that are accepted: waves take the positions in turn.
 template <typename E>
-__device__ __forceinline__ int accepted(const Args& a, int lo, int n, int& first) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  if (threadIdx.x == 0) first = n - 1;
+__global__ __launch_bounds__(kThreads) void decide_kernel(Args a) {
+  __shared__ int first;
+  const int b = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int lo, n;
+  row_span(a, b, lo, n);
+  if (threadIdx.x == 0) {
+    first = n - 1;
+    a.ticket[b * kTicket] = 0;
+  }
+  if (n == 0) {
+    if (threadIdx.x == 0) a.rows[b] = int4{lo, 0, 0, 0};
+    write_row(a, b, lo, 0, -1);
+    return;
+  }
   __syncthreads();
   for (int j = w; j < n - 1; j += kThreads / 64) {
     const int64_t pos = lo + j;
@@ -235,17 +247,39 @@ __device__ __forceinline__ int accepted(const Args& a, int lo, int n, int& first
     if (lane == 0 && !((double)a.accept_u[pos] * (double)qd < p)) atomicMin(&first, j);
   }
   __syncthreads();
-  return first;
+  if (w != 0) return;
+  const int taken = first;
+  const float top = wave_max(lane < a.parts ? a.stats[(int64_t)(lo + taken) * a.parts + lane].x : kNegInf);
+  if (lane == 0) a.rows[b] = int4{lo, n, taken, __float_as_int(top)};
 }
 
-// Inclusive sums over the workgroup's threads; `all` their total.
+// x of another lane by a DPP move, 0 where the move names none.
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)u, kCtrl, kRowMask, 0xF, true);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), kCtrl, kRowMask, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Inclusive sums over the lanes of a wave: within rows of 16 lanes, then across
+// them (a lane that a move leaves out adds 0).
+__device__ __forceinline__ double wave_scan(double x) {
+  x += dpp<0x111, 0xF>(x);  // row_shr:1
+  x += dpp<0x112, 0xF>(x);  // row_shr:2
+  x += dpp<0x114, 0xF>(x);  // row_shr:4
+  x += dpp<0x118, 0xF>(x);  // row_shr:8
+  x += dpp<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
+  x += dpp<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
+// Inclusive sums over the workgroup's threads; `all` their total.  `part` is this
+// call's own.
 __device__ __forceinline__ double block_scan(double x, double (&part)[4], double& all) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  for (int d = 1; d < 64; d <<= 1) {
-    const double y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  if (lane == 63) part[w] = x;
+  const int w = threadIdx.x >> 6;
+  x = wave_scan(x);
+  if ((threadIdx.x & 63) == 63) part[w] = x;
   __syncthreads();
   double ahead = 0.;
   all = 0.;
@@ -254,45 +288,44 @@ __device__ __forceinline__ double block_scan(double x, double (&part)[4], double
     if (i < w) ahead += part[i];
     all += part[i];
   }
-  __syncthreads();
   return ahead + x;
 }
 
-// The first thread with `hit`, or the last one with `some`, or -1.
-__device__ __forceinline__ int first_thread(bool hit, bool some, int (&at)[2]) {
-  if (threadIdx.x == 0) {
-    at[0] = kThreads;
-    at[1] = -1;
+// The first thread with `hit`, or the last one with `some`, or -1.  `at` is this
+// call's own.
+__device__ __forceinline__ int find_thread(bool hit, bool some, int2 (&at)[4]) {
+  const uint64_t h = __ballot(hit), m = __ballot(some);
+  if ((threadIdx.x & 63) == 0)
+    at[threadIdx.x >> 6] = int2{h ? __builtin_ctzll(h) : -1, m ? 63 - __builtin_clzll(m) : -1};
+  __syncthreads();
+  int last = -1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (at[i].x >= 0) return 64 * i + at[i].x;
+    if (at[i].y >= 0) last = 64 * i + at[i].y;
   }
-  __syncthreads();
-  if (hit) atomicMin(&at[0], (int)threadIdx.x);
-  if (some) atomicMax(&at[1], (int)threadIdx.x);
-  __syncthreads();
-  const int found = at[0] < kThreads ? at[0] : at[1];
-  __syncthreads();
-  return found;
+  return last;
 }
 
 // kTotal: only the sums of exponentials of the drawn position.  Else its
 // weights, and the draw by the row's last workgroup.
 template <typename E, bool kTotal>
 __global__ __launch_bounds__(kThreads) void draw_kernel(Args a) {
-  __shared__ int first, at[2];
-  __shared__ double part[4];
+  __shared__ double part[5][4];
+  __shared__ int2 at[2][4];
+  __shared__ int found_chunk, token;
+  __shared__ double found_ahead;
   __shared__ bool mine;
   const int b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-  const int tid = threadIdx.x, lane = tid & 63;
-  int lo, n;
-  row_span(a, b, lo, n);
-  if (n == 0) {
-    if (!kTotal && chunk == 0) write_row(a, b, lo, 0, -1);
-    return;
-  }
-  const int taken = accepted<E>(a, lo, n, first);
-  const int64_t pos = lo + taken;
+  const int tid = threadIdx.x;
+  const int4 r = a.rows[b];
+  if (r.y == 0) return;
+  const int taken = r.z;
+  const float top = __int_as_float(r.w);
+  const int64_t pos = r.x + taken;
   const E* row = static_cast<const E*>(a.logits) + pos * a.lg_sn;
-  const float top = wave_max(lane < a.parts ? a.stats[pos * a.parts + lane].x : kNegInf);
-  const bool refused = taken < n - 1;
+  const bool refused = taken < r.y - 1;
+  if (kTotal && !refused) return;
   const int64_t draft = refused && a.probs == nullptr ? a.tokens[pos + 1] : -1;
   const float* q = refused && a.probs != nullptr ? a.probs + pos * a.dp_sn : nullptr;
   const int before = lead(row);
@@ -300,20 +333,26 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Args a) {
   if (!kTotal && q != nullptr) {
     double s = 0.;
     for (int i = tid; i < a.chunks; i += kThreads) s += a.total[(int64_t)b * a.chunks + i];
-    block_scan(s, part, sum_exp);
+    block_scan(s, part[0], sum_exp);
   }
-  // Weights of this thread's eight tokens of chunk c: (left after the draft, all).
+  // Weights of this thread's eight tokens of chunk c: left after the draft, all.
   const auto weights = [&](int c, double (&left)[kGroup], double (&all)[kGroup]) {
     const int start = c * kChunk + tid * kGroup - before;
-    float x[kGroup];
+    float x[kGroup], y[kGroup];
     load8(row, start, a.V, kNegInf, x);
+    if (q != nullptr) {
+      // Aligned like the logits only if the rows are.
+      if ((reinterpret_cast<uintptr_t>(q + start) & 15u) == 0) load8(q, start, a.V, 0.f, y);
+      else
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e) y[e] = start + e >= 0 && start + e < a.V ? q[start + e] : 0.f;
+    }
 #pragma unroll
     for (int e = 0; e < kGroup; ++e) {
       const int i = start + e;
-      const bool in = i >= 0 && i < a.V;
-      all[e] = in ? exp_of(a, x[e], top) : 0.;
+      all[e] = i >= 0 && i < a.V ? exp_of(a, x[e], top) : 0.;
       left[e] = all[e];
-      if (q != nullptr && in) left[e] = fmax(all[e] - (double)q[i] * sum_exp, 0.);
+      if (q != nullptr) left[e] = fmax(all[e] - (double)y[e] * sum_exp, 0.);
       if (i == draft) left[e] = 0.;
     }
   };
@@ -325,12 +364,12 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Args a) {
     sa += all[e];
   }
   double chunk_left, chunk_all;
-  block_scan(sa, part, chunk_all);
+  block_scan(sa, part[1], chunk_all);
   if (kTotal) {
     if (tid == 0) a.total[(int64_t)b * a.chunks + chunk] = chunk_all;
     return;
   }
-  block_scan(sl, part, chunk_left);
+  block_scan(sl, part[2], chunk_left);
   if (tid == 0) {
     double2* s = a.sums + (int64_t)b * a.chunks + chunk;
     __hip_atomic_store(&s->x, chunk_left, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -341,77 +380,69 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Args a) {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     s_waitcnt_vm(0);
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    mine = __hip_atomic_fetch_add(&a.ticket[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+    mine = __hip_atomic_fetch_add(&a.ticket[b * kTicket], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
            a.chunks - 1;
   }
   __syncthreads();
   if (!mine) return;
-  // Totals over the chunks, then the chunk, thread and token of the crossing.
+  // The chunk of the crossing: a thread adds up `per` neighbouring chunks, the
+  // thread of the crossing walks them.
+  const int per = (a.chunks + kThreads - 1) / kThreads;
   const auto chunk_sum = [&](int c, bool use_left) {
-    if (c >= a.chunks) return 0.;
     double2* s = a.sums + (int64_t)b * a.chunks + c;
     return __hip_atomic_load(use_left ? &s->x : &s->y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   };
   bool use_left = true;
-  double total = 0.;
-  for (int pass = 0; pass < 2; ++pass) {
-    double s = 0.;
-    total = 0.;
-    for (int c0 = 0; c0 < a.chunks; c0 += kThreads) {
-      block_scan(chunk_sum(c0 + tid, use_left), part, s);
-      total += s;
-    }
+  double total, s, upto;
+  for (int pass = 0;; ++pass) {
+    s = 0.;
+    for (int c = tid * per; c < min((tid + 1) * per, a.chunks); ++c) s += chunk_sum(c, use_left);
+    upto = block_scan(s, part[3 + pass], total);
     if (total > 0. && total < (double)__builtin_huge_val()) break;
-    use_left = false;
     if (pass == 1) {
-      write_row(a, b, lo, taken, -1);
+      write_row(a, b, r.x, taken, -1);
       return;
     }
+    use_left = false;  // nothing left after the draft: from all of p
   }
   const double mark = (double)a.sample_u[b] * total;
-  int found = -1;
-  double ahead = 0., found_ahead = 0.;
-  for (int c0 = 0; c0 < a.chunks; c0 += kThreads) {
-    const double s = chunk_sum(c0 + tid, use_left);
-    double batch;
-    const double upto = ahead + block_scan(s, part, batch);
-    const bool hit = upto > mark && s > 0.;
-    const int t = first_thread(hit, s > 0., at);
-    if (t >= 0) {
-      found = c0 + t;
-      // Sums ahead of the chunk, from its thread.
-      if (tid == t) part[0] = upto - s;
-      __syncthreads();
-      found_ahead = part[0];
-      __syncthreads();
+  if (tid == find_thread(upto > mark && s > 0., s > 0., at[0])) {
+    double ahead = upto - s, passed = 0.;
+    for (int c = tid * per; c < min((tid + 1) * per, a.chunks); ++c) {
+      const double here = chunk_sum(c, use_left);
+      if (!(here > 0.)) continue;
+      ahead += passed;
+      passed = here;
+      found_chunk = c;
+      if (ahead + here > mark) break;
     }
-    ahead += batch;
-    if (__syncthreads_or(hit)) break;
+    found_ahead = ahead;
   }
+  __syncthreads();
+  const int found = found_chunk;
   weights(found, left, all);
-  double s = 0.;
+  s = 0.;
 #pragma unroll
   for (int e = 0; e < kGroup; ++e) s += use_left ? left[e] : all[e];
   double whole;
-  const double upto = found_ahead + block_scan(s, part, whole);
-  const int t = first_thread(upto > mark && s > 0., s > 0., at);
-  if (tid == t) {
+  upto = found_ahead + block_scan(s, part[1], whole);
+  if (tid == find_thread(upto > mark && s > 0., s > 0., at[1])) {
     double sum = upto - s;
-    int token = -1;
+    int here = -1;
     bool crossed = false;
 #pragma unroll
     for (int e = 0; e < kGroup; ++e) {
       const double w = use_left ? left[e] : all[e];
       sum += w;
       if (!crossed && w > 0.) {
-        token = found * kChunk + tid * kGroup - before + e;
+        here = found * kChunk + tid * kGroup - before + e;
         crossed = sum > mark;
       }
     }
-    at[0] = token;
+    token = here;
   }
   __syncthreads();
-  write_row(a, b, lo, taken, at[0]);
+  write_row(a, b, r.x, taken, token);
 }
 
 int parts_of(int T, int V) {
@@ -432,10 +463,10 @@ extern "C" int64_t qf_verify_workspace(int T, int B, int V) {
   using namespace qf::verify;
   if (T < 1 || B < 1 || V < 1) return QF_ERR_INVALID_ARG;
   if (V > 0x7fffffff - 2 * kChunk || (int64_t)T * kMaxParts > 0x7fffffff ||
-      (int64_t)B * chunks_of(V) > 0x7fffffff)
+      (int64_t)B * chunks_of(V) > 0x7fffffff || B > 0x7fffffff / kTicket)
     return QF_ERR_UNSUPPORTED;
   const int64_t sums = (int64_t)B * chunks_of(V);
-  return round16((int64_t)T * parts_of(T, V) * 8) + sums * 16 + round16(sums * 8) + (int64_t)B * 4;
+  return round16((int64_t)T * parts_of(T, V) * 8) + sums * 16 + round16(sums * 8) + (int64_t)B * (16 + 4 * kTicket);
 }
 
 namespace qf {
@@ -450,6 +481,7 @@ int launch(const Args& a, bool greedy, hipStream_t st) {
     return (int)hipGetLastError();
   }
   hipLaunchKernelGGL((stats_kernel<E, false>), all, block, 0, st, a);
+  hipLaunchKernelGGL(decide_kernel<E>, dim3(a.B), block, 0, st, a);
   const dim3 draw((unsigned)(a.B * a.chunks));
   if (a.probs != nullptr) hipLaunchKernelGGL((draw_kernel<E, true>), draw, block, 0, st, a);
   hipLaunchKernelGGL((draw_kernel<E, false>), draw, block, 0, st, a);
@@ -505,7 +537,8 @@ extern "C" int qf_verify_drafts(const void* logits, int dtype, int64_t lg_sn, co
   p += verify::round16((int64_t)T * a.parts * 8);
   a.total = reinterpret_cast<double*>(p);
   p += verify::round16(sums * 8);
-  a.ticket = reinterpret_cast<int32_t*>(p);
+  a.rows = reinterpret_cast<int4*>(p);
+  a.ticket = reinterpret_cast<int32_t*>(p + (int64_t)B * 16);
   hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == QF_F16 ? launch<f16>(a, greedy, st) : launch<float>(a, greedy, st);
 }
