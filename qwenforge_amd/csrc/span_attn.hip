@@ -188,7 +188,7 @@ template <int kQB>
 struct State {
   f16x8 q[kQB][2];
   int lim[kQB];     // the column sees slots [lo, lim)
-  int lo;
+  int lo, seen;     // every column of the wave sees [lo, seen)
   float m[kQB];     // running reference, log2 units
   f32x4 l[kQB];     // running sum of p, in every row of the column
   f32x4 o[kQB][4];
@@ -219,8 +219,10 @@ __device__ __forceinline__ void init_state(State<kQB>& s, int lo, float scale_lo
   }
 }
 
-__device__ __forceinline__ bool special2(unsigned w) {  // either half an infinity or NaN
-  return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+// Bits 15 and 31 set for halves of w that are infinities or NaN (an exponent of
+// ones carries into the sign's place).
+__device__ __forceinline__ unsigned special2(unsigned w) {
+  return (w & 0x7FFF7FFFu) + 0x04000400u;
 }
 
 // The infinities and NaNs of a masked tile's V: out of the operands, so that a
@@ -239,10 +241,8 @@ __device__ __forceinline__ void masked_values(u32x2 (&vr)[2][4][2], const State<
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          unsigned w = vr[ch][t][h][x];
-          if ((w & 0x7C00u) == 0x7C00u) w &= 0xFFFF0000u;
-          if ((w & 0x7C000000u) == 0x7C000000u) w &= 0xFFFFu;
-          vr[ch][t][h][x] = w;
+          const unsigned bad = (special2(vr[ch][t][h][x]) & 0x80008000u) >> 15;
+          vr[ch][t][h][x] &= ~(bad * 0xFFFFu);
         }
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
 #pragma unroll
@@ -334,40 +334,30 @@ __device__ __forceinline__ void scores(f32x4 (&sc)[kQB][4], const KTile& k, cons
         }
 }
 
-// Whether a query of the wave does not see all of the tile at key0.
-template <int kQB>
-__device__ __forceinline__ bool is_masked(const State<kQB>& s, int key0) {
-  bool masked = key0 < s.lo;
-#pragma unroll
-  for (int b = 0; b < kQB; ++b) masked = masked || __any(s.lim[b] < key0 + kBN);
-  return masked;
-}
-
-template <int kQB>
+// Drops the scores of keys past each column's bound, and below the unit's first
+// slot where its first tile holds such keys (narrow units only: the others
+// start on a tile's edge).
+template <int kQB, bool kLow>
 __device__ __forceinline__ void mask(f32x4 (&sc)[kQB][4], const State<kQB>& s, int key0) {
   const int grp = (threadIdx.x & 63) >> 4;
 #pragma unroll
-  for (int b = 0; b < kQB; ++b)
+  for (int b = 0; b < kQB; ++b) {
+    const int left = s.lim[b] - key0 - 8 * grp, skip = s.lo - key0 - 8 * grp;
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = key0 + 32 * (blk >> 1) + 8 * grp + 4 * (blk & 1) + i;
-        if (key < s.lo || key >= s.lim[b]) sc[b][blk][i] = kNegInf;
+        const int key = 32 * (blk >> 1) + 4 * (blk & 1) + i;
+        if (key >= left || (kLow && key < skip)) sc[b][blk][i] = kNegInf;
       }
+  }
 }
 
 // Largest score of each lane, log2 units.
 template <int kQB>
-__device__ __forceinline__ void tops(float (&mx)[kQB], const f32x4 (&sc)[kQB][4], float ks2) {
+__device__ __forceinline__ void tops(float (&mx)[kQB], f32x4 (&sc)[kQB][4], float ks2) {
 #pragma unroll
-  for (int b = 0; b < kQB; ++b) {
-    float t[4];
-#pragma unroll
-    for (int blk = 0; blk < 4; ++blk)
-      t[blk] = fmaxf(fmaxf(sc[b][blk][0], sc[b][blk][1]), fmaxf(sc[b][blk][2], sc[b][blk][3]));
-    mx[b] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * ks2;
-  }
+  for (int b = 0; b < kQB; ++b) mx[b] = max16(sc[b]) * ks2;
 }
 
 // Moves the references of the columns whose scores grew past them.  A column
@@ -432,14 +422,14 @@ __device__ __forceinline__ void add_values(State<kQB>& s, const f16x8 (&pb)[kQB]
 template <int kQB>
 __device__ __forceinline__ void check_values(VTile& v, State<kQB>& s, const f16x8 (&pb)[kQB][2],
                                              int key0, const unsigned char* Vs) {
-  bool bad = false;
+  unsigned bad = 0;
 #pragma unroll
   for (int ch = 0; ch < 2; ++ch)
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) bad = bad || special2(v.r[ch][t][h][0]) || special2(v.r[ch][t][h][1]);
-  if (__any(bad)) masked_values<kQB>(v.r, s, pb, key0, s.o, Vs);
+      for (int h = 0; h < 2; ++h) bad |= special2(v.r[ch][t][h][0]) | special2(v.r[ch][t][h][1]);
+  if (__any((bad & 0x80008000u) != 0)) masked_values<kQB>(v.r, s, pb, key0, s.o, Vs);
 }
 
 // Scores, online softmax and PV product of the tile of keys [key0, key0 + 64)
@@ -452,8 +442,8 @@ __device__ __forceinline__ void tile_step(State<kQB>& s, int key0, const unsigne
   wait_k(k);
   f32x4 sc[kQB][4];
   scores(sc, k, s);
-  const bool masked = is_masked(s, key0);
-  if (masked) mask(sc, s, key0);
+  const bool masked = key0 < s.lo || key0 + kBN > s.seen;
+  if (masked) mask<kQB, true>(sc, s, key0);
   float mx[kQB];
   tops(mx, sc, s.ks2);
   raise(s, mx);
@@ -530,6 +520,11 @@ __device__ __forceinline__ void load_queries(State<kQB>& s, const Args& a, const
     }
     s.lim[b] = r < u.rows ? row_limit(a, u, token) : u.k1;
   }
+  int least = s.lim[0];
+#pragma unroll
+  for (int b = 1; b < kQB; ++b) least = min(least, s.lim[b]);
+  for (int d = 8; d > 0; d >>= 1) least = min(least, __shfl_xor(least, d));  // columns: 16 lanes
+  s.seen = __builtin_amdgcn_readfirstlane(least);
 }
 
 // o / l of a column, zero where nothing was seen.
@@ -608,9 +603,9 @@ __device__ __forceinline__ void wide_unit(const Args& a, const Unit& u, unsigned
   }
   for (int i = 0, st = 0; i < n; ++i, st = after(st, 1)) {
     const int key0 = first + i * kBN;
-    const bool masked = is_masked(s, key0);
+    const bool masked = key0 + kBN > s.seen;
     if (masked) {
-      mask(sc, s, key0);
+      mask<kQB, false>(sc, s, key0);
       tops(mx, sc, s.ks2);
     }
     raise(s, mx);
