@@ -429,7 +429,12 @@ __device__ __forceinline__ void check_values(VTile& v, State<kQB>& s, const f16x
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) bad |= special2(v.r[ch][t][h][0]) | special2(v.r[ch][t][h][1]);
-  if (__any((bad & 0x80008000u) != 0)) masked_values<kQB>(v.r, s, pb, key0, s.o, Vs);
+  if (__any((bad & 0x80008000u) != 0)) {
+    masked_values<kQB>(v.r, s, pb, key0, s.o, Vs);
+    // lgkmcnt(0) where the compiler sees it: it would wait for these LDS reads at
+    // the end of the branch's other side too, among reads it does not know.
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+  }
 }
 
 // Scores, online softmax and PV product of the tile of keys [key0, key0 + 64)
@@ -601,7 +606,9 @@ __device__ __forceinline__ void wide_unit(const Args& a, const Unit& u, unsigned
     read_k(k, s.koff, stage(1, 0));
     wait_k(k);
   }
-  for (int i = 0, st = 0; i < n; ++i, st = after(st, 1)) {
+  int st = 0;
+  // Step i from its scores `sc`; `next` becomes step i + 1's.
+  const auto step = [&](int i, f32x4 (&sc)[kQB][4], f32x4 (&next)[kQB][4]) __attribute__((always_inline)) {
     const int key0 = first + i * kBN;
     const bool masked = key0 + kBN > s.seen;
     if (masked) {
@@ -613,9 +620,9 @@ __device__ __forceinline__ void wide_unit(const Args& a, const Unit& u, unsigned
     // reads in flight are not the compiler's.
     VTile v;
     read_v(v, s.voff, stage(st, 1));
-    f32x4 next[kQB][4];  // past the last tile: of its K again, unused
+    __builtin_amdgcn_sched_barrier(0);
     f16x8 pb[kQB][2];
-    scores(next, k, s);
+    scores(next, k, s);  // past the last tile: of its K again, unused
 #pragma unroll
     for (int b = 0; b < kQB; ++b) weights(pb, sc, s, b);
     // One matrix product, then vector work for the 16 cycles that it takes.
@@ -636,13 +643,16 @@ __device__ __forceinline__ void wide_unit(const Args& a, const Unit& u, unsigned
     load(i + 4, after(st, 4));
     if (masked) check_values(v, s, pb, key0, stage(st, 1));
     read_k(k, s.koff, stage(i + 2 < n ? after(st, 2) : st, 0));
+    __builtin_amdgcn_sched_barrier(0);
     add_values(s, pb, v);
     tops(mx, next, s.ks2);
     wait_k(k);
-#pragma unroll
-    for (int b = 0; b < kQB; ++b)
-#pragma unroll
-      for (int blk = 0; blk < 4; ++blk) sc[b][blk] = next[b][blk];
+    st = after(st, 1);
+  };
+  f32x4 next[kQB][4];
+  for (int i = 0; i < n; i += 2) {  // in pairs, so that no scores are copied
+    step(i, sc, next);
+    if (i + 1 < n) step(i + 1, next, sc);
   }
   const int col = threadIdx.x & 15;
   const Args& late = late_args();
