@@ -794,46 +794,74 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
   }
 }
 
-// Joins the `n` partials of each (token, kv head, query head): one wave each,
-// lane j holding the weights of partials j and j + 64, then 16 lanes of 4 dims
-// for each of four partials at a time.
+// Joins the `n` partials of each (token, kv head, query head).  kSubs groups of 16
+// lanes, a lane for 4 dims, share a query: one where there are few partials (four
+// queries to a wave), four where there are many.  A lane loads the statistics of
+// a partial of its own, kEach times, and hands the weights around; then each
+// group takes every kSubs-th partial, eight loads in flight together.
+template <int kSubs, int kEach>
 __global__ __launch_bounds__(256) void span_merge_kernel(Args a, int n) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= (int64_t)a.tokens * a.KVH * a.G) return;
-  const int g = (int)(id % a.G);
-  const int64_t th = id / a.G;
+  constexpr int kLanes = 16 * kSubs;  // of one query
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t id = (int64_t)blockIdx.x * (16 / kSubs) + tid / (16 * kSubs);
+  const bool in = id < (int64_t)a.tokens * a.KVH * a.G;
+  const int64_t id0 = in ? id : 0;
+  const int g = (int)(id0 % a.G);
+  const int64_t th = id0 / a.G;
   const int hk = (int)(th % a.KVH), token = (int)(th / a.KVH);
   const int64_t p0 = th * n * a.G + g;
-  float2 x[2];
+  const int mine = lane & (kLanes - 1), base = lane & ~(kLanes - 1);
+  float2 x[kEach];
+  float top = kNegInf;
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    x[h] = lane + 64 * h < n ? a.ml[p0 + (int64_t)(lane + 64 * h) * a.G] : float2{kNegInf, 0.f};
-  float top = fmaxf(x[0].x, x[1].x);
-  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  float wt[2], sum = 0.f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    wt[h] = x[h].y == 0.f ? 0.f : x[h].x == top ? 1.f : fast_exp2(x[h].x - top);
-    sum += x[h].y == 0.f ? 0.f : wt[h] * x[h].y;
+  for (int h = 0; h < kEach; ++h) {
+    const int j = mine + kLanes * h;
+    x[h] = j < n ? a.ml[p0 + (int64_t)j * a.G] : float2{kNegInf, 0.f};
+    top = fmaxf(top, x[h].x);
   }
-  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-  uint64_t there[2];
+  for (int d = kLanes / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  float sum = 0.f;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) there[h] = __ballot(x[h].y != 0.f);
+  for (int h = 0; h < kEach; ++h) {
+    // Absent partials have l = 0, whatever their accumulators hold.
+    const float w = x[h].y == 0.f ? 0.f : x[h].x == top ? 1.f : fast_exp2(x[h].x - top);
+    sum += x[h].y == 0.f ? 0.f : w * x[h].y;
+    x[h].x = w;
+  }
+  for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  const int sub = (tid >> 4) & (kSubs - 1), d0 = 4 * (lane & 15);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  const int sub = lane >> 4, d = 4 * (lane & 15);
+  constexpr int kRounds = kLanes * kEach / kSubs;  // partials of a group
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    for (int j0 = 0; j0 < 64 && 64 * h + j0 < n; j0 += 4) {
-      const int j = j0 + sub;
-      const float w = __shfl(wt[h], j);
-      if (there[h] >> j & 1)
-        o += *reinterpret_cast<const f32x4*>(a.acc + (p0 + (int64_t)(64 * h + j) * a.G) * kD + d) * w;
+  for (int i0 = 0; i0 < kRounds; i0 += 8) {
+    if (i0 * kSubs >= n) break;
+    f32x4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8 && i0 + i < kRounds; ++i) {
+      const int j = min(sub + kSubs * (i0 + i), n - 1);
+      v[i] = *reinterpret_cast<const f32x4*>(a.acc + (p0 + (int64_t)j * a.G) * kD + d0);
     }
 #pragma unroll
-  for (int c = 0; c < 4; ++c) o[c] = col_sum(o[c]);
-  if (sub == 0) store_out(a, token, hk, g, d, o, sum);
+    for (int i = 0; i < 8 && i0 + i < kRounds; ++i) {
+      const int j = sub + kSubs * (i0 + i);
+      float w = 0.f, l = 0.f;
+#pragma unroll
+      for (int h = 0; h < kEach; ++h) {
+        const float wh = __shfl(x[h].x, base + (j & (kLanes - 1)));
+        const float lh = __shfl(x[h].y, base + (j & (kLanes - 1)));
+        if (j / kLanes == h) {
+          w = wh;
+          l = lh;
+        }
+      }
+      if (j < n && l != 0.f) o += v[i] * w;
+    }
+  }
+  if constexpr (kSubs > 1) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = col_sum(o[c]);
+  }
+  if (in && (kSubs == 1 || lane < 16)) store_out(a, token, hk, g, d0, o, sum);
 }
 
 // K (rotated with cos / sin if given) and V of every new token into its slot:
@@ -943,7 +971,10 @@ int launch(const Args& a, const Plan& p, hipStream_t st) {
   const int n = kDecode ? a.splits + a.own_splits : a.splits;
   if (rc == 0 && (kDecode || n > 1)) {
     const int64_t queries = (int64_t)a.tokens * a.KVH * a.G;
-    hipLaunchKernelGGL(span_merge_kernel, dim3((unsigned)((queries + 3) / 4)), dim3(256), 0, st, a, n);
+    const dim3 all((unsigned)((queries + 15) / 16)), quarter((unsigned)((queries + 3) / 4));
+    if (n <= 8) hipLaunchKernelGGL((span_merge_kernel<1, 1>), all, dim3(256), 0, st, a, n);
+    else if (n <= 64) hipLaunchKernelGGL((span_merge_kernel<4, 1>), quarter, dim3(256), 0, st, a, n);
+    else hipLaunchKernelGGL((span_merge_kernel<4, 2>), quarter, dim3(256), 0, st, a, n);
     rc = (int)hipGetLastError();
   }
   return rc;
