@@ -31,9 +31,10 @@ constexpr int kBN = 64;                      // keys per tile
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kTileBytes = kBN * kRowBytes;  // of K or V
-constexpr int kStages = 5;                   // ring of the wide units: two workgroups fill a CU's LDS
+constexpr int kStages = 4;                   // ring of the wide units
 constexpr int kMaxSplits = 64;               // of either kind of unit
 constexpr int kMinKeys = 128;                // least keys of a split
+constexpr int kStepKeys = kWaves * kBN;      // a step of a narrow unit's waves
 
 struct Args {
   const f16* q;
@@ -462,12 +463,10 @@ __device__ __forceinline__ void tile_step(State<kQB>& s, int key0, const unsigne
   add_values(s, pb, v);
 }
 
-// All but this wave's newest `ahead` tiles of loads (four each) have landed, and
-// after the barrier that holds for every wave.
+// All but this wave's newest `ahead` tiles of loads (0 or 1, of four) have
+// landed, and after the barrier that holds for every wave.
 __device__ __forceinline__ void stage_ready(int ahead) {
-  if (ahead >= 2) __builtin_amdgcn_s_waitcnt(0x0F78);       // vmcnt(8)
-  else if (ahead == 1) __builtin_amdgcn_s_waitcnt(0x0F74);  // vmcnt(4)
-  else __builtin_amdgcn_s_waitcnt(0x0F70);
+  s_waitcnt_vm(ahead == 0 ? 0 : 4);
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __builtin_amdgcn_s_barrier();
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -565,11 +564,22 @@ __device__ __forceinline__ void empty_unit(const Args& a, const Unit& u, int n_r
   }
 }
 
+// Places [from, to) of a unit's queries hold nothing.
+__device__ __forceinline__ void no_parts(const Args& a, const Unit& u, int n_rows, int from, int to) {
+  n_rows = min(n_rows, u.rows - u.r0);
+  for (int i = threadIdx.x; i < (to - from) * n_rows; i += kThreads) {
+    const int split = from + i / n_rows, r = u.r0 + i % n_rows;
+    const int64_t th = (int64_t)(u.tok0 + r / a.G) * a.KVH + u.hk;
+    a.ml[(th * u.n_split + split) * a.G + r % a.G] = float2{kNegInf, 0.f};
+  }
+}
+
 // kQB * 64 query rows, kQB * 16 per wave; the waves share the key tiles, on a
 // ring of kStages.  A step takes tile i's probabilities while the matrix cores
 // form tile i + 1's scores (its K came into registers during the step before),
-// then reads tile i + 2's K behind tile i's output product; tiles i + 3 and
-// i + 4 are on their way.
+// then reads tile i + 2's K behind tile i's output product; tile i + 3 is on its
+// way (one more stage, and tile i + 4 too, took 194 us where this takes 189: a
+// 2048-token chunk behind 16384 slots).
 template <int kQB>
 __device__ __forceinline__ void wide_unit(const Args& a, const Unit& u, unsigned char* lds) {
   if (u.k1 <= u.k0) {
@@ -593,11 +603,10 @@ __device__ __forceinline__ void wide_unit(const Args& a, const Unit& u, unsigned
   load_queries(s, a, u, row0);
   load(1, 1);
   load(2, 2);
-  load(3, 3);
   f32x4 sc[kQB][4];
   float mx[kQB];
   KTile k;
-  stage_ready(n - 2);  // tiles 0 and, if there is one, 1
+  stage_ready(n > 2 ? 1 : 0);  // tiles 0 and, if there is one, 1
   read_k(k, s.koff, stage(0, 0));
   wait_k(k);
   scores(sc, k, s);
@@ -638,9 +647,9 @@ __device__ __forceinline__ void wide_unit(const Args& a, const Unit& u, unsigned
     for (int b = 0; b < kQB; ++b) asm volatile("" : "+v"(pb[b][0]), "+v"(pb[b][1]));
     wait_v(v);
     // Tile i + 2 is there, and every wave is past tile i - 1, whose stage takes
-    // tile i + 4.
-    stage_ready(min(n - 3 - i, 1));
-    load(i + 4, after(st, 4));
+    // tile i + 3.
+    stage_ready(0);
+    load(i + 3, after(st, 3));
     if (masked) check_values(v, s, pb, key0, stage(st, 1));
     read_k(k, s.koff, stage(i + 2 < n ? after(st, 2) : st, 0));
     __builtin_amdgcn_sched_barrier(0);
@@ -720,10 +729,11 @@ __device__ __forceinline__ void narrow_unit(const Args& a, const Unit& u, unsign
   store_part(late_args(), u, u.r0 + (lane & 15), w, o, top, sum, w == 0);
 }
 
-// Slots [k0, k1) of split s of `n` splits over [lo, hi), cut at multiples of 64.
-__device__ __forceinline__ void cut(int lo, int hi, int s, int n, int& k0, int& k1) {
+// Slots [k0, k1) of split s of `n` splits of at least `least` over [lo, hi), cut at
+// multiples of 64.
+__device__ __forceinline__ void cut(int lo, int hi, int s, int n, int least, int& k0, int& k1) {
   const int first = lo & ~(kBN - 1);
-  const int len = max((int)(((int64_t)hi - first + n * kBN - 1) / (n * kBN)) * kBN, kMinKeys);
+  const int len = max((int)(((int64_t)hi - first + n * kBN - 1) / (n * kBN)) * kBN, least);
   const int64_t at = first + (int64_t)s * len;
   k0 = (int)(at < hi ? (s == 0 ? lo : at) : hi);
   k1 = (int)(at + len < hi ? at + len : hi);
@@ -737,15 +747,21 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
   static_assert(kStages >= kWaves, "the narrow units' four tiles fit too");
   __shared__ __attribute__((aligned(16))) unsigned char lds[kStages * 2 * kTileBytes];
   constexpr int kTr = kForm == 0 ? 16 : 64 * kForm;
-  const int n_first = a.n_tiles * a.KVH * a.splits;
+  const int n_first = a.n_tiles * ((a.KVH * a.splits + 7) & ~7);
   Unit u;
   u.ctx = -1;
   u.n_split = kDecode ? a.splits + a.own_splits : a.splits > 1 ? a.splits : 0;
   int before;
   if (!kDecode || (int)blockIdx.x < n_first) {
-    const int tile = blockIdx.x % a.n_tiles, rest = blockIdx.x / a.n_tiles;
+    // Workgroups go to the XCDs in turn.  Query tiles that read the same keys
+    // share an XCD and its L2: pairs of a kv head and a split are dealt out in
+    // turn, where there are XCDs enough for that.
+    int id = blockIdx.x;
+    if (a.KVH * a.splits >= 8) id = (id / (8 * a.n_tiles) * 8 + id % 8) * a.n_tiles + id / 8 % a.n_tiles;
+    const int tile = id % a.n_tiles, rest = id / a.n_tiles;
     u.hk = rest % a.KVH;
     u.split = rest / a.KVH;
+    if (u.split >= a.splits) return;
     const Segment g = find_segment(a, kTr, before, [&](int, int, int ahead, int tiles) {
       return tile < ahead + tiles;
     });
@@ -766,7 +782,7 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
       const int newest = (min(u.r0 + kTr, u.rows) - 1) / a.G;   // last token of the tile
       end = u.ctx < 0 ? 0 : min(u.ctx + newest + 1, a.cap);
     }
-    cut(0, end, u.split, a.splits, u.k0, u.k1);
+    cut(0, end, u.split, a.splits, kMinKeys, u.k0, u.k1);
     if constexpr (kForm == 0) narrow_unit(a, u, lds);
     else wide_unit<kForm>(a, u, lds);
   } else {
@@ -785,11 +801,10 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
     u.rows = a.G;
     u.r0 = 0;
     if (g.index < 0) {  // in no group: no workgroup reports on its shared slots
-      u.k0 = u.k1 = 0;
-      for (u.split = s; u.split < a.splits; u.split += a.own_splits) empty_unit(a, u, 16);
+      if (s == 0) no_parts(a, u, 16, 0, a.splits);
     }
     u.split = a.splits + s;
-    cut(lo, end, s, a.own_splits, u.k0, u.k1);
+    cut(lo, end, s, a.own_splits, kStepKeys, u.k0, u.k1);
     narrow_unit(a, u, lds);
   }
 }
@@ -832,30 +847,31 @@ __global__ __launch_bounds__(256) void span_merge_kernel(Args a, int n) {
   const int sub = (tid >> 4) & (kSubs - 1), d0 = 4 * (lane & 15);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   constexpr int kRounds = kLanes * kEach / kSubs;  // partials of a group
-#pragma unroll
+#pragma unroll 1
   for (int i0 = 0; i0 < kRounds; i0 += 8) {
     if (i0 * kSubs >= n) break;
     f32x4 v[8];
-#pragma unroll
-    for (int i = 0; i < 8 && i0 + i < kRounds; ++i) {
-      const int j = min(sub + kSubs * (i0 + i), n - 1);
-      v[i] = *reinterpret_cast<const f32x4*>(a.acc + (p0 + (int64_t)j * a.G) * kD + d0);
-    }
+    float w[8];
 #pragma unroll
     for (int i = 0; i < 8 && i0 + i < kRounds; ++i) {
       const int j = sub + kSubs * (i0 + i);
-      float w = 0.f, l = 0.f;
+      float l = 0.f;
+      w[i] = 0.f;
 #pragma unroll
       for (int h = 0; h < kEach; ++h) {
         const float wh = __shfl(x[h].x, base + (j & (kLanes - 1)));
         const float lh = __shfl(x[h].y, base + (j & (kLanes - 1)));
         if (j / kLanes == h) {
-          w = wh;
+          w[i] = wh;
           l = lh;
         }
       }
-      if (j < n && l != 0.f) o += v[i] * w;
+      v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (l != 0.f)
+        v[i] = *reinterpret_cast<const f32x4*>(a.acc + (p0 + (int64_t)j * a.G) * kD + d0);
     }
+#pragma unroll
+    for (int i = 0; i < 8 && i0 + i < kRounds; ++i) o += v[i] * w[i];
   }
   if constexpr (kSubs > 1) {
 #pragma unroll
@@ -930,10 +946,12 @@ int pick_form(int64_t rows_per_segment) {
   return rows_per_segment <= 16 ? 0 : rows_per_segment <= 64 ? 1 : 2;
 }
 
-// Splits so that the units fill the CUs twice, none for less than kMinKeys.
-int pick_splits(int64_t units, int cap, int fill) {
-  const int by_len = (int)std::min<int64_t>(kMaxSplits, ((int64_t)cap + kMinKeys - 1) / kMinKeys);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(by_len, fill / std::max<int64_t>(1, units)));
+// Splits of at least `least` keys, so that no more units are made than the two
+// workgroups per CU that run at once: some more would take a second round (286
+// units of 16 ragged rows behind 2048 slots: 56 us whole, 62 cut in two).
+int pick_splits(int64_t units, int cap, int least) {
+  const int64_t by_len = std::min<int64_t>(kMaxSplits, ((int64_t)cap + least - 1) / least);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(by_len, 2 * kCus / units));
 }
 
 Plan decode_plan(int B, int KVH, int G, int n_groups, int cap) {
@@ -942,8 +960,10 @@ Plan decode_plan(int B, int KVH, int G, int n_groups, int cap) {
   p.form = pick_form((rows + n_groups - 1) / n_groups);
   const int tr = p.form == 0 ? 16 : 64 * p.form;
   p.n_tiles = (int)(rows / tr) + n_groups;
-  p.splits = pick_splits((int64_t)p.n_tiles * KVH, cap, 2 * kCus);
-  p.own_splits = pick_splits((int64_t)B * KVH, cap, 2 * kCus);
+  // Half as many as kMinKeys allows: the merge reads them all (24 rows in three
+  // groups behind up to 4096 shared slots: 14.9 us with all, 14.3 with these).
+  p.splits = pick_splits((int64_t)p.n_tiles * KVH, cap, 2 * kMinKeys);
+  p.own_splits = pick_splits((int64_t)B * KVH, cap, kStepKeys);
   return p;
 }
 
@@ -953,14 +973,14 @@ Plan extend_plan(int B, int KVH, int G, int total, int cap) {
   p.form = pick_form((rows + B - 1) / B);
   const int tr = p.form == 0 ? 16 : 64 * p.form;
   p.n_tiles = (int)(rows / tr) + B;
-  p.splits = pick_splits((int64_t)p.n_tiles * KVH, cap, 2 * kCus);
+  p.splits = pick_splits((int64_t)p.n_tiles * KVH, cap, kMinKeys);
   p.own_splits = 0;
   return p;
 }
 
 template <bool kDecode>
 int launch(const Args& a, const Plan& p, hipStream_t st) {
-  const int64_t grid = (int64_t)a.n_tiles * a.KVH * a.splits +
+  const int64_t grid = a.n_tiles * (((int64_t)a.KVH * a.splits + 7) & ~(int64_t)7) +
                        (kDecode ? (int64_t)a.tokens * a.KVH * a.own_splits : 0);
   if (grid > 0x7fffffff) return QF_ERR_UNSUPPORTED;
   const dim3 g((unsigned)grid), b(kThreads);
