@@ -354,6 +354,8 @@ _lib: C.CDLL | None = None
 def load() -> C.CDLL:
     """Load ``_qf_attn.so`` once; raise ``RuntimeError`` if it is unavailable."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -102,16 +102,17 @@ __device__ __forceinline__ int scan_sum(int x, int n) {
   return x;
 }
 
-// One segment: its tokens [lo, hi) and its index, -1 if there is none.
+// One segment: its tokens [lo, hi), its index, -1 if there is none, and its plen
+// or cached slots (-1: none, parked), clamped.
 struct Segment {
-  int index, lo, hi;
+  int index, lo, hi, slots;
 };
 
 // Walks the segments 64 at a time and takes the first one for which `pick(lo,
 // hi, tiles ahead, its tiles)` is true, tiles holding tr query rows; `before`
 // becomes the tiles ahead of it.  Any contents of bounds give segments that ascend, do not
 // overlap and stay within the tokens.
-template <typename Pick>
+template <bool kDecode, typename Pick>
 __device__ __forceinline__ Segment find_segment(const Args& a, int tr, int& before, Pick&& pick) {
   const int lane = threadIdx.x & 63;
   int top = 0;
@@ -119,6 +120,8 @@ __device__ __forceinline__ Segment find_segment(const Args& a, int tr, int& befo
   for (int i0 = 0; i0 < a.n_seg; i0 += 64) {
     const int n = min(a.n_seg - i0, 64);
     const int i = i0 + min(lane, n - 1);
+    // Loaded with the bounds: the walk waits for memory once.
+    const int slots = kDecode ? clampi(a.plen[i], 0, a.pcap) : clampi(a.last[i * a.last_sb], -1, a.cap);
     const int hi = scan_max(max(top, clampi(a.bounds[i + 1], 0, a.tokens)), n);
     int lo = clampi(a.bounds[i], 0, a.tokens);
     lo = max(max(top, scan_max(lo, n)), 0);
@@ -129,12 +132,13 @@ __device__ __forceinline__ Segment find_segment(const Args& a, int tr, int& befo
     if (hit != 0) {
       const int j = __builtin_ctzll(hit);
       before += __builtin_amdgcn_readlane(upto - tiles, j);
-      return {i0 + j, __builtin_amdgcn_readlane(lo, j), __builtin_amdgcn_readlane(end, j)};
+      return {i0 + j, __builtin_amdgcn_readlane(lo, j), __builtin_amdgcn_readlane(end, j),
+              __builtin_amdgcn_readlane(slots, j)};
     }
     before += __builtin_amdgcn_readlane(upto, n - 1);
     top = __builtin_amdgcn_readlane(end, n - 1);
   }
-  return {-1, 0, 0};
+  return {-1, 0, 0, 0};
 }
 
 // A range of slots of a row's pages, read tile by tile.  A tile's address takes a
@@ -762,7 +766,7 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
     u.hk = rest % a.KVH;
     u.split = rest / a.KVH;
     if (u.split >= a.splits) return;
-    const Segment g = find_segment(a, kTr, before, [&](int, int, int ahead, int tiles) {
+    const Segment g = find_segment<kDecode>(a, kTr, before, [&](int, int, int ahead, int tiles) {
       return tile < ahead + tiles;
     });
     if (g.index < 0) return;
@@ -774,11 +778,11 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
       const bool given = a.ptable != nullptr;
       u.pages = given ? a.ptable + (int64_t)g.index * a.pt_sb : a.table + (int64_t)g.lo * a.t_sb;
       u.n_pages = given ? a.pppr : a.ppr;
-      end = clampi(a.plen[g.index], 0, a.pcap);
+      end = g.slots;
     } else {
       u.pages = a.table + (int64_t)g.index * a.t_sb;
       u.n_pages = a.ppr;
-      u.ctx = clampi(a.last[g.index * a.last_sb], -1, a.cap);
+      u.ctx = g.slots;
       const int newest = (min(u.r0 + kTr, u.rows) - 1) / a.G;   // last token of the tile
       end = u.ctx < 0 ? 0 : min(u.ctx + newest + 1, a.cap);
     }
@@ -790,11 +794,12 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
     const int s = id % a.own_splits, rest = id / a.own_splits;
     u.hk = rest % a.KVH;
     const int token = rest / a.KVH;
-    const Segment g = find_segment(a, kTr, before, [&](int lo, int hi, int, int) {
+    const int64_t last = a.last[token * a.last_sb];
+    const Segment g = find_segment<true>(a, kTr, before, [&](int lo, int hi, int, int) {
       return lo <= token && token < hi;
     });
-    const int end = clampi(a.last[token * a.last_sb], -1, a.cap - 1) + 1;
-    const int lo = min(g.index < 0 ? 0 : clampi(a.plen[g.index], 0, a.pcap), end);
+    const int end = clampi(last, -1, a.cap - 1) + 1;
+    const int lo = min(g.slots, end);  // 0 in no group
     u.tok0 = token;
     u.pages = a.table + (int64_t)token * a.t_sb;
     u.n_pages = a.ppr;

@@ -37,7 +37,7 @@ MIN_PAGE, MAX_PAGE = 64, 4096
 
 
 def _check_page_size(page_size: int) -> None:
-    if not (MIN_PAGE <= page_size <= MAX_PAGE) or page_size & (page_size - 1):
+    if not MIN_PAGE <= page_size <= MAX_PAGE or page_size & (page_size - 1):
         raise ValueError(f"page_size must be a power of two in [{MIN_PAGE}, {MAX_PAGE}] (got {page_size})")
 
 
@@ -335,9 +335,9 @@ def copy_pages(pools, src, dst, slots=None) -> None:
     if isinstance(pools, torch.Tensor):
         if pools.dim() < 4 or not pools.is_contiguous():
             raise ValueError("pools must be a contiguous (..., n_pages, KVH, P, 64) tensor, or a list")
-        _require_cuda_fp16("pools", pools)
+        _half("pools", pools, pools.dim())
         first, shape, stride = pools, pools.shape[-4:], pools.stride()[-4:]
-        step = shape.numel()
+        step = shape[0] * stride[0]
         per = pools.numel() // step if step else 0
         bases = (pools.data_ptr(),)
     else:
@@ -479,7 +479,8 @@ def flash_decode_attention_prefix_paged(grouped: torch.Tensor, k_pool: torch.Ten
         shared = (prefix_table.data_ptr(), prefix_table.stride(0), prefix_table.shape[1])
     dev = grouped.device
     if out is None:
-        out = torch.empty((b, kvh, g, d), device=dev, dtype=torch.float16)
+        out = (torch.empty_like(grouped) if grouped.is_contiguous()
+               else torch.empty((b, kvh, g, d), device=dev, dtype=torch.float16))
     else:
         _half("out", out, 4)
         if out.shape != grouped.shape or out.get_device() != index:

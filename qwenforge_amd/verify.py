@@ -79,9 +79,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     else:
         accept_u = sample_u = draft_probs = None
     _check_rows(cu_seqlens, total, max_seqlen, lengths)
-    # The counts lie behind the rows' tokens, in one allocation.
-    both = torch.empty(b * (max_seqlen + 1), device=dev, dtype=torch.int64)
-    out, count = both[:b * max_seqlen].view(b, max_seqlen), both[b * max_seqlen:]
+    out = torch.empty((b, max_seqlen), device=dev, dtype=torch.int64)
+    count = torch.empty(b, device=dev, dtype=torch.int64)
     ws = _workspace(_lib.load().qf_verify_workspace(total, b, vocab), "qf_verify_workspace", dev)
     _call("qf_verify_drafts", index, logits.data_ptr(), kind, logits.stride(0) if total > 1 else vocab,
           tokens.data_ptr(), cu_seqlens.data_ptr(), _ptr(accept_u), _ptr(sample_u), _ptr(draft_probs),
