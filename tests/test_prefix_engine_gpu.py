@@ -109,13 +109,16 @@ def test_forked_rows_extend_and_decode_apart(dev, model):
         assert torch.equal(torch.cat(kv.gather(i, 1, 100)), kept[i])
 
 
+@pytest.mark.parametrize("once", [True, False])
 @pytest.mark.parametrize("max_batch,tiles", [(1, True), (3, True), (6, True), (3, False), (33, True)])
-def test_serving_behind_a_prefix(dev, model, max_batch, tiles):
-    """Every step form: fused, wide and torch; rows are reused, and a request's
-    tokens are those it gets alone in the same step shape."""
+def test_serving_behind_a_prefix(dev, model, monkeypatch, max_batch, tiles, once):
+    """Every step form: fused, wide and torch, reading the prefix once or row by
+    row; rows are reused, and a request's tokens are those it gets alone in the
+    same step shape."""
     w, eng = model
     if not tiles:
         eng = PagedDecodeEngine(CFG, eng.w, dev, fused_step=False)
+    monkeypatch.setattr(eng, "reads_prefix_once", lambda batch, slots: once)
     gen = torch.Generator().manual_seed(5)
     prefix = _ids(gen, 150)
     prompts, news = [_ids(gen, n) for n in (9, 40, 1, 17, 30)], [6, 1, 9, 4, 7]
@@ -132,6 +135,13 @@ def test_serving_behind_a_prefix(dev, model, max_batch, tiles):
         alone = eng.serve([prompts[i].to(dev), prompts[1].to(dev)], [news[i], 1], max_batch=max_batch,
                           n_pages=pages, prefix=prefix.to(dev))[0]
         assert torch.equal(alone, got[i])
+
+
+def test_when_a_prefix_is_read_once(dev, model):
+    _, eng = model
+    assert not eng.reads_prefix_once(1, 16384) and not eng.reads_prefix_once(4, 1024)
+    assert eng.reads_prefix_once(2, 4096) and eng.reads_prefix_once(4, 16384)
+    assert not eng.reads_prefix_once(8, 16384) and eng.reads_prefix_once(32, 16384)
 
 
 def test_prefix_serving_refuses_and_runs_out(dev, model):
