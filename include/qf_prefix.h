@@ -37,8 +37,8 @@ extern "C" {
  * page holds afterwards is unspecified.  n_pairs = 0 launches nothing.
  */
 int qf_copy_pages(const void* const* pools, int n_pools, int per, int64_t step,
-                  int64_t sp, int64_t sh, int64_t sn, const int32_t* src, const int32_t* dst, const int32_t* slots, int n_pairs,
-                  int n_pages, int KVH, int page_size, int D, void* stream);
+                  int64_t sp, int64_t sh, int64_t sn, const int32_t* src, const int32_t* dst,
+                  const int32_t* slots, int n_pairs, int n_pages, int KVH, int page_size, int D, void* stream);
 
 /*
  * Decode attention of a batch whose rows share prefixes: the result of
@@ -91,7 +91,9 @@ int qf_decode_attn_prefix_paged(const void* q, int64_t q_sb, int64_t q_sh, int64
  * to slots [0, context[b] + i].
  *
  *   q, out (T, QH, D), k, v (T, KVH, D): strides *_sh per head, *_sn per token;
- *          T = total = cu_seqlens[B]; a row may have no tokens
+ *          a row may have no tokens; tokens of no row (before cu_seqlens[0],
+ *          from cu_seqlens[B] to T = total) are not appended, and their rows of
+ *          out are left as they were
  *   context  int64 on the device, row b reads context[b * ctx_sb]; negative:
  *          the row's tokens are not appended and their outputs are zero
  *   cos, sin (T, D), token stride cs_sn, or both NULL: rotate-half RoPE of q

@@ -32,7 +32,7 @@ extern "C" {
  *   sample_u    fp32[B] in [0, 1): for the row's last new token
  *   draft_probs NULL, or fp32 (T, V), row stride dp_sn: the distribution q_j that
  *               position j's draft was drawn from
- *   temperature T > 0: p_j = softmax(logits[j] / T).  Draft d is accepted while
+ *   temperature T > 0 (1 / T a normal fp32 number): p_j = softmax(logits[j] / T).  Draft d is accepted while
  *               accept_u q_j(d) < p_j(d) (q_j(d) = 1 without draft_probs).  After
  *               the first rejection the row's next token is drawn from
  *               max(p_j - q_j, 0) (without draft_probs from p_j without d; from

@@ -467,10 +467,13 @@ __global__ __launch_bounds__(256) void prefill_tokens_kernel(const int* cu, int 
     }
     b = lo;
     pos = t - cu[b];
-    if (context != nullptr) {  // behind the row's cached slots; a parked row appends nothing
+    if (context != nullptr) {
+      // Behind the row's cached slots; a parked row and a token of no row append
+      // nothing.
       const int64_t c = context[b * ctx_sb];
-      S = c < 0 || c > cap ? 0 : cap;
-      pos += (int)(c < 0 ? 0 : c > cap ? cap : c);
+      const bool mine = pos >= 0 && pos <= t && t < cu[b + 1] && c >= 0 && c <= cap;
+      S = mine ? cap : 0;
+      pos = mine ? pos + (int)c : 0;
     }
   } else {
     b = t / S;
@@ -809,6 +812,7 @@ extern "C" int qf_extend_layers(const QfPrefillLayer* layers, int n_layers, void
   if (!cu || !context || !block_table || B < 1 || cap < 1) return QF_ERR_INVALID_ARG;
   if (page_log2(page_size, pages_per_row, n_pages) < 0) return QF_ERR_UNSUPPORTED;
   if (cap > pages_per_row * page_size) return QF_ERR_INVALID_ARG;
+  if ((int64_t)cap + T > 0x7fffffff) return QF_ERR_UNSUPPORTED;
   return run_layers(layers, n_layers, hidden_p, T, B, 1, cu, context, ctx_sb, cap, inv_freq,
                     block_table, bt_sb, pages_per_row, n_pages, page_size, ws, ws_bytes, eps, H, QH,
                     KVH, D, I, stream);

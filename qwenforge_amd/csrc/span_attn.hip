@@ -819,16 +819,18 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(Args a) {
 // queries to a wave), four where there are many.  A lane loads the statistics of
 // a partial of its own, kEach times, and hands the weights around; then each
 // group takes every kSubs-th partial, eight loads in flight together.
-template <int kSubs, int kEach>
+template <int kSubs, int kEach, bool kDecode>
 __global__ __launch_bounds__(256) void span_merge_kernel(Args a, int n) {
   constexpr int kLanes = 16 * kSubs;  // of one query
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t id = (int64_t)blockIdx.x * (16 / kSubs) + tid / (16 * kSubs);
-  const bool in = id < (int64_t)a.tokens * a.KVH * a.G;
+  bool in = id < (int64_t)a.tokens * a.KVH * a.G;
   const int64_t id0 = in ? id : 0;
   const int g = (int)(id0 % a.G);
   const int64_t th = id0 / a.G;
   const int hk = (int)(th % a.KVH), token = (int)(th / a.KVH);
+  // New tokens outside every row were no unit's.
+  if (!kDecode) in = in && token >= a.bounds[0] && token < a.bounds[a.n_seg];
   const int64_t p0 = th * n * a.G + g;
   const int mine = lane & (kLanes - 1), base = lane & ~(kLanes - 1);
   float2 x[kEach];
@@ -997,9 +999,9 @@ int launch(const Args& a, const Plan& p, hipStream_t st) {
   if (rc == 0 && (kDecode || n > 1)) {
     const int64_t queries = (int64_t)a.tokens * a.KVH * a.G;
     const dim3 all((unsigned)((queries + 15) / 16)), quarter((unsigned)((queries + 3) / 4));
-    if (n <= 8) hipLaunchKernelGGL((span_merge_kernel<1, 1>), all, dim3(256), 0, st, a, n);
-    else if (n <= 64) hipLaunchKernelGGL((span_merge_kernel<4, 1>), quarter, dim3(256), 0, st, a, n);
-    else hipLaunchKernelGGL((span_merge_kernel<4, 2>), quarter, dim3(256), 0, st, a, n);
+    if (n <= 8) hipLaunchKernelGGL((span_merge_kernel<1, 1, kDecode>), all, dim3(256), 0, st, a, n);
+    else if (n <= 64) hipLaunchKernelGGL((span_merge_kernel<4, 1, kDecode>), quarter, dim3(256), 0, st, a, n);
+    else if (kDecode) hipLaunchKernelGGL((span_merge_kernel<4, 2, true>), quarter, dim3(256), 0, st, a, n);
     rc = (int)hipGetLastError();
   }
   return rc;
@@ -1030,7 +1032,7 @@ int fill(Args& a, const void* q, const void* k_pool, int64_t kp_sp, int64_t kp_s
   if (kp_sn < kD || vp_sn < kD || kp_sn > 0x3fffffff / page_size || vp_sn > 0x3fffffff / page_size ||
       kp_sp < 0 || vp_sp < 0 || kp_sp >> 3 > 0x7fffffff || vp_sp >> 3 > 0x7fffffff)
     return QF_ERR_UNSUPPORTED;
-  if ((int64_t)tokens * G > 0x3fffffff || (int64_t)tokens * KVH * G > 0x7fffffff ||
+  if (n_seg > 0x3fffffff || (int64_t)tokens * G > 0x3fffffff || (int64_t)tokens * KVH * G > 0x7fffffff ||
       (int64_t)cap + tokens > 0x7fffffff)
     return QF_ERR_UNSUPPORTED;
   a = Args{};
@@ -1066,7 +1068,8 @@ void set_parts(Args& a, const Plan& p, void* ws) {
 extern "C" int64_t qf_decode_attn_prefix_workspace(int B, int KVH, int G, int n_groups, int cap) {
   using namespace qf::span;
   if (B < 1 || KVH < 1 || n_groups < 1 || cap < 1) return QF_ERR_INVALID_ARG;
-  if (G < 1 || G > 16 || (int64_t)B * KVH * G > 0x7fffffff) return QF_ERR_UNSUPPORTED;
+  if (G < 1 || G > 16 || (int64_t)B * KVH * G > 0x7fffffff || n_groups > 0x3fffffff)
+    return QF_ERR_UNSUPPORTED;
   const Plan p = decode_plan(B, KVH, G, n_groups, cap);
   return part_bytes((int64_t)B * KVH * G, p.splits + p.own_splits);
 }
@@ -1107,7 +1110,7 @@ extern "C" int qf_decode_attn_prefix_paged(
 extern "C" int64_t qf_prefill_extend_workspace(int B, int QH, int KVH, int total, int cap) {
   using namespace qf::span;
   if (B < 1 || KVH < 1 || QH < KVH || QH % KVH != 0 || total < 1 || cap < 1) return QF_ERR_INVALID_ARG;
-  if (QH / KVH > 16 || (int64_t)total * QH > 0x7fffffff) return QF_ERR_UNSUPPORTED;
+  if (QH / KVH > 16 || (int64_t)total * QH > 0x7fffffff || B > 0x3fffffff) return QF_ERR_UNSUPPORTED;
   const Plan p = extend_plan(B, KVH, QH / KVH, total, cap);
   return p.splits > 1 ? part_bytes((int64_t)total * QH, p.splits) : 0;
 }

@@ -88,7 +88,8 @@ __device__ __forceinline__ int lead(const E* row) {
 }
 
 // Maximum and sum of exponentials of one part of a position (kArgmax: the
-// maximum and its lowest index).
+// maximum and its lowest index; with a NaN, index -1 and a maximum that none
+// exceeds).
 template <typename E, bool kArgmax>
 __global__ __launch_bounds__(kThreads) void stats_kernel(Args a) {
   __shared__ float sm[4], sl[4];
@@ -102,6 +103,7 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(Args a) {
   const int end = min((part + 1) * per, groups);
   float m = kNegInf, l = 0.f;
   int at = 0x7fffffff;
+  bool nan = false;
 #pragma unroll 2
   for (int g = part * per + tid; g < end; g += kThreads) {
     float x[kGroup];
@@ -114,6 +116,8 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(Args a) {
           m = x[e];
           at = first + e;
         }
+#pragma unroll
+      for (int e = 0; e < kGroup; e += 2) nan |= __builtin_isunordered(x[e], x[e + 1]);
     } else {
       float top = m;
 #pragma unroll
@@ -125,6 +129,10 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(Args a) {
       l = l * fast_exp2((m - ref) * a.k2) + s;   // m = -inf: l is 0 (or NaN and stays so)
       m = top;
     }
+  }
+  if (kArgmax && nan) {
+    m = __builtin_huge_valf();
+    at = -1;
   }
   for (int d = 32; d > 0; d >>= 1) {
     const float m2 = __shfl_xor(m, d);
@@ -187,7 +195,8 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
-// Argmax of a position from its parts (one per lane), -1 if nothing is above -inf.
+// Argmax of a position from its parts (one per lane), -1 if nothing is above -inf
+// or there is a NaN.
 __device__ __forceinline__ int best_token(const Args& a, int pos) {
   const int lane = threadIdx.x & 63;
   const float2 x = lane < a.parts ? a.stats[(int64_t)pos * a.parts + lane]
@@ -505,8 +514,9 @@ extern "C" int qf_verify_drafts(const void* logits, int dtype, int64_t lg_sn, co
   if (!logits || !tokens || !cu_seqlens || !out || !count || !ws || width < 1 || lg_sn < V ||
       !(temperature >= 0.) || !std::isfinite(temperature))
     return QF_ERR_INVALID_ARG;
-  if (!greedy && (!accept_u || !sample_u || (draft_probs != nullptr && dp_sn < V) ||
-                  !std::isfinite(1. / temperature) || !std::isfinite(kLog2e / (float)temperature)))
+  // Past the normal fp32 numbers a masked logit times k2 would be no number.
+  const float k2 = greedy ? 0.f : (float)(1.4426950408889634 / temperature);
+  if (!greedy && (!accept_u || !sample_u || (draft_probs != nullptr && dp_sn < V) || !std::isnormal(k2)))
     return QF_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(logits) & (dtype == QF_F16 ? 1u : 3u)) != 0 ||
       (reinterpret_cast<uintptr_t>(ws) & 15u) != 0)
@@ -522,7 +532,7 @@ extern "C" int qf_verify_drafts(const void* logits, int dtype, int64_t lg_sn, co
   a.probs = greedy ? nullptr : draft_probs;
   a.dp_sn = dp_sn;
   a.inv_t = greedy ? 0. : 1. / temperature;
-  a.k2 = greedy ? 0.f : (float)(1.4426950408889634 / temperature);
+  a.k2 = k2;
   a.out = out;
   a.count = count;
   a.width = width;

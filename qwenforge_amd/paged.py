@@ -454,9 +454,10 @@ def flash_decode_attention_prefix_paged(grouped: torch.Tensor, k_pool: torch.Ten
     [0, prefix_len[g]) hold the same K and V in every row (forked rows'); they
     are read from the pages of the group's first row, or of row g of
     ``prefix_table`` (N, pages) int32 -- needed where the first row may have
-    nothing mapped.  Rows outside the groups share nothing.  ``kv_last`` (B,) int64 is each row's last slot; a row with a
-    negative one (parked) gets zeros.  The three are read on the device when the
-    kernels run.  Returns (B, KVH, G, 64), written to ``out`` if given.
+    nothing mapped.  Rows outside the groups share nothing.  ``kv_last`` (B,)
+    int64 is each row's last slot; a row with a negative one (parked) gets zeros.
+    All of these are read on the device when the kernels run.  Returns
+    (B, KVH, G, 64), written to ``out`` if given.
     """
     _half("grouped", grouped, 4)
     b, kvh, g, d = grouped.shape
@@ -471,7 +472,8 @@ def flash_decode_attention_prefix_paged(grouped: torch.Tensor, k_pool: torch.Ten
     last_sb = _int_rows("kv_last", kv_last, b, torch.int64, index)
     shared = (None, 0, 0)
     if prefix_table is not None:
-        if prefix_table.dtype is not torch.int32 or prefix_table.get_device() != index:
+        if (not isinstance(prefix_table, torch.Tensor) or prefix_table.dtype is not torch.int32
+                or prefix_table.get_device() != index):
             raise TypeError(f"prefix_table must be an int32 tensor on cuda:{index}")
         if (prefix_table.dim() != 2 or prefix_table.shape[0] != groups or prefix_table.shape[1] < 1
                 or prefix_table.stride(1) != 1):

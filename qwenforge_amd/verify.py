@@ -71,7 +71,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
         _vector("accept_u", accept_u, total, torch.float32, index)
         _vector("sample_u", sample_u, b, torch.float32, index)
         if draft_probs is not None:
-            if draft_probs.dtype is not torch.float32 or draft_probs.get_device() != index:
+            if (not isinstance(draft_probs, torch.Tensor) or draft_probs.dtype is not torch.float32
+                    or draft_probs.get_device() != index):
                 raise TypeError(f"draft_probs must be a float32 tensor on {dev}")
             if draft_probs.shape != logits.shape or draft_probs.stride(1) != 1:
                 raise ValueError("draft_probs must have the logits' shape and unit last stride")

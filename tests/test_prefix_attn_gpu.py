@@ -488,6 +488,96 @@ def test_captured_extension_follows_contexts(dev):
         assert (got.cpu().double() - ref).abs().max().item() <= TOL * vp.abs().max().item()
 
 
+@pytest.mark.parametrize("ppr", [1, 5])                  # whole rows, and rows cut into splits
+def test_tokens_behind_the_last_row_are_left_alone(dev, ppr):
+    """A captured call whose offsets shrink: padding is neither appended nor
+    attended, and its outputs stay as they were."""
+    gen = torch.Generator().manual_seed(37)
+    lens, ctx = [3, 4], [9, 20]
+    q, k, v, kp, vp, table = _extend_case(gen, dev, [6, 6], [0, 0], 14, 2, 64, extra=ppr - 1)
+    cu = torch.tensor([0, 6, 12], dtype=torch.int32, device=dev)
+    context = torch.tensor(ctx, device=dev)
+    t = table.to(dev)
+    kp0, vp0 = kp.clone(), vp.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = paged.prefill_extend_paged(q, k, v, cu, 6, context, None, None, kp, vp, t)
+    for first in (0, 2):
+        bounds = _starts(lens, first)
+        cu.copy_(torch.tensor(bounds, dtype=torch.int32))
+        kp.copy_(kp0), vp.copy_(vp0), got.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        ref, kr, vr = _extend_ref(q, k, v, bounds, ctx, kp0, vp0, table, 64 * ppr)
+        assert torch.equal(kp.cpu(), kr) and torch.equal(vp.cpu(), vr)
+        rows = slice(bounds[0], bounds[-1])
+        assert (got[rows].cpu().double() - ref[rows]).abs().max().item() <= TOL * vp.abs().max().item()
+        assert (got[:bounds[0]] == 7).all() and (got[bounds[-1]:] == 7).all()
+
+
+def test_offsets_past_32_bits(dev):
+    """Pages 2^31 elements apart, heads 2^30: attention, appends and copies."""
+    gen = torch.Generator().manual_seed(38)
+    sp, sh = 2**31 + 1024, 2**30 + 512
+    pools = []
+    for _ in range(2):
+        store = torch.empty(2 * sp + sh + 64 * D, device=dev, dtype=torch.float16)
+        pool = store.as_strided((3, 2, 64, D), (sp, sh, D, 1))
+        pool.copy_(torch.randn(3, 2, 64, D, generator=gen))
+        pools.append(pool)
+    kp, vp = pools
+    table = torch.tensor([[0, 2], [0, 1]], dtype=torch.int32)
+    lens = [110, 70]
+    q = torch.randn(2, 2, 7, D, generator=gen).half().to(dev)
+    got = paged.flash_decode_attention_prefix_paged(
+        q, kp, vp, table.to(dev), torch.tensor([0, 2], dtype=torch.int32, device=dev),
+        torch.tensor([64], dtype=torch.int32, device=dev), torch.tensor([n - 1 for n in lens], device=dev))
+    tol = TOL * vp.abs().max().item()
+    assert (got.cpu().double() - _prefix_ref(q, kp, vp, table, lens)).abs().max().item() <= tol
+    qkv = torch.randn(5, 18, D, generator=gen).half().to(dev)
+    q, k, v = qkv[:, :14], qkv[:, 14:16], qkv[:, 16:]
+    ref, kr, vr = _extend_ref(q, k, v, [0, 3, 5], lens, kp, vp, table, 128)
+    got = paged.prefill_extend_paged(q, k, v, torch.tensor([0, 3, 5], dtype=torch.int32, device=dev), 3,
+                                     torch.tensor(lens, device=dev), None, None, kp, vp, table.to(dev))
+    assert torch.equal(kp.cpu(), kr) and torch.equal(vp.cpu(), vr)
+    assert (got.cpu().double() - ref).abs().max().item() <= TOL * max(vp.abs().max().item(), v.abs().max().item())
+    paged.copy_pages([kp, vp], [2], [0], slots=[50])
+    kr[0, :, :50], vr[0, :, :50] = kr[2, :, :50], vr[2, :, :50]
+    assert torch.equal(kp.cpu(), kr) and torch.equal(vp.cpu(), vr)
+
+
+def test_two_streams_at_once(dev):
+    """Calls that overlap take scratch of their own: every result has the bits of
+    the same call alone."""
+    gen = torch.Generator().manual_seed(39)
+    decode, extend = [], []
+    for n in (3, 5):
+        lens = [2000 + 77 * i for i in range(n)]
+        kp, vp, table = _prefix_case(gen, dev, [n], lens, [1900], 2, 64)
+        q = torch.randn(n, 2, 7, D, generator=gen).half().to(dev)
+        decode.append((q, kp, vp, table.to(dev), torch.tensor([0, n], dtype=torch.int32, device=dev),
+                       torch.tensor([1900], dtype=torch.int32, device=dev),
+                       torch.tensor([x - 1 for x in lens], device=dev)))
+        q, k, v, kp, vp, table = _extend_case(gen, dev, [6] * n, lens, 14, 2, 64)
+        extend.append((q, k, v, torch.tensor(_starts([6] * n), dtype=torch.int32, device=dev), 6,
+                       torch.tensor(lens, device=dev), None, None, kp, vp, table.to(dev)))
+    calls = [(f, args) for f, a in ((paged.flash_decode_attention_prefix_paged, decode),
+                                    (paged.prefill_extend_paged, extend)) for args in a]
+    want = [f(*args) for f, args in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = []
+    for _ in range(5):
+        for s, (f, args) in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(f(*args))
+    torch.cuda.synchronize()
+    for i, w in enumerate(want):
+        assert all(torch.equal(g, w) for g in got[i::len(calls)])
+
+
 def test_extension_refusals(dev):
     gen = torch.Generator().manual_seed(36)
     q, k, v, kp, vp, table = _extend_case(gen, dev, [4, 6], [10, 20], 14, 2, 64)

@@ -102,7 +102,7 @@ def test_verify_refusals_without_a_gpu():
     assert call(sn=99) == -1 and call(tokens=None) == -1 and call(au=None) == -1 and call(su=None) == -1
     assert call(q=16, qsn=99) == -1 and call(width=0) == -1 and call(ws=8) == -1
     assert call(temp=-0.5) == -1 and call(temp=float("nan")) == -1 and call(temp=float("inf")) == -1
-    assert call(temp=1e-320) == -1
+    assert call(temp=1e-320) == -1 and call(temp=1e39) == -1 and call(temp=1e-39) == -1
     assert call(bytes_=8) == -3
     assert lib.qf_verify_workspace(4, 2, 100) > 0
     with pytest.raises(RuntimeError, match="no CPU path"):
@@ -127,6 +127,9 @@ def test_span_attention_refusals_without_a_gpu():
     assert prefix(bytes_=100) == -3
     assert lib.qf_decode_attn_prefix_workspace(0, 2, 7, 1, 64) == -1
     assert lib.qf_decode_attn_prefix_workspace(1, 2, 17, 1, 64) == -2
+    assert prefix(groups=2**31 - 1) == -2
+    assert lib.qf_decode_attn_prefix_workspace(1, 2, 7, 2**31 - 1, 64) == -2
+    assert lib.qf_prefill_extend_workspace(2**31 - 1, 14, 2, 1, 64) == -2
 
     def extend(q=16, cu=16, total=8, ctx=16, cos=None, sin=None, cap=256, ws=16, bytes_=1 << 30, out=16, b=2,
                qh=14, kvh=2, d=64, k_sn=1152, ppr=4):

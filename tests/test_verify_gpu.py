@@ -168,7 +168,12 @@ def test_masked_and_unusable_logits(dev, dtype):
     assert out[:, 0].tolist() == [2999, -1, -1, -1, 1500, 17]
     assert count.tolist() == [1, 0, 0, 0, 1, 1]
     count, out = verify.verify_drafts(x, tokens, _cu([1] * 6, dev), 1, None, None, temperature=0)
-    assert out[:, 0].tolist() == [2999, -1, 0, 7, 0, 17] and count.tolist() == [1, 0, 1, 1, 1, 1]
+    assert out[:, 0].tolist() == [2999, -1, -1, 7, 0, 17] and count.tolist() == [1, 0, 0, 1, 1, 1]
+    for at in (0, 1, 2047, 2048, v - 1):                # a NaN anywhere beside an infinity
+        x[3, at], x[3, 7] = math.nan, math.inf
+        _, out = verify.verify_drafts(x, tokens, _cu([1] * 6, dev), 1, None, None, temperature=0)
+        assert out[:, 0].tolist() == [2999, -1, -1, -1, 0, 17]
+        x[3, at] = 0.5
     # A draft in front of an unusable position: accepted, then nothing drawn.
     x2 = torch.stack([x[0], x[1]])
     count, out = verify.verify_drafts(x2, torch.tensor([1, 2999], device=dev), _cu([2], dev), 2, u[:2], r[:1])
@@ -259,6 +264,33 @@ def test_two_streams_at_once(dev):
             assert torch.equal(count.cpu(), want[0]) and torch.equal(out.cpu(), want[1])
 
 
+@pytest.mark.parametrize("lens", [[1, 2], [1, 1, 1]])
+def test_rows_more_than_32_bits_apart(dev, lens):
+    gen = torch.Generator().manual_seed(23)
+    v = 2500
+    x, tokens, u, r, q = _case(gen, dev, lens, v, torch.float16, 1.0, True)
+    step = 2**31 + 8
+    far_x = torch.empty(2 * step + v, device=dev, dtype=torch.float16).as_strided((3, v), (step, 1))
+    far_q = torch.empty(2 * step + v, device=dev).as_strided((3, v), (step, 1))
+    far_x.copy_(x), far_q.copy_(q)
+    for probs, temp in ((far_q, 1.0), (None, 1.0), (None, 0.0)):
+        count, out = verify.verify_drafts(far_x, tokens, _cu(lens, dev), 3, u, r, temperature=temp,
+                                          draft_probs=probs)
+        want = _expect(x, tokens, lens, u, r, temp, None if probs is None else q, 3)
+        assert torch.equal(count.cpu(), want[0]) and torch.equal(out.cpu(), want[1])
+
+
+def test_more_positions_than_parts_to_go_round(dev):
+    """One part to a position, and more rows than a workgroup has lanes."""
+    gen = torch.Generator().manual_seed(24)
+    lens = [1 + i % 9 for i in range(600)]
+    logits, tokens, u, r, probs = _case(gen, dev, lens, 211, torch.float32, 0.9, True)
+    count, out = verify.verify_drafts(logits, tokens, _cu(lens, dev), 9, u, r, temperature=0.9,
+                                      draft_probs=probs, lengths=lens)
+    want = _expect(logits, tokens, lens, u, r, 0.9, probs, 9)
+    assert torch.equal(count.cpu(), want[0]) and torch.equal(out.cpu(), want[1])
+
+
 def test_refusals(dev):
     x = torch.zeros(4, 10, device=dev)
     ok = dict(logits=x, tokens=torch.zeros(4, dtype=torch.int64, device=dev), cu_seqlens=_cu([2, 2], dev),
@@ -274,6 +306,7 @@ def test_refusals(dev):
                          (dict(accept_u=None), TypeError), (dict(sample_u=ok["sample_u"].double()), TypeError),
                          (dict(temperature=-1.0), ValueError), (dict(temperature=math.nan), ValueError),
                          (dict(temperature=math.inf), ValueError), (dict(temperature=1e-320), RuntimeError),
+                         (dict(temperature=1e39), RuntimeError), (dict(draft_probs=[0.5]), TypeError),
                          (dict(draft_probs=x.half()), TypeError), (dict(draft_probs=x[:, :5]), ValueError)):
         with pytest.raises(kind):
             verify.verify_drafts(**{**ok, **change})
