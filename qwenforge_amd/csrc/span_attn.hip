@@ -18,6 +18,19 @@
 // lds_tile.h; scores and output are computed transposed (qf_common.h).  Slots
 // past a unit's last one read as zero, and masked slots count for nothing
 // whatever K and V hold there (masked_values).
+//
+// A wave's step of 32 queries and 64 keys is 36 matrix products of 16 cycles, and
+// more than as many cycles of vector work: 32 exponentials of 16 cycles, their
+// fma and conversion, maxima, addresses.  So the vector unit bounds the
+// long cases, not memory: MI355X, 14 query heads on 2 kv heads, GPU time of the
+// whole call in a replayed graph: 2048 tokens behind 16384 slots 188 us (680
+// TF/s; 111 us at the rate of a large fp16 product), 16 rows of 9 to 301 tokens
+// behind 2048 slots 56 us (its 286 units leave most CUs one workgroup of the
+// two that they hold), decode of 96 rows of one 32768-slot prefix 36 us (7 us
+// of memory traffic, 10 of products; each row alone over the shared pages 7 ms
+// in plain tensor operations).  Four rows of a 512-slot prefix take 9.4 us, four
+// times five tokens behind 2000 slots 12.1 us: two or three launches and their
+// dependent loads (bounds, table, tile).
 #include <algorithm>
 
 #include "lds_tile.h"
