@@ -30,6 +30,7 @@ namespace qf {
 namespace verify {
 
 constexpr int kThreads = 256;
+constexpr int kDecide = 512;               // of decide_kernel
 constexpr int kGroup = 8;                  // consecutive logits of a thread
 constexpr int kChunk = kThreads * kGroup;  // tokens of a draw_kernel workgroup
 constexpr int kMaxParts = 64;              // chunks of a position in stats_kernel
@@ -231,9 +232,10 @@ __device__ __forceinline__ double exp_of(const Args& a, float x, float top) {
   return exp(((double)x - (double)top) * a.inv_t);
 }
 
-// Drafts of the row that are accepted: waves take the positions in turn.
+// Drafts of the row that are accepted: waves take the positions in turn, each
+// three dependent loads.
 template <typename E>
-__global__ __launch_bounds__(kThreads) void decide_kernel(Args a) {
+__global__ __launch_bounds__(kDecide) void decide_kernel(Args a) {
   __shared__ int first;
   const int b = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int lo, n;
@@ -248,7 +250,7 @@ __global__ __launch_bounds__(kThreads) void decide_kernel(Args a) {
     return;
   }
   __syncthreads();
-  for (int j = w; j < n - 1; j += kThreads / 64) {
+  for (int j = w; j < n - 1; j += kDecide / 64) {
     const int64_t pos = lo + j;
     const int64_t d = a.tokens[pos + 1];
     const bool known = d >= 0 && d < a.V;
@@ -424,7 +426,9 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Args a) {
   const double mark = (double)a.sample_u[b] * total;
   if (tid == find_thread(upto > mark && s > 0., s > 0., at[0])) {
     double ahead = upto - s, passed = 0.;
-    for (int c = tid * per; c < min((tid + 1) * per, a.chunks); ++c) {
+    // One chunk to a thread: no second trip to memory for it.
+    if (per == 1) found_chunk = tid;
+    else for (int c = tid * per; c < min((tid + 1) * per, a.chunks); ++c) {
       const double here = chunk_sum(c, use_left);
       if (!(here > 0.)) continue;
       ahead += passed;
@@ -497,7 +501,7 @@ int launch(const Args& a, bool greedy, hipStream_t st) {
     return (int)hipGetLastError();
   }
   hipLaunchKernelGGL((stats_kernel<E, false>), all, block, 0, st, a);
-  hipLaunchKernelGGL(decide_kernel<E>, dim3(a.B), block, 0, st, a);
+  hipLaunchKernelGGL(decide_kernel<E>, dim3(a.B), dim3(kDecide), 0, st, a);
   const dim3 draw((unsigned)(a.B * a.chunks));
   if (a.probs != nullptr) hipLaunchKernelGGL((draw_kernel<E, true>), draw, block, 0, st, a);
   hipLaunchKernelGGL((draw_kernel<E, false>), draw, block, 0, st, a);

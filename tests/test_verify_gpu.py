@@ -280,6 +280,17 @@ def test_rows_more_than_32_bits_apart(dev, lens):
         assert torch.equal(count.cpu(), want[0]) and torch.equal(out.cpu(), want[1])
 
 
+@pytest.mark.parametrize("drafter", [False, True])
+def test_more_chunks_than_threads(dev, drafter):
+    """A vocabulary of which a thread adds up several chunks."""
+    gen = torch.Generator().manual_seed(25)
+    lens, v = [2, 1, 3], 1200007
+    logits, tokens, u, r, probs = _case(gen, dev, lens, v, torch.float16, 1.0, drafter)
+    count, out = verify.verify_drafts(logits, tokens, _cu(lens, dev), 3, u, r, draft_probs=probs)
+    want = _expect(logits, tokens, lens, u, r, 1.0, probs, 3)
+    assert torch.equal(count.cpu(), want[0]) and torch.equal(out.cpu(), want[1])
+
+
 def test_more_positions_than_parts_to_go_round(dev):
     """One part to a position, and more rows than a workgroup has lanes."""
     gen = torch.Generator().manual_seed(24)
