@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "extend.h"
 #include "step_common.h"
 #include "../../include/qf_prefill.h"
 #include "../../include/qf_prefix.h"

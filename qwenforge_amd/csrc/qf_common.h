@@ -187,22 +187,6 @@ __device__ __forceinline__ float col_sum(float x) {
 // Compute units of the device of `st` (prefill_attn.hip), 0 if unknown.
 int stream_cus(hipStream_t st);
 
-// Attention of packed new tokens whose K and V are in the pages already
-// (span_attn.hip), for rows that hold context[b * ctx_sb] slots before them;
-// arguments and workspace as in qf_prefill_extend_paged.
-struct ExtendCall {
-  const int32_t* cu;
-  const int64_t* context;
-  int64_t ctx_sb;
-  const int32_t* table;
-  int64_t t_sb;
-  int ppr, n_pages, page_size, cap, B, T, QH, KVH;
-};
-int extend_attention(const ExtendCall& c, const void* q, int64_t q_sh, int64_t q_sn, void* out,
-                     int64_t o_sh, int64_t o_sn, const void* k_pool, int64_t kp_sp, int64_t kp_sh,
-                     int64_t kp_sn, const void* v_pool, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn,
-                     void* ws, int64_t ws_bytes, float scale, hipStream_t st);
-
 // Paged KV caches (host side): page_size must be a power of two in
 // [64, 4096] (a 32-key decode tile and a 64-key prefill tile then never
 // straddle a page), with at least one page per row and a non-empty pool.

@@ -33,6 +33,7 @@
 // dependent loads (bounds, table, tile).
 #include <algorithm>
 
+#include "extend.h"
 #include "lds_tile.h"
 #include "../../include/qf_prefix.h"
 
