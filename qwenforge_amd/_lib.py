@@ -344,8 +344,8 @@ for _name in ("qf_decode_attn", "qf_decode_attn_paged"):
 
 # Entry points that do not return an int status.
 RESTYPES = {"qf_error_string": C.c_char_p, "qf_prefill_layers_workspace": _i64,
-            "qf_decode_attn_prefix_workspace": _i64, "qf_prefill_extend_workspace": _i64, "qf_extend_layers_workspace": _i64,
-            "qf_verify_workspace": _i64}
+            "qf_decode_attn_prefix_workspace": _i64, "qf_prefill_extend_workspace": _i64,
+            "qf_extend_layers_workspace": _i64, "qf_verify_workspace": _i64}
 
 _lock = threading.Lock()
 _lib: C.CDLL | None = None

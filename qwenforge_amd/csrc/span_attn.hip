@@ -124,8 +124,8 @@ struct Segment {
 
 // Walks the segments 64 at a time and takes the first one for which `pick(lo,
 // hi, tiles ahead, its tiles)` is true, tiles holding tr query rows; `before`
-// becomes the tiles ahead of it.  Any contents of bounds give segments that ascend, do not
-// overlap and stay within the tokens.
+// becomes the tiles ahead of it.  Any contents of bounds give segments that
+// ascend, do not overlap and stay within the tokens.
 template <bool kDecode, typename Pick>
 __device__ __forceinline__ Segment find_segment(const Args& a, int tr, int& before, Pick&& pick) {
   const int lane = threadIdx.x & 63;
@@ -1099,8 +1099,8 @@ extern "C" int qf_decode_attn_prefix_paged(
     int64_t kp_sh, int64_t kp_sn, const void* v_pool, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn,
     const int32_t* block_table, int64_t bt_sb, int pages_per_row, int n_pages, int page_size,
     const int32_t* prefix_rows, const int32_t* prefix_len, int n_groups, const int32_t* prefix_table,
-    int64_t pt_sb, int prefix_pages, const int64_t* kv_last, int64_t kv_last_sb, void* ws, int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh,
-    int64_t o_sg, int B, int KVH, int G, int D, float scale, void* stream) {
+    int64_t pt_sb, int prefix_pages, const int64_t* kv_last, int64_t kv_last_sb, void* ws,
+    int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh, int64_t o_sg, int B, int KVH, int G, int D, float scale, void* stream) {
   using namespace qf;
   using namespace qf::span;
   Args a;

@@ -79,6 +79,32 @@ def test_extension_in_pieces_matches_the_oracle(dev, model, monkeypatch, native)
                 assert (got.float().cpu() - ref[0, :, :n]).abs().max().item() <= 2e-2
 
 
+@pytest.mark.parametrize("bounds", [[0, 3, 6], [2, 5, 8], [0, 6, 6]])
+def test_layers_of_padded_tokens_append_none_of_them(dev, model, bounds):
+    """Tokens before the first row and behind the last reach no page."""
+    from qwenforge_amd import prefill_ops
+
+    _, eng = model
+    gen = torch.Generator().manual_seed(4)
+    kv = eng.new_paged_cache(2, 6, 64, 3)
+    for r in range(2):
+        kv.map_row(r, 192)
+    contexts = [5, 70]
+    hidden = (torch.randn(10, CFG.hidden, generator=gen) * 0.1).half().to(dev)
+    layers = prefill_ops.layer_table(CFG, eng.w["layers"], kv.pools, hidden.device,
+                                     (kv.n_pages, kv.kv_heads, kv.page_size, CFG.head_dim))
+    prefill_ops.extend_layers(CFG, layers, hidden, torch.tensor(bounds, dtype=torch.int32, device=dev),
+                              torch.tensor(contexts, device=dev), 192, eng.inv_freq, kv.table, kv.n_pages,
+                              kv.page_size)
+    written = (kv.store != 0).any(dim=-1).cpu()             # (layers, 2, page, head, slot)
+    want = torch.zeros_like(written)
+    for r, c in enumerate(contexts):
+        for slot in range(c, c + bounds[r + 1] - bounds[r]):
+            want[:, :, int(kv.table[r, slot // 64]), :, slot % 64] = True
+    assert torch.equal(written, want)
+    assert hidden[bounds[0]:bounds[-1]].isfinite().all()
+
+
 def test_forked_rows_extend_and_decode_apart(dev, model):
     """Two rows forked from one go on with texts of their own; the first row's pages stay its own."""
     w, eng = model
