@@ -1100,7 +1100,8 @@ extern "C" int qf_decode_attn_prefix_paged(
     const int32_t* block_table, int64_t bt_sb, int pages_per_row, int n_pages, int page_size,
     const int32_t* prefix_rows, const int32_t* prefix_len, int n_groups, const int32_t* prefix_table,
     int64_t pt_sb, int prefix_pages, const int64_t* kv_last, int64_t kv_last_sb, void* ws,
-    int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh, int64_t o_sg, int B, int KVH, int G, int D, float scale, void* stream) {
+    int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh, int64_t o_sg, int B,
+    int KVH, int G, int D, float scale, void* stream) {
   using namespace qf;
   using namespace qf::span;
   Args a;

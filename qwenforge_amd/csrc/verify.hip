@@ -18,8 +18,9 @@
 // probabilities 46.5 us in a replayed graph, of which stats_kernel 18 (78 MB, 4.3
 // TB/s: memory; four groups in flight or twice the parts were slower), decide_kernel
 // 5 (6 with four waves), the sums of exponentials 8, the draw 18 (exps in 64 bits,
-// 29 MB, and the last workgroup's search, some 5 us of dependent steps).  One row of 5 positions 14.5 us, 8 rows at temperature 0 8.5 us: the
-// launches and each one's chain of dependent loads.
+// 29 MB, and the last workgroup's search, some 5 us of dependent steps).  One row
+// of 5 positions 14.5 us, 8 rows at temperature 0 8.5 us: the launches and each
+// one's chain of dependent loads.
 #include <algorithm>
 #include <cmath>
 
@@ -486,7 +487,8 @@ extern "C" int64_t qf_verify_workspace(int T, int B, int V) {
       (int64_t)B * chunks_of(V) > 0x7fffffff || B > 0x7fffffff / kTicket)
     return QF_ERR_UNSUPPORTED;
   const int64_t sums = (int64_t)B * chunks_of(V);
-  return round16((int64_t)T * parts_of(T, V) * 8) + sums * 16 + round16(sums * 8) + (int64_t)B * (16 + 4 * kTicket);
+  return round16((int64_t)T * parts_of(T, V) * 8) + sums * 16 + round16(sums * 8) +
+         (int64_t)B * (16 + 4 * kTicket);
 }
 
 namespace qf {
