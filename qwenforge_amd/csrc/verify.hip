@@ -372,7 +372,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Args a) {
       all[e] = i >= 0 && i < a.V ? exp_of(a, x[e], top) : 0.;
       left[e] = all[e];
       if (q != nullptr) left[e] = fmax(all[e] - (double)y[e] * sum_exp, 0.);
-      if (i == draft) left[e] = 0.;
+      if (i == draft) left[e] *= 0.;  // a NaN stays: no distribution, nothing drawn
     }
   };
   double left[kGroup], all[kGroup], sl = 0., sa = 0.;
