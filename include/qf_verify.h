@@ -47,9 +47,10 @@ extern "C" {
  * A draft outside [0, V) is rejected.  A position whose logits give no
  * distribution (NaN, or with T > 0 an infinity of +; nothing above -infinity)
  * rejects its draft and draws nothing.  A row without positions gets 0 tokens; no
- * row uses more than `width` positions.  exp and the sums that the drawn token
- * depends on are in 64 bits.  ws: 16-byte aligned, of qf_verify_workspace bytes,
- * else QF_ERR_SCRATCH_LIMIT; not to be shared by calls that overlap in time.
+ * row uses more than `width` positions.  Every new token, accepted or drawn, is
+ * the one that exponentials and sums in 64 bits give.  ws: 16-byte aligned, of
+ * qf_verify_workspace bytes, else QF_ERR_SCRATCH_LIMIT; not to be shared by calls
+ * that overlap in time.
  */
 int64_t qf_verify_workspace(int T, int B, int V);
 

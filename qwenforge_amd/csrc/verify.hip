@@ -3,16 +3,17 @@
 // first rejection leave exactly p.
 //
 // stats_kernel reads every logit once: maximum and sum of exponentials (or the
-// argmax) of each chunk of each position, fp32 within a thread's few values.
-// decide_kernel, a workgroup per row, finds the row's first rejection from
-// those.  draw_kernel, a workgroup per row and chunk of 2048 tokens, goes over the
-// logits of that one position again.  Its weights and sums are in 64 bits: the
-// token drawn is where a running sum over the vocabulary crosses a number, and a
-// sum off by 2^-24 would move that crossing past a token in some draws out of a
-// hundred.  The workgroup that completes a row adds up its chunks and searches
-// the one of the crossing.  With draft probabilities the sum of exponentials has
-// to be known in 64 bits before max(p - q, 0) can be formed, so a first launch of
-// the kernel takes it.
+// argmax) of each chunk of each position, in fp32.  decide_kernel, a workgroup per
+// row, finds the row's first rejection from those; where an acceptance is closer
+// than fp32 sums tell (2e-5 of it at 151936 logits), it takes that position's
+// sum again in 64 bits.  draw_kernel, a workgroup per row and chunk of 2048 tokens,
+// goes over the logits of the last position once more.  Its weights and sums are in
+// 64 bits: the token drawn is where a running sum over the vocabulary crosses a
+// number, and a sum off by 2^-24 would move that crossing past a token in some draws
+// out of a hundred.  The workgroup that completes a row adds up its chunks and
+// searches the one of the crossing.  With draft probabilities the sum of
+// exponentials has to be known in 64 bits before max(p - q, 0) can be formed, so a
+// first launch of the kernel takes it.
 //
 // MI355X, 151936 fp16 logits a position: 32 rows of 8 positions with draft
 // probabilities 46.5 us in a replayed graph, of which stats_kernel 18 (78 MB, 4.3
@@ -51,6 +52,7 @@ struct Args {
   int64_t dp_sn;
   double inv_t;
   float k2;            // log2(e) / temperature
+  double slack;        // sides of an acceptance that are closer than this factor are close
   int64_t* out;
   int64_t* count;
   float2* stats;       // (T, parts): max, sum (argmax: max, index)
@@ -234,15 +236,20 @@ __device__ __forceinline__ double exp_of(const Args& a, float x, float top) {
 }
 
 // Drafts of the row that are accepted: waves take the positions in turn, each
-// three dependent loads.
+// three dependent loads.  The statistics' sum of exponentials decides where it is
+// certain to (Args::slack); the few positions whose two sides are closer take
+// their sum anew in 64 bits, one after the other.
 template <typename E>
 __global__ __launch_bounds__(kDecide) void decide_kernel(Args a) {
-  __shared__ int first;
+  constexpr int kWaves = kDecide / 64;
+  __shared__ int first, close;  // refused, too close to say: the first of each
+  __shared__ double part[kWaves];
   const int b = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int lo, n;
   row_span(a, b, lo, n);
   if (threadIdx.x == 0) {
     first = n - 1;
+    close = n;
     a.ticket[b * kTicket] = 0;
   }
   if (n == 0) {
@@ -251,21 +258,48 @@ __global__ __launch_bounds__(kDecide) void decide_kernel(Args a) {
     return;
   }
   __syncthreads();
-  for (int j = w; j < n - 1; j += kDecide / 64) {
-    const int64_t pos = lo + j;
-    const int64_t d = a.tokens[pos + 1];
-    const bool known = d >= 0 && d < a.V;
-    const float2 x = lane < a.parts ? a.stats[pos * a.parts + lane] : float2{kNegInf, 0.f};
-    const float xd = known ? (float)static_cast<const E*>(a.logits)[pos * a.lg_sn + d] : kNegInf;
-    const float qd = a.probs == nullptr ? 1.f : known ? a.probs[pos * a.dp_sn + d] : 0.f;
-    const float top = wave_max(x.x), ref = top == kNegInf ? 0.f : top;
-    // An absent part (-inf, 0) adds 0; a NaN sum stays.
-    const double sum = wave_sum((double)x.y * (double)fast_exp2((x.x - ref) * a.k2));
-    const bool fine = sum > 0. && sum < (double)__builtin_huge_valf();
-    const double p = fine && known ? exp_of(a, xd, top) / sum : 0.;
-    if (lane == 0 && !((double)a.accept_u[pos] * (double)qd < p)) atomicMin(&first, j);
+  int from = 0;
+  for (;;) {
+    for (int j = from + w; j < n - 1; j += kWaves) {
+      const int64_t pos = lo + j;
+      const int64_t d = a.tokens[pos + 1];
+      const bool known = d >= 0 && d < a.V;
+      const float2 x = lane < a.parts ? a.stats[pos * a.parts + lane] : float2{kNegInf, 0.f};
+      const float xd = known ? (float)static_cast<const E*>(a.logits)[pos * a.lg_sn + d] : kNegInf;
+      const float qd = a.probs == nullptr ? 1.f : known ? a.probs[pos * a.dp_sn + d] : 0.f;
+      const float top = wave_max(x.x), ref = top == kNegInf ? 0.f : top;
+      // An absent part (-inf, 0) adds 0; a NaN sum stays.
+      const double sum = wave_sum((double)x.y * (double)fast_exp2((x.x - ref) * a.k2));
+      const bool fine = sum > 0. && sum < (double)__builtin_huge_valf();
+      // u q < e / sum, both sides times the sum.
+      const double e = fine && known ? exp_of(a, xd, top) : 0.;
+      const double uq = (double)a.accept_u[pos] * (double)qd, lhs = uq * sum;
+      if (lane == 0) {
+        if (e > 0. && lhs <= e * a.slack && e <= lhs * a.slack) atomicMin(&close, j);
+        else if (!(e > 0. && lhs < e)) atomicMin(&first, j);
+      }
+    }
+    __syncthreads();
+    const int j = close;
+    if (j >= first) break;
+    const int64_t pos = lo + j, d = a.tokens[pos + 1];
+    const E* row = static_cast<const E*>(a.logits) + pos * a.lg_sn;
+    const float top = wave_max(lane < a.parts ? a.stats[pos * a.parts + lane].x : kNegInf);
+    double s = 0.;
+    for (int i = threadIdx.x; i < a.V; i += kDecide) s += exp_of(a, (float)row[i], top);
+    s = wave_sum(s);
+    if (lane == 0) part[w] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double sum = 0.;
+      for (int i = 0; i < kWaves; ++i) sum += part[i];
+      const float qd = a.probs == nullptr ? 1.f : a.probs[pos * a.dp_sn + d];
+      if (!((double)a.accept_u[pos] * (double)qd < exp_of(a, (float)row[d], top) / sum)) first = j;
+      close = n;
+    }
+    __syncthreads();
+    from = j + 1;  // once one is refused, no position from here on comes before it
   }
-  __syncthreads();
   if (w != 0) return;
   const int taken = first;
   const float top = wave_max(lane < a.parts ? a.stats[(int64_t)(lo + taken) * a.parts + lane].x : kNegInf);
@@ -472,6 +506,21 @@ int parts_of(int T, int V) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({by_len, kMaxParts, 2048 / T}));
 }
 
+// By which factor the two sides of an acceptance have to be apart for the fp32 sums to
+// say which is larger; u = 2^-24.  An exponential's argument of -a log2 units comes of
+// three roundings, 3 u a ln 2 of its value, and the weighted mean of a is at most
+// log2 V < 31: 65 u of the sum.  The exponential and a thread's eight terms are 9
+// more; each of the nine joins of threads and waves, the join of parts and each
+// further group of a thread 4 (exponential, product, sum).  That is less than x =
+// (128 + 4 groups) u, and 1 / (1 - x) < 1 + 2.5 x below 0.1; from there on every
+// position is looked at again.
+double slack_of(int V, int parts) {
+  const int64_t groups = ((int64_t)V + 2 * kGroup - 1) / kGroup;
+  const int64_t per = (groups + parts - 1) / parts;
+  const double x = (128. + 4. * (double)((per + kThreads - 1) / kThreads)) * 0x1p-24;
+  return x < 0.1 ? 1. + 2.5 * x : HUGE_VAL;
+}
+
 // With the elements that groups may start before the row.
 int chunks_of(int V) { return (int)(((int64_t)V + kGroup - 1 + kChunk - 1) / kChunk); }
 
@@ -551,6 +600,7 @@ extern "C" int qf_verify_drafts(const void* logits, int dtype, int64_t lg_sn, co
   a.width = width;
   a.T = T; a.B = B; a.V = V;
   a.parts = parts_of(T, V);
+  a.slack = slack_of(V, a.parts);
   a.chunks = chunks_of(V);
   unsigned char* p = static_cast<unsigned char*>(ws);
   const int64_t sums = (int64_t)B * a.chunks;
