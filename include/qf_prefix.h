@@ -68,7 +68,8 @@ int qf_copy_pages(const void* const* pools, int n_pools, int per, int64_t step,
  *
  * All device arrays are read when the kernels run; any contents keep every
  * access in bounds.  Infinities and NaN in slots that a row does not see do not
- * reach its output.
+ * reach its output.  Where every score that a query sees is -infinity its output is
+ * NaN, here and in the extension, as from qf_decode_attn and qf_prefill_attn.
  */
 int64_t qf_decode_attn_prefix_workspace(int B, int KVH, int G, int n_groups, int cap);
 

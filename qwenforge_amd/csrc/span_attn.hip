@@ -49,6 +49,7 @@ constexpr int kStages = 4;                   // ring of the wide units
 constexpr int kMaxSplits = 64;               // of either kind of unit
 constexpr int kMinKeys = 128;                // least keys of a split
 constexpr int kStepKeys = kWaves * kBN;      // a step of a narrow unit's waves
+constexpr float kHuge = 3.402823466e38f;
 
 struct Args {
   const f16* q;
@@ -549,10 +550,12 @@ __device__ __forceinline__ void load_queries(State<kQB>& s, const Args& a, const
   s.seen = __builtin_amdgcn_readfirstlane(least);
 }
 
-// o / l of a column, zero where nothing was seen.
+// o / l of a column.  Where all that it sees scored -infinity, o and l are 0 and
+// the quotient, as the softmax, is NaN; `sees` is false where it sees nothing, and
+// the output zero.
 __device__ __forceinline__ void store_out(const Args& a, int token, int hk, int g, int d, f32x4 o,
-                                          float l) {
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+                                          float l, bool sees) {
+  const float inv = sees ? 1.f / l : 0.f;
   const f16x4 r = {(f16)(o[0] * inv), (f16)(o[1] * inv), (f16)(o[2] * inv), (f16)(o[3] * inv)};
   *reinterpret_cast<f16x4*>(a.out + token * a.o_st + hk * a.o_sh + g * a.o_sg + d) = r;
 }
@@ -563,12 +566,14 @@ __device__ __forceinline__ void store_part(const Args& a, const Unit& u, int r, 
   if (r >= u.rows) return;
   const int token = u.tok0 + r / a.G, g = r % a.G;
   if (u.n_split == 0) {
-    store_out(a, token, u.hk, g, 16 * t + 4 * grp, o, l);
+    store_out(a, token, u.hk, g, 16 * t + 4 * grp, o, l, true);
     return;
   }
   const int64_t p = part_index(a, u, token, g);
   *reinterpret_cast<f32x4*>(a.acc + p * kD + 16 * t + 4 * grp) = o;
-  if (stats && grp == 0) a.ml[p] = float2{m, l};
+  // New tokens all see their split 0, which says to the merge that they see
+  // something where it holds scores of -infinity alone.
+  if (stats && grp == 0) a.ml[p] = float2{l == 0.f && u.split == 0 ? -kHuge : m, l};
 }
 
 // A unit with no slot: every query's partial is absent (l = 0), the output zero.
@@ -577,7 +582,7 @@ __device__ __forceinline__ void empty_unit(const Args& a, const Unit& u, int n_r
     const int r = u.r0 + (i >> 4), d = 4 * (i & 15);
     if (r >= u.rows) break;
     const int token = u.tok0 + r / a.G, g = r % a.G;
-    if (u.n_split == 0) store_out(a, token, u.hk, g, d, f32x4{0.f, 0.f, 0.f, 0.f}, 0.f);
+    if (u.n_split == 0) store_out(a, token, u.hk, g, d, f32x4{0.f, 0.f, 0.f, 0.f}, 0.f, false);
     else if (d == 0) a.ml[part_index(a, u, token, g)] = float2{kNegInf, 0.f};
   }
 }
@@ -900,7 +905,8 @@ __global__ __launch_bounds__(256) void span_merge_kernel(Args a, int n) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) o[c] = col_sum(o[c]);
   }
-  if (in && (kSubs == 1 || lane < 16)) store_out(a, token, hk, g, d0, o, sum);
+  const bool sees = kDecode ? a.last[token * a.last_sb] >= 0 : top > kNegInf;
+  if (in && (kSubs == 1 || lane < 16)) store_out(a, token, hk, g, d0, o, sum, sees);
 }
 
 // K (rotated with cos / sin if given) and V of every new token into its slot:
