@@ -26,6 +26,7 @@ and can be admitted and retired independently.  The ops call the C ABI in
 from __future__ import annotations
 
 import ctypes as C
+import operator
 
 import torch
 
@@ -131,7 +132,7 @@ class PagedKvCache:
         ``rows`` (unmapped before): whole pages are shared, a partly filled last
         page is copied into a page of the row's own, for all rows and layers in
         one launch.  ``map_row`` then grows the rows as usual."""
-        rows = [int(r) for r in rows]
+        rows = [operator.index(r) for r in rows]
         pages = self._rows.get(src, [])
         if not 0 <= n_slots <= len(pages) * self.page_size:
             raise ValueError(f"row {src} has {len(pages) * self.page_size} slots mapped, not {n_slots}")
@@ -314,7 +315,7 @@ def _slot_args(slots: torch.Tensor, batch: int, device):
 # --------------------------------------------------------------------------
 
 def _page_list(name: str, pages, n: int, low: int, high: int) -> list:
-    pages = [int(p) for p in pages]
+    pages = [operator.index(p) for p in pages]
     if len(pages) != n or any(not low <= p < high for p in pages):
         raise ValueError(f"{name} must be {n} whole numbers in [{low}, {high})")
     return pages
