@@ -39,15 +39,23 @@ from .rope import cos_sin
 
 
 def lookup_drafts(tokens, n: int, longest: int = 3) -> list:
-    """Up to ``n`` tokens that followed the last earlier occurrence of the
-    sequence's end (its last ``longest`` tokens, else fewer)."""
-    tokens = list(tokens)
-    for k in range(min(longest, len(tokens) - 1), 0, -1):
-        end = tokens[-k:]
-        for i in range(len(tokens) - k - 1, -1, -1):
-            if tokens[i:i + k] == end:
-                return tokens[i + k:i + k + n]
-    return []
+    """Up to ``n`` tokens that followed an earlier occurrence of the sequence's
+    end (its last ``longest`` tokens, else fewer): of the last occurrence with n
+    tokens behind it, or of the one with the most, as in a text that repeats
+    itself within n tokens."""
+    back = list(tokens)[::-1]
+    length = behind = i = 0               # of the best occurrence; i tokens stand behind one found
+    while (length < longest or behind < n) and back:
+        try:
+            i = back.index(back[0], i + 1)
+        except ValueError:
+            break
+        k = 1
+        while k < longest and i + k < len(back) and back[i + k] == back[k]:
+            k += 1
+        if k > length or (k == length and behind < n):
+            length, behind = k, i
+    return back[max(behind - n, 0):behind][::-1]
 
 
 class PagedDecodeEngine(DecodeEngine):
