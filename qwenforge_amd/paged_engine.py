@@ -194,15 +194,25 @@ class PagedDecodeEngine(DecodeEngine):
     def reads_prefix_once(self, batch: int, slots: int) -> bool:
         """Whether ``serve``'s steps attend ``batch`` rows with a common prefix of
         ``slots`` slots by ``flash_decode_attention_prefix_paged``, rather than each
-        row alone over the pages it shares.  Measured on MI355X, ms per step of 24
-        layers, alone / together: B=2 1024 0.58 / 0.65, 4096 0.71 / 0.69, 16384
-        1.25 / 0.77; B=4 1024 0.62 / 0.73, 4096 0.75 / 0.76, 16384 1.28 / 0.82; B=8
-        4096 0.73 / 0.82, 16384 0.86 / 0.90; B=32 1024 0.95 / 1.07, 4096 1.07 /
-        1.09, 16384 1.57 / 1.20 (the fused step cuts a row into at most eight
-        pieces, the wide one into as many as fill the CUs)."""
+        row alone over the pages it shares.
+
+        Alone, a row's slots are cut into as many pieces as the step has for it, so
+        its time grows with slots / pieces, however many of the rows are parked (4 of
+        32 rows behind 16384 slots take what 32 take); together it hardly grows.  The
+        fused step has four pieces for any row, the others CUs / (rows * kv heads).
+        MI355X, us per layer of the step, alone / together, at heads / kv heads:
+        fused, 2 rows of 14/2 2048 slots 27.2 / 27.6, 4096 30.6 / 28.9; of 16/8 3072
+        29.8 / 30.7, 4096 31.8 / 31.6; 3 rows of 16/8 4096 32.0 / 32.2; 4 rows of
+        14/2 4096 31.8 / 31.6, 6144 35.5 / 32.7; of 16/8 4096 33.0 / 35.7, 6144 36.9
+        / 36.7.  Wide, by rows * kv heads * slots: 262144 (8 and 32 rows of 14/2)
+        36.6 / 38.8 and 45.4 / 46.5, (8 of 16/8) 37.2 / 38.6, (16 of 8/1) 36.6 /
+        39.8; 327680 (5 of 14/2, 5 of 16/8) 41.6 / 39.6 and 39.2 / 38.6; 524288 (16
+        of 14/2, 8 of 16/8, 32 of 8/1) 46.1 / 43.5, 44.2 / 40.9 and 48.8 / 46.1."""
+        if batch < 2:
+            return False
         if self.uses_fused_step(batch):
-            return batch > 1 and slots >= 4096
-        return batch * slots > 131072
+            return slots >= (4096 if batch == 2 else 6144)
+        return batch * self.cfg.kv_heads * slots >= 327680
 
     def _attend_prefix(self, ctx, grouped, kp, vp):
         rows, length, table = ctx["prefix"]
