@@ -59,7 +59,8 @@ int qf_prefill_layers(const QfPrefillLayer* layers, int n_layers, void* hidden, 
 /* qf_prefill_layers for packed new tokens of rows that hold slots already, over
  * paged caches (qf_prefill_extend_paged in qf_prefix.h: cu, context, ctx_sb and
  * cap as there): token i of row b has position and slot context[b] + i and
- * attends to slots [0, context[b] + i].  ws as above, of at least
+ * attends to slots [0, context[b] + i].  Tokens of no row append nothing; what
+ * their rows of hidden hold afterwards is unspecified.  ws as above, of at least
  * qf_extend_layers_workspace bytes. */
 int64_t qf_extend_layers_workspace(int T, int hidden, int QH, int KVH, int D, int I, int B, int cap);
 

@@ -6,7 +6,8 @@
 // thread, all layers' K and V in one launch, so memory bounds it: 700 pages of 64
 // slots in 24 layers (1.1 GB read and written) take 213 us, 5.2 TB/s, where a
 // copy of 1 GiB runs at 4.8.  A partly filled page of one row takes 2.7 us, the
-// launch.
+// launch; called from Python 8.6 us with indices on the device and 30 with lists,
+// which are checked and copied there (700 pages 211 and 229).
 #include "qf_common.h"
 #include "../../include/qf_prefix.h"
 

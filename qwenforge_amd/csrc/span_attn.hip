@@ -19,18 +19,21 @@
 // past a unit's last one read as zero, and masked slots count for nothing
 // whatever K and V hold there (masked_values).
 //
-// A wave's step of 32 queries and 64 keys is 36 matrix products of 16 cycles, and
-// more than as many cycles of vector work: 32 exponentials of 16 cycles, their
-// fma and conversion, maxima, addresses.  So the vector unit bounds the
-// long cases, not memory: MI355X, 14 query heads on 2 kv heads, GPU time of the
-// whole call in a replayed graph: 2048 tokens behind 16384 slots 188 us (680
-// TF/s; 111 us at the rate of a large fp16 product), 16 rows of 9 to 301 tokens
-// behind 2048 slots 56 us (its 286 units leave most CUs one workgroup of the
-// two that they hold), decode of 96 rows of one 32768-slot prefix 36 us (7 us
-// of memory traffic, 10 of products; each row alone over the shared pages 7 ms
-// in plain tensor operations).  Four rows of a 512-slot prefix take 9.4 us, four
-// times five tokens behind 2000 slots 12.1 us: two or three launches and their
-// dependent loads (bounds, table, tile).
+// A wave's step of 32 queries and 64 keys is 36 matrix products of 16 cycles and
+// some 120 vector instructions, 32 of them exponentials of 16 cycles.  No unit is
+// full, and memory is not the bound: counted over 2048 tokens behind 16384 slots
+// (96 rows of a 32768-slot prefix), the vector unit issues in 44% (42%) of the SIMDs'
+// cycles and the matrix cores are busy in 33% (23%); a wave spends 23% (38%) of its
+// time waiting for tiles and barriers and 29% (24%) for its turn to issue, with 1.5
+// waves to a SIMD.  MI355X, 14 query heads on 2 kv heads, GPU time of the whole call
+// in a replayed graph: that chunk 189 us (680 TF/s; 111 us at the rate of a large
+// fp16 product), 16 rows of 9 to 301 tokens behind 2048 slots 56 us (its 286 units
+// leave most CUs one workgroup of the two that they hold), four times five tokens
+// behind 2000 slots 12.2 us (three launches and their dependent loads).  Decode,
+// and in brackets each row alone over the shared pages (flash_decode_attention_paged):
+// 96 rows of the 32768-slot prefix 36 us (235), 24 rows in three groups of up to
+// 4096 shared slots 12.8 (14.1), four rows of a 512-slot prefix 9.4 (6.3): the two
+// launches, of which the merge is 3 us, pay from long prefixes or many rows on.
 #include <algorithm>
 
 #include "extend.h"
@@ -979,9 +982,11 @@ int pick_form(int64_t rows_per_segment) {
   return rows_per_segment <= 16 ? 0 : rows_per_segment <= 64 ? 1 : 2;
 }
 
-// Splits of at least `least` keys, so that no more units are made than the two
+// Splits of at least `least` keys, so that these units are no more than the two
 // workgroups per CU that run at once: some more would take a second round (286
-// units of 16 ragged rows behind 2048 slots: 56 us whole, 62 cut in two).
+// units of 16 ragged rows behind 2048 slots: 56 us whole, 62 cut in two).  A decode's
+// own slots are counted by themselves, though they share the launch: 96 rows of a
+// 32768-slot prefix are 504 wide and 384 narrow workgroups.
 int pick_splits(int64_t units, int cap, int least) {
   const int64_t by_len = std::min<int64_t>(kMaxSplits, ((int64_t)cap + least - 1) / least);
   return (int)std::max<int64_t>(1, std::min<int64_t>(by_len, 2 * kCus / units));

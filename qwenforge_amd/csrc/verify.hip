@@ -16,12 +16,13 @@
 // first launch of the kernel takes it.
 //
 // MI355X, 151936 fp16 logits a position: 32 rows of 8 positions with draft
-// probabilities 46.5 us in a replayed graph, of which stats_kernel 18 (78 MB, 4.3
-// TB/s: memory; four groups in flight or twice the parts were slower), decide_kernel
-// 5 (6 with four waves), the sums of exponentials 8, the draw 18 (exps in 64 bits,
-// 29 MB, and the last workgroup's search, some 5 us of dependent steps).  One row
-// of 5 positions 14.5 us, 8 rows at temperature 0 8.5 us: the launches and each
-// one's chain of dependent loads.
+// probabilities 47.5 us in a replayed graph (fp32 logits 59).  Traced one by one,
+// which adds 0.5 to 2 us to each: stats_kernel 18.2 (78 MB, 4.3 TB/s: memory; four
+// groups in flight or twice the parts were slower), decide_kernel 4.8 (6 with four
+// waves), the sums of exponentials 8.2, the draw 18.9 (exps in 64 bits, 29 MB, and
+// the last workgroup's search, some 5 us of dependent steps).  One row of 5
+// positions 14.6 us, 8 rows at temperature 0 8.5 us: the launches and each one's
+// chain of dependent loads.
 #include <algorithm>
 #include <cmath>
 
