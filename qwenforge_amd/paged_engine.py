@@ -43,7 +43,7 @@ def lookup_drafts(tokens, n: int, longest: int = 3) -> list:
     end (its last ``longest`` tokens, else fewer): of the last occurrence with n
     tokens behind it, or of the one with the most, as in a text that repeats
     itself within n tokens."""
-    back = list(tokens)[::-1]
+    back = list(tokens)[::-1] if longest > 0 else []
     length = behind = i = 0               # of the best occurrence; i tokens stand behind one found
     while (length < longest or behind < n) and back:
         try:
