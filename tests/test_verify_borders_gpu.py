@@ -82,3 +82,22 @@ def test_several_borders_in_a_row(dev):
         kept = n - 1 if above is None else above
         assert count.tolist() == [kept + 1]
         assert out[0, :kept].tolist() == tokens[1:kept + 1].tolist()
+
+
+def test_borders_of_a_few_rows_among_many_positions(dev):
+    """So many positions that each is one workgroup's, whose threads add up 75 groups of logits."""
+    gen = torch.Generator(dev).manual_seed(9)
+    rows, v = 550, 151936
+    logits = torch.randn(2 * rows, v, generator=gen, device=dev, dtype=torch.float16) * 2
+    tokens = torch.zeros(2 * rows, dtype=torch.int64, device=dev)
+    looked = list(range(0, rows, 61)) + [rows - 1]
+    p = torch.softmax(logits[[2 * r for r in looked]].cpu().double(), dim=-1)
+    draft = p.argmax(dim=-1)
+    tokens[[2 * r + 1 for r in looked]] = draft.to(dev)
+    sides = np.array([_sides(b) for b in p.gather(1, draft[:, None])[:, 0].tolist()])
+    for side in (0, 1):
+        u = torch.full((2 * rows,), 0.5, device=dev)
+        u[[2 * r for r in looked]] = torch.tensor(sides[:, side], dtype=torch.float32, device=dev)
+        _, out = verify.verify_drafts(logits, tokens, _cu([2] * rows, dev), 2, u, torch.full((rows,), 0.5, device=dev))
+        took = (out[looked, 1] >= 0).cpu()
+        assert took.all() if side == 0 else not took.any(), (side, took.tolist())
