@@ -201,8 +201,8 @@ class PagedDecodeEngine(DecodeEngine):
         32 rows behind 16384 slots take what 32 take); together it hardly grows.  The
         fused step has four pieces for any row, the others CUs / (rows * kv heads).
         MI355X, us per layer of the step, alone / together, at heads / kv heads:
-        fused, 2 rows of 14/2 2048 slots 27.2 / 27.6, 4096 30.6 / 28.9; of 16/8 3072
-        29.8 / 30.7, 4096 31.8 / 31.6; 3 rows of 16/8 4096 32.0 / 32.2; 4 rows of
+        fused, 2 rows of 14/2 2048 slots 27.2 / 27.6, 4096 30.6 / 28.9; of 16/8 2048
+        28.2 / 29.7, 4096 31.8 / 31.6; 3 rows of 16/8 4096 32.0 / 32.2; 4 rows of
         14/2 4096 31.8 / 31.6, 6144 35.5 / 32.7; of 16/8 4096 33.0 / 35.7, 6144 36.9
         / 36.7.  Wide, by rows * kv heads * slots: 262144 (8 and 32 rows of 14/2)
         36.6 / 38.8 and 45.4 / 46.5, (8 of 16/8) 37.2 / 38.6, (16 of 8/1) 36.6 /

@@ -17,7 +17,7 @@ TIMED = [
     (14, 2, 8, 32768, 43.9, 40.0), (14, 2, 16, 8192, 39.3, 41.4), (14, 2, 16, 16384, 46.1, 43.5),
     (14, 2, 32, 4096, 45.4, 46.5), (14, 2, 32, 8192, 52.2, 48.0), (14, 2, 48, 2048, 89.2, 91.3),
     (14, 2, 48, 4096, 96.6, 91.5),
-    (16, 8, 2, 3072, 29.8, 30.7), (16, 8, 2, 8192, 39.1, 36.6), (16, 8, 3, 6144, 36.1, 33.6),
+    (16, 8, 2, 2048, 28.2, 29.7), (16, 8, 2, 8192, 39.1, 36.6), (16, 8, 3, 6144, 36.1, 33.6),
     (16, 8, 4, 4096, 33.0, 35.7), (16, 8, 4, 8192, 40.5, 37.4), (16, 8, 5, 8192, 39.2, 38.6),
     (16, 8, 8, 4096, 37.2, 38.6), (16, 8, 8, 8192, 44.2, 40.9), (16, 8, 16, 4096, 47.6, 42.0),
     (16, 8, 32, 2048, 52.1, 47.6), (16, 8, 48, 2048, 114.1, 96.9),
