@@ -1,6 +1,7 @@
 """ctypes binding of the C ABI in ``include/qf_attn.h``, ``include/qf_step.h``,
 ``include/qf_wide.h``, ``include/qf_prefill.h``, ``include/qf_paged.h``,
-``include/qf_prefix.h``, ``include/qf_verify.h`` and ``include/qf_probe.h``.
+``include/qf_prefix.h``, ``include/qf_verify.h``, ``include/qf_paged8.h`` and
+``include/qf_probe.h``.
 
 The shared object is built in-tree by ``qwenforge_amd.build``.  There is no
 fallback: if it is missing or does not load, every op raises.
@@ -15,6 +16,17 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().with_name("_qf_attn.so")
 
 _i64, _i32, _f32, _vp = C.c_int64, C.c_int, C.c_float, C.c_void_p
+
+
+
+class Pool8(C.Structure):
+    """``QfPool8`` (``include/qf_paged8.h``)."""
+
+    _fields_ = ([(n, _vp) for n in ("k", "v", "k_scale", "v_scale")]
+                + [(n, _i64) for n in ("sl", "sp", "sh", "ssl", "ssp", "ssh")]
+                + [("table", _vp), ("bt_sb", _i64)]
+                + [(n, C.c_int32) for n in ("pages_per_row", "n_pages", "page_size", "layers", "KVH", "code")])
+
 
 # name -> argument types, in header order.  Every entry point returns int.
 SIGNATURES = {
@@ -320,6 +332,26 @@ SIGNATURES = {
         _vp, _vp, _vp, _i64, C.c_double,  # accept_u, sample_u, draft_probs, dp_sn, temperature
         _vp, _i32, _vp, _vp, _i64,      # out, width, count, ws, ws_bytes
         _i32, _i32, _i32, _vp,          # T, B, V, stream
+    ],
+    # include/qf_paged8.h
+    "qf_append_paged8": [
+        _vp, _i64, _i64, _i64,          # k, k_sl, k_sh, k_sn
+        _vp, _i64, _i64, _i64,          # v
+        _vp, _i32, _i32,                # cu_seqlens, total, max_seqlen
+        _vp, _i64,                      # context, ctx_sb
+        _vp, _vp, _i64,                 # cos, sin, cs_sn
+        C.POINTER(Pool8), _i32, _i32, _vp,  # pool, B, D, stream
+    ],
+    "qf_read_paged8": [
+        _vp, _i64, _i64, _i64,          # k, k_sl, k_sh, k_sn
+        _vp, _i64, _i64, _i64,          # v
+        _vp, _i32, _i32,                # cu_seqlens, total, max_seqlen
+        _vp, _i64,                      # first, first_sb
+        C.POINTER(Pool8), _i32, _i32, _vp,  # pool, B, D, stream
+    ],
+    "qf_copy_pages8": [
+        _vp, _i32, _i64, _i64, _i64,    # store, layers, layer_step, step, bytes
+        _vp, _vp, _i32, _i32, _vp,      # src, dst, n_pairs, n_pages, stream
     ],
     # include/qf_probe.h
     "qf_stream_read": [_vp, _i64, _vp, _i32, _vp],   # src, bytes, sink, workgroups, stream

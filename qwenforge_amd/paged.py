@@ -71,13 +71,19 @@ class PagedKvCache:
         self.kv_heads = kv_heads
         self.pages_per_row = pages_per_row
         self.device = torch.device(device)
-        self.store = torch.zeros((layers, 2, n_pages, kv_heads, page_size, HEAD_DIM),
-                                 device=self.device, dtype=dtype)
-        self.pools = [(layer[0], layer[1]) for layer in self.store]
+        self._allocate(layers, dtype)
         self.table = torch.full((max_rows, pages_per_row), -1, device=self.device, dtype=torch.int32)
         self._free = list(range(n_pages))
         self._rows: dict[int, list[int]] = {}
         self._holders = [0] * n_pages          # rows that hold each page
+
+    def _allocate(self, layers: int, dtype) -> None:
+        self.store = torch.zeros((layers, 2, self.n_pages, self.kv_heads, self.page_size, HEAD_DIM),
+                                 device=self.device, dtype=dtype)
+        self.pools = [(layer[0], layer[1]) for layer in self.store]
+
+    def _copy(self, src, dst, slots=None) -> None:
+        copy_pages(self.store, src, dst, slots=slots)
 
     @property
     def capacity(self) -> int:
@@ -144,7 +150,7 @@ class PagedKvCache:
             raise RuntimeError(f"page pool exhausted: need {len(rows)}, {len(self._free)} free")
         own = self._free[:len(rows)] if rest else []
         if own:
-            copy_pages(self.store, [pages[whole]] * len(rows), own, slots=[rest] * len(rows))
+            self._copy([pages[whole]] * len(rows), own, slots=[rest] * len(rows))
         for i, row in enumerate(rows):
             if rest:
                 self._take()
@@ -171,7 +177,7 @@ class PagedKvCache:
         if len(at) > len(self._free):
             raise RuntimeError(f"page pool exhausted: need {len(at)}, {len(self._free)} free")
         if at:
-            copy_pages(self.store, [pages[j] for j in at], self._free[:len(at)])
+            self._copy([pages[j] for j in at], self._free[:len(at)])
             for j in at:
                 self._holders[pages[j]] -= 1
                 pages[j] = self._take()
@@ -187,7 +193,7 @@ class PagedKvCache:
         dst = [p for p in self._free if p < len(used)]
         if not src:
             return 0
-        copy_pages(self.store, src, dst)
+        self._copy(src, dst)
         to = dict(zip(src, dst))
         for pages in self._rows.values():
             pages[:] = [to.get(p, p) for p in pages]
