@@ -112,6 +112,68 @@ int qf_read_paged8(void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn,
 int qf_copy_pages8(void* store, int layers, int64_t layer_step, int64_t step, int64_t bytes,
                    const int32_t* src, const int32_t* dst, int n_pairs, int n_pages, void* stream);
 
+/*
+ * Decode attention of single tokens: softmax(scale q K^T) V over each row's slots
+ * [0, kv_last], as qf_decode_attn_paged without a bias.
+ *
+ *   q, out   (B, KVH, G, D), strides *_sb, *_sh, *_sg
+ *   kv_last  int64 on the device, row b reads kv_last[b * kv_last_sb]: its last
+ *            slot (inclusive).  A row with kv_last < 0 (parked) gets zeros
+ *   pool     of one layer
+ *   ws       16-byte aligned scratch of at least qf_decode_attn_paged8_workspace
+ *            bytes for these sizes (cap = pages_per_row * page_size; NULL where
+ *            that is 0), else QF_ERR_SCRATCH_LIMIT; free again when the call's work
+ *            is done, and not to be shared by calls that overlap in time
+ *   scale    > 0
+ *
+ * Slots that a row does not see may hold anything.  A block that reads as NaN makes
+ * NaN of the rows that see any of it; where every score is -infinity the output is NaN.
+ */
+int64_t qf_decode_attn_paged8_workspace(int B, int KVH, int G, int cap);
+
+int qf_decode_attn_paged8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sg,
+                          const QfPool8* pool, const int64_t* kv_last, int64_t kv_last_sb,
+                          void* ws, int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh,
+                          int64_t o_sg, int B, int G, int D, float scale, void* stream);
+
+/*
+ * Its split phase alone: the partials acc (B, KVH, splits, G, D), m and l (B, KVH,
+ * splits, G) of qf_decode_split_paged, for qf_decode_combine or qf_attn_merge_o_proj
+ * (m in natural units; a range without a slot leaves acc = l = 0 and m = -infinity).
+ * acc is 16-byte aligned.
+ */
+int qf_decode_split_paged8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sg,
+                           const QfPool8* pool, const int64_t* kv_last, int64_t kv_last_sb,
+                           float* acc, float* m, float* l, int splits, int B, int G, int D,
+                           float scale, void* stream);
+
+/*
+ * New tokens behind cached ones: qf_append_paged8 of a layer's k and v, then token i of
+ * row b attends to slots [0, context[b] + i] of its pages -- all of them as the pages
+ * hold them, the new ones too.
+ *
+ *   q, out  (T, QH, D), strides *_sh per head, *_sn per token, QH a multiple of the
+ *           pool's KVH.  Rows of out for tokens of no row are left as they were; those
+ *           of a parked row (context < 0) become zero
+ *   cos, sin  as in the append; q is rotated with them too
+ *   max_seqlen  the most tokens of a row; further ones get no output
+ *   cap     slots of a row that the call may use, at most pages_per_row *
+ *           page_size: a bound on every row's context + tokens, from which the
+ *           work is split.  Tokens past it are not appended and see the slots below
+ *   ws      as above, qf_prefill_extend_paged8_workspace bytes
+ */
+int64_t qf_prefill_extend_paged8_workspace(int B, int QH, int KVH, int total, int max_seqlen, int cap);
+
+int qf_prefill_extend_paged8(const void* q, int64_t q_sh, int64_t q_sn,
+                             const void* k, int64_t k_sh, int64_t k_sn,
+                             const void* v, int64_t v_sh, int64_t v_sn,
+                             const int32_t* cu_seqlens, int total, int max_seqlen,
+                             const int64_t* context, int64_t ctx_sb,
+                             const void* cos, const void* sin, int64_t cs_sn,
+                             const QfPool8* pool, int cap, void* ws, int64_t ws_bytes,
+                             void* out, int64_t o_sh, int64_t o_sn,
+                             int B, int QH, int D, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

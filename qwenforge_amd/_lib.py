@@ -353,6 +353,33 @@ SIGNATURES = {
         _vp, _i32, _i64, _i64, _i64,    # store, layers, layer_step, step, bytes
         _vp, _vp, _i32, _i32, _vp,      # src, dst, n_pairs, n_pages, stream
     ],
+    "qf_decode_attn_paged8_workspace": [_i32, _i32, _i32, _i32],        # B, KVH, G, cap
+    "qf_decode_attn_paged8": [
+        _vp, _i64, _i64, _i64,          # q, q_sb, q_sh, q_sg
+        C.POINTER(Pool8), _vp, _i64,    # pool, kv_last, kv_last_sb
+        _vp, _i64,                      # ws, ws_bytes
+        _vp, _i64, _i64, _i64,          # out, o_sb, o_sh, o_sg
+        _i32, _i32, _i32, _f32, _vp,    # B, G, D, scale, stream
+    ],
+    "qf_decode_split_paged8": [
+        _vp, _i64, _i64, _i64,          # q
+        C.POINTER(Pool8), _vp, _i64,    # pool, kv_last, kv_last_sb
+        _vp, _vp, _vp, _i32,            # acc, m, l, splits
+        _i32, _i32, _i32, _f32, _vp,    # B, G, D, scale, stream
+    ],
+    "qf_prefill_extend_paged8_workspace": [_i32, _i32, _i32, _i32, _i32, _i32],  # B, QH, KVH, total, longest, cap
+    "qf_prefill_extend_paged8": [
+        _vp, _i64, _i64,                # q, q_sh, q_sn
+        _vp, _i64, _i64,                # k
+        _vp, _i64, _i64,                # v
+        _vp, _i32, _i32,                # cu_seqlens, total, max_seqlen
+        _vp, _i64,                      # context, ctx_sb
+        _vp, _vp, _i64,                 # cos, sin, cs_sn
+        C.POINTER(Pool8), _i32,         # pool, cap
+        _vp, _i64,                      # ws, ws_bytes
+        _vp, _i64, _i64,                # out, o_sh, o_sn
+        _i32, _i32, _i32, _f32, _vp,    # B, QH, D, scale, stream
+    ],
     # include/qf_probe.h
     "qf_stream_read": [_vp, _i64, _vp, _i32, _vp],   # src, bytes, sink, workgroups, stream
     "qf_launch_probe": [_vp, _i64, _vp, _vp,          # src, bytes, index, sink
@@ -377,7 +404,8 @@ for _name in ("qf_decode_attn", "qf_decode_attn_paged"):
 # Entry points that do not return an int status.
 RESTYPES = {"qf_error_string": C.c_char_p, "qf_prefill_layers_workspace": _i64,
             "qf_decode_attn_prefix_workspace": _i64, "qf_prefill_extend_workspace": _i64,
-            "qf_extend_layers_workspace": _i64, "qf_verify_workspace": _i64}
+            "qf_extend_layers_workspace": _i64, "qf_verify_workspace": _i64,
+            "qf_decode_attn_paged8_workspace": _i64, "qf_prefill_extend_paged8_workspace": _i64}
 
 _lock = threading.Lock()
 _lib: C.CDLL | None = None

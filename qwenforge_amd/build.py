@@ -24,7 +24,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 SOURCES = ["decode_attn.hip", "decode_attn_fused_vec.hip", "prefill_attn.hip", "prefill_gemm.hip", "rope_append.hip",
            "decode_step.hip", "decode_wide.hip", "pages.hip", "span_attn.hip", "verify.hip", "paged8.hip",
-           "probe.hip", "decode_valu.hip", "capi.cpp"]
+           "paged8_attn.hip", "probe.hip", "decode_valu.hip", "capi.cpp"]
 # Packed-fp32 VALU forms are disabled for all device code (they have produced
 # silently wrong results on this hardware pool); hipcc's host pass warns that it
 # does not know the feature, which is harmless.

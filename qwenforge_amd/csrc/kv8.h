@@ -88,6 +88,12 @@ inline int make_pool(const QfPool8* h, Pool& p) {
   return QF_OK;
 }
 
+// qf_append_paged8 into the rows' slots below cap (paged8.hip).
+int append(const void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn, const void* v, int64_t v_sl,
+           int64_t v_sh, int64_t v_sn, const int32_t* cu_seqlens, int total, int max_seqlen,
+           const int64_t* context, int64_t ctx_sb, const void* cos, const void* sin, int64_t cs_sn,
+           const QfPool8* pool, int cap, int B, int D, hipStream_t st);
+
 __device__ __forceinline__ int clampi(int64_t x, int lo, int hi) {
   return (int)(x < lo ? lo : x > hi ? hi : x);
 }

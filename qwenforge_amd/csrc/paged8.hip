@@ -28,7 +28,7 @@ struct RowsArgs {
   const int32_t* cu;
   const int64_t* first;      // first slot of each row's tokens
   int64_t first_sb;
-  int B, total;
+  int B, total, cap;         // slots of a row from cap on are not there
   const f16* cos;
   const f16* sin;
   int64_t cs_sn;
@@ -201,7 +201,8 @@ __global__ __launch_bounds__(64 * kWaves) void append_kernel(RowsArgs a) {
   uint8_t* kp = a.p.k + at + (int64_t)in_page * kD;     // 16 slots x 64
   uint8_t* vp = a.p.v + at + (int64_t)(in_page >> 6) * 64 * kD + (in_page & 63);
   const bool begun = u.lo > 0;
-  const int end = u.lo + u.n;                           // slots [lo, end) of the block are new
+  const int end = min(u.lo + u.n, a.cap - slot0);       // slots [lo, end) of the block are new
+  if (end <= u.lo) return;
   const float ks_old = a.p.ks[sat], vs_old = a.p.vs[sat];
 
   // K: slot t, dims 8c and 32 + 8c.
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_kernel(RowsArgs a) {
   }
   u32x2 old_lo = {0, 0}, old_hi = {0, 0};
   u32x4 old_v = {0, 0, 0, 0};
-  if (u.n < kBlock) {
+  if (begun || end < kBlock) {
     old_lo = *reinterpret_cast<const u32x2*>(kp + t * kD + c);
     old_hi = *reinterpret_cast<const u32x2*>(kp + t * kD + c + 32);
     old_v = *reinterpret_cast<const u32x4*>(vp + lane * 64);
@@ -347,7 +348,7 @@ int make_rows(RowsArgs& a, dim3& grid, const void* k, int64_t k_sl, int64_t k_sh
               const void* v, int64_t v_sl, int64_t v_sh, int64_t v_sn, const int32_t* cu, int total,
               int max_seqlen, const int64_t* first, int64_t first_sb, const QfPool8* pool, int B, int D) {
   if (D != kD) return QF_ERR_UNSUPPORTED;
-  if (!k || !v || !cu || !first || B < 1 || total < 1 || max_seqlen < 1 || max_seqlen > total)
+  if (!pool || !k || !v || !cu || !first || B < 1 || total < 1 || max_seqlen < 1 || max_seqlen > total)
     return QF_ERR_INVALID_ARG;
   if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) != 0 ||
       ((k_sl | k_sh | k_sn | v_sl | v_sh | v_sn) & 7) != 0)
@@ -364,6 +365,7 @@ int make_rows(RowsArgs& a, dim3& grid, const void* k, int64_t k_sl, int64_t k_sh
   a.first = first;
   a.first_sb = first_sb;
   a.B = B; a.total = total;
+  a.cap = pool->pages_per_row * pool->page_size;
   // A row's n tokens touch at most n / 16 + 2 blocks, one of them if n is 1.
   const int64_t blocks = max_seqlen == 1 ? B : (int64_t)total / kBlock + 2 * (int64_t)std::min(B, total);
   grid = dim3((unsigned)((blocks + kWaves - 1) / kWaves), (unsigned)(pool->KVH * pool->layers));
@@ -373,14 +375,10 @@ int make_rows(RowsArgs& a, dim3& grid, const void* k, int64_t k_sl, int64_t k_sh
 }  // namespace kv8
 }  // namespace qf
 
-extern "C" int qf_append_paged8(const void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn,
-                                const void* v, int64_t v_sl, int64_t v_sh, int64_t v_sn,
-                                const int32_t* cu_seqlens, int total, int max_seqlen,
-                                const int64_t* context, int64_t ctx_sb, const void* cos,
-                                const void* sin, int64_t cs_sn, const QfPool8* pool, int B, int D,
-                                void* stream) {
-  using namespace qf;
-  using namespace qf::kv8;
+int qf::kv8::append(const void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn, const void* v, int64_t v_sl,
+                    int64_t v_sh, int64_t v_sn, const int32_t* cu_seqlens, int total, int max_seqlen,
+                    const int64_t* context, int64_t ctx_sb, const void* cos, const void* sin,
+                    int64_t cs_sn, const QfPool8* pool, int cap, int B, int D, hipStream_t st) {
   RowsArgs a;
   dim3 grid;
   const int rc = make_rows(a, grid, k, k_sl, k_sh, k_sn, v, v_sl, v_sh, v_sn, cu_seqlens, total,
@@ -393,12 +391,22 @@ extern "C" int qf_append_paged8(const void* k, int64_t k_sl, int64_t k_sh, int64
   a.cos = static_cast<const f16*>(cos);
   a.sin = static_cast<const f16*>(sin);
   a.cs_sn = cs_sn;
-  hipStream_t st = static_cast<hipStream_t>(stream);
+  a.cap = std::min(a.cap, cap);
   if (pool->code == QF_CODE_E4M3)
     hipLaunchKernelGGL(append_kernel<true>, grid, dim3(64 * kWaves), 0, st, a);
   else
     hipLaunchKernelGGL(append_kernel<false>, grid, dim3(64 * kWaves), 0, st, a);
   return (int)hipGetLastError();
+}
+
+extern "C" int qf_append_paged8(const void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn,
+                                const void* v, int64_t v_sl, int64_t v_sh, int64_t v_sn,
+                                const int32_t* cu_seqlens, int total, int max_seqlen,
+                                const int64_t* context, int64_t ctx_sb, const void* cos,
+                                const void* sin, int64_t cs_sn, const QfPool8* pool, int B, int D,
+                                void* stream) {
+  return qf::kv8::append(k, k_sl, k_sh, k_sn, v, v_sl, v_sh, v_sn, cu_seqlens, total, max_seqlen, context,
+                         ctx_sb, cos, sin, cs_sn, pool, 0x7fffffff, B, D, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int qf_read_paged8(void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn, void* v, int64_t v_sl,

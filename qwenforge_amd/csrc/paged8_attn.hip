@@ -1,0 +1,667 @@
+// Attention over paged caches held in 8 bits (gfx950; the format is qf_paged8.h's):
+// single tokens of a batch, and new tokens behind cached ones.
+//
+// softmax(q K^T) V over slots [0, lim) of a row's pages, lim differing by query, is
+// cut into units: up to 16 kNC query rows (token, query head of one kv head) times
+// a range of slots.  The waves of a unit's workgroup take tiles of 64 slots in turn and
+// join their states in LDS; what several ranges of a query leave is joined by
+// merge_kernel.
+//
+// A tile is 8 KB of codes, K and V both loaded straight into matrix-core operands,
+// 16 bytes a lane: with lane group g = lane / 16,
+//   K  lane r + 16 g of load (u, j) has dims [16 g, 16 g + 16) of slot
+//      16 (r / 4) + 8 u + 4 j + r % 4, so that element i of score tile (u, j) is
+//      slot 16 g + 8 u + 4 j + i;
+//   V  lane r + 16 g of load t has slots [16 g, 16 g + 16) of dim 16 t + r, which the
+//      dim-major pages hold side by side: no transposition anywhere.
+// So all 16 slots whose scores and values a lane has are one block of the cache, and a
+// tile's scales are two floats a lane.  K's scale goes into the factor that the scores
+// have anyway; V's into the conversion of its codes to fp16, which is exact.
+#include <algorithm>
+
+#include "kv8.h"
+#include "lds_tile.h"
+
+namespace qf {
+namespace kv8 {
+
+constexpr int kTile = 64;                    // slots
+constexpr int kMaxSplits = 64;
+
+struct AttnArgs {
+  Pool p;
+  const f16* q;
+  int64_t q_st, q_sh, q_sg;                  // token, kv head, query head of the kv head
+  const int32_t* cu;                         // extension: the rows' tokens
+  const int64_t* last;                       // decode: last slot; extension: cached slots
+  int64_t last_sb;
+  int B, tokens, G, cap;
+  int n_tiles, splits;                       // query tiles of a row, splits of a row's slots
+  float* acc;                                // (token, kv head, split, query head, 64)
+  float* m;                                  // (token, kv head, split, query head), times m_unit
+  float* l;
+  float m_unit;                              // ln 2 where a caller's own merge reads m
+  int fill;                                  // ranges without a slot leave partials too
+  f16* out;
+  int64_t o_st, o_sh, o_sg;
+  float scale_log2;
+  const f16* cos;
+  const f16* sin;
+  int64_t cs_sn;
+};
+
+// Slots [k0, k1) of split s of [0, end): cut at multiples of `least` and 64.
+__device__ __forceinline__ void cut(int end, int s, int n, int& k0, int& k1) {
+  const int tiles = (end + kTile - 1) / kTile;
+  const int len = (tiles + n - 1) / n * kTile;
+  const int64_t at = (int64_t)s * len;
+  k0 = (int)(at < end ? at : end);
+  k1 = (int)(at + len < end ? at + len : end);
+}
+
+struct Unit {
+  int tok0, rows, r0;     // the row's first token, its query rows, the unit's first one
+  int row, hk, split;
+  int ctx;                // extension: cached slots, -1 parked
+  int k0, k1;
+};
+
+// What the query row of `token` sees: slots [0, lim).
+template <bool kDecode>
+__device__ __forceinline__ int row_limit(const AttnArgs& a, const Unit& u, int token) {
+  if (kDecode) return u.k1;
+  return min(u.ctx + (token - u.tok0) + 1, a.cap);
+}
+
+struct Raw {
+  u32x4 k[4], v[4];
+  float ks, vs;
+};
+
+// A row's pages of one kv head, read tile by tile in ascending order.
+struct Source {
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* ks;
+  const float* vs;
+  const int32_t* row;
+  int64_t sp, ssp;
+  int pid, pwin;          // lane j: page of logical page pwin + j
+  int log2p, ppr, n_pages;
+  int koff, voff;         // of the lane within a tile
+};
+
+__device__ __forceinline__ void load_pids(Source& s, int win) {
+  const int j = min(win + (int)(threadIdx.x & 63), s.ppr - 1);
+  s.pid = min(max(s.row[j], 0), s.n_pages - 1);
+  s.pwin = win;
+}
+
+__device__ __forceinline__ u32x4 load_nt(const uint8_t* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+}
+
+template <bool kNt>
+__device__ __forceinline__ void load_tile(Raw& r, Source& s, int slot0) {
+  const int lp = slot0 >> s.log2p;
+  if (lp - s.pwin >= 64) load_pids(s, lp);
+  const int page = __builtin_amdgcn_readlane(s.pid, lp - s.pwin);
+  const int in_page = slot0 & ((1 << s.log2p) - 1);
+  const uint8_t* k = s.k + page * s.sp + in_page * kD;
+  const uint8_t* v = s.v + page * s.sp + in_page * kD;
+  const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r.k[i] = kNt ? load_nt(k + s.koff + i * 4 * kD) : *reinterpret_cast<const u32x4*>(k + s.koff + i * 4 * kD);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r.v[i] = kNt ? load_nt(v + s.voff + i * 16 * kTile) : *reinterpret_cast<const u32x4*>(v + s.voff + i * 16 * kTile);
+  r.ks = s.ks[page * s.ssp + (in_page >> 4) + g];
+  r.vs = s.vs[page * s.ssp + (in_page >> 4) + g];
+}
+
+// The softmax state of kNC blocks of 16 query columns.
+template <int kNC>
+struct State {
+  f16x8 q[kNC][2];      // dims 16 g + 8 h ..
+  int lim[kNC];
+  int seen;             // every column sees [0, seen)
+  float m[kNC];         // log2 units
+  f32x4 l[kNC];
+  f32x4 o[kNC][4];
+};
+
+template <int kNC, bool kDecode>
+__device__ __forceinline__ void load_queries(State<kNC>& s, const AttnArgs& a, const Unit& u) {
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  int least = 0x7fffffff;
+#pragma unroll
+  for (int b = 0; b < kNC; ++b) {
+    const int r = u.r0 + 16 * b + col;
+    const int rr = min(r, u.rows - 1);
+    const int token = u.tok0 + rr / a.G, h = rr % a.G;
+    const f16* qp = a.q + token * a.q_st + u.hk * a.q_sh + h * a.q_sg + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) s.q[b][i] = load16(qp + 8 * i);
+    if (!kDecode && a.cos != nullptr) {
+      // The other half of the rotated pairs is the lane's 32 away.
+      const f16* other = qp + (g < 2 ? 32 : -32);
+      const int64_t co = token * a.cs_sn + 16 * (g & 1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f16x8 x = g < 2 ? s.q[b][i] : load16(other + 8 * i);
+        f16x8 y = g < 2 ? load16(other + 8 * i) : s.q[b][i];
+        rope_pair(x, y, load16(a.cos + co + 8 * i), load16(a.sin + co + 8 * i),
+                  load16(a.cos + co + 8 * i + 32), load16(a.sin + co + 8 * i + 32));
+        s.q[b][i] = g < 2 ? x : y;
+      }
+    }
+    s.lim[b] = r < u.rows ? min(row_limit<kDecode>(a, u, token), u.k1) : u.k1;
+    least = min(least, s.lim[b]);
+    s.m[b] = kNegInf;
+    s.l[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) s.o[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (kDecode) {
+    s.seen = u.k1;
+  } else {
+    for (int d = 8; d > 0; d >>= 1) least = min(least, __shfl_xor(least, d));
+    s.seen = __builtin_amdgcn_readfirstlane(least);
+  }
+}
+
+// Scores, online softmax and PV product of the tile at key0.  `next` loads what
+// comes after it, once the tile's codes are in fp16.
+template <bool kE4m3, int kNC, typename Next>
+__device__ __forceinline__ void tile_step(State<kNC>& s, Raw& r, int key0, int k1, float scale_log2,
+                                          Next&& next) {
+  const int g = (threadIdx.x & 63) >> 4;
+  const bool masked = key0 + kTile > s.seen;
+  float vs = r.vs;
+  const float ks2 = r.ks * scale_log2;
+  if (key0 + kTile > k1) {
+    // Slots behind the last one may hold anything: their values become zeros.
+    const int have = k1 - key0 - 16 * g;  // of the lane's 16
+    if (have <= 0) vs = 1.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = min(max(have - 4 * i, 0), 4);
+      const unsigned keep = n == 4 ? ~0u : (1u << (8 * n)) - 1u;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) r.v[t][i] &= keep;
+    }
+  }
+  // A block that reads as NaN: zeros here, and NaN probabilities for who sees it.
+  const bool bad = !(vs == vs);
+  if (bad) vs = 0.f;
+  f16x8 k[4][2], v[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) k[i][h] = codes8<kE4m3>(r.k[i][2 * h], r.k[i][2 * h + 1], 1.f);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) v[t][h] = values8<kE4m3>(r.v[t][2 * h], r.v[t][2 * h + 1], vs);
+  next();
+  const f16x8 ones = {(f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f};
+#pragma unroll
+  for (int b = 0; b < kNC; ++b) {
+    f32x4 sc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc[i] = mfma16x16x32(k[i][0], s.q[b][0], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc[i] = mfma16x16x32(k[i][1], s.q[b][1], sc[i]);
+    float f = ks2;
+    const int left = s.lim[b] - key0 - 16 * g;
+    if (masked) {
+      if (left <= 0) f = 1.f;   // whatever scale an unseen block has
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i >= left) sc[i / 4][i % 4] = kNegInf;
+    }
+    const float mx = max16(sc) * f;
+    if (__any(mx > s.m[b] + kRescaleSlack)) {
+      const float top = col_max(mx);
+      const float m_new = top > s.m[b] + kRescaleSlack ? top : s.m[b];
+      const float c = m_new == s.m[b] ? 1.f : fast_exp2(s.m[b] - m_new);
+      s.l[b] *= c;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) s.o[b][t] *= c;
+      s.m[b] = m_new;
+    }
+    const float neg_m = s.m[b] == kNegInf ? 0.f : -s.m[b];
+    f16x8 p[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        p[u][e] = (f16)fast_exp2(__builtin_fmaf(sc[2 * u + e / 4][e % 4], f, neg_m));
+    if (__any(bad && left > 0)) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (bad && left > 0) p[u][e] = (f16)__builtin_nanf("");
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      // The sum adds the rounded p, so that the weights add to one.
+      s.l[b] = mfma16x16x32(ones, p[u], s.l[b]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) s.o[b][t] = mfma16x16x32(v[t][u], p[u], s.o[b][t]);
+    }
+  }
+}
+
+__device__ __forceinline__ void store_out(const AttnArgs& a, int token, int hk, int g, int d, f32x4 o,
+                                          float l, bool sees) {
+  const float inv = sees ? 1.f / l : 0.f;
+  const f16x4 r = {(f16)(o[0] * inv), (f16)(o[1] * inv), (f16)(o[2] * inv), (f16)(o[3] * inv)};
+  *reinterpret_cast<f16x4*>(a.out + token * a.o_st + hk * a.o_sh + g * a.o_sg + d) = r;
+}
+
+__device__ __forceinline__ int64_t part_index(const AttnArgs& a, const Unit& u, int token, int g) {
+  return (((int64_t)token * a.p.kvh + u.hk) * a.splits + u.split) * a.G + g;
+}
+
+// A unit without a slot.
+__device__ __forceinline__ void empty_unit(const AttnArgs& a, const Unit& u, int n_rows) {
+  if (a.splits > 1 && !a.fill) return;
+  for (int i = threadIdx.x; i < n_rows * 16; i += blockDim.x) {
+    const int r = u.r0 + (i >> 4), d = 4 * (i & 15);
+    if (r >= u.rows) break;
+    const int token = u.tok0 + r / a.G, g = r % a.G;
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    if (a.splits == 1 && !a.fill) {
+      store_out(a, token, u.hk, g, d, zero, 0.f, false);
+    } else {
+      const int64_t p = part_index(a, u, token, g);
+      *reinterpret_cast<f32x4*>(a.acc + p * kD + d) = zero;
+      if (d == 0) {
+        a.m[p] = kNegInf;
+        a.l[p] = 0.f;
+      }
+    }
+  }
+}
+
+template <bool kE4m3, int kNC, bool kDecode>
+__device__ __forceinline__ void run_unit(const AttnArgs& a, const Unit& u, f32x4* lds) {
+  if (u.k1 <= u.k0) {
+    empty_unit(a, u, 16 * kNC);
+    return;
+  }
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int n = (u.k1 - u.k0 + kTile - 1) / kTile;
+  Source src;
+  src.k = a.p.k + u.hk * a.p.sh;
+  src.v = a.p.v + u.hk * a.p.sh;
+  src.ks = a.p.ks + u.hk * a.p.ssh;
+  src.vs = a.p.vs + u.hk * a.p.ssh;
+  src.row = a.p.table + u.row * a.p.t_sb;
+  src.sp = a.p.sp;
+  src.ssp = a.p.ssp;
+  src.log2p = a.p.log2p; src.ppr = a.p.ppr; src.n_pages = a.p.n_pages;
+  src.koff = (16 * (col >> 2) + (col & 3)) * kD + 16 * g;
+  src.voff = col * kTile + 16 * g;
+  Raw r;
+  if (w < n) {
+    load_pids(src, (u.k0 + w * kTile) >> a.p.log2p);
+    load_tile<kDecode>(r, src, u.k0 + w * kTile);
+  }
+  State<kNC> s;
+  load_queries<kNC, kDecode>(s, a, u);
+  for (int i = w; i < n; i += nw) {
+    tile_step<kE4m3, kNC>(s, r, u.k0 + i * kTile, u.k1, a.scale_log2, [&] {
+      if (i + nw < n) load_tile<kDecode>(r, src, u.k0 + (i + nw) * kTile);
+    });
+  }
+  // The waves' states, a block of columns at a time.
+  f32x4* so = lds;                                          // [wave][d tile][lane]
+  float2* sml = reinterpret_cast<float2*>(lds + nw * 256);  // [wave][column]
+#pragma unroll
+  for (int b = 0; b < kNC; ++b) {
+    if (b > 0) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 4; ++t) so[(w * 4 + t) * 64 + lane] = s.o[b][t];
+    if (g == 0) sml[w * 16 + col] = float2{s.m[b], s.l[b][0]};
+    __syncthreads();
+    const int rr = u.r0 + 16 * b + col;
+    const int t = w;   // dims 16 t ..
+    if (w < 4 && rr < u.rows) {
+      float top = kNegInf;
+      for (int i = 0; i < nw; ++i) top = fmaxf(top, sml[i * 16 + col].x);
+      float sum = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < nw; ++i) {
+        const float2 x = sml[i * 16 + col];
+        const float c = x.x == top ? 1.f : fast_exp2(x.x - top);
+        sum += x.y * c;
+        o += so[(i * 4 + t) * 64 + lane] * c;
+      }
+      const int token = u.tok0 + rr / a.G, h = rr % a.G;
+      if (a.splits == 1 && !a.fill) {
+        store_out(a, token, u.hk, h, 16 * t + 4 * g, o, sum, true);
+      } else {
+        const int64_t p = part_index(a, u, token, h);
+        *reinterpret_cast<f32x4*>(a.acc + p * kD + 16 * t + 4 * g) = o;
+        if (t == 0 && g == 0) {
+          a.m[p] = top * a.m_unit;
+          a.l[p] = sum;
+        }
+      }
+    }
+  }
+}
+
+template <bool kE4m3>
+__global__ __launch_bounds__(1024) void decode_kernel(AttnArgs a) {
+  extern __shared__ f32x4 lds[];
+  Unit u;
+  int id = blockIdx.x;
+  u.split = id % a.splits;
+  id /= a.splits;
+  u.hk = id % a.p.kvh;
+  u.row = u.tok0 = id / a.p.kvh;
+  u.rows = a.G;
+  u.r0 = 0;
+  u.ctx = -1;
+  const int end = clampi(a.last[u.row * a.last_sb], -1, a.cap - 1) + 1;
+  cut(end, u.split, a.splits, u.k0, u.k1);
+  run_unit<kE4m3, 1, true>(a, u, lds);
+}
+
+template <bool kE4m3, int kNC>
+__global__ __launch_bounds__(256, 2) void extend_kernel(AttnArgs a) {
+  extern __shared__ f32x4 lds[];
+  // Query tiles that read the same slots share an XCD (workgroups go to the XCDs in
+  // turn) and its L2, where there are XCDs enough.
+  const int groups = a.B * a.p.kvh * a.splits;
+  int id = blockIdx.x;
+  if (groups >= 8) id = (id / (8 * a.n_tiles) * 8 + id % 8) * a.n_tiles + id / 8 % a.n_tiles;
+  Unit u;
+  const int tile = id % a.n_tiles;
+  id /= a.n_tiles;
+  if (id >= groups) return;
+  u.split = id % a.splits;
+  id /= a.splits;
+  u.hk = id % a.p.kvh;
+  u.row = id / a.p.kvh;
+  const int lo = clampi(a.cu[u.row], 0, a.tokens), hi = clampi(a.cu[u.row + 1], lo, a.tokens);
+  u.tok0 = lo;
+  u.rows = (hi - lo) * a.G;
+  u.r0 = tile * 16 * kNC;
+  if (u.r0 >= u.rows) return;
+  u.ctx = clampi(a.last[u.row * a.last_sb], -1, a.cap);
+  // All tiles of a row are cut alike; a tile stops where its newest token does.
+  const int end = u.ctx < 0 ? 0 : min(u.ctx + hi - lo, a.cap);
+  cut(end, u.split, a.splits, u.k0, u.k1);
+  if (u.ctx >= 0) {
+    const int newest = (min(u.r0 + 16 * kNC, u.rows) - 1) / a.G;
+    u.k1 = min(u.k1, min(u.ctx + newest + 1, a.cap));
+  }
+  run_unit<kE4m3, kNC, false>(a, u, lds);
+}
+
+// Joins the partials of each (token, kv head, query head).  kSubs groups of 16 lanes,
+// a lane for 4 dims, share a query.
+template <int kSubs, bool kDecode>
+__global__ __launch_bounds__(256) void merge_kernel(AttnArgs a) {
+  constexpr int kLanes = 16 * kSubs;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t id = (int64_t)blockIdx.x * (256 / kLanes) + tid / kLanes;
+  const bool in = id < (int64_t)a.tokens * a.p.kvh * a.G;
+  const int64_t id0 = in ? id : 0;
+  const int g = (int)(id0 % a.G);
+  const int64_t th = id0 / a.G;
+  const int hk = (int)(th % a.p.kvh), token = (int)(th / a.p.kvh);
+  int end, lim;
+  bool mine = in;
+  if (kDecode) {
+    end = lim = clampi(a.last[token * a.last_sb], -1, a.cap - 1) + 1;
+  } else {
+    // The token's row: the last one that starts at or before it.
+    int lo = 0, hi = a.B;
+    while (lo + 1 < hi) {
+      const int mid = (lo + hi) / 2;
+      if (a.cu[mid] <= token) lo = mid;
+      else hi = mid;
+    }
+    const int t0 = clampi(a.cu[lo], 0, a.tokens), t1 = clampi(a.cu[lo + 1], t0, a.tokens);
+    mine = mine && token >= t0 && token < t1;
+    const int ctx = clampi(a.last[lo * a.last_sb], -1, a.cap);
+    end = ctx < 0 ? 0 : min(ctx + t1 - t0, a.cap);
+    lim = ctx < 0 ? 0 : min(ctx + token - t0 + 1, a.cap);
+  }
+  int n = 0;   // splits that hold a slot below lim
+  if (lim > 0) {
+    const int len = ((end + kTile - 1) / kTile + a.splits - 1) / a.splits * kTile;
+    n = (lim + len - 1) / len;
+  }
+  const int64_t p0 = th * a.splits * a.G + g;
+  float top = kNegInf;
+  for (int j = lane & (kLanes - 1); j < n; j += kLanes) top = fmaxf(top, a.m[p0 + (int64_t)j * a.G]);
+  for (int d = kLanes / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const int sub = (tid >> 4) & (kSubs - 1), d0 = 4 * (lane & 15);
+  float sum = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int j = sub; j < n; j += kSubs) {
+    const int64_t p = p0 + (int64_t)j * a.G;
+    const float m = a.m[p], l = a.l[p];
+    const f32x4 x = *reinterpret_cast<const f32x4*>(a.acc + p * kD + d0);
+    const float c = m == top ? 1.f : fast_exp2(m - top);
+    sum += l * c;
+    o += x * c;
+  }
+  if constexpr (kSubs > 1) {
+    sum = col_sum(sum);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = col_sum(o[c]);
+  }
+  if (mine && (kSubs == 1 || lane < 16)) store_out(a, token, hk, g, d0, o, sum, lim > 0);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+
+constexpr int kCus = 256;
+
+int64_t part_bytes(int64_t queries, int n) { return n <= 1 ? 0 : queries * n * (kD + 2) * 4; }
+
+struct Plan {
+  int waves, splits, cols, n_tiles;
+};
+
+Plan decode_plan(int B, int KVH, int cap) {
+  const int64_t pairs = (int64_t)B * KVH, tiles = (cap + kTile - 1) / kTile;
+  Plan p = {4, 1, 1, 1};
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, (tiles + p.waves - 1) / p.waves, 2 * kCus / pairs}));
+  return p;
+}
+
+Plan extend_plan(int B, int KVH, int G, int total, int max_seqlen, int cap) {
+  Plan p = {4, 1, 1, 1};
+  const int64_t rows = (int64_t)max_seqlen * G;
+  p.cols = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.n_tiles = (int)((rows + 16 * p.cols - 1) / (16 * p.cols));
+  const int64_t units = (int64_t)KVH * std::min<int64_t>((int64_t)B * p.n_tiles, (int64_t)total * G / (16 * p.cols) + B);
+  const int64_t tiles = (cap + kTile - 1) / kTile;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, (tiles + p.waves - 1) / p.waves, 2 * kCus / units}));
+  return p;
+}
+
+size_t lds_bytes(int waves) { return waves * (256 * sizeof(f32x4) + 16 * sizeof(float2)); }
+
+template <bool kDecode>
+int launch_merge(const AttnArgs& a, hipStream_t st) {
+  const int64_t queries = (int64_t)a.tokens * a.p.kvh * a.G;
+  if (a.splits <= 8)
+    hipLaunchKernelGGL((merge_kernel<1, kDecode>), dim3((unsigned)((queries + 15) / 16)), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((merge_kernel<4, kDecode>), dim3((unsigned)((queries + 3) / 4)), dim3(256), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+int launch_decode(const AttnArgs& a, int code, int waves, hipStream_t st) {
+  const int64_t grid = (int64_t)a.B * a.p.kvh * a.splits;
+  if (grid > 0x7fffffff) return QF_ERR_UNSUPPORTED;
+  const dim3 g((unsigned)grid), b(64 * waves);
+  if (code == QF_CODE_E4M3) hipLaunchKernelGGL(decode_kernel<true>, g, b, lds_bytes(waves), st, a);
+  else hipLaunchKernelGGL(decode_kernel<false>, g, b, lds_bytes(waves), st, a);
+  return (int)hipGetLastError();
+}
+
+template <int kNC>
+int launch_extend(const AttnArgs& a, int code, int waves, hipStream_t st) {
+  const int64_t grid = (((int64_t)a.B * a.p.kvh * a.splits + 7) & ~(int64_t)7) * a.n_tiles;
+  if (grid > 0x7fffffff) return QF_ERR_UNSUPPORTED;
+  const dim3 g((unsigned)grid), b(64 * waves);
+  if (code == QF_CODE_E4M3) hipLaunchKernelGGL((extend_kernel<true, kNC>), g, b, lds_bytes(waves), st, a);
+  else hipLaunchKernelGGL((extend_kernel<false, kNC>), g, b, lds_bytes(waves), st, a);
+  return (int)hipGetLastError();
+}
+
+// Checks and fills what the entry points share.
+int fill_args(AttnArgs& a, const void* q, const QfPool8* pool, const int64_t* last, int64_t last_sb,
+              int B, int tokens, int G, int D, int cap, float scale) {
+  if (D != kD || G < 1 || G > 16) return QF_ERR_UNSUPPORTED;
+  a = AttnArgs{};
+  const int rc = make_pool(pool, a.p);
+  if (rc != QF_OK) return rc;
+  if (!q || !last || B < 1 || tokens < 1 || cap < 1 || cap > pool->pages_per_row * pool->page_size ||
+      pool->layers != 1 || !(scale > 0.f) || !(scale < 1e30f))
+    return QF_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(q) & 15u) != 0) return QF_ERR_INVALID_ARG;
+  if (B > 0x3fffffff || (int64_t)tokens * G > 0x3fffffff || (int64_t)tokens * a.p.kvh * G > 0x7fffffff ||
+      (int64_t)cap + tokens > 0x7fffffff - kTile)
+    return QF_ERR_UNSUPPORTED;
+  a.q = static_cast<const f16*>(q);
+  a.last = last;
+  a.last_sb = last_sb;
+  a.B = B; a.tokens = tokens; a.G = G; a.cap = cap;
+  a.scale_log2 = scale * kLog2e;
+  a.m_unit = 1.f;
+  return QF_OK;
+}
+
+bool bad_out(const void* out, int64_t st, int64_t sh, int64_t sg) {
+  return !out || (reinterpret_cast<uintptr_t>(out) & 7u) != 0 || ((st | sh | sg) & 3) != 0;
+}
+
+int set_parts(AttnArgs& a, void* ws, int64_t ws_bytes) {
+  if (a.splits <= 1) return QF_OK;
+  const int64_t queries = (int64_t)a.tokens * a.p.kvh * a.G;
+  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u) != 0) return QF_ERR_INVALID_ARG;
+  if (ws_bytes < part_bytes(queries, a.splits)) return QF_ERR_SCRATCH_LIMIT;
+  a.acc = static_cast<float*>(ws);
+  a.m = a.acc + queries * a.splits * kD;
+  a.l = a.m + queries * a.splits;
+  return QF_OK;
+}
+
+}  // namespace kv8
+}  // namespace qf
+
+extern "C" int64_t qf_decode_attn_paged8_workspace(int B, int KVH, int G, int cap) {
+  using namespace qf::kv8;
+  if (B < 1 || KVH < 1 || cap < 1) return QF_ERR_INVALID_ARG;
+  if (G < 1 || G > 16 || (int64_t)B * KVH * G > 0x7fffffff) return QF_ERR_UNSUPPORTED;
+  return part_bytes((int64_t)B * KVH * G, decode_plan(B, KVH, cap).splits);
+}
+
+extern "C" int qf_decode_attn_paged8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sg,
+                                     const QfPool8* pool, const int64_t* kv_last, int64_t kv_last_sb,
+                                     void* ws, int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh,
+                                     int64_t o_sg, int B, int G, int D, float scale, void* stream) {
+  using namespace qf;
+  using namespace qf::kv8;
+  AttnArgs a;
+  const int cap = pool ? pool->pages_per_row * pool->page_size : 0;
+  int rc = fill_args(a, q, pool, kv_last, kv_last_sb, B, B, G, D, cap, scale);
+  if (rc != QF_OK) return rc;
+  if (((q_sb | q_sh | q_sg) & 7) != 0 || bad_out(out, o_sb, o_sh, o_sg)) return QF_ERR_INVALID_ARG;
+  a.q_st = q_sb; a.q_sh = q_sh; a.q_sg = q_sg;
+  a.out = static_cast<f16*>(out);
+  a.o_st = o_sb; a.o_sh = o_sh; a.o_sg = o_sg;
+  const Plan p = decode_plan(B, pool->KVH, cap);
+  a.splits = p.splits;
+  rc = set_parts(a, ws, ws_bytes);
+  if (rc != QF_OK) return rc;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  rc = launch_decode(a, pool->code, p.waves, st);
+  return rc == 0 && a.splits > 1 ? launch_merge<true>(a, st) : rc;
+}
+
+extern "C" int qf_decode_split_paged8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sg,
+                                      const QfPool8* pool, const int64_t* kv_last, int64_t kv_last_sb,
+                                      float* acc, float* m, float* l, int splits, int B, int G, int D,
+                                      float scale, void* stream) {
+  using namespace qf;
+  using namespace qf::kv8;
+  AttnArgs a;
+  const int cap = pool ? pool->pages_per_row * pool->page_size : 0;
+  const int rc = fill_args(a, q, pool, kv_last, kv_last_sb, B, B, G, D, cap, scale);
+  if (rc != QF_OK) return rc;
+  if (((q_sb | q_sh | q_sg) & 7) != 0 || !acc || (reinterpret_cast<uintptr_t>(acc) & 15u) != 0 || !m ||
+      !l || splits < 1 || splits > 1024)
+    return QF_ERR_INVALID_ARG;
+  a.q_st = q_sb; a.q_sh = q_sh; a.q_sg = q_sg;
+  a.acc = acc;
+  a.m = m;
+  a.l = l;
+  a.m_unit = kLn2;
+  a.fill = 1;
+  a.splits = splits;
+  return launch_decode(a, pool->code, 4, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int64_t qf_prefill_extend_paged8_workspace(int B, int QH, int KVH, int total, int max_seqlen,
+                                                      int cap) {
+  using namespace qf::kv8;
+  if (B < 1 || KVH < 1 || QH < KVH || QH % KVH != 0 || total < 1 || max_seqlen < 1 || cap < 1)
+    return QF_ERR_INVALID_ARG;
+  if (QH / KVH > 16 || (int64_t)total * QH > 0x7fffffff || B > 0x3fffffff) return QF_ERR_UNSUPPORTED;
+  return part_bytes((int64_t)total * QH, extend_plan(B, KVH, QH / KVH, total, max_seqlen, cap).splits);
+}
+
+extern "C" int qf_prefill_extend_paged8(
+    const void* q, int64_t q_sh, int64_t q_sn, const void* k, int64_t k_sh, int64_t k_sn, const void* v,
+    int64_t v_sh, int64_t v_sn, const int32_t* cu_seqlens, int total, int max_seqlen,
+    const int64_t* context, int64_t ctx_sb, const void* cos, const void* sin, int64_t cs_sn,
+    const QfPool8* pool, int cap, void* ws, int64_t ws_bytes, void* out, int64_t o_sh, int64_t o_sn,
+    int B, int QH, int D, float scale, void* stream) {
+  using namespace qf;
+  using namespace qf::kv8;
+  if (!pool || pool->KVH < 1 || QH < pool->KVH || QH % pool->KVH != 0) return QF_ERR_INVALID_ARG;
+  const int G = QH / pool->KVH;
+  AttnArgs a;
+  int rc = fill_args(a, q, pool, context, ctx_sb, B, total, G, D, cap, scale);
+  if (rc != QF_OK) return rc;
+  if (!cu_seqlens || max_seqlen < 1 || max_seqlen > total || ((q_sh | q_sn) & 7) != 0 ||
+      bad_out(out, o_sn, o_sh, 0))
+    return QF_ERR_INVALID_ARG;
+  a.q_st = q_sn; a.q_sh = G * q_sh; a.q_sg = q_sh;
+  a.out = static_cast<f16*>(out);
+  a.o_st = o_sn; a.o_sh = G * o_sh; a.o_sg = o_sh;
+  a.cu = cu_seqlens;
+  a.cos = static_cast<const f16*>(cos);
+  a.sin = static_cast<const f16*>(sin);
+  a.cs_sn = cs_sn;
+  const Plan p = extend_plan(B, pool->KVH, G, total, max_seqlen, cap);
+  a.splits = p.splits;
+  a.n_tiles = p.n_tiles;
+  rc = set_parts(a, ws, ws_bytes);
+  if (rc != QF_OK) return rc;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  rc = append(k, 0, k_sh, k_sn, v, 0, v_sh, v_sn, cu_seqlens, total, max_seqlen, context, ctx_sb, cos, sin,
+              cs_sn, pool, cap, B, D, st);
+  if (rc != QF_OK) return rc;
+  if (p.cols == 1) rc = launch_extend<1>(a, pool->code, p.waves, st);
+  else if (p.cols == 2) rc = launch_extend<2>(a, pool->code, p.waves, st);
+  else rc = launch_extend<4>(a, pool->code, p.waves, st);
+  return rc == 0 && a.splits > 1 ? launch_merge<false>(a, st) : rc;
+}

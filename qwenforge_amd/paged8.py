@@ -19,6 +19,10 @@ where a few channels are far larger than the others.
 * ``PagedKv8Cache`` -- ``paged.PagedKvCache`` over such pools.
 * ``append_paged8`` -- new tokens quantised into their pages, with RoPE if asked.
 * ``read_paged8`` -- slots of rows back in fp16.
+* ``flash_decode_attention_paged8`` / ``flash_decode_split_paged8`` -- attention of
+  single tokens (SE:834-874 semantics).
+* ``prefill_extend_paged8`` -- new tokens appended and attended with the slots before
+  them.
 * ``copy_pages8`` -- pages of every layer copied to other pages in one launch.
 """
 
@@ -27,8 +31,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib, paged
-from .ops import HEAD_DIM, _ptr
-from .paged import _call, _check_page_size, _check_rows, _half, _int_rows, _page_list
+from .ops import HEAD_DIM, _ptr, _scratch_args
+from .paged import _call, _check_page_size, _check_rows, _half, _int_rows, _page_list, _workspace
 
 BLOCK = 16
 CODES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
@@ -261,3 +265,105 @@ def copy_pages8(store: torch.Tensor, src, dst) -> None:
         src, dst = torch.tensor([a, b], dtype=torch.int32).to(store.device)
     _call("qf_copy_pages8", index, store.data_ptr(), layers, n_pages * size, size, size, src.data_ptr(),
           dst.data_ptr(), n, n_pages)
+
+
+# --------------------------------------------------------------------------
+# attention
+# --------------------------------------------------------------------------
+
+def _decode_args(grouped, pools, block_table, kv_last):
+    _half("grouped", grouped, 4)
+    b, kvh, _, _ = grouped.shape
+    index = grouped.get_device()
+    pool, cap = _pools8(pools, block_table, b, index)
+    if pool.KVH != kvh:
+        raise ValueError(f"pools hold {pool.KVH} kv heads, grouped {kvh}")
+    return index, pool, cap, _int_rows("kv_last", kv_last, b, torch.int64, index)
+
+
+def flash_decode_attention_paged8(grouped: torch.Tensor, pools, block_table: torch.Tensor,
+                                  kv_last: torch.Tensor, scale: float | None = None,
+                                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention of a batch over pages held in 8 bits.
+
+    grouped (B, KVH, G, 64) fp16, G at most 16; ``pools`` one layer's; block_table (B,
+    pages_per_row) int32; ``kv_last`` (B,) int64 is each row's last slot, read on the
+    device, and a row with a negative one (parked) gets zeros.  ``scale`` defaults to
+    64 ** -0.5.  Returns (B, KVH, G, 64), written to ``out`` if given.  A row's result
+    does not depend on the other rows.
+    """
+    index, pool, cap, last_sb = _decode_args(grouped, pools, block_table, kv_last)
+    b, kvh, g, d = grouped.shape
+    if out is None:
+        out = (torch.empty_like(grouped) if grouped.is_contiguous()
+               else torch.empty((b, kvh, g, d), device=grouped.device, dtype=torch.float16))
+    else:
+        _half("out", out, 4)
+        if out.shape != grouped.shape or out.get_device() != index:
+            raise ValueError(f"out must be {tuple(grouped.shape)} on {grouped.device}")
+    need = _lib.load().qf_decode_attn_paged8_workspace(b, kvh, g, cap)
+    ws = None if need == 0 else _workspace(need, "qf_decode_attn_paged8_workspace", grouped.device)
+    _call("qf_decode_attn_paged8", index, grouped.data_ptr(), *grouped.stride()[:3], pool, kv_last.data_ptr(),
+          last_sb, _ptr(ws), max(need, 0), out.data_ptr(), *out.stride()[:3], b, g, d,
+          d ** -0.5 if scale is None else scale)
+    return out
+
+
+def flash_decode_split_paged8(grouped: torch.Tensor, pools, block_table: torch.Tensor, flash,
+                              kv_last: torch.Tensor, scale: float | None = None):
+    """The split launch alone: fills ``flash[0:3]`` = (acc, m, l) of
+    ``ops.make_flash_scratch``, for ``ops.flash_decode_combine`` or
+    ``step_ops.attn_merge_o_proj``."""
+    index, pool, cap, last_sb = _decode_args(grouped, pools, block_table, kv_last)
+    acc, m, l, _, _, splits, _, _ = _scratch_args(grouped, cap, None, flash, kv_last)
+    b, _, g, d = grouped.shape
+    _call("qf_decode_split_paged8", index, grouped.data_ptr(), *grouped.stride()[:3], pool, kv_last.data_ptr(),
+          last_sb, acc.data_ptr(), m.data_ptr(), l.data_ptr(), splits, b, g, d,
+          d ** -0.5 if scale is None else scale)
+    return acc, m, l
+
+
+def prefill_extend_paged8(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                          cu_seqlens: torch.Tensor, max_seqlen: int, context: torch.Tensor,
+                          cos: torch.Tensor | None, sin: torch.Tensor | None, pools,
+                          block_table: torch.Tensor, lengths=None, max_slots: int | None = None,
+                          scale: float | None = None) -> torch.Tensor:
+    """New tokens appended to rows that hold slots already, and attended.
+
+    ``append_paged8`` of key and value, then token i of row b, packed query (T, QH,
+    64), attends to slots [0, context[b] + i] as the pages hold them, its own and the
+    call's other tokens among them.  ``cos``/``sin`` rotate query and key.
+    ``max_slots`` bounds every row's context + tokens (default: the table's): the work
+    is split by it, and slots past it are neither written nor read.  A parked row
+    (negative context) gets zeros.  Returns (T, QH, 64).
+    """
+    _half("query", query, 3)
+    _half("key", key, 3)
+    _half("value", value, 3)
+    total, qh, d = query.shape
+    kvh = key.shape[1]
+    if key.shape[0] != total or value.shape != key.shape or kvh < 1 or qh % kvh != 0:
+        raise ValueError("packed extension shapes: query (T, QH, D), key/value (T, KVH, D)")
+    index = query.get_device()
+    if key.get_device() != index or value.get_device() != index:
+        raise ValueError(f"query, key and value must be on one device ({query.device})")
+    b, ctx_sb = _packed(cu_seqlens, total, max_seqlen, context, "context", index, lengths)
+    pool, cap = _pools8(pools, block_table, b, index)
+    if pool.KVH != kvh:
+        raise ValueError(f"pools hold {pool.KVH} kv heads, key {kvh}")
+    if max_slots is not None:
+        if not max_seqlen <= max_slots <= cap:
+            raise ValueError(f"max_slots must be in [{max_seqlen}, {cap}] (got {max_slots})")
+        cap = int(max_slots)
+    elif max_seqlen > cap:
+        raise ValueError(f"max_seqlen exceeds the row capacity {cap}")
+    cos, sin, cs_sn = _rope(cos, sin, total, index)
+    out = torch.empty((total, qh, d), device=query.device, dtype=torch.float16)
+    need = _lib.load().qf_prefill_extend_paged8_workspace(b, qh, kvh, total, max_seqlen, cap)
+    ws = None if need == 0 else _workspace(need, "qf_prefill_extend_paged8_workspace", query.device)
+    qs, ks, vs = query.stride(), key.stride(), value.stride()
+    _call("qf_prefill_extend_paged8", index, query.data_ptr(), qs[1], qs[0], key.data_ptr(), ks[1], ks[0],
+          value.data_ptr(), vs[1], vs[0], cu_seqlens.data_ptr(), total, max_seqlen, context.data_ptr(), ctx_sb,
+          _ptr(cos), _ptr(sin), cs_sn, pool, cap, _ptr(ws), max(need, 0), out.data_ptr(), d, qh * d, b, qh, d,
+          d ** -0.5 if scale is None else scale)
+    return out

@@ -1,0 +1,347 @@
+"""Attention over caches held in 8 bits against the definition in 64 bits, over the
+values that the pages hold.
+
+Tolerance: the output is sum_j w_j v_j with |v| <= V, v exact in fp16.  The kernel rounds
+each p_j to fp16 (half a step, 2^-11) and divides by the sum of the rounded ones, so a
+weight is off by at most 2 * 2^-11 relative and the output by 2 * 2^-11 V; p below
+fp16's normal range (2^-14 of a reference that is at most 2^8 below the row's largest) is
+off by half a step of 2^-24, together at most n * 2^-25 V over a sum of at least 2^-8 --
+2^-17 n V, less than 0.02 * 2^-11 V per 64 slots only where that many lie so low, which
+random scores within +-16 do not do.  The fp16 output adds 2^-11 V.  Scores are fp32 sums
+of 64 products: 64 * 2^-24 * sum |q k| / 8 < 2^-15 for the sizes here, which moves p by as
+much.  In all 3.1 * 2^-11 V with room for the fp32 sums of p and p v.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv8
+from qwenforge_amd import ops, paged8
+from test_paged8_gpu import make_pools, make_table, row_state
+
+pytestmark = pytest.mark.gpu
+TOL = 3.1 * 2.0 ** -11
+D = 64
+
+
+def fill_rows(gen, layer, table, rows, dev, size=1.0):
+    """K and V of the rows' slots appended (random), everything else left as it was."""
+    lens = [max(n, 0) for n in rows]
+    kvh = layer[0].shape[1]
+    if sum(lens) == 0:
+        return
+    x = (torch.randn(sum(lens), 2 * kvh, D, generator=gen) * size).half().to(dev)
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=dev)
+    paged8.append_paged8(x[:, :kvh], x[:, kvh:], cu, max(lens),
+                         torch.zeros(len(lens), dtype=torch.int64, device=dev), None, None, layer, table,
+                         lengths=lens)
+
+
+def values_of(layer, table_row, n):
+    """K and V (n, KVH, 64) in 64 bits of a row's first n slots."""
+    state = row_state(layer, table_row, -(-n // 16) * 16)
+    return [kv8.dense(*s)[:n] for s in state]
+
+
+def check(got, want, v_max, what):
+    off = np.abs(got.cpu().double().numpy() - want).max()
+    assert off <= TOL * v_max, (what, off, TOL * v_max)
+
+
+DECODE = [
+    # rows' slots, kv heads, heads of each, page, pages a row
+    ([1], 1, 1, 64, None),
+    ([64], 2, 7, 64, None),
+    ([65], 2, 7, 64, 40),
+    ([1, 2, 15, 16, 17, 63, 64, 65, 127, 129], 2, 7, 64, None),
+    ([1023, 0, 300, 4097], 2, 7, 64, None),
+    ([5000], 1, 16, 64, 100),
+    ([700, 3, 0, 1500, 200], 8, 2, 128, None),
+    ([2000, 1111], 3, 5, 256, None),
+    ([12345], 2, 8, 4096, None),
+    ([33 * i % 500 for i in range(70)], 1, 4, 64, None),
+]
+
+
+def decode_case(gen, case, code, dev, size=1.0):
+    rows, kvh, g, page, ppr = DECODE[case]
+    ppr = ppr or max(1, -(-max(rows) // page))
+    n_pages = sum(-(-n // page) for n in rows) + 3
+    layer = tuple(t[0] for t in make_pools(gen, n_pages, kvh, page, code, dev))
+    table, host = make_table(gen, rows, page, n_pages, ppr, dev)
+    fill_rows(gen, layer, table, rows, dev, size)
+    q = torch.randn(len(rows), kvh, g, D, generator=gen).half().to(dev)
+    last = torch.tensor([n - 1 for n in rows], dtype=torch.int64, device=dev)
+    return rows, layer, table, host, q, last
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("case", range(len(DECODE)))
+def test_decode(dev, case, code):
+    gen = torch.Generator().manual_seed(200 + case)
+    rows, layer, table, host, q, last = decode_case(gen, case, code, dev)
+    got = paged8.flash_decode_attention_paged8(q, layer, table, last)
+    assert got.shape == q.shape
+    for r, n in enumerate(rows):
+        if n == 0:
+            assert torch.equal(got[r], torch.zeros_like(got[r]))
+            continue
+        k, v = values_of(layer, host[r], n)
+        want = kv8.attend(q[r].reshape(-1, D).cpu().double().numpy(), k, v)
+        check(got[r].reshape(-1, D), want, np.abs(v).max(), (case, r, n))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("splits", [1, 3, 16, 40])
+def test_split_phase_and_the_framework_s_merges(dev, code, splits):
+    """Partials of any split count, merged by the merge of the fp16 caches."""
+    gen = torch.Generator().manual_seed(31)
+    rows, layer, table, host, q, last = decode_case(gen, 3, code, dev)
+    b, kvh, g, _ = q.shape
+    flash = ops.make_flash_scratch(b, kvh, g, table.shape[1] * 64, dev, splits=splits, fused=False)
+    for t in flash[:3]:
+        t.fill_(float("nan"))
+    paged8.flash_decode_split_paged8(q, layer, table, flash, last)
+    got = ops.flash_decode_combine(flash)
+    for r, n in enumerate(rows):
+        k, v = values_of(layer, host[r], n)
+        want = kv8.attend(q[r].reshape(-1, D).cpu().double().numpy(), k, v)
+        check(got[r].reshape(-1, D), want, np.abs(v).max(), (r, n))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_strided_queries_outputs_and_tables(dev, code):
+    gen = torch.Generator().manual_seed(37)
+    rows, layer, table, host, q, last = decode_case(gen, 4, code, dev)
+    want = paged8.flash_decode_attention_paged8(q, layer, table, last, scale=0.3)
+    b, kvh, g, _ = q.shape
+    wide = torch.zeros(b, kvh, g + 2, 2 * D, device=dev, dtype=torch.float16)
+    wide[:, :, 1:1 + g, D:] = q
+    out = torch.full((b, g, kvh, D), 7.0, device=dev, dtype=torch.float16).transpose(1, 2)
+    wide_table = torch.full((b, table.shape[1] + 3), -5, dtype=torch.int32, device=dev)
+    wide_table[:, :table.shape[1]] = table
+    lasts = torch.full((b, 3), 99, dtype=torch.int64, device=dev)
+    lasts[:, 1] = last
+    got = paged8.flash_decode_attention_paged8(wide[:, :, 1:1 + g, D:], layer, wide_table[:, :table.shape[1]],
+                                               lasts[:, 1], scale=0.3, out=out)
+    assert got is out and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_rows_do_not_depend_on_their_company(dev, code):
+    """Nor on a row's place: the same rows in another order, bit for bit."""
+    gen = torch.Generator().manual_seed(41)
+    rows, layer, table, host, q, last = decode_case(gen, 4, code, dev)
+    want = paged8.flash_decode_attention_paged8(q, layer, table, last)
+    order = torch.tensor([3, 1, 0, 2], device=dev)
+    got = paged8.flash_decode_attention_paged8(q[order], layer, table[order].contiguous(), last[order])
+    assert torch.equal(got, want[order])
+    parked = last.clone()
+    parked[0] = parked[3] = -1
+    got = paged8.flash_decode_attention_paged8(q, layer, table, parked)
+    assert torch.equal(got[2], want[2]) and not got[0].any() and not got[3].any()
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_unseen_slots_may_hold_anything(dev, code):
+    """Slots behind the last one: NaN codes, NaN and infinite scales, in its block, tile and page."""
+    for n in (1, 16, 20, 48, 63, 64, 100):
+        gen = torch.Generator().manual_seed(43 + n)
+        layer = tuple(t[0] for t in make_pools(gen, 4, 2, 64, code, dev, junk=False))
+        table, host = make_table(gen, [128], 64, 4, 2, dev)
+        fill_rows(gen, layer, table, [n], dev)
+        q = torch.randn(1, 2, 7, D, generator=gen).half().to(dev)
+        last = torch.tensor([n - 1], device=dev)
+        want = paged8.flash_decode_attention_paged8(q, layer, table, last)
+        for s in range(n, 128):
+            page, off = int(host[0, s // 64]), s % 64
+            layer[0].view(torch.uint8)[page, :, off] = 0x7F
+            layer[1].view(torch.uint8)[page, :, 0, :, off] = 0xFF
+            if s % 16 == 0:
+                for t, x in zip(layer[2:], (float("nan"), float("inf")) if s % 32 else (-float("inf"), float("nan"))):
+                    t[page, :, off // 16] = x
+        assert torch.equal(paged8.flash_decode_attention_paged8(q, layer, table, last), want), n
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_nan_blocks_reach_who_sees_them(dev, code):
+    gen = torch.Generator().manual_seed(47)
+    layer = tuple(t[0] for t in make_pools(gen, 4, 2, 64, code, dev))
+    table, host = make_table(gen, [200], 64, 4, 4, dev)
+    fill_rows(gen, layer, table, [200], dev)
+    q = torch.randn(1, 2, 7, D, generator=gen).half().to(dev)
+    for which in (2, 3):
+        keep = layer[which].clone()
+        layer[which][int(host[0, 2]), 1, 1] = float("nan")            # slots 144 .. 159 of head 1
+        seen = [paged8.flash_decode_attention_paged8(q, layer, table, torch.tensor([n - 1], device=dev))
+                for n in (144, 145, 200)]
+        assert torch.isfinite(seen[0]).all()
+        for x in seen[1:]:
+            assert torch.isnan(x[0, 1]).all() and torch.isfinite(x[0, 0]).all()
+        layer[which].copy_(keep)
+
+
+def test_scores_of_minus_infinity_alone(dev):
+    """An infinite query against keys of the other sign: NaN, as from the fp16 caches."""
+    for code in ("int8", "e4m3"):
+        kv = paged8.PagedKv8Cache(1, 1, 2, 64, 1, 2, dev, code)
+        kv.map_row(0, 100)
+        x = torch.ones(100, 1, D, device=dev, dtype=torch.float16)
+        cu = torch.tensor([0, 100], dtype=torch.int32, device=dev)
+        paged8.append_paged8(-x, x, cu, 100, torch.zeros(1, dtype=torch.int64, device=dev), None, None,
+                             kv.pools[0], kv.table)
+        q = torch.ones(1, 1, 2, D, device=dev, dtype=torch.float16)
+        q[0, 0, 1] = float("inf")
+        got = paged8.flash_decode_attention_paged8(q, kv.pools[0], kv.table, torch.tensor([99], device=dev))
+        assert torch.isnan(got[0, 0, 1]).all() and torch.equal(got[0, 0, 0], x[0, 0])
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_values_of_very_different_sizes(dev, code):
+    """Blocks whose scales lie far apart: a query that looks at the small ones gets them to their own precision."""
+    gen = torch.Generator().manual_seed(53)
+    kv = paged8.PagedKv8Cache(1, 1, 4, 64, 1, 4, dev, code)
+    kv.map_row(0, 256)
+    v = torch.randn(256, 1, D, generator=gen)
+    size = torch.ones(256)
+    size[:64], size[64:128], size[128:192], size[192:] = 6e4 / 5, 1.0, 2.0 ** -10, 2.0 ** -18
+    v = (v.clamp(-5, 5) * size[:, None, None]).half()
+    k = torch.zeros(256, 1, D)
+    for j in range(4):
+        k[64 * j:64 * j + 64, 0, j] = 8.0
+    cu = torch.tensor([0, 256], dtype=torch.int32, device=dev)
+    paged8.append_paged8(k.half().to(dev), v.to(dev), cu, 256, torch.zeros(1, dtype=torch.int64, device=dev), None,
+                         None, kv.pools[0], kv.table)
+    q = torch.zeros(1, 1, 4, D)
+    for j in range(4):
+        q[0, 0, j, j] = 64.0                          # 64 a score: the others' weight is e^-64
+    got = paged8.flash_decode_attention_paged8(q.half().to(dev), kv.pools[0], kv.table,
+                                               torch.tensor([255], device=dev))[0, 0]
+    vals = values_of(kv.pools[0], kv.table[0].cpu(), 256)[1][:, 0]
+    for j in range(4):
+        part = vals[64 * j:64 * j + 64]
+        off = np.abs(got[j].cpu().double().numpy() - part.mean(axis=0))
+        # p are 1; the fp16 output's step below 2^-14 is 2^-24.
+        assert (off <= TOL * np.abs(part).max() + 2.0 ** -25).all(), (j, off.max())
+
+
+EXTEND = [
+    # new tokens, slots before them, kv heads, heads of each, page
+    ([1], [0], 1, 1, 64),
+    ([5, 5], [300, 2011], 2, 7, 64),
+    ([1, 8, 3], [15, 0, 64], 2, 7, 64),
+    ([30], [100], 2, 7, 64),
+    ([0, 17, 4, 2, 1], [5, 3, -1, 1000, 63], 8, 2, 128),
+    ([70, 9, 130], [16, 1031, 0], 2, 7, 64),
+    ([200], [700], 1, 16, 256),
+    ([3] * 9, [100 * i for i in range(9)], 2, 8, 64),
+    ([2], [5000], 1, 4, 64),
+]
+
+
+def extend_case(gen, case, code, dev):
+    lens, ctx, kvh, g, page = EXTEND[case]
+    need = [max(c, 0) + n for n, c in zip(lens, ctx)]
+    n_pages = sum(-(-n // page) for n in need) + 3
+    layer = tuple(t[0] for t in make_pools(gen, n_pages, kvh, page, code, dev))
+    table, host = make_table(gen, need, page, n_pages, max(1, -(-max(need) // page)), dev)
+    fill_rows(gen, layer, table, ctx, dev)
+    total = sum(lens)
+    qkv = torch.randn(total, (g + 2) * kvh, D, generator=gen).half().to(dev)
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=dev)
+    return (lens, ctx, kvh, g, layer, table, host, qkv[:, :g * kvh], qkv[:, g * kvh:(g + 1) * kvh],
+            qkv[:, (g + 1) * kvh:], cu, torch.tensor(ctx, device=dev))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("case", range(len(EXTEND)))
+def test_extend(dev, case, code):
+    gen = torch.Generator().manual_seed(300 + case)
+    lens, ctx, kvh, g, layer, table, host, q, k, v, cu, context = extend_case(gen, case, code, dev)
+    other = tuple(t.clone() for t in layer)
+    most = max(n + c for n, c in zip(lens, ctx))
+    got = paged8.prefill_extend_paged8(q, k, v, cu, max(lens), context, None, None, layer, table, lengths=lens,
+                                       max_slots=most)
+    paged8.append_paged8(k, v, cu, max(lens), context, None, None, other, table, lengths=lens)
+    for a, b in zip(layer, other):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for r, (n, c) in enumerate(zip(lens, ctx)):
+        lo = sum(lens[:r])
+        if c < 0:
+            assert not got[lo:lo + n].any()
+            continue
+        if n == 0:
+            continue
+        kk, vv = values_of(layer, host[r], c + n)
+        for i in range(n):
+            want = kv8.attend(q[lo + i].cpu().double().numpy(), kk[:c + i + 1], vv[:c + i + 1])
+            check(got[lo + i], want, np.abs(vv).max(), (case, r, i))
+    again = paged8.prefill_extend_paged8(q, k, v, cu, max(lens), context, None, None, layer, table)
+    assert torch.equal(again, got) or most < table.shape[1] * layer[0].shape[2]
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_extend_rotates_queries_and_keys(dev, code):
+    gen = torch.Generator().manual_seed(59)
+    lens, ctx, kvh, g, layer, table, host, q, k, v, cu, context = extend_case(gen, 5, code, dev)
+    n = q.shape[0]
+    ang = torch.rand(n, 32, generator=gen) * 6
+    cos, sin = (torch.cat([f(ang), f(ang)], dim=1).half().to(dev) for f in (torch.cos, torch.sin))
+    other = tuple(t.clone() for t in layer)
+    got = paged8.prefill_extend_paged8(q, k, v, cu, max(lens), context, cos, sin, layer, table, lengths=lens)
+
+    def turn(x):
+        cache = torch.zeros(n, kvh, 64, D, device=dev, dtype=torch.float16)
+        y = ops.rope_append(x[:, :, None].contiguous(), k[:, :, None].contiguous(), v[:, :, None].contiguous(),
+                            cos.view(n, 1, D), sin.view(n, 1, D), cache, cache.clone(),
+                            torch.zeros(1, dtype=torch.int64, device=dev))
+        return y[:, :, 0], cache[:, :, 0]
+
+    q2, k2 = turn(q)
+    want = paged8.prefill_extend_paged8(q2, k2, v, cu, max(lens), context, None, None, other, table, lengths=lens)
+    assert torch.equal(got, want)
+    for a, b in zip(layer, other):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_nan_tokens_reach_later_blocks_only(dev, code):
+    """A token that is not finite: its block's queries and the later ones, not those of earlier blocks."""
+    gen = torch.Generator().manual_seed(61)
+    for which in (0, 1):
+        layer = tuple(t[0] for t in make_pools(gen, 3, 1, 64, code, dev))
+        table, host = make_table(gen, [90], 64, 3, 2, dev)
+        fill_rows(gen, layer, table, [20], dev)
+        x = torch.randn(2, 60, 1, D, generator=gen).half()
+        x[which, 17, 0, 3] = float("nan")                              # slot 37, block 32 .. 47
+        k, v = x.to(dev)
+        q = torch.randn(60, 2, D, generator=gen).half().to(dev)
+        cu = torch.tensor([0, 60], dtype=torch.int32, device=dev)
+        got = paged8.prefill_extend_paged8(q, k, v, cu, 60, torch.tensor([20], device=dev), None, None, layer, table)
+        assert torch.isfinite(got[:12]).all() and torch.isnan(got[12:]).all()
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_max_slots_bounds_writes_and_reads(dev, code):
+    gen = torch.Generator().manual_seed(67)
+    layer = tuple(t[0] for t in make_pools(gen, 4, 1, 64, code, dev))
+    table, host = make_table(gen, [200], 64, 4, 4, dev)
+    fill_rows(gen, layer, table, [90], dev)
+    x = torch.randn(30, 4, D, generator=gen).half().to(dev)
+    cu = torch.tensor([0, 30], dtype=torch.int32, device=dev)
+    ctx = torch.tensor([90], device=dev)
+    other = tuple(t.clone() for t in layer)
+    before = row_state(layer, host[0], 128)
+    got = paged8.prefill_extend_paged8(x[:, :2], x[:, 2:3], x[:, 3:], cu, 30, ctx, None, None, layer, table,
+                                       max_slots=100)
+    for which, at in ((0, 2), (1, 3)):
+        values, scales = before[which]
+        kv8.append(values, scales, 90, x[:10, at:at + 1].cpu().double().numpy(), code)
+        after = row_state(layer, host[0], 128)[which]
+        assert np.array_equal(after[0], values) and np.array_equal(after[1], scales)
+    kk, vv = values_of(layer, host[0], 100)
+    for i in (0, 9, 10, 29):
+        n = min(91 + i, 100)
+        want = kv8.attend(x[i, :2].cpu().double().numpy(), kk[:n], vv[:n])
+        check(got[i], want, np.abs(vv).max(), i)
