@@ -47,10 +47,12 @@ extern "C" {
 /* Slots of one scale. */
 #define QF_BLOCK8 16
 
-/* The pools of `layers` layers and the rows' pages (HOST struct, read during the
- * call).  Strides of codes in bytes, of scales in floats, alike for K and V; the
- * codes of one page and head are contiguous, and so are its scales.  Code
- * pointers and strides are multiples of 16. */
+/* Arguments come in HOST structs of 8-byte fields, read during the call: a caller
+ * whose language is slow at passing many arguments packs them into one buffer.
+ *
+ * The pools of `layers` layers and the rows' pages.  Strides of codes in bytes, of
+ * scales in floats, alike for K and V; the codes of one page and head are contiguous,
+ * and so are its scales.  Code pointers and strides are multiples of 16. */
 typedef struct {
   void* k;
   void* v;
@@ -60,45 +62,45 @@ typedef struct {
   int64_t ssl, ssp, ssh;
   const int32_t* table;      /* (rows, pages_per_row), row stride bt_sb */
   int64_t bt_sb;
-  int32_t pages_per_row, n_pages, page_size;
-  int32_t layers, KVH, code;
+  int64_t pages_per_row, n_pages, page_size;
+  int64_t layers, KVH, code;
 } QfPool8;
 
+/* Packed tokens of B rows: row b has tokens [cu_seqlens[b], cu_seqlens[b + 1]) of
+ * `total`, at most max_seqlen, and they are its slots first[b * first_sb] + i. */
+typedef struct {
+  QfPool8 pool;
+  void* k;                   /* (layers, T, KVH, D): strides per layer, head, token */
+  int64_t k_sl, k_sh, k_sn;
+  void* v;
+  int64_t v_sl, v_sh, v_sn;
+  const int32_t* cu_seqlens;
+  int64_t total, max_seqlen;
+  const int64_t* first;
+  int64_t first_sb;
+  const void* cos;           /* (T, D), token stride cs_sn, or both NULL */
+  const void* sin;
+  int64_t cs_sn;
+  int64_t B, D;
+} QfRows8;
+
 /*
- * Quantises new tokens into their pages.  Row b's tokens, [cu_seqlens[b],
- * cu_seqlens[b + 1]) of the packed k and v, go to its slots context[b] + i.
- *
- *   k, v  (layers, T, KVH, D): strides *_sl per layer, *_sn per token, *_sh per
- *         head.  Tokens of no row are not read
- *   context  int64 on the device, row b reads context[b * ctx_sb]; a negative one
- *         appends nothing.  Slots past the row's pages are not written
- *   cos, sin (T, D), token stride cs_sn, or both NULL: rotate-half RoPE of k as in
- *         qf_rope_append, before it is quantised
- *   max_seqlen  the most tokens of a row
+ * Quantises new tokens into their pages.  A row with a negative first slot (parked)
+ * appends nothing; slots past the row's pages are not written; tokens of no row are
+ * not read.  With cos and sin k gets the rotate-half RoPE of qf_rope_append before it
+ * is quantised.
  *
  * Slots of the last block behind the row's last token keep their codes.  No page
  * may be written by two rows of a call.
  */
-int qf_append_paged8(const void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn,
-                     const void* v, int64_t v_sl, int64_t v_sh, int64_t v_sn,
-                     const int32_t* cu_seqlens, int total, int max_seqlen,
-                     const int64_t* context, int64_t ctx_sb,
-                     const void* cos, const void* sin, int64_t cs_sn,
-                     const QfPool8* pool, int B, int D, void* stream);
+int qf_append_paged8(const QfRows8* rows, void* stream);
 
 /*
- * Slots first[b] .. of each row back in fp16, packed: token i of row b is slot
- * first[b] + i.
- *
- *   k, v  (layers, T, KVH, D) as above, written.  Tokens of no row are left as they
- *         were; those of a row with a negative first, and of slots past the row's
- *         pages, become zero
+ * The rows' slots back in fp16: k and v are written (cos and sin NULL).  Tokens of no
+ * row are left as they were; those of a row with a negative first slot, and of slots
+ * past the row's pages, become zero.
  */
-int qf_read_paged8(void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn,
-                   void* v, int64_t v_sl, int64_t v_sh, int64_t v_sn,
-                   const int32_t* cu_seqlens, int total, int max_seqlen,
-                   const int64_t* first, int64_t first_sb,
-                   const QfPool8* pool, int B, int D, void* stream);
+int qf_read_paged8(const QfRows8* rows, void* stream);
 
 /*
  * Copies whole page records within every layer: page dst[i] becomes page src[i].
@@ -112,67 +114,80 @@ int qf_read_paged8(void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn,
 int qf_copy_pages8(void* store, int layers, int64_t layer_step, int64_t step, int64_t bytes,
                    const int32_t* src, const int32_t* dst, int n_pairs, int n_pages, void* stream);
 
+/* Queries of single tokens: q and out (B, KVH, G, D), one layer's pool. */
+typedef struct {
+  QfPool8 pool;
+  const void* q;
+  int64_t q_sb, q_sh, q_sg;
+  const int64_t* kv_last;    /* row b's last slot: kv_last[b * kv_last_sb] */
+  int64_t kv_last_sb;
+  void* out;
+  int64_t o_sb, o_sh, o_sg;
+  void* ws;
+  int64_t ws_bytes;
+  int64_t B, G, D;
+  const void* k_new;         /* (B, KVH, D): strides per row and head; or both NULL */
+  int64_t kn_sb, kn_sh;
+  const void* v_new;
+  int64_t vn_sb, vn_sh;
+  double scale;              /* > 0 */
+} QfDecode8;
+
 /*
  * Decode attention of single tokens: softmax(scale q K^T) V over each row's slots
- * [0, kv_last], as qf_decode_attn_paged without a bias.
+ * [0, kv_last], as qf_decode_attn_paged without a bias.  A row with kv_last < 0
+ * (parked) gets zeros.  With k_new and v_new row b's token is appended at slot
+ * kv_last first, as by qf_append_paged8 (a slot past the row's pages appends nothing).
  *
- *   q, out   (B, KVH, G, D), strides *_sb, *_sh, *_sg
- *   kv_last  int64 on the device, row b reads kv_last[b * kv_last_sb]: its last
- *            slot (inclusive).  A row with kv_last < 0 (parked) gets zeros
- *   pool     of one layer
- *   ws       16-byte aligned scratch of at least qf_decode_attn_paged8_workspace
- *            bytes for these sizes (cap = pages_per_row * page_size; NULL where
- *            that is 0), else QF_ERR_SCRATCH_LIMIT; free again when the call's work
- *            is done, and not to be shared by calls that overlap in time
- *   scale    > 0
+ * ws is 16-byte aligned scratch of at least qf_decode_attn_paged8_workspace bytes for
+ * these sizes (cap = pages_per_row * page_size; NULL where that is 0), else
+ * QF_ERR_SCRATCH_LIMIT; free again when the call's work is done, and not to be shared
+ * by calls that overlap in time.
  *
  * Slots that a row does not see may hold anything.  A block that reads as NaN makes
  * NaN of the rows that see any of it; where every score is -infinity the output is NaN.
  */
 int64_t qf_decode_attn_paged8_workspace(int B, int KVH, int G, int cap);
 
-int qf_decode_attn_paged8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sg,
-                          const QfPool8* pool, const int64_t* kv_last, int64_t kv_last_sb,
-                          void* ws, int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh,
-                          int64_t o_sg, int B, int G, int D, float scale, void* stream);
+int qf_decode_attn_paged8(const QfDecode8* args, void* stream);
 
 /*
- * Its split phase alone: the partials acc (B, KVH, splits, G, D), m and l (B, KVH,
- * splits, G) of qf_decode_split_paged, for qf_decode_combine or qf_attn_merge_o_proj
- * (m in natural units; a range without a slot leaves acc = l = 0 and m = -infinity).
- * acc is 16-byte aligned.
+ * Its split phase alone (out and ws unused): the partials acc (B, KVH, splits, G, D),
+ * m and l (B, KVH, splits, G) of qf_decode_split_paged, for qf_decode_combine or
+ * qf_attn_merge_o_proj (m in natural units; a range without a slot leaves acc = l = 0
+ * and m = -infinity).  acc is 16-byte aligned.
  */
-int qf_decode_split_paged8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sg,
-                           const QfPool8* pool, const int64_t* kv_last, int64_t kv_last_sb,
-                           float* acc, float* m, float* l, int splits, int B, int G, int D,
-                           float scale, void* stream);
+int qf_decode_split_paged8(const QfDecode8* args, float* acc, float* m, float* l, int splits,
+                           void* stream);
+
+/* New tokens with their queries: q and out (T, QH, D), QH a multiple of the pool's KVH. */
+typedef struct {
+  QfRows8 rows;              /* k and v appended at first[b] + i, one layer */
+  const void* q;
+  int64_t q_sh, q_sn;
+  void* out;
+  int64_t o_sh, o_sn;
+  int64_t cap;               /* slots of a row that the call may use */
+  void* ws;
+  int64_t ws_bytes;
+  int64_t QH;
+  double scale;              /* > 0 */
+} QfExtend8;
 
 /*
  * New tokens behind cached ones: qf_append_paged8 of a layer's k and v, then token i of
- * row b attends to slots [0, context[b] + i] of its pages -- all of them as the pages
- * hold them, the new ones too.
+ * row b attends to slots [0, first[b] + i] of its pages -- all of them as the pages
+ * hold them, the new ones too.  cos and sin rotate q as well.
  *
- *   q, out  (T, QH, D), strides *_sh per head, *_sn per token, QH a multiple of the
- *           pool's KVH.  Rows of out for tokens of no row are left as they were; those
- *           of a parked row (context < 0) become zero
- *   cos, sin  as in the append; q is rotated with them too
- *   max_seqlen  the most tokens of a row; further ones get no output
- *   cap     slots of a row that the call may use, at most pages_per_row *
- *           page_size: a bound on every row's context + tokens, from which the
- *           work is split.  Tokens past it are not appended and see the slots below
- *   ws      as above, qf_prefill_extend_paged8_workspace bytes
+ * Rows of out for tokens of no row, and past a row's max_seqlen, are left as they were;
+ * those of a parked row become zero.  cap is at most pages_per_row * page_size, a
+ * bound on every row's first + tokens, from which the work is split; tokens past it
+ * are not appended and see the slots below.  ws as above,
+ * qf_prefill_extend_paged8_workspace bytes.
  */
 int64_t qf_prefill_extend_paged8_workspace(int B, int QH, int KVH, int total, int max_seqlen, int cap);
 
-int qf_prefill_extend_paged8(const void* q, int64_t q_sh, int64_t q_sn,
-                             const void* k, int64_t k_sh, int64_t k_sn,
-                             const void* v, int64_t v_sh, int64_t v_sn,
-                             const int32_t* cu_seqlens, int total, int max_seqlen,
-                             const int64_t* context, int64_t ctx_sb,
-                             const void* cos, const void* sin, int64_t cs_sn,
-                             const QfPool8* pool, int cap, void* ws, int64_t ws_bytes,
-                             void* out, int64_t o_sh, int64_t o_sn,
-                             int B, int QH, int D, float scale, void* stream);
+int qf_prefill_extend_paged8(const QfExtend8* args, void* stream);
 
 #ifdef __cplusplus
 }

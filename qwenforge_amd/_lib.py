@@ -18,16 +18,6 @@ LIB_PATH = Path(__file__).resolve().with_name("_qf_attn.so")
 _i64, _i32, _f32, _vp = C.c_int64, C.c_int, C.c_float, C.c_void_p
 
 
-
-class Pool8(C.Structure):
-    """``QfPool8`` (``include/qf_paged8.h``)."""
-
-    _fields_ = ([(n, _vp) for n in ("k", "v", "k_scale", "v_scale")]
-                + [(n, _i64) for n in ("sl", "sp", "sh", "ssl", "ssp", "ssh")]
-                + [("table", _vp), ("bt_sb", _i64)]
-                + [(n, C.c_int32) for n in ("pages_per_row", "n_pages", "page_size", "layers", "KVH", "code")])
-
-
 # name -> argument types, in header order.  Every entry point returns int.
 SIGNATURES = {
     "qf_decode_attn": [
@@ -334,52 +324,17 @@ SIGNATURES = {
         _i32, _i32, _i32, _vp,          # T, B, V, stream
     ],
     # include/qf_paged8.h
-    "qf_append_paged8": [
-        _vp, _i64, _i64, _i64,          # k, k_sl, k_sh, k_sn
-        _vp, _i64, _i64, _i64,          # v
-        _vp, _i32, _i32,                # cu_seqlens, total, max_seqlen
-        _vp, _i64,                      # context, ctx_sb
-        _vp, _vp, _i64,                 # cos, sin, cs_sn
-        C.POINTER(Pool8), _i32, _i32, _vp,  # pool, B, D, stream
-    ],
-    "qf_read_paged8": [
-        _vp, _i64, _i64, _i64,          # k, k_sl, k_sh, k_sn
-        _vp, _i64, _i64, _i64,          # v
-        _vp, _i32, _i32,                # cu_seqlens, total, max_seqlen
-        _vp, _i64,                      # first, first_sb
-        C.POINTER(Pool8), _i32, _i32, _vp,  # pool, B, D, stream
-    ],
+    "qf_append_paged8": [C.c_char_p, _vp],   # QfRows8, stream
+    "qf_read_paged8": [C.c_char_p, _vp],     # QfRows8, stream
     "qf_copy_pages8": [
         _vp, _i32, _i64, _i64, _i64,    # store, layers, layer_step, step, bytes
         _vp, _vp, _i32, _i32, _vp,      # src, dst, n_pairs, n_pages, stream
     ],
     "qf_decode_attn_paged8_workspace": [_i32, _i32, _i32, _i32],        # B, KVH, G, cap
-    "qf_decode_attn_paged8": [
-        _vp, _i64, _i64, _i64,          # q, q_sb, q_sh, q_sg
-        C.POINTER(Pool8), _vp, _i64,    # pool, kv_last, kv_last_sb
-        _vp, _i64,                      # ws, ws_bytes
-        _vp, _i64, _i64, _i64,          # out, o_sb, o_sh, o_sg
-        _i32, _i32, _i32, _f32, _vp,    # B, G, D, scale, stream
-    ],
-    "qf_decode_split_paged8": [
-        _vp, _i64, _i64, _i64,          # q
-        C.POINTER(Pool8), _vp, _i64,    # pool, kv_last, kv_last_sb
-        _vp, _vp, _vp, _i32,            # acc, m, l, splits
-        _i32, _i32, _i32, _f32, _vp,    # B, G, D, scale, stream
-    ],
+    "qf_decode_attn_paged8": [C.c_char_p, _vp],                         # QfDecode8, stream
+    "qf_decode_split_paged8": [C.c_char_p, _vp, _vp, _vp, _i32, _vp],   # QfDecode8, acc, m, l, splits, stream
     "qf_prefill_extend_paged8_workspace": [_i32, _i32, _i32, _i32, _i32, _i32],  # B, QH, KVH, total, longest, cap
-    "qf_prefill_extend_paged8": [
-        _vp, _i64, _i64,                # q, q_sh, q_sn
-        _vp, _i64, _i64,                # k
-        _vp, _i64, _i64,                # v
-        _vp, _i32, _i32,                # cu_seqlens, total, max_seqlen
-        _vp, _i64,                      # context, ctx_sb
-        _vp, _vp, _i64,                 # cos, sin, cs_sn
-        C.POINTER(Pool8), _i32,         # pool, cap
-        _vp, _i64,                      # ws, ws_bytes
-        _vp, _i64, _i64,                # out, o_sh, o_sn
-        _i32, _i32, _i32, _f32, _vp,    # B, QH, D, scale, stream
-    ],
+    "qf_prefill_extend_paged8": [C.c_char_p, _vp],                      # QfExtend8, stream
     # include/qf_probe.h
     "qf_stream_read": [_vp, _i64, _vp, _i32, _vp],   # src, bytes, sink, workgroups, stream
     "qf_launch_probe": [_vp, _i64, _vp, _vp,          # src, bytes, index, sink

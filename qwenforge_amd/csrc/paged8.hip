@@ -1,18 +1,11 @@
 // Tokens quantised into paged caches held in 8 bits, slots read back, pages copied
 // (gfx950; the format is qf_paged8.h's).
 //
-// A wave takes one block of 16 slots of one kv head, K and V:
-//   scale = max(the scale of the slots already there, 2^e), the least e >= -24 with
-//           max |x| <= Q 2^e (Q = 127 or 448), read off the exponent and mantissa
-//           of the largest magnitude;
-//   code  = rne(x 2^-e), which is exact before the rounding.
-// K goes through it as four lanes a slot, each with the dims [8c, 8c + 8) and
-// [32 + 8c, 40 + 8c) that a rotate-half pair needs; V as a lane a dim, whose 16
-// slots of the block are 16 bytes of the dim-major page.  Four waves are a
-// workgroup, so a page's 64-byte lines of V are written on one CU.
+// A wave takes one block of 16 slots of one kv head, K and V (kv8_block.h).  Four waves
+// are a workgroup, so a page's 64-byte lines of V are written on one CU.
 #include <algorithm>
 
-#include "kv8.h"
+#include "kv8_block.h"
 
 namespace qf {
 namespace kv8 {
@@ -60,8 +53,20 @@ __device__ __forceinline__ void row_tokens(const RowsArgs& a, int r, int& lo, in
   hi = clampi(a.cu[r + 1], lo, a.total);
 }
 
-// The id-th of the blocks that the rows' tokens touch, counted row by row.
+// The id-th of the blocks that the rows' tokens touch, counted row by row.  kSingle: no
+// row has more than one token, and row id has the block.
+template <bool kSingle>
 __device__ __forceinline__ Unit find_unit(const RowsArgs& a, int id) {
+  if constexpr (kSingle) {
+    if (id >= a.B) return {0, 0, 0, 0, 0};
+    int lo, hi;
+    row_tokens(a, id, lo, hi);
+    const int64_t first = a.first[id * a.first_sb];
+    if (first < 0) return {id, lo, min(hi - lo, 1), -1, 0};
+    const int64_t block = first / kBlock;
+    return {id, lo, min(hi - lo, 1), (int)(first % kBlock),
+            (int)(block < 0x7fffffff / kBlock ? block : 0x7fffffff / kBlock)};
+  }
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int i0 = 0; i0 < a.B; i0 += 64) {
@@ -97,182 +102,22 @@ __device__ __forceinline__ Unit find_unit(const RowsArgs& a, int id) {
   return {0, 0, 0, 0, 0};
 }
 
-// The least scale of a block whose largest magnitude has these fp16 bits.
-template <bool kE4m3>
-__device__ __forceinline__ float scale_for(unsigned top) {
-  if (top >= 0x7C00u) return __builtin_nanf("");
-  const unsigned f = __float_as_uint((float)__builtin_bit_cast(f16, (unsigned short)top));
-  // Q = 1.984375 * 2^6 or 1.75 * 2^8.
-  const int e = (int)(f >> 23) - 127 - (kE4m3 ? 8 : 6) +
-                ((f & 0x7FFFFFu) > (kE4m3 ? 0x600000u : 0x7E0000u) ? 1 : 0);
-  return __uint_as_float((unsigned)(max(e, kMinExp) + 127) << 23);
-}
-
-// Largest magnitude at scale s whose value fp16 holds: 65504 / s rounded down to a
-// code.  It is below Q where the scale is the largest there is alone.
-template <bool kE4m3>
-__device__ __forceinline__ float code_top(float s) {
-  if (kE4m3) return s >= 256.f ? 240.f : 448.f;
-  return s >= 1024.f ? 63.f : 127.f;
-}
-
-// Four codes of y[0..3] = x / scale.
-template <bool kE4m3>
-__device__ __forceinline__ unsigned encode4(const float (&y)[4], float top) {
-  float z[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) z[i] = __builtin_amdgcn_fmed3f(y[i], -top, top);
-  if constexpr (kE4m3) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], w, true);
-  } else {
-    // Adding 1.5 * 2^23 rounds to a whole number, ties to even, in the low bits.
-    unsigned b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(z[i] + 12582912.f);
-    const unsigned lo = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u);
-    const unsigned hi = __builtin_amdgcn_perm(b[3], b[2], 0x0C0C0400u);
-    return lo | hi << 16;
-  }
-}
-
-template <bool kE4m3>
-__device__ __forceinline__ unsigned encode4(f16 a, f16 b, f16 c, f16 d, float inv, float top) {
-  return encode4<kE4m3>({(float)a * inv, (float)b * inv, (float)c * inv, (float)d * inv}, top);
-}
-
-// Four codes at the ratio old scale / new scale.
-template <bool kE4m3>
-__device__ __forceinline__ unsigned recode4(unsigned w, float ratio, float top) {
-  const unsigned u = flip8<kE4m3>(w);
-  const f16x2 a = code_pair<kE4m3, false>(u, 1.f), b = code_pair<kE4m3, true>(u, 1.f);
-  return encode4<kE4m3>({(float)a[0] * ratio, (float)a[1] * ratio, (float)b[0] * ratio,
-                         (float)b[1] * ratio}, top);
-}
-
-__device__ __forceinline__ unsigned magnitudes(f16x8 x) {
-  const u32x4 w = __builtin_bit_cast(u32x4, x);
-  unsigned top = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
-  return top;
-}
-
-__device__ __forceinline__ unsigned wave_max(unsigned x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x = max(x, (unsigned)__shfl_xor((int)x, d));
-  return x;
-}
-
-// The block's new scale, and what its old codes are multiplied by (1: left alone).
-struct Scales {
-  float s, inv, top, ratio;
-  bool bad;
-};
-
-template <bool kE4m3>
-__device__ __forceinline__ Scales new_scale(unsigned top, float old, bool begun) {
-  Scales r;
-  const float need = scale_for<kE4m3>(top);
-  r.s = need;
-  if (begun && !(old < need)) r.s = need == need ? old : need;  // NaN of either stays
-  r.bad = !(r.s == r.s);
-  r.inv = r.bad ? 0.f : 1.f / r.s;
-  r.top = code_top<kE4m3>(r.s);
-  r.ratio = begun && old < r.s ? old * r.inv : 1.f;
-  return r;
-}
-
-template <bool kE4m3>
+template <bool kE4m3, bool kSingle>
 __global__ __launch_bounds__(64 * kWaves) void append_kernel(RowsArgs a) {
-  const int lane = threadIdx.x & 63;
   const int id = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
   const int hk = blockIdx.y % a.p.kvh, layer = blockIdx.y / a.p.kvh;
-  const Unit u = find_unit(a, id);
+  const Unit u = find_unit<kSingle>(a, id);
   if (u.n <= 0 || u.lo < 0) return;
   const int slot0 = u.block << 4;                       // of the block
   const int lp = slot0 >> a.p.log2p;
   if (lp >= a.p.ppr) return;
-  const int page = a.p.table[u.row * a.p.t_sb + lp];
-  if (page < 0 || page >= a.p.n_pages) return;
-  const int in_page = slot0 & ((1 << a.p.log2p) - 1);
-  const int64_t at = layer * a.p.sl + page * a.p.sp + hk * a.p.sh;
-  const int64_t sat = layer * a.p.ssl + page * a.p.ssp + hk * a.p.ssh + (in_page >> 4);
-  uint8_t* kp = a.p.k + at + (int64_t)in_page * kD;     // 16 slots x 64
-  uint8_t* vp = a.p.v + at + (int64_t)(in_page >> 6) * 64 * kD + (in_page & 63);
-  const bool begun = u.lo > 0;
-  const int end = min(u.lo + u.n, a.cap - slot0);       // slots [lo, end) of the block are new
+  const int end = min(u.lo + u.n, a.cap - slot0);
   if (end <= u.lo) return;
-  const float ks_old = a.p.ks[sat], vs_old = a.p.vs[sat];
-
-  // K: slot t, dims 8c and 32 + 8c.
-  const int t = lane >> 2, c = 8 * (lane & 3);
-  const bool fresh = t >= u.lo && t < end;
-  const int64_t tok = u.tok + (fresh ? t - u.lo : 0);
-  const f16* src = a.k + layer * a.k_sl + hk * a.k_sh + tok * a.k_sn + c;
-  f16x8 klo = load16(src), khi = load16(src + 32);
-  // V: dim `lane`, the block's 16 slots.
-  const f16* vsrc = a.v + layer * a.v_sl + hk * a.v_sh + (int64_t)u.tok * a.v_sn + lane;
-  f16 x[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const bool in = j >= u.lo && j < end;
-    x[j] = in ? vsrc[(j - u.lo) * a.v_sn] : (f16)0.f;
-  }
-  u32x2 old_lo = {0, 0}, old_hi = {0, 0};
-  u32x4 old_v = {0, 0, 0, 0};
-  if (begun || end < kBlock) {
-    old_lo = *reinterpret_cast<const u32x2*>(kp + t * kD + c);
-    old_hi = *reinterpret_cast<const u32x2*>(kp + t * kD + c + 32);
-    old_v = *reinterpret_cast<const u32x4*>(vp + lane * 64);
-  }
-  if (a.cos != nullptr) {
-    const int64_t co = tok * a.cs_sn + c;
-    rope_pair(klo, khi, load16(a.cos + co), load16(a.sin + co), load16(a.cos + co + 32),
-              load16(a.sin + co + 32));
-  }
-  const Scales k = new_scale<kE4m3>(
-      wave_max(fresh ? max(magnitudes(klo), magnitudes(khi)) : 0u), ks_old, begun);
-  unsigned vtop = 0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    vtop = max(vtop, (unsigned)__builtin_bit_cast(unsigned short, x[j]) & 0x7FFFu);
-  const Scales v = new_scale<kE4m3>(wave_max(vtop), vs_old, begun);
-
-  if (fresh || (t < u.lo && k.ratio != 1.f)) {
-    u32x2 lo, hi;
-    if (fresh) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        lo[i] = k.bad ? 0u : encode4<kE4m3>(klo[4 * i], klo[4 * i + 1], klo[4 * i + 2], klo[4 * i + 3], k.inv, k.top);
-        hi[i] = k.bad ? 0u : encode4<kE4m3>(khi[4 * i], khi[4 * i + 1], khi[4 * i + 2], khi[4 * i + 3], k.inv, k.top);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        lo[i] = recode4<kE4m3>(old_lo[i], k.ratio, k.top);
-        hi[i] = recode4<kE4m3>(old_hi[i], k.ratio, k.top);
-      }
-    }
-    *reinterpret_cast<u32x2*>(kp + t * kD + c) = lo;
-    *reinterpret_cast<u32x2*>(kp + t * kD + c + 32) = hi;
-  }
-  u32x4 out;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const unsigned w = v.bad ? 0u : encode4<kE4m3>(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], v.inv, v.top);
-    // Bytes of slots that are new, and of those before them.
-    const int n0 = min(max(u.lo - 4 * i, 0), 4), n1 = min(max(end - 4 * i, 0), 4);
-    const unsigned below = n0 == 4 ? ~0u : (1u << (8 * n0)) - 1u;
-    const unsigned upto = n1 == 4 ? ~0u : (1u << (8 * n1)) - 1u;
-    const unsigned had = v.ratio != 1.f ? recode4<kE4m3>(old_v[i], v.ratio, v.top) : old_v[i];
-    out[i] = (w & upto & ~below) | (had & below) | (old_v[i] & ~upto);
-  }
-  *reinterpret_cast<u32x4*>(vp + lane * 64) = out;
-  if (lane == 0) {
-    a.p.ks[sat] = k.s;
-    a.p.vs[sat] = v.s;
-  }
+  const Tokens t = {a.k + layer * a.k_sl + hk * a.k_sh + u.tok * a.k_sn, a.k_sn,
+                    a.v + layer * a.v_sl + hk * a.v_sh + u.tok * a.v_sn, a.v_sn,
+                    a.cos == nullptr ? nullptr : a.cos + u.tok * a.cs_sn,
+                    a.cos == nullptr ? nullptr : a.sin + u.tok * a.cs_sn, a.cs_sn};
+  append_block<kE4m3>(a.p, layer, hk, a.p.table[u.row * a.p.t_sb + lp], slot0, u.lo, end, t);
 }
 
 template <bool kE4m3>
@@ -280,7 +125,7 @@ __global__ __launch_bounds__(64 * kWaves) void read_kernel(RowsArgs a) {
   const int lane = threadIdx.x & 63;
   const int id = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
   const int hk = blockIdx.y % a.p.kvh, layer = blockIdx.y / a.p.kvh;
-  const Unit u = find_unit(a, id);
+  const Unit u = find_unit<false>(a, id);
   if (u.n <= 0) return;
   const int slot0 = u.block << 4;
   const int lp = slot0 >> a.p.log2p;
@@ -291,30 +136,35 @@ __global__ __launch_bounds__(64 * kWaves) void read_kernel(RowsArgs a) {
   const int64_t at = layer * a.p.sl + page * a.p.sp + hk * a.p.sh;
   const int64_t sat = layer * a.p.ssl + page * a.p.ssp + hk * a.p.ssh + (in_page >> 4);
   const float ks = a.p.ks[sat], vs = a.p.vs[sat];
-  // Four lanes a slot, 16 dims each.
+  // K: four lanes a slot, 16 dims each.  V: dims 2d and 2d + 1, slots j0 .. j0 + 7.
   const int t = lane >> 2, c = 16 * (lane & 3);
+  const int d = lane & 31, j0 = lane >> 5 << 3;
   const u32x4 kw = *reinterpret_cast<const u32x4*>(a.p.k + at + (int64_t)in_page * kD + t * kD + c);
-  const u32x4 vw = *reinterpret_cast<const u32x4*>(a.p.v + at + (int64_t)(in_page >> 6) * 64 * kD +
-                                                   (in_page & 63) + lane * 64);
-  const f16 nan = (f16)__builtin_nanf("");
-  f16x8 k0 = values8<kE4m3>(kw[0], kw[1], ks), k1 = values8<kE4m3>(kw[2], kw[3], ks);
-  f16x8 v0 = values8<kE4m3>(vw[0], vw[1], vs), v1 = values8<kE4m3>(vw[2], vw[3], vs);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    k0[i] = none ? (f16)0.f : ks == ks ? k0[i] : nan;
-    k1[i] = none ? (f16)0.f : ks == ks ? k1[i] : nan;
-    v0[i] = none ? (f16)0.f : vs == vs ? v0[i] : nan;
-    v1[i] = none ? (f16)0.f : vs == vs ? v1[i] : nan;
-  }
+  const uint8_t* vp = a.p.v + at + (int64_t)(in_page >> 6) * 64 * kD + (in_page & 63) + 128 * d + j0;
+  const u32x2 vw0 = *reinterpret_cast<const u32x2*>(vp), vw1 = *reinterpret_cast<const u32x2*>(vp + 64);
+  u32x4 k0 = __builtin_bit_cast(u32x4, values8<kE4m3>(kw[0], kw[1], ks));
+  u32x4 k1 = __builtin_bit_cast(u32x4, values8<kE4m3>(kw[2], kw[3], ks));
+  u32x4 v0 = __builtin_bit_cast(u32x4, values8<kE4m3>(vw0[0], vw0[1], vs));
+  u32x4 v1 = __builtin_bit_cast(u32x4, values8<kE4m3>(vw1[0], vw1[1], vs));
+  const unsigned ksay = none ? 0u : ks == ks ? ~0u : 0x7E007E00u, vsay = none ? 0u : vs == vs ? ~0u : 0x7E007E00u;
   if (t >= lo && t < lo + u.n) {
     f16* dst = a.k + layer * a.k_sl + hk * a.k_sh + (int64_t)(u.tok + t - lo) * a.k_sn + c;
-    store16(dst, k0);
-    store16(dst + 8, k1);
-  }
-  f16* dst = a.v + layer * a.v_sl + hk * a.v_sh + (int64_t)u.tok * a.v_sn + lane;
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (j >= lo && j < lo + u.n) dst[(j - lo) * a.v_sn] = j < 8 ? v0[j & 7] : v1[j & 7];
+    for (int i = 0; i < 4; ++i) {
+      k0[i] = ksay == ~0u ? k0[i] : ksay;
+      k1[i] = ksay == ~0u ? k1[i] : ksay;
+    }
+    store16(dst, __builtin_bit_cast(f16x8, k0));
+    store16(dst + 8, __builtin_bit_cast(f16x8, k1));
+  }
+  f16* dst = a.v + layer * a.v_sl + hk * a.v_sh + (int64_t)u.tok * a.v_sn + 2 * d;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    // Slot j of both dims, as one word.
+    const unsigned w = __builtin_amdgcn_perm(v1[j / 2], v0[j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+    if (j0 + j >= lo && j0 + j < lo + u.n)
+      *reinterpret_cast<unsigned*>(dst + (j0 + j - lo) * a.v_sn) = vsay == ~0u ? w : vsay;
+  }
 }
 
 constexpr int kCopyThreads = 256, kCopyUnroll = 4;
@@ -344,84 +194,75 @@ __global__ __launch_bounds__(kCopyThreads) void copy_kernel(uint8_t* store, int6
 }
 
 // Checks and fills what the append and the read share, and the launch's size.
-int make_rows(RowsArgs& a, dim3& grid, const void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn,
-              const void* v, int64_t v_sl, int64_t v_sh, int64_t v_sn, const int32_t* cu, int total,
-              int max_seqlen, const int64_t* first, int64_t first_sb, const QfPool8* pool, int B, int D) {
-  if (D != kD) return QF_ERR_UNSUPPORTED;
-  if (!pool || !k || !v || !cu || !first || B < 1 || total < 1 || max_seqlen < 1 || max_seqlen > total)
+int make_rows(RowsArgs& a, dim3& grid, const QfRows8& h) {
+  if (h.D != kD) return QF_ERR_UNSUPPORTED;
+  if (!h.k || !h.v || !h.cu_seqlens || !h.first || h.B < 1 || h.total < 1 || h.max_seqlen < 1 ||
+      h.max_seqlen > h.total)
     return QF_ERR_INVALID_ARG;
-  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) != 0 ||
-      ((k_sl | k_sh | k_sn | v_sl | v_sh | v_sn) & 7) != 0)
+  if (((reinterpret_cast<uintptr_t>(h.k) | reinterpret_cast<uintptr_t>(h.v)) & 15u) != 0 ||
+      ((h.k_sl | h.k_sh | h.k_sn | h.v_sl | h.v_sh | h.v_sn) & 7) != 0)
     return QF_ERR_INVALID_ARG;
-  if (B > 0x3fffffff || total > 0x3fffffff) return QF_ERR_UNSUPPORTED;
+  if (h.B > 0x3fffffff || h.total > 0x3fffffff) return QF_ERR_UNSUPPORTED;
   a = RowsArgs{};
-  const int rc = make_pool(pool, a.p);
+  const int rc = make_pool(h.pool, a.p);
   if (rc != QF_OK) return rc;
-  a.k = static_cast<f16*>(const_cast<void*>(k));
-  a.k_sl = k_sl; a.k_sh = k_sh; a.k_sn = k_sn;
-  a.v = static_cast<f16*>(const_cast<void*>(v));
-  a.v_sl = v_sl; a.v_sh = v_sh; a.v_sn = v_sn;
-  a.cu = cu;
-  a.first = first;
-  a.first_sb = first_sb;
-  a.B = B; a.total = total;
-  a.cap = pool->pages_per_row * pool->page_size;
+  a.k = static_cast<f16*>(h.k);
+  a.k_sl = h.k_sl; a.k_sh = h.k_sh; a.k_sn = h.k_sn;
+  a.v = static_cast<f16*>(h.v);
+  a.v_sl = h.v_sl; a.v_sh = h.v_sh; a.v_sn = h.v_sn;
+  a.cu = h.cu_seqlens;
+  a.first = h.first;
+  a.first_sb = h.first_sb;
+  a.B = (int)h.B; a.total = (int)h.total;
+  a.cap = row_cap(a.p);
   // A row's n tokens touch at most n / 16 + 2 blocks, one of them if n is 1.
-  const int64_t blocks = max_seqlen == 1 ? B : (int64_t)total / kBlock + 2 * (int64_t)std::min(B, total);
-  grid = dim3((unsigned)((blocks + kWaves - 1) / kWaves), (unsigned)(pool->KVH * pool->layers));
+  const int64_t blocks = h.max_seqlen == 1 ? h.B : h.total / kBlock + 2 * std::min(h.B, h.total);
+  grid = dim3((unsigned)((blocks + kWaves - 1) / kWaves), (unsigned)(h.pool.KVH * h.pool.layers));
   return QF_OK;
 }
 
 }  // namespace kv8
 }  // namespace qf
 
-int qf::kv8::append(const void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn, const void* v, int64_t v_sl,
-                    int64_t v_sh, int64_t v_sn, const int32_t* cu_seqlens, int total, int max_seqlen,
-                    const int64_t* context, int64_t ctx_sb, const void* cos, const void* sin,
-                    int64_t cs_sn, const QfPool8* pool, int cap, int B, int D, hipStream_t st) {
+int qf::kv8::append(const QfRows8& h, int cap, hipStream_t st) {
   RowsArgs a;
   dim3 grid;
-  const int rc = make_rows(a, grid, k, k_sl, k_sh, k_sn, v, v_sl, v_sh, v_sn, cu_seqlens, total,
-                           max_seqlen, context, ctx_sb, pool, B, D);
+  const int rc = make_rows(a, grid, h);
   if (rc != QF_OK) return rc;
-  if ((cos == nullptr) != (sin == nullptr) ||
-      ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15u) != 0 ||
-      (cos != nullptr && (cs_sn & 7) != 0))
+  if ((h.cos == nullptr) != (h.sin == nullptr) ||
+      ((reinterpret_cast<uintptr_t>(h.cos) | reinterpret_cast<uintptr_t>(h.sin)) & 15u) != 0 ||
+      (h.cos != nullptr && (h.cs_sn & 7) != 0))
     return QF_ERR_INVALID_ARG;
-  a.cos = static_cast<const f16*>(cos);
-  a.sin = static_cast<const f16*>(sin);
-  a.cs_sn = cs_sn;
+  a.cos = static_cast<const f16*>(h.cos);
+  a.sin = static_cast<const f16*>(h.sin);
+  a.cs_sn = h.cs_sn;
   a.cap = std::min(a.cap, cap);
-  if (pool->code == QF_CODE_E4M3)
-    hipLaunchKernelGGL(append_kernel<true>, grid, dim3(64 * kWaves), 0, st, a);
-  else
-    hipLaunchKernelGGL(append_kernel<false>, grid, dim3(64 * kWaves), 0, st, a);
+  const dim3 block(64 * kWaves);
+  const bool e4m3 = h.pool.code == QF_CODE_E4M3;
+  if (h.max_seqlen == 1) {
+    if (e4m3) hipLaunchKernelGGL((append_kernel<true, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((append_kernel<false, true>), grid, block, 0, st, a);
+  } else {
+    if (e4m3) hipLaunchKernelGGL((append_kernel<true, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((append_kernel<false, false>), grid, block, 0, st, a);
+  }
   return (int)hipGetLastError();
 }
 
-extern "C" int qf_append_paged8(const void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn,
-                                const void* v, int64_t v_sl, int64_t v_sh, int64_t v_sn,
-                                const int32_t* cu_seqlens, int total, int max_seqlen,
-                                const int64_t* context, int64_t ctx_sb, const void* cos,
-                                const void* sin, int64_t cs_sn, const QfPool8* pool, int B, int D,
-                                void* stream) {
-  return qf::kv8::append(k, k_sl, k_sh, k_sn, v, v_sl, v_sh, v_sn, cu_seqlens, total, max_seqlen, context,
-                         ctx_sb, cos, sin, cs_sn, pool, 0x7fffffff, B, D, static_cast<hipStream_t>(stream));
+extern "C" int qf_append_paged8(const QfRows8* rows, void* stream) {
+  if (!rows) return QF_ERR_INVALID_ARG;
+  return qf::kv8::append(*rows, 0x7fffffff, static_cast<hipStream_t>(stream));
 }
 
-extern "C" int qf_read_paged8(void* k, int64_t k_sl, int64_t k_sh, int64_t k_sn, void* v, int64_t v_sl,
-                              int64_t v_sh, int64_t v_sn, const int32_t* cu_seqlens, int total,
-                              int max_seqlen, const int64_t* first, int64_t first_sb,
-                              const QfPool8* pool, int B, int D, void* stream) {
-  using namespace qf;
+extern "C" int qf_read_paged8(const QfRows8* rows, void* stream) {
   using namespace qf::kv8;
   RowsArgs a;
   dim3 grid;
-  const int rc = make_rows(a, grid, k, k_sl, k_sh, k_sn, v, v_sl, v_sh, v_sn, cu_seqlens, total,
-                           max_seqlen, first, first_sb, pool, B, D);
+  if (!rows || rows->cos || rows->sin) return QF_ERR_INVALID_ARG;
+  const int rc = make_rows(a, grid, *rows);
   if (rc != QF_OK) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (pool->code == QF_CODE_E4M3)
+  if (rows->pool.code == QF_CODE_E4M3)
     hipLaunchKernelGGL(read_kernel<true>, grid, dim3(64 * kWaves), 0, st, a);
   else
     hipLaunchKernelGGL(read_kernel<false>, grid, dim3(64 * kWaves), 0, st, a);

@@ -19,7 +19,7 @@
 // have anyway; V's into the conversion of its codes to fp16, which is exact.
 #include <algorithm>
 
-#include "kv8.h"
+#include "kv8_block.h"
 #include "lds_tile.h"
 
 namespace qf {
@@ -27,6 +27,8 @@ namespace kv8 {
 
 constexpr int kTile = 64;                    // slots
 constexpr int kMaxSplits = 64;
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 struct AttnArgs {
   Pool p;
@@ -48,6 +50,10 @@ struct AttnArgs {
   const f16* cos;
   const f16* sin;
   int64_t cs_sn;
+  const f16* kn;                             // decode: the token of slot `last`, appended
+  int64_t kn_sb, kn_sh;
+  const f16* vn;
+  int64_t vn_sb, vn_sh;
 };
 
 // Slots [k0, k1) of split s of [0, end): cut at multiples of `least` and 64.
@@ -65,13 +71,6 @@ struct Unit {
   int ctx;                // extension: cached slots, -1 parked
   int k0, k1;
 };
-
-// What the query row of `token` sees: slots [0, lim).
-template <bool kDecode>
-__device__ __forceinline__ int row_limit(const AttnArgs& a, const Unit& u, int token) {
-  if (kDecode) return u.k1;
-  return min(u.ctx + (token - u.tok0) + 1, a.cap);
-}
 
 struct Raw {
   u32x4 k[4], v[4];
@@ -97,27 +96,29 @@ __device__ __forceinline__ void load_pids(Source& s, int win) {
   s.pwin = win;
 }
 
-__device__ __forceinline__ u32x4 load_nt(const uint8_t* p) {
-  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-}
-
+// Loads the tile at slot0 where `valid`; without it nothing is fetched, but the loads
+// count: what a wave waits for then does not depend on where its tiles end.
 template <bool kNt>
-__device__ __forceinline__ void load_tile(Raw& r, Source& s, int slot0) {
-  const int lp = slot0 >> s.log2p;
+__device__ __forceinline__ void load_tile(Raw& r, Source& s, int slot0, bool valid) {
+  const int lp = valid ? slot0 >> s.log2p : s.pwin;
   if (lp - s.pwin >= 64) load_pids(s, lp);
-  const int page = __builtin_amdgcn_readlane(s.pid, lp - s.pwin);
+  const int64_t page = __builtin_amdgcn_readlane(s.pid, lp - s.pwin);
   const int in_page = slot0 & ((1 << s.log2p) - 1);
-  const uint8_t* k = s.k + page * s.sp + in_page * kD;
-  const uint8_t* v = s.v + page * s.sp + in_page * kD;
+  const int64_t at = page * s.sp + in_page * kD, sat = page * s.ssp + (in_page >> 4);
   const int g = (threadIdx.x & 63) >> 4;
+  constexpr int aux = kNt ? 2 : 0;
+  const __amdgpu_buffer_rsrc_t rk = buffer_rsrc(s.k + at, valid ? kTile * kD : 0);
+  const __amdgpu_buffer_rsrc_t rv = buffer_rsrc(s.v + at, valid ? kTile * kD : 0);
+  const __amdgpu_buffer_rsrc_t rks = buffer_rsrc(s.ks + sat, valid ? 16 : 0);
+  const __amdgpu_buffer_rsrc_t rvs = buffer_rsrc(s.vs + sat, valid ? 16 : 0);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    r.k[i] = kNt ? load_nt(k + s.koff + i * 4 * kD) : *reinterpret_cast<const u32x4*>(k + s.koff + i * 4 * kD);
+    r.k[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, s.koff + i * 4 * kD, 0, aux));
+  r.ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rks, 4 * g, 0, 0));
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    r.v[i] = kNt ? load_nt(v + s.voff + i * 16 * kTile) : *reinterpret_cast<const u32x4*>(v + s.voff + i * 16 * kTile);
-  r.ks = s.ks[page * s.ssp + (in_page >> 4) + g];
-  r.vs = s.vs[page * s.ssp + (in_page >> 4) + g];
+    r.v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, s.voff + i * 16 * kTile, 0, aux));
+  r.vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rvs, 4 * g, 0, 0));
 }
 
 // The softmax state of kNC blocks of 16 query columns.
@@ -131,15 +132,14 @@ struct State {
   f32x4 o[kNC][4];
 };
 
+// The unit's queries; what each sees is set_limits'.
 template <int kNC, bool kDecode>
 __device__ __forceinline__ void load_queries(State<kNC>& s, const AttnArgs& a, const Unit& u) {
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  int least = 0x7fffffff;
 #pragma unroll
   for (int b = 0; b < kNC; ++b) {
-    const int r = u.r0 + 16 * b + col;
-    const int rr = min(r, u.rows - 1);
-    const int token = u.tok0 + rr / a.G, h = rr % a.G;
+    const int rr = min(u.r0 + 16 * b + col, u.rows - 1);
+    const int token = kDecode ? u.tok0 : u.tok0 + rr / a.G, h = kDecode ? rr : rr % a.G;
     const f16* qp = a.q + token * a.q_st + u.hk * a.q_sh + h * a.q_sg + 16 * g;
 #pragma unroll
     for (int i = 0; i < 2; ++i) s.q[b][i] = load16(qp + 8 * i);
@@ -156,19 +156,31 @@ __device__ __forceinline__ void load_queries(State<kNC>& s, const AttnArgs& a, c
         s.q[b][i] = g < 2 ? x : y;
       }
     }
-    s.lim[b] = r < u.rows ? min(row_limit<kDecode>(a, u, token), u.k1) : u.k1;
-    least = min(least, s.lim[b]);
     s.m[b] = kNegInf;
     s.l[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < 4; ++t) s.o[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if (kDecode) {
-    s.seen = u.k1;
-  } else {
-    for (int d = 8; d > 0; d >>= 1) least = min(least, __shfl_xor(least, d));
-    s.seen = __builtin_amdgcn_readfirstlane(least);
+}
+
+template <int kNC, bool kDecode>
+__device__ __forceinline__ void set_limits(State<kNC>& s, const AttnArgs& a, const Unit& u) {
+  const int col = threadIdx.x & 15;
+  int least = u.k1;
+#pragma unroll
+  for (int b = 0; b < kNC; ++b) {
+    s.lim[b] = u.k1;
+    if (!kDecode) {
+      const int r = u.r0 + 16 * b + col;
+      if (r < u.rows) s.lim[b] = min(u.ctx + r / a.G + 1, u.k1);
+      least = min(least, s.lim[b]);
+    }
   }
+  if (!kDecode) {
+    for (int d = 8; d > 0; d >>= 1) least = min(least, __shfl_xor(least, d));
+    least = __builtin_amdgcn_readfirstlane(least);
+  }
+  s.seen = least;
 }
 
 // Scores, online softmax and PV product of the tile at key0.  `next` loads what
@@ -200,30 +212,47 @@ __device__ __forceinline__ void tile_step(State<kNC>& s, Raw& r, int key0, int k
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int h = 0; h < 2; ++h) k[i][h] = codes8<kE4m3>(r.k[i][2 * h], r.k[i][2 * h + 1], 1.f);
+  if (kE4m3 || !__any(vs > kAffineMost)) {
+    const Affine f = affine(vs);
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) v[t][h] = values8<kE4m3>(r.v[t][2 * h], r.v[t][2 * h + 1], vs);
+      for (int h = 0; h < 2; ++h) v[t][h] = values8<kE4m3>(r.v[t][2 * h], r.v[t][2 * h + 1], vs, f);
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v[t][h] = values8<kE4m3>(r.v[t][2 * h], r.v[t][2 * h + 1], vs);
+  }
   next();
-  const f16x8 ones = {(f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f};
+  f32x4 sc[kNC][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int b = 0; b < kNC; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sc[b][i] = mfma16x16x32(k[i][h], s.q[b][h], h == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[b][i]);
+  float f[kNC], mx[kNC];
+  bool grew = false;
 #pragma unroll
   for (int b = 0; b < kNC; ++b) {
-    f32x4 sc[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sc[i] = mfma16x16x32(k[i][0], s.q[b][0], f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sc[i] = mfma16x16x32(k[i][1], s.q[b][1], sc[i]);
-    float f = ks2;
-    const int left = s.lim[b] - key0 - 16 * g;
+    f[b] = ks2;
     if (masked) {
-      if (left <= 0) f = 1.f;   // whatever scale an unseen block has
+      const int left = s.lim[b] - key0 - 16 * g;
+      if (left <= 0) f[b] = 1.f;   // whatever scale an unseen block has
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (i >= left) sc[i / 4][i % 4] = kNegInf;
+        if (i >= left) sc[b][i / 4][i % 4] = kNegInf;
     }
-    const float mx = max16(sc) * f;
-    if (__any(mx > s.m[b] + kRescaleSlack)) {
-      const float top = col_max(mx);
+    mx[b] = max16(sc[b]) * f[b];
+    grew = grew || mx[b] > s.m[b] + kRescaleSlack;
+  }
+  // Moves the references of the columns whose own scores grew past them.
+  if (__any(grew)) {
+#pragma unroll
+    for (int b = 0; b < kNC; ++b) {
+      const float top = col_max(mx[b]);
       const float m_new = top > s.m[b] + kRescaleSlack ? top : s.m[b];
       const float c = m_new == s.m[b] ? 1.f : fast_exp2(s.m[b] - m_new);
       s.l[b] *= c;
@@ -231,26 +260,47 @@ __device__ __forceinline__ void tile_step(State<kNC>& s, Raw& r, int key0, int k
       for (int t = 0; t < 4; ++t) s.o[b][t] *= c;
       s.m[b] = m_new;
     }
+  }
+  f16x8 p[kNC][2];
+  const f16x8 ones = {(f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f};
+  const auto weights = [&](int b) {
     const float neg_m = s.m[b] == kNegInf ? 0.f : -s.m[b];
-    f16x8 p[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u) {
+      f32x8 x;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        p[u][e] = (f16)fast_exp2(__builtin_fmaf(sc[2 * u + e / 4][e % 4], f, neg_m));
-    if (__any(bad && left > 0)) {
+      for (int e = 0; e < 8; ++e) x[e] = fast_exp2(__builtin_fmaf(sc[b][2 * u + e / 4][e % 4], f[b], neg_m));
+      p[b][u] = __builtin_convertvector(x, f16x8);
+    }
+  };
+  const auto products = [&](int b) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      // The sum adds the rounded p, so that the weights add to one.
+      s.l[b] = mfma16x16x32(ones, p[b][u], s.l[b]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) s.o[b][t] = mfma16x16x32(v[t][u], p[b][u], s.o[b][t]);
+    }
+  };
+  if (__any(bad)) {
+#pragma unroll
+    for (int b = 0; b < kNC; ++b) {
+      weights(b);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (bad && left > 0) p[u][e] = (f16)__builtin_nanf("");
+          if (bad && s.lim[b] > key0 + 16 * g) p[b][u][e] = (f16)__builtin_nanf("");
+      products(b);
     }
+    return;
+  }
+  weights(0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      // The sum adds the rounded p, so that the weights add to one.
-      s.l[b] = mfma16x16x32(ones, p[u], s.l[b]);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) s.o[b][t] = mfma16x16x32(v[t][u], p[u], s.o[b][t]);
+  for (int b = 0; b < kNC; ++b) {
+    products(b);
+    if (b + 1 < kNC) {
+      weights(b + 1);
     }
   }
 }
@@ -287,8 +337,29 @@ __device__ __forceinline__ void empty_unit(const AttnArgs& a, const Unit& u, int
   }
 }
 
+// The row's pages, with the first 64 table entries on their way.
+__device__ __forceinline__ Source make_source(const AttnArgs& a, const Unit& u) {
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  Source s;
+  s.row = a.p.table + u.row * a.p.t_sb;
+  s.ppr = a.p.ppr; s.n_pages = a.p.n_pages;
+  load_pids(s, 0);
+  s.k = a.p.k + u.hk * a.p.sh;
+  s.v = a.p.v + u.hk * a.p.sh;
+  s.ks = a.p.ks + u.hk * a.p.ssh;
+  s.vs = a.p.vs + u.hk * a.p.ssh;
+  s.sp = a.p.sp;
+  s.ssp = a.p.ssp;
+  s.log2p = a.p.log2p;
+  s.koff = (16 * (col >> 2) + (col & 3)) * kD + 16 * g;
+  s.voff = col * kTile + 16 * g;
+  return s;
+}
+
+// A unit whose queries are in s.
 template <bool kE4m3, int kNC, bool kDecode>
-__device__ __forceinline__ void run_unit(const AttnArgs& a, const Unit& u, f32x4* lds) {
+__device__ __forceinline__ void run_unit(const AttnArgs& a, const Unit& u, Source& src, State<kNC>& s,
+                                         f32x4* lds) {
   if (u.k1 <= u.k0) {
     empty_unit(a, u, 16 * kNC);
     return;
@@ -296,28 +367,30 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Unit& u, f32x4
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int n = (u.k1 - u.k0 + kTile - 1) / kTile;
-  Source src;
-  src.k = a.p.k + u.hk * a.p.sh;
-  src.v = a.p.v + u.hk * a.p.sh;
-  src.ks = a.p.ks + u.hk * a.p.ssh;
-  src.vs = a.p.vs + u.hk * a.p.ssh;
-  src.row = a.p.table + u.row * a.p.t_sb;
-  src.sp = a.p.sp;
-  src.ssp = a.p.ssp;
-  src.log2p = a.p.log2p; src.ppr = a.p.ppr; src.n_pages = a.p.n_pages;
-  src.koff = (16 * (col >> 2) + (col & 3)) * kD + 16 * g;
-  src.voff = col * kTile + 16 * g;
-  Raw r;
-  if (w < n) {
-    load_pids(src, (u.k0 + w * kTile) >> a.p.log2p);
-    load_tile<kDecode>(r, src, u.k0 + w * kTile);
-  }
-  State<kNC> s;
-  load_queries<kNC, kDecode>(s, a, u);
-  for (int i = w; i < n; i += nw) {
-    tile_step<kE4m3, kNC>(s, r, u.k0 + i * kTile, u.k1, a.scale_log2, [&] {
-      if (i + nw < n) load_tile<kDecode>(r, src, u.k0 + (i + nw) * kTile);
-    });
+  const int mine = (n - w + nw - 1) / nw;      // tiles of this wave, from w on every nw-th
+  const auto slot = [&](int j) { return u.k0 + (w + j * nw) * kTile; };
+  if constexpr (kNC == 1) {
+    // Two tiles ahead: a wave that is alone on its SIMD takes a tile in less time than
+    // memory answers in.
+    Raw r0, r1;
+    load_tile<kDecode>(r0, src, slot(0), 0 < mine);
+    load_tile<kDecode>(r1, src, slot(1), 1 < mine);
+    set_limits<kNC, kDecode>(s, a, u);
+    int j = 0;
+    for (; j + 2 <= mine; j += 2) {
+      tile_step<kE4m3, kNC>(s, r0, slot(j), u.k1, a.scale_log2,
+                            [&] { load_tile<kDecode>(r0, src, slot(j + 2), j + 2 < mine); });
+      tile_step<kE4m3, kNC>(s, r1, slot(j + 1), u.k1, a.scale_log2,
+                            [&] { load_tile<kDecode>(r1, src, slot(j + 3), j + 3 < mine); });
+    }
+    if (j < mine) tile_step<kE4m3, kNC>(s, r0, slot(j), u.k1, a.scale_log2, [] {});
+  } else {
+    Raw r;
+    load_tile<kDecode>(r, src, slot(0), 0 < mine);
+    set_limits<kNC, kDecode>(s, a, u);
+    for (int j = 0; j < mine; ++j)
+      tile_step<kE4m3, kNC>(s, r, slot(j), u.k1, a.scale_log2,
+                            [&] { load_tile<kDecode>(r, src, slot(j + 1), j + 1 < mine); });
   }
   // The waves' states, a block of columns at a time.
   f32x4* so = lds;                                          // [wave][d tile][lane]
@@ -358,7 +431,7 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Unit& u, f32x4
 }
 
 template <bool kE4m3>
-__global__ __launch_bounds__(1024) void decode_kernel(AttnArgs a) {
+__global__ __launch_bounds__(512, 2) void decode_kernel(AttnArgs a) {
   extern __shared__ f32x4 lds[];
   Unit u;
   int id = blockIdx.x;
@@ -369,9 +442,26 @@ __global__ __launch_bounds__(1024) void decode_kernel(AttnArgs a) {
   u.rows = a.G;
   u.r0 = 0;
   u.ctx = -1;
-  const int end = clampi(a.last[u.row * a.last_sb], -1, a.cap - 1) + 1;
-  cut(end, u.split, a.splits, u.k0, u.k1);
-  run_unit<kE4m3, 1, true>(a, u, lds);
+  // The table and the queries are loaded while the row's length is.
+  const int64_t last = a.last[u.row * a.last_sb];
+  Source src = make_source(a, u);
+  State<1> s;
+  load_queries<1, true>(s, a, u);
+  cut(clampi(last, -1, a.cap - 1) + 1, u.split, a.splits, u.k0, u.k1);
+  if (a.kn != nullptr && last >= u.k0 && last < u.k1) {
+    // The unit that sees the new token writes it; its block is in no other unit.  The
+    // waves of a workgroup share a first-level cache, so they see it past the barrier.
+    if (threadIdx.x < 64) {
+      const int slot = (int)last, lo = slot % kBlock;
+      const Tokens t = {a.kn + u.row * a.kn_sb + u.hk * a.kn_sh, 0, a.vn + u.row * a.vn_sb + u.hk * a.vn_sh,
+                        0, nullptr, nullptr, 0};
+      append_block<kE4m3>(a.p, 0, u.hk, src.row[slot >> a.p.log2p], slot - lo, lo, lo + 1, t);
+      s_waitcnt_vm(0);
+    }
+    __threadfence_block();
+    __syncthreads();
+  }
+  run_unit<kE4m3, 1, true>(a, u, src, s, lds);
 }
 
 template <bool kE4m3, int kNC>
@@ -403,12 +493,15 @@ __global__ __launch_bounds__(256, 2) void extend_kernel(AttnArgs a) {
     const int newest = (min(u.r0 + 16 * kNC, u.rows) - 1) / a.G;
     u.k1 = min(u.k1, min(u.ctx + newest + 1, a.cap));
   }
-  run_unit<kE4m3, kNC, false>(a, u, lds);
+  Source src = make_source(a, u);
+  State<kNC> s;
+  load_queries<kNC, false>(s, a, u);
+  run_unit<kE4m3, kNC, false>(a, u, src, s, lds);
 }
 
-// Joins the partials of each (token, kv head, query head).  kSubs groups of 16 lanes,
-// a lane for 4 dims, share a query.
-template <int kSubs, bool kDecode>
+// Joins the at most kSubs * kEach partials of each (token, kv head, query head).  kSubs
+// groups of 16 lanes, a lane for 4 dims, share a query.
+template <int kSubs, int kEach, bool kDecode>
 __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a) {
   constexpr int kLanes = 16 * kSubs;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -442,20 +535,29 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a) {
     n = (lim + len - 1) / len;
   }
   const int64_t p0 = th * a.splits * a.G + g;
-  float top = kNegInf;
-  for (int j = lane & (kLanes - 1); j < n; j += kLanes) top = fmaxf(top, a.m[p0 + (int64_t)j * a.G]);
-  for (int d = kLanes / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  // All of a lane's partials at once.  Those past n hold anything, but are there.
   const int sub = (tid >> 4) & (kSubs - 1), d0 = 4 * (lane & 15);
+  float mv[kEach], lv[kEach], top = kNegInf;
+  f32x4 x[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int64_t p = p0 + (int64_t)min(sub + kSubs * e, a.splits - 1) * a.G;
+    mv[e] = a.m[p];
+    lv[e] = a.l[p];
+    x[e] = *reinterpret_cast<const f32x4*>(a.acc + p * kD + d0);
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    if (sub + kSubs * e < n) top = fmaxf(top, mv[e]);
+  if constexpr (kSubs > 1) top = col_max(top);
   float sum = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int j = sub; j < n; j += kSubs) {
-    const int64_t p = p0 + (int64_t)j * a.G;
-    const float m = a.m[p], l = a.l[p];
-    const f32x4 x = *reinterpret_cast<const f32x4*>(a.acc + p * kD + d0);
-    const float c = m == top ? 1.f : fast_exp2(m - top);
-    sum += l * c;
-    o += x * c;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (sub + kSubs * e >= n) continue;
+    const float c = mv[e] == top ? 1.f : fast_exp2(mv[e] - top);
+    sum += lv[e] * c;
+    o += x[e] * c;
   }
   if constexpr (kSubs > 1) {
     sum = col_sum(sum);
@@ -476,21 +578,32 @@ struct Plan {
   int waves, splits, cols, n_tiles;
 };
 
+// Rows of at most 1024 slots whole, by one launch; longer ones in ranges of at least a
+// tile a wave, as many as let two workgroups a CU run at once, at least two from 4096
+// slots on.  MI355X, 2 kv heads of 7 queries, us in a replayed graph, in one piece /
+// in the best number of pieces: one row of 512 slots 5.5 / 7.3, 1024 7.6 / 7.5, 2048
+// 10.2 / 7.6, 16384 51.8 / 9.8; 16 rows of 1024 8.8 / 8.5; 64 of 512 7.0 / 8.7, of 32768
+// 169 / 87.  Two pieces a row where there are more pairs of a row and a kv head than
+// CUs: 160 rows of 8192 slots 72 / 65, 128 rows of 200 to 8192 36 / 31, but 200 rows of
+// 8192 79 / 84.  Eight waves to a row in one piece take one of 512 slots in 5.5 where
+// four take 6.1, but 200 rows of 1024 in 17.6 where those take 15.7.
 Plan decode_plan(int B, int KVH, int cap) {
-  const int64_t pairs = (int64_t)B * KVH, tiles = (cap + kTile - 1) / kTile;
-  Plan p = {4, 1, 1, 1};
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, (tiles + p.waves - 1) / p.waves, 2 * kCus / pairs}));
-  return p;
+  const int64_t pairs = (int64_t)B * KVH, tiles = ((int64_t)cap + kTile - 1) / kTile;
+  if (tiles <= 16) return {pairs <= kCus / 2 ? 8 : 4, 1, 1, 1};
+  const int64_t fill = std::max<int64_t>(2 * kCus / pairs, tiles >= 64 ? 2 : 1);
+  return {4, (int)std::min<int64_t>({(tiles + 3) / 4, fill, kMaxSplits}), 1, 1};
 }
 
+// As many splits as let two workgroups a CU run at once.
 Plan extend_plan(int B, int KVH, int G, int total, int max_seqlen, int cap) {
   Plan p = {4, 1, 1, 1};
   const int64_t rows = (int64_t)max_seqlen * G;
-  p.cols = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.cols = rows <= 16 ? 1 : 2;
   p.n_tiles = (int)((rows + 16 * p.cols - 1) / (16 * p.cols));
-  const int64_t units = (int64_t)KVH * std::min<int64_t>((int64_t)B * p.n_tiles, (int64_t)total * G / (16 * p.cols) + B);
-  const int64_t tiles = (cap + kTile - 1) / kTile;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, (tiles + p.waves - 1) / p.waves, 2 * kCus / units}));
+  const int64_t units = (int64_t)KVH * std::min<int64_t>((int64_t)B * p.n_tiles,
+                                                         (int64_t)total * G / (16 * p.cols) + B);
+  const int64_t tiles = ((int64_t)cap + kTile - 1) / kTile;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, (tiles + 3) / 4, 2 * kCus / units}));
   return p;
 }
 
@@ -499,10 +612,10 @@ size_t lds_bytes(int waves) { return waves * (256 * sizeof(f32x4) + 16 * sizeof(
 template <bool kDecode>
 int launch_merge(const AttnArgs& a, hipStream_t st) {
   const int64_t queries = (int64_t)a.tokens * a.p.kvh * a.G;
-  if (a.splits <= 8)
-    hipLaunchKernelGGL((merge_kernel<1, kDecode>), dim3((unsigned)((queries + 15) / 16)), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((merge_kernel<4, kDecode>), dim3((unsigned)((queries + 3) / 4)), dim3(256), 0, st, a);
+  const dim3 all((unsigned)((queries + 15) / 16)), quarter((unsigned)((queries + 3) / 4)), b(256);
+  if (a.splits <= 4) hipLaunchKernelGGL((merge_kernel<1, 4, kDecode>), all, b, 0, st, a);
+  else if (a.splits <= 16) hipLaunchKernelGGL((merge_kernel<4, 4, kDecode>), quarter, b, 0, st, a);
+  else hipLaunchKernelGGL((merge_kernel<4, 16, kDecode>), quarter, b, 0, st, a);
   return (int)hipGetLastError();
 }
 
@@ -526,24 +639,24 @@ int launch_extend(const AttnArgs& a, int code, int waves, hipStream_t st) {
 }
 
 // Checks and fills what the entry points share.
-int fill_args(AttnArgs& a, const void* q, const QfPool8* pool, const int64_t* last, int64_t last_sb,
-              int B, int tokens, int G, int D, int cap, float scale) {
+int fill_args(AttnArgs& a, const void* q, const QfPool8& pool, const int64_t* last, int64_t last_sb,
+              int64_t B, int64_t tokens, int64_t G, int64_t D, double scale) {
   if (D != kD || G < 1 || G > 16) return QF_ERR_UNSUPPORTED;
   a = AttnArgs{};
   const int rc = make_pool(pool, a.p);
   if (rc != QF_OK) return rc;
-  if (!q || !last || B < 1 || tokens < 1 || cap < 1 || cap > pool->pages_per_row * pool->page_size ||
-      pool->layers != 1 || !(scale > 0.f) || !(scale < 1e30f))
+  if (!q || !last || B < 1 || tokens < 1 || pool.layers != 1 || !(scale > 0.) || !(scale < 1e30) ||
+      (reinterpret_cast<uintptr_t>(q) & 15u) != 0)
     return QF_ERR_INVALID_ARG;
-  if ((reinterpret_cast<uintptr_t>(q) & 15u) != 0) return QF_ERR_INVALID_ARG;
-  if (B > 0x3fffffff || (int64_t)tokens * G > 0x3fffffff || (int64_t)tokens * a.p.kvh * G > 0x7fffffff ||
-      (int64_t)cap + tokens > 0x7fffffff - kTile)
+  a.cap = row_cap(a.p);
+  if (B > 0x3fffffff || tokens > 0x3fffffff / G || tokens * G > 0x7fffffff / a.p.kvh ||
+      a.cap + tokens > 0x7fffffff - kTile)
     return QF_ERR_UNSUPPORTED;
   a.q = static_cast<const f16*>(q);
   a.last = last;
   a.last_sb = last_sb;
-  a.B = B; a.tokens = tokens; a.G = G; a.cap = cap;
-  a.scale_log2 = scale * kLog2e;
+  a.B = (int)B; a.tokens = (int)tokens; a.G = (int)G;
+  a.scale_log2 = (float)scale * kLog2e;
   a.m_unit = 1.f;
   return QF_OK;
 }
@@ -563,6 +676,23 @@ int set_parts(AttnArgs& a, void* ws, int64_t ws_bytes) {
   return QF_OK;
 }
 
+int decode_args(AttnArgs& a, const QfDecode8* h) {
+  if (!h) return QF_ERR_INVALID_ARG;
+  const int rc = fill_args(a, h->q, h->pool, h->kv_last, h->kv_last_sb, h->B, h->B, h->G, h->D, h->scale);
+  if (rc != QF_OK) return rc;
+  if (((h->q_sb | h->q_sh | h->q_sg) & 7) != 0) return QF_ERR_INVALID_ARG;
+  a.q_st = h->q_sb; a.q_sh = h->q_sh; a.q_sg = h->q_sg;
+  if ((h->k_new == nullptr) != (h->v_new == nullptr) ||
+      ((reinterpret_cast<uintptr_t>(h->k_new) | reinterpret_cast<uintptr_t>(h->v_new)) & 15u) != 0 ||
+      (h->k_new != nullptr && ((h->kn_sb | h->kn_sh | h->vn_sb | h->vn_sh) & 7) != 0))
+    return QF_ERR_INVALID_ARG;
+  a.kn = static_cast<const f16*>(h->k_new);
+  a.kn_sb = h->kn_sb; a.kn_sh = h->kn_sh;
+  a.vn = static_cast<const f16*>(h->v_new);
+  a.vn_sb = h->vn_sb; a.vn_sh = h->vn_sh;
+  return QF_OK;
+}
+
 }  // namespace kv8
 }  // namespace qf
 
@@ -573,50 +703,40 @@ extern "C" int64_t qf_decode_attn_paged8_workspace(int B, int KVH, int G, int ca
   return part_bytes((int64_t)B * KVH * G, decode_plan(B, KVH, cap).splits);
 }
 
-extern "C" int qf_decode_attn_paged8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sg,
-                                     const QfPool8* pool, const int64_t* kv_last, int64_t kv_last_sb,
-                                     void* ws, int64_t ws_bytes, void* out, int64_t o_sb, int64_t o_sh,
-                                     int64_t o_sg, int B, int G, int D, float scale, void* stream) {
+extern "C" int qf_decode_attn_paged8(const QfDecode8* h, void* stream) {
   using namespace qf;
   using namespace qf::kv8;
   AttnArgs a;
-  const int cap = pool ? pool->pages_per_row * pool->page_size : 0;
-  int rc = fill_args(a, q, pool, kv_last, kv_last_sb, B, B, G, D, cap, scale);
+  int rc = decode_args(a, h);
   if (rc != QF_OK) return rc;
-  if (((q_sb | q_sh | q_sg) & 7) != 0 || bad_out(out, o_sb, o_sh, o_sg)) return QF_ERR_INVALID_ARG;
-  a.q_st = q_sb; a.q_sh = q_sh; a.q_sg = q_sg;
-  a.out = static_cast<f16*>(out);
-  a.o_st = o_sb; a.o_sh = o_sh; a.o_sg = o_sg;
-  const Plan p = decode_plan(B, pool->KVH, cap);
+  if (bad_out(h->out, h->o_sb, h->o_sh, h->o_sg)) return QF_ERR_INVALID_ARG;
+  a.out = static_cast<f16*>(h->out);
+  a.o_st = h->o_sb; a.o_sh = h->o_sh; a.o_sg = h->o_sg;
+  const Plan p = decode_plan(a.B, a.p.kvh, a.cap);
   a.splits = p.splits;
-  rc = set_parts(a, ws, ws_bytes);
+  rc = set_parts(a, h->ws, h->ws_bytes);
   if (rc != QF_OK) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  rc = launch_decode(a, pool->code, p.waves, st);
+  rc = launch_decode(a, (int)h->pool.code, p.waves, st);
   return rc == 0 && a.splits > 1 ? launch_merge<true>(a, st) : rc;
 }
 
-extern "C" int qf_decode_split_paged8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sg,
-                                      const QfPool8* pool, const int64_t* kv_last, int64_t kv_last_sb,
-                                      float* acc, float* m, float* l, int splits, int B, int G, int D,
-                                      float scale, void* stream) {
+extern "C" int qf_decode_split_paged8(const QfDecode8* h, float* acc, float* m, float* l, int splits,
+                                      void* stream) {
   using namespace qf;
   using namespace qf::kv8;
   AttnArgs a;
-  const int cap = pool ? pool->pages_per_row * pool->page_size : 0;
-  const int rc = fill_args(a, q, pool, kv_last, kv_last_sb, B, B, G, D, cap, scale);
+  const int rc = decode_args(a, h);
   if (rc != QF_OK) return rc;
-  if (((q_sb | q_sh | q_sg) & 7) != 0 || !acc || (reinterpret_cast<uintptr_t>(acc) & 15u) != 0 || !m ||
-      !l || splits < 1 || splits > 1024)
+  if (!acc || (reinterpret_cast<uintptr_t>(acc) & 15u) != 0 || !m || !l || splits < 1 || splits > 1024)
     return QF_ERR_INVALID_ARG;
-  a.q_st = q_sb; a.q_sh = q_sh; a.q_sg = q_sg;
   a.acc = acc;
   a.m = m;
   a.l = l;
   a.m_unit = kLn2;
   a.fill = 1;
   a.splits = splits;
-  return launch_decode(a, pool->code, 4, static_cast<hipStream_t>(stream));
+  return launch_decode(a, (int)h->pool.code, 4, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t qf_prefill_extend_paged8_workspace(int B, int QH, int KVH, int total, int max_seqlen,
@@ -628,40 +748,36 @@ extern "C" int64_t qf_prefill_extend_paged8_workspace(int B, int QH, int KVH, in
   return part_bytes((int64_t)total * QH, extend_plan(B, KVH, QH / KVH, total, max_seqlen, cap).splits);
 }
 
-extern "C" int qf_prefill_extend_paged8(
-    const void* q, int64_t q_sh, int64_t q_sn, const void* k, int64_t k_sh, int64_t k_sn, const void* v,
-    int64_t v_sh, int64_t v_sn, const int32_t* cu_seqlens, int total, int max_seqlen,
-    const int64_t* context, int64_t ctx_sb, const void* cos, const void* sin, int64_t cs_sn,
-    const QfPool8* pool, int cap, void* ws, int64_t ws_bytes, void* out, int64_t o_sh, int64_t o_sn,
-    int B, int QH, int D, float scale, void* stream) {
+extern "C" int qf_prefill_extend_paged8(const QfExtend8* h, void* stream) {
   using namespace qf;
   using namespace qf::kv8;
-  if (!pool || pool->KVH < 1 || QH < pool->KVH || QH % pool->KVH != 0) return QF_ERR_INVALID_ARG;
-  const int G = QH / pool->KVH;
+  if (!h) return QF_ERR_INVALID_ARG;
+  const QfRows8& r = h->rows;
+  if (r.pool.KVH < 1 || h->QH < r.pool.KVH || h->QH % r.pool.KVH != 0) return QF_ERR_INVALID_ARG;
+  const int64_t G = h->QH / r.pool.KVH;
   AttnArgs a;
-  int rc = fill_args(a, q, pool, context, ctx_sb, B, total, G, D, cap, scale);
+  int rc = fill_args(a, h->q, r.pool, r.first, r.first_sb, r.B, r.total, G, r.D, h->scale);
   if (rc != QF_OK) return rc;
-  if (!cu_seqlens || max_seqlen < 1 || max_seqlen > total || ((q_sh | q_sn) & 7) != 0 ||
-      bad_out(out, o_sn, o_sh, 0))
+  if (!r.cu_seqlens || r.max_seqlen < 1 || r.max_seqlen > r.total || h->cap < 1 || h->cap > a.cap ||
+      ((h->q_sh | h->q_sn) & 7) != 0 || bad_out(h->out, h->o_sn, h->o_sh, 0))
     return QF_ERR_INVALID_ARG;
-  a.q_st = q_sn; a.q_sh = G * q_sh; a.q_sg = q_sh;
-  a.out = static_cast<f16*>(out);
-  a.o_st = o_sn; a.o_sh = G * o_sh; a.o_sg = o_sh;
-  a.cu = cu_seqlens;
-  a.cos = static_cast<const f16*>(cos);
-  a.sin = static_cast<const f16*>(sin);
-  a.cs_sn = cs_sn;
-  const Plan p = extend_plan(B, pool->KVH, G, total, max_seqlen, cap);
+  a.cap = (int)h->cap;
+  a.q_st = h->q_sn; a.q_sh = G * h->q_sh; a.q_sg = h->q_sh;
+  a.out = static_cast<f16*>(h->out);
+  a.o_st = h->o_sn; a.o_sh = G * h->o_sh; a.o_sg = h->o_sh;
+  a.cu = r.cu_seqlens;
+  a.cos = static_cast<const f16*>(r.cos);
+  a.sin = static_cast<const f16*>(r.sin);
+  a.cs_sn = r.cs_sn;
+  const Plan p = extend_plan(a.B, a.p.kvh, a.G, a.tokens, (int)r.max_seqlen, a.cap);
   a.splits = p.splits;
   a.n_tiles = p.n_tiles;
-  rc = set_parts(a, ws, ws_bytes);
+  rc = set_parts(a, h->ws, h->ws_bytes);
   if (rc != QF_OK) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  rc = append(k, 0, k_sh, k_sn, v, 0, v_sh, v_sn, cu_seqlens, total, max_seqlen, context, ctx_sb, cos, sin,
-              cs_sn, pool, cap, B, D, st);
+  rc = append(r, a.cap, st);
   if (rc != QF_OK) return rc;
-  if (p.cols == 1) rc = launch_extend<1>(a, pool->code, p.waves, st);
-  else if (p.cols == 2) rc = launch_extend<2>(a, pool->code, p.waves, st);
-  else rc = launch_extend<4>(a, pool->code, p.waves, st);
+  const int code = (int)r.pool.code;
+  rc = p.cols == 1 ? launch_extend<1>(a, code, p.waves, st) : launch_extend<2>(a, code, p.waves, st);
   return rc == 0 && a.splits > 1 ? launch_merge<false>(a, st) : rc;
 }

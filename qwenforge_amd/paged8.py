@@ -28,11 +28,14 @@ where a few channels are far larger than the others.
 
 from __future__ import annotations
 
+import functools
+import struct
+
 import torch
 
 from . import _lib, paged
-from .ops import HEAD_DIM, _ptr, _scratch_args
-from .paged import _call, _check_page_size, _check_rows, _half, _int_rows, _page_list, _workspace
+from .ops import HEAD_DIM, _scratch_args
+from .paged import MAX_PAGE, _check_page_size, _check_rows, _half, _int_rows, _page_list
 
 BLOCK = 16
 CODES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
@@ -90,48 +93,96 @@ class PagedKv8Cache(paged.PagedKvCache):
 # argument helpers
 # --------------------------------------------------------------------------
 
-def _pools8(pools, block_table, batch: int, index: int, layers: int = 0):
-    """The ``Pool8`` of a layer's pools -- with ``layers``, of ``layers`` layers' as
-    ``PagedKv8Cache.all_pools`` -- and the rows' table on GPU ``index``, and the slots
-    of a row."""
+# The structs of the C ABI, all of 8-byte fields: packed here in one go, where
+# handing that many arguments to ctypes would take longer than the launch.
+_ROWS = struct.Struct("=36q")         # QfPool8 (18), then QfRows8's own
+_DECODE = struct.Struct("=39qd")      # QfPool8, then QfDecode8's own
+_EXTEND = struct.Struct("=46qd")      # QfRows8, then QfExtend8's own
+
+
+def _explain_pools(pools, index: int, lead: int) -> None:
+    """Raises for what ``_pools8`` refused."""
     if not isinstance(pools, (tuple, list)) or len(pools) != 4:
         raise TypeError("pools must be (k, v, k_scale, v_scale)")
     k, v, ks, vs = pools
-    for name, t in (("k", k), ("v", v), ("k_scale", ks), ("v_scale", vs)):
-        if not isinstance(t, torch.Tensor) or t.get_device() != index or index < 0:
+    for name, t in zip(("k", "v", "k_scale", "v_scale"), pools):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != index:
             raise RuntimeError(f"{name} must be a tensor on cuda:{index}; there is no CPU path")
-    kind = _KINDS.get(k.dtype)
-    if kind is None or v.dtype is not k.dtype or ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
+    if k.dtype not in _KINDS or v.dtype is not k.dtype or ks.dtype is not torch.float32 \
+            or vs.dtype is not torch.float32:
         raise TypeError("k and v must both be int8 or float8_e4m3fn, k_scale and v_scale float32 "
                         f"(got {k.dtype}, {v.dtype}, {ks.dtype}, {vs.dtype})")
-    lead = 1 if layers else 0
-    shape, strides = k.shape, k.stride()
-    if len(shape) != 4 + lead or (layers and shape[0] != layers):
-        raise ValueError(f"k must be {'(layers, ' if layers else '('}n_pages, KVH, P, 64) (got {tuple(shape)})")
-    n_pages, kvh, page, d = shape[lead:]
+    shape = tuple(k.shape)
+    if len(shape) != 4 + lead or 0 in shape or shape[-1] != HEAD_DIM:
+        raise ValueError(f"k must be {'(layers, ' if lead else '('}n_pages, KVH, P, 64) (got {shape})")
+    page, outer = shape[-2], shape[:lead + 2]
     _check_page_size(page)
-    if (d != HEAD_DIM or n_pages < 1 or kvh < 1
-            or v.shape != (*shape[:lead + 2], page // 64, HEAD_DIM, 64)
-            or ks.shape != (*shape[:lead + 2], page // BLOCK) or vs.shape != ks.shape):
-        raise ValueError(f"pools of {n_pages} pages of {kvh} heads and {page} slots need v (n_pages, KVH, "
-                         f"P / 64, 64, 64) and scales (n_pages, KVH, P / {BLOCK})")
-    scale_strides = ks.stride()
-    outer, scale_outer = strides[:lead + 2], scale_strides[:lead + 2]
-    if (v.stride() != (*outer, 4096, 64, 1) or strides[lead + 2:] != (64, 1)
-            or vs.stride() != scale_strides or scale_strides[-1] != 1):
-        raise ValueError("k and v must have the same page and head strides, and so must the scales; "
-                         "what a page and head holds must be contiguous")
+    if v.shape != (*outer, page // 64, HEAD_DIM, 64) or ks.shape != (*outer, page // BLOCK) or vs.shape != ks.shape:
+        raise ValueError(f"pools of {outer} pages and heads of {page} slots need v (.., P / 64, 64, 64) and "
+                         f"scales (.., P / {BLOCK})")
+    raise ValueError("k and v must have the same page and head strides, and so must the scales; "
+                     "what a page and head holds must be contiguous")
+
+
+def _pools8(pools, block_table, batch: int, index: int, lead: int = 0):
+    """``QfPool8``'s fields for a layer's pools -- with ``lead`` 1 for all layers', as
+    ``PagedKv8Cache.all_pools`` -- and the rows' table on GPU ``index``; the pools' kv
+    heads and the slots of a row.  Reads as few tensor properties as it can and
+    explains itself only when it refuses."""
+    try:
+        k, v, ks, vs = pools
+        shape, strides, scale_strides = k.shape, k.stride(), ks.stride()
+        *_, n_pages, kvh, page, d = shape
+        kind = _KINDS[k.dtype]
+        ok = (len(shape) == 4 + lead and d == HEAD_DIM and n_pages * kvh > 0 and shape[0] > 0
+              and 64 <= page <= MAX_PAGE and not page & (page - 1)
+              and v.shape == (*shape[:-2], page // 64, HEAD_DIM, 64) and ks.shape == (*shape[:-2], page // BLOCK)
+              and vs.shape == ks.shape
+              and v.stride() == (*strides[:-2], 4096, 64, 1) and strides[-2:] == (64, 1)
+              and vs.stride() == scale_strides and scale_strides[-1] == 1
+              and v.dtype is k.dtype and ks.dtype is torch.float32 and vs.dtype is torch.float32
+              and k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == index >= 0)
+    except (AttributeError, KeyError, TypeError, ValueError):
+        ok = False
+    if not ok:
+        _explain_pools(pools, index, lead)
     if (not isinstance(block_table, torch.Tensor) or block_table.dtype is not torch.int32
             or block_table.get_device() != index):
         raise TypeError(f"block_table must be an int32 tensor on cuda:{index}")
-    if block_table.dim() != 2 or block_table.shape[0] != batch or block_table.stride(1) != 1:
+    table_shape, table_strides = block_table.shape, block_table.stride()
+    if len(table_shape) != 2 or table_shape[0] != batch or table_strides[1] != 1:
         raise ValueError(f"block_table must be (B={batch}, pages_per_row) with unit inner stride")
-    ppr = block_table.shape[1]
-    if lead == 0:
-        outer, scale_outer = (0, *outer), (0, *scale_outer)
-    return _lib.Pool8(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), *outer, *scale_outer,
-                      block_table.data_ptr(), block_table.stride(0), ppr, n_pages, page, layers or 1, kvh,
-                      kind), ppr * page
+    ppr = table_shape[1]
+    if lead:
+        outer = (*strides[:3], *scale_strides[:3])
+    else:
+        outer = (0, *strides[:2], 0, *scale_strides[:2])
+    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), *outer, block_table.data_ptr(),
+            table_strides[0], ppr, n_pages, page, shape[0] if lead else 1, kvh, kind), kvh, ppr * page
+
+
+def _call8(name: str, index: int, *args) -> None:
+    """Entry point ``name`` on GPU ``index`` and its current stream."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name: str, *sizes) -> int:
+    need = getattr(_lib.load(), name)(*sizes)
+    if need < 0:
+        _lib.check(need, name)
+    return need
+
+
+def _scratch(need: int, device):
+    return torch.empty(need, device=device, dtype=torch.uint8) if need else None
 
 
 def _packed(cu_seqlens, total: int, max_seqlen: int, first, name: str, index: int, lengths):
@@ -161,6 +212,10 @@ def _rope(cos, sin, total: int, index: int):
     return cos, sin, cos.stride(0)
 
 
+def _address(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 # --------------------------------------------------------------------------
 # writing, reading, copying
 # --------------------------------------------------------------------------
@@ -185,26 +240,25 @@ def append_paged8(key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tens
     that grew.  Tokens with infinities or NaN make their blocks read as NaN until
     the first slot is written again.  Pages written to must be the row's own.
     """
-    layers = key.shape[0] if isinstance(key, torch.Tensor) and key.dim() == 4 else 0
-    lead = 1 if layers else 0
+    lead = 1 if isinstance(key, torch.Tensor) and key.dim() == 4 else 0
     _half("key", key, 3 + lead)
     _half("value", value, 3 + lead)
-    index = key.get_device()
-    shape = key.shape
+    index, shape = key.get_device(), key.shape
     total, kvh = shape[lead], shape[lead + 1]
     if value.shape != shape or value.get_device() != index:
         raise ValueError(f"key and value must be alike (got {tuple(shape)}, {tuple(value.shape)})")
     b, ctx_sb = _packed(cu_seqlens, total, max_seqlen, context, "context", index, lengths)
-    pool, cap = _pools8(pools, block_table, b, index, layers)
-    if pool.KVH != kvh:
-        raise ValueError(f"pools hold {pool.KVH} kv heads, key {kvh}")
+    pool, heads, cap = _pools8(pools, block_table, b, index, lead)
+    if heads != kvh or (lead and pool[15] != shape[0]):
+        raise ValueError(f"pools of {pool[15]} layers and {heads} kv heads do not match key {tuple(shape)}")
     if max_seqlen > cap:
         raise ValueError(f"max_seqlen exceeds the row capacity {cap}")
     cos, sin, cs_sn = _rope(cos, sin, total, index)
     ks, vs = key.stride(), value.stride()
-    _call("qf_append_paged8", index, key.data_ptr(), ks[0] if layers else 0, ks[lead + 1], ks[lead],
-          value.data_ptr(), vs[0] if layers else 0, vs[lead + 1], vs[lead], cu_seqlens.data_ptr(), total,
-          max_seqlen, context.data_ptr(), ctx_sb, _ptr(cos), _ptr(sin), cs_sn, pool, b, HEAD_DIM)
+    _call8("qf_append_paged8", index, _ROWS.pack(
+        *pool, key.data_ptr(), ks[0] if lead else 0, ks[lead + 1], ks[lead], value.data_ptr(),
+        vs[0] if lead else 0, vs[lead + 1], vs[lead], cu_seqlens.data_ptr(), total, max_seqlen,
+        context.data_ptr(), ctx_sb, _address(cos), _address(sin), cs_sn, b, HEAD_DIM))
 
 
 def read_paged8(pools, block_table: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int,
@@ -222,20 +276,19 @@ def read_paged8(pools, block_table: torch.Tensor, cu_seqlens: torch.Tensor, max_
     k = pools[0] if isinstance(pools, (tuple, list)) and len(pools) == 4 else None
     if not isinstance(k, torch.Tensor) or not k.is_cuda or k.dim() not in (4, 5):
         raise RuntimeError("pools must be (k, v, k_scale, v_scale) HIP device tensors; there is no CPU path")
-    index, layers = k.get_device(), k.shape[0] if k.dim() == 5 else 0
+    index, lead = k.get_device(), k.dim() - 4
     if total is None:
         total = sum(lengths) if lengths is not None else int(cu_seqlens[-1])
     b, first_sb = _packed(cu_seqlens, total, max_seqlen, first, "first", index, lengths)
-    pool, _ = _pools8(pools, block_table, b, index, layers)
-    shape = (2, layers or 1, total, pool.KVH, HEAD_DIM)
-    out = torch.empty(shape, device=k.device, dtype=torch.float16)
-    step = total * pool.KVH * HEAD_DIM
-    at = out.data_ptr()
-    _call("qf_read_paged8", index, at, step, HEAD_DIM, pool.KVH * HEAD_DIM, at + 2 * step * (layers or 1), step,
-          HEAD_DIM, pool.KVH * HEAD_DIM, cu_seqlens.data_ptr(), total, max_seqlen, first.data_ptr(), first_sb,
-          pool, b, HEAD_DIM)
-    k, v = out.unbind(0)
-    return (k, v) if layers else (k[0], v[0])
+    pool, kvh, _ = _pools8(pools, block_table, b, index, lead)
+    layers, row = pool[15], kvh * HEAD_DIM
+    out = torch.empty((2, layers, total, kvh, HEAD_DIM) if lead else (2, total, kvh, HEAD_DIM),
+                      device=k.device, dtype=torch.float16)
+    at, step = out.data_ptr(), total * row
+    _call8("qf_read_paged8", index, _ROWS.pack(
+        *pool, at, step, HEAD_DIM, row, at + 2 * step * layers, step, HEAD_DIM, row, cu_seqlens.data_ptr(), total,
+        max_seqlen, first.data_ptr(), first_sb, 0, 0, 0, b, HEAD_DIM))
+    return out.unbind(0)
 
 
 def copy_pages8(store: torch.Tensor, src, dst) -> None:
@@ -263,27 +316,40 @@ def copy_pages8(store: torch.Tensor, src, dst) -> None:
         if len(set(b)) != n or set(a) & set(b):
             raise ValueError("no page may be written twice, or both written and read")
         src, dst = torch.tensor([a, b], dtype=torch.int32).to(store.device)
-    _call("qf_copy_pages8", index, store.data_ptr(), layers, n_pages * size, size, size, src.data_ptr(),
-          dst.data_ptr(), n, n_pages)
+    _call8("qf_copy_pages8", index, store.data_ptr(), layers, n_pages * size, size, size, src.data_ptr(),
+           dst.data_ptr(), n, n_pages)
 
 
 # --------------------------------------------------------------------------
 # attention
 # --------------------------------------------------------------------------
 
-def _decode_args(grouped, pools, block_table, kv_last):
+def _decode_args(grouped, pools, block_table, kv_last, key, value):
+    """``QfDecode8``'s fields up to kv_last's, the call's GPU, shape and capacity, and
+    the fields of the new tokens."""
     _half("grouped", grouped, 4)
-    b, kvh, _, _ = grouped.shape
-    index = grouped.get_device()
-    pool, cap = _pools8(pools, block_table, b, index)
-    if pool.KVH != kvh:
-        raise ValueError(f"pools hold {pool.KVH} kv heads, grouped {kvh}")
-    return index, pool, cap, _int_rows("kv_last", kv_last, b, torch.int64, index)
+    shape, index = grouped.shape, grouped.get_device()
+    pool, kvh, cap = _pools8(pools, block_table, shape[0], index)
+    if kvh != shape[1]:
+        raise ValueError(f"pools hold {kvh} kv heads, grouped {shape[1]}")
+    last_sb = _int_rows("kv_last", kv_last, shape[0], torch.int64, index)
+    strides, new = grouped.stride(), (0, 0, 0, 0, 0, 0)
+    if (key is None) != (value is None):
+        raise ValueError("key and value go together")
+    if key is not None:
+        for name, t in (("key", key), ("value", value)):
+            _half(name, t, 3)
+            if t.shape != (shape[0], kvh, HEAD_DIM) or t.get_device() != index:
+                raise ValueError(f"{name} must be {(shape[0], kvh, HEAD_DIM)} on cuda:{index}")
+        new = (key.data_ptr(), *key.stride()[:2], value.data_ptr(), *value.stride()[:2])
+    return (*pool, grouped.data_ptr(), strides[0], strides[1], strides[2], kv_last.data_ptr(),
+            last_sb), index, shape, cap, new
 
 
 def flash_decode_attention_paged8(grouped: torch.Tensor, pools, block_table: torch.Tensor,
                                   kv_last: torch.Tensor, scale: float | None = None,
-                                  out: torch.Tensor | None = None) -> torch.Tensor:
+                                  out: torch.Tensor | None = None, key: torch.Tensor | None = None,
+                                  value: torch.Tensor | None = None) -> torch.Tensor:
     """Decode attention of a batch over pages held in 8 bits.
 
     grouped (B, KVH, G, 64) fp16, G at most 16; ``pools`` one layer's; block_table (B,
@@ -291,35 +357,39 @@ def flash_decode_attention_paged8(grouped: torch.Tensor, pools, block_table: tor
     device, and a row with a negative one (parked) gets zeros.  ``scale`` defaults to
     64 ** -0.5.  Returns (B, KVH, G, 64), written to ``out`` if given.  A row's result
     does not depend on the other rows.
+
+    With ``key`` and ``value`` (B, KVH, 64) each row's new token is first appended at slot
+    kv_last, as ``append_paged8`` does, in the same launch: a decoding step's.
     """
-    index, pool, cap, last_sb = _decode_args(grouped, pools, block_table, kv_last)
-    b, kvh, g, d = grouped.shape
+    head, index, shape, cap, new = _decode_args(grouped, pools, block_table, kv_last, key, value)
+    b, kvh, g, d = shape
     if out is None:
-        out = (torch.empty_like(grouped) if grouped.is_contiguous()
-               else torch.empty((b, kvh, g, d), device=grouped.device, dtype=torch.float16))
+        out = torch.empty(shape, device=grouped.device, dtype=torch.float16)
     else:
         _half("out", out, 4)
-        if out.shape != grouped.shape or out.get_device() != index:
-            raise ValueError(f"out must be {tuple(grouped.shape)} on {grouped.device}")
-    need = _lib.load().qf_decode_attn_paged8_workspace(b, kvh, g, cap)
-    ws = None if need == 0 else _workspace(need, "qf_decode_attn_paged8_workspace", grouped.device)
-    _call("qf_decode_attn_paged8", index, grouped.data_ptr(), *grouped.stride()[:3], pool, kv_last.data_ptr(),
-          last_sb, _ptr(ws), max(need, 0), out.data_ptr(), *out.stride()[:3], b, g, d,
-          d ** -0.5 if scale is None else scale)
+        if out.shape != shape or out.get_device() != index:
+            raise ValueError(f"out must be {tuple(shape)} on {grouped.device}")
+    need = _workspace_bytes("qf_decode_attn_paged8_workspace", b, kvh, g, cap)
+    ws = _scratch(need, grouped.device)
+    strides = out.stride()
+    _call8("qf_decode_attn_paged8", index, _DECODE.pack(
+        *head, out.data_ptr(), strides[0], strides[1], strides[2], _address(ws), need, b, g, d, *new,
+        d ** -0.5 if scale is None else scale))
     return out
 
 
 def flash_decode_split_paged8(grouped: torch.Tensor, pools, block_table: torch.Tensor, flash,
-                              kv_last: torch.Tensor, scale: float | None = None):
+                              kv_last: torch.Tensor, scale: float | None = None,
+                              key: torch.Tensor | None = None, value: torch.Tensor | None = None):
     """The split launch alone: fills ``flash[0:3]`` = (acc, m, l) of
     ``ops.make_flash_scratch``, for ``ops.flash_decode_combine`` or
-    ``step_ops.attn_merge_o_proj``."""
-    index, pool, cap, last_sb = _decode_args(grouped, pools, block_table, kv_last)
+    ``step_ops.attn_merge_o_proj``; ``key`` and ``value`` as in
+    ``flash_decode_attention_paged8``."""
+    head, index, (b, _, g, d), cap, new = _decode_args(grouped, pools, block_table, kv_last, key, value)
     acc, m, l, _, _, splits, _, _ = _scratch_args(grouped, cap, None, flash, kv_last)
-    b, _, g, d = grouped.shape
-    _call("qf_decode_split_paged8", index, grouped.data_ptr(), *grouped.stride()[:3], pool, kv_last.data_ptr(),
-          last_sb, acc.data_ptr(), m.data_ptr(), l.data_ptr(), splits, b, g, d,
-          d ** -0.5 if scale is None else scale)
+    _call8("qf_decode_split_paged8", index, _DECODE.pack(
+        *head, 0, 0, 0, 0, 0, 0, b, g, d, *new, d ** -0.5 if scale is None else scale),
+        acc.data_ptr(), m.data_ptr(), l.data_ptr(), splits)
     return acc, m, l
 
 
@@ -340,17 +410,17 @@ def prefill_extend_paged8(query: torch.Tensor, key: torch.Tensor, value: torch.T
     _half("query", query, 3)
     _half("key", key, 3)
     _half("value", value, 3)
-    total, qh, d = query.shape
-    kvh = key.shape[1]
-    if key.shape[0] != total or value.shape != key.shape or kvh < 1 or qh % kvh != 0:
+    (total, qh, d), shape = query.shape, key.shape
+    kvh = shape[1]
+    if shape[0] != total or value.shape != shape or kvh < 1 or qh % kvh != 0:
         raise ValueError("packed extension shapes: query (T, QH, D), key/value (T, KVH, D)")
     index = query.get_device()
     if key.get_device() != index or value.get_device() != index:
         raise ValueError(f"query, key and value must be on one device ({query.device})")
     b, ctx_sb = _packed(cu_seqlens, total, max_seqlen, context, "context", index, lengths)
-    pool, cap = _pools8(pools, block_table, b, index)
-    if pool.KVH != kvh:
-        raise ValueError(f"pools hold {pool.KVH} kv heads, key {kvh}")
+    pool, heads, cap = _pools8(pools, block_table, b, index)
+    if heads != kvh:
+        raise ValueError(f"pools hold {heads} kv heads, key {kvh}")
     if max_slots is not None:
         if not max_seqlen <= max_slots <= cap:
             raise ValueError(f"max_slots must be in [{max_seqlen}, {cap}] (got {max_slots})")
@@ -359,11 +429,11 @@ def prefill_extend_paged8(query: torch.Tensor, key: torch.Tensor, value: torch.T
         raise ValueError(f"max_seqlen exceeds the row capacity {cap}")
     cos, sin, cs_sn = _rope(cos, sin, total, index)
     out = torch.empty((total, qh, d), device=query.device, dtype=torch.float16)
-    need = _lib.load().qf_prefill_extend_paged8_workspace(b, qh, kvh, total, max_seqlen, cap)
-    ws = None if need == 0 else _workspace(need, "qf_prefill_extend_paged8_workspace", query.device)
+    need = _workspace_bytes("qf_prefill_extend_paged8_workspace", b, qh, kvh, total, max_seqlen, cap)
+    ws = _scratch(need, query.device)
     qs, ks, vs = query.stride(), key.stride(), value.stride()
-    _call("qf_prefill_extend_paged8", index, query.data_ptr(), qs[1], qs[0], key.data_ptr(), ks[1], ks[0],
-          value.data_ptr(), vs[1], vs[0], cu_seqlens.data_ptr(), total, max_seqlen, context.data_ptr(), ctx_sb,
-          _ptr(cos), _ptr(sin), cs_sn, pool, cap, _ptr(ws), max(need, 0), out.data_ptr(), d, qh * d, b, qh, d,
-          d ** -0.5 if scale is None else scale)
+    _call8("qf_prefill_extend_paged8", index, _EXTEND.pack(
+        *pool, key.data_ptr(), 0, ks[1], ks[0], value.data_ptr(), 0, vs[1], vs[0], cu_seqlens.data_ptr(), total,
+        max_seqlen, context.data_ptr(), ctx_sb, _address(cos), _address(sin), cs_sn, b, d, query.data_ptr(), qs[1],
+        qs[0], out.data_ptr(), d, qh * d, cap, _address(ws), need, qh, d ** -0.5 if scale is None else scale))
     return out

@@ -16,7 +16,8 @@ pools (``paged.PagedKvCache``):
   its pages and extend them by their own prompts, and a long prefix is read once
   for all rows in each step;
 * ``generate_drafted`` runs a row's last token and drafted ones in one pass and
-  keeps those that the model would have drawn.
+  keeps those that the model would have drawn;
+* all three hold their cache in 8 bits on request (``kv_code``, ``paged8``).
 
 The captured step is the dense engine's step with the paged kernels: for 1..4
 rows the fused weight-streaming kernels (QKV + RoPE + paged append, paged
@@ -33,7 +34,7 @@ from collections import deque
 import torch
 import torch.nn.functional as F
 
-from . import ops, paged, prefill_ops, step_ops, verify, wide_ops
+from . import ops, paged, paged8, prefill_ops, step_ops, verify, wide_ops
 from .engine import DecodeEngine
 from .rope import cos_sin
 
@@ -61,11 +62,12 @@ def lookup_drafts(tokens, n: int, longest: int = 3) -> list:
 class PagedDecodeEngine(DecodeEngine):
     """``DecodeEngine`` whose decode step reads and writes a paged KV cache."""
 
-    def new_paged_cache(self, max_rows: int, n_pages: int, page_size: int,
-                        pages_per_row: int) -> paged.PagedKvCache:
+    def new_paged_cache(self, max_rows: int, n_pages: int, page_size: int, pages_per_row: int,
+                        code: str | None = None) -> paged.PagedKvCache:
+        """A cache in fp16, or in 8 bits of ``code`` (``paged8.CODES``)."""
         cfg = self.cfg
-        return paged.PagedKvCache(cfg.layers, cfg.kv_heads, n_pages, page_size, max_rows,
-                                  pages_per_row, self.device)
+        kind, more = (paged.PagedKvCache, ()) if code is None else (paged8.PagedKv8Cache, (code,))
+        return kind(cfg.layers, cfg.kv_heads, n_pages, page_size, max_rows, pages_per_row, self.device, *more)
 
     # ------------------------------------------------------------------ prefill
     @torch.no_grad()
@@ -74,10 +76,14 @@ class PagedDecodeEngine(DecodeEngine):
         pages mapped beforehand) -> last-token logits (len(rows), vocab).
 
         One packed varlen launch per layer (``_prefill_ragged`` semantics,
-        SE:1162-1204): row b's tokens land in its slots [0, len_b)."""
+        SE:1162-1204): row b's tokens land in its slots [0, len_b).  A cache in 8
+        bits is filled behind the pass, whose own attention is over the fp16
+        keys and values."""
         rows = list(rows)
         if len(rows) != len(prompts):
             raise ValueError("one row per prompt")
+        if isinstance(kv, paged8.PagedKv8Cache):
+            return self._prefill_paged8(prompts, kv, rows)
         table = self._table_rows(kv, rows)
         return self._prefill_packed(
             prompts, lambda i, q, k, v, cu, n, cos, sin, lengths: paged.prefill_varlen_paged(
@@ -87,6 +93,35 @@ class PagedDecodeEngine(DecodeEngine):
                 hidden, kv.pools, (kv.n_pages, kv.kv_heads, kv.page_size, self.cfg.head_dim),
                 len(prompts), longest, cu=cu, block_table=table, n_pages=kv.n_pages,
                 page_size=kv.page_size))
+
+    def _prefill_paged8(self, prompts, kv: paged8.PagedKv8Cache, rows):
+        """The prompts through dense fp16 caches of their own, which are then quantised:
+        every layer's tokens of a row in one launch.  Prompts go together as far as
+        those caches take a 64th of the GPU's memory, 2 GiB at least."""
+        cfg = self.cfg
+        lengths = [int(p.numel()) for p in prompts]
+        if max(lengths) > kv.capacity:
+            raise ValueError(f"a prompt exceeds the row capacity {kv.capacity}")
+        slot_bytes = cfg.layers * 2 * cfg.kv_heads * cfg.head_dim * 2
+        memory = max(2 << 30, torch.cuda.get_device_properties(self.device).total_memory // 64)
+        logits, at = [], 0
+        while at < len(prompts):
+            n, longest = 1, lengths[at]
+            while at + n < len(prompts) and (n + 1) * max(longest, lengths[at + n]) * slot_bytes <= memory:
+                longest = max(longest, lengths[at + n])
+                n += 1
+            dense = torch.zeros((2, cfg.layers, n, cfg.kv_heads, longest, cfg.head_dim), device=self.device,
+                                dtype=torch.float16)
+            logits.append(self.prefill_ragged(prompts[at:at + n], list(zip(*dense))))
+            zero = torch.zeros(1, device=self.device, dtype=torch.int64)
+            for j in range(n):
+                m = lengths[at + j]
+                k, v = dense[:, :, j, :, :m].transpose(2, 3)
+                cu = torch.tensor([0, m], device=self.device, dtype=torch.int32)
+                r = rows[at + j]
+                paged8.append_paged8(k, v, cu, m, zero, None, None, kv.all_pools, kv.table[r:r + 1], lengths=[m])
+            at += n
+        return torch.cat(logits)
 
     def _table_rows(self, kv: paged.PagedKvCache, rows):
         if rows == list(range(rows[0], rows[0] + len(rows))):
@@ -101,7 +136,8 @@ class PagedDecodeEngine(DecodeEngine):
         after every token (packed) without ``last_only``.
 
         The slots must be mapped; pages of theirs that another row holds too are
-        copied first (``PagedKvCache.own_slots``)."""
+        copied first (``PagedKvCache.own_slots``).  Over a cache in 8 bits the
+        projections are torch's."""
         cfg, dev = self.cfg, self.device
         rows, contexts = list(rows), [int(c) for c in contexts]
         lengths = [int(c.numel()) for c in chunks]
@@ -124,12 +160,15 @@ class PagedDecodeEngine(DecodeEngine):
             pos = torch.cat([torch.arange(c, c + n, device=dev) for c, n in zip(contexts, lengths)])
             cos, sin = cos_sin(pos, self.inv_freq)
             qh, kvh, d = cfg.heads, cfg.kv_heads, cfg.head_dim
-            for layer, (kp, vp) in zip(self.w["layers"], kv.pools):
+            for layer, pools in zip(self.w["layers"], kv.pools):
                 proj = F.linear(self._rms(hidden, layer["input_norm"]), layer["qkv_weight"],
                                 layer["qkv_bias"]).view(total, qh + 2 * kvh, d)
-                att = paged.prefill_extend_paged(proj[:, :qh], proj[:, qh:qh + kvh], proj[:, qh + kvh:],
-                                                 cu, max(lengths), ctx, cos, sin, kp, vp, table,
-                                                 lengths=lengths, max_slots=most, scale=self.scale)
+                new = (proj[:, :qh], proj[:, qh:qh + kvh], proj[:, qh + kvh:], cu, max(lengths), ctx, cos, sin)
+                last = dict(lengths=lengths, max_slots=most, scale=self.scale)
+                if isinstance(kv, paged8.PagedKv8Cache):
+                    att = paged8.prefill_extend_paged8(*new, pools, table, **last)
+                else:
+                    att = paged.prefill_extend_paged(*new, *pools, table, **last)
                 hidden = hidden + F.linear(att.reshape(total, qh * d), layer["o_weight"])
                 hidden = hidden + self._mlp(self._rms(hidden, layer["post_norm"]), layer)
         return self._last_logits(hidden[cu[1:].long() - 1] if last_only else hidden)
@@ -138,7 +177,7 @@ class PagedDecodeEngine(DecodeEngine):
         """Every layer of an extension in one native call, or False where the
         model's or the caches' layout is one it does not take."""
         cfg = self.cfg
-        if (hidden.dtype != torch.float16 or not hidden.is_cuda
+        if (isinstance(kv, paged8.PagedKv8Cache) or hidden.dtype != torch.float16 or not hidden.is_cuda
                 or prefill_ops.workspace_bytes(cfg, hidden.shape[0]) < 0):
             return False
         layers = prefill_ops.layer_table(cfg, self.w["layers"], kv.pools, hidden.device,
@@ -186,10 +225,37 @@ class PagedDecodeEngine(DecodeEngine):
             "prefix": prefix,
         }
         self._step_buffers(ctx, batch)
-        if prefix is not None:
-            ctx["att"] = torch.zeros(batch, cfg.kv_heads, cfg.groups, cfg.head_dim, device=dev,
-                                     dtype=torch.float16)
+        f16 = dict(device=dev, dtype=torch.float16)
+        ctx["kv8"] = isinstance(kv, paged8.PagedKv8Cache)
+        if ctx["kv8"]:
+            if prefix is not None:
+                raise ValueError("a prefix is read once for all rows over caches in fp16 only")
+            # The step's keys and values pass through a page of fp16 for each row.
+            ctx["new"] = tuple(torch.zeros(2, batch, cfg.kv_heads, paged.MIN_PAGE, cfg.head_dim, **f16))
+            ctx["new_table"] = torch.arange(batch, device=dev, dtype=torch.int32).view(batch, 1)
+            ctx["new_slot"] = torch.zeros(batch, device=dev, dtype=torch.long)
+        if prefix is not None or ctx["kv8"]:
+            ctx["att"] = torch.zeros(batch, cfg.kv_heads, cfg.groups, cfg.head_dim, **f16)
         return ctx
+
+    def _write_to(self, ctx, i: int):
+        """Where the QKV launch of layer i appends the step's keys and values: pools,
+        table and slots."""
+        if ctx["kv8"]:
+            return (*ctx["new"], ctx["new_table"], ctx["new_slot"])
+        return (*ctx["kv"].pools[i], ctx["table"], ctx["pos"])
+
+    def _attend(self, ctx, i: int, grouped):
+        """Attention of layer i's step over the slots up to the one just written."""
+        kv, table, pos = ctx["kv"], ctx["table"], ctx["pos"]
+        if ctx["kv8"]:
+            return paged8.flash_decode_attention_paged8(grouped, kv.pools[i], table, pos, scale=self.scale,
+                                                        out=ctx["att"], key=ctx["new"][0][:, :, 0],
+                                                        value=ctx["new"][1][:, :, 0])
+        if ctx["prefix"] is not None:
+            return self._attend_prefix(ctx, grouped, *kv.pools[i])
+        return paged.flash_decode_attention_paged(grouped, *kv.pools[i], table, None, ctx["flash"], kv_last=pos,
+                                                  scale=self.scale, share_rows=ctx["share_rows"])
 
     def reads_prefix_once(self, batch: int, slots: int) -> bool:
         """Whether ``serve``'s steps attend ``batch`` rows with a common prefix of
@@ -237,25 +303,30 @@ class PagedDecodeEngine(DecodeEngine):
         kv, table, pos = ctx["kv"], ctx["table"], ctx["pos"]
         rope = (pos, self.inv_freq)                              # each row's own position
         hidden, q_rot, h = ctx["hidden"], ctx["q_rot"], ctx["h"]
-        for i, (layer, (kp, vp)) in enumerate(zip(self.w["layers"], kv.pools)):
+        for i, layer in enumerate(self.w["layers"]):
             w_qkv, w_gate_up = self.projection_weights(i, b)
             if i == 0:
                 paged.rms_qkv_rope_append_paged(self.w["embed"], layer["input_norm"], eps,
                                                 w_qkv, layer["qkv_bias"], None, None,
-                                                kp, vp, table, pos, q_rot, token=ctx["token"],
+                                                *self._write_to(ctx, i), q_rot, token=ctx["token"],
                                                 hidden_out=hidden, positions=rope)
             else:
                 paged.rms_qkv_rope_append_paged(hidden, layer["input_norm"], eps,
                                                 w_qkv, layer["qkv_bias"], None, None,
-                                                kp, vp, table, pos, q_rot, positions=rope)
+                                                *self._write_to(ctx, i), q_rot, positions=rope)
             grouped = q_rot.view(b, cfg.kv_heads, cfg.groups, cfg.head_dim)
             # The slot just written is the row's last valid one.
             if ctx["prefix"] is not None:
-                att = self._attend_prefix(ctx, grouped, kp, vp)
+                att = self._attend_prefix(ctx, grouped, *kv.pools[i])
                 step_ops.gemv_residual(att.view(b, -1), layer["o_weight"], hidden)
             else:
-                paged.flash_decode_split_paged(grouped, kp, vp, table, None, ctx["flash"], kv_last=pos,
-                                               scale=self.scale)
+                if ctx["kv8"]:
+                    paged8.flash_decode_split_paged8(grouped, kv.pools[i], table, ctx["flash"], pos,
+                                                     scale=self.scale, key=ctx["new"][0][:, :, 0],
+                                                     value=ctx["new"][1][:, :, 0])
+                else:
+                    paged.flash_decode_split_paged(grouped, *kv.pools[i], table, None, ctx["flash"],
+                                                   kv_last=pos, scale=self.scale)
                 step_ops.attn_merge_o_proj(ctx["flash"], self.o_proj_weight(i, b), hidden)
             step_ops.rms_gate_up_swiglu(hidden, layer["post_norm"], eps, w_gate_up, h)
             step_ops.gemv_residual(h, layer["down_weight"], hidden)
@@ -264,39 +335,25 @@ class PagedDecodeEngine(DecodeEngine):
         step_ops.argmax_step(ctx["keys"], ctx["token"], ctx["rows"], ctx["step"], None, pos)
 
     def _step_wide_paged(self, ctx):
-        kv, table, pos = ctx["kv"], ctx["table"], ctx["pos"]
-
         def qkv(i, layer, w_qkv):
             wide_ops.rms_qkv_rope_append_paged(ctx["hidden"], layer["input_norm"], self.cfg.rms_eps,
-                                               w_qkv, layer["qkv_bias"], (pos, self.inv_freq),
-                                               *kv.pools[i], table, pos, ctx["q_rot"])
+                                               w_qkv, layer["qkv_bias"], (ctx["pos"], self.inv_freq),
+                                               *self._write_to(ctx, i), ctx["q_rot"])
 
-        def attend(i, grouped):
-            if ctx["prefix"] is not None:
-                return self._attend_prefix(ctx, grouped, *kv.pools[i])
-            return paged.flash_decode_attention_paged(grouped, *kv.pools[i], table, None,
-                                                      ctx["flash"], kv_last=pos, scale=self.scale,
-                                                      share_rows=ctx["share_rows"])
-
-        self._wide_body(ctx, qkv, attend, None)
+        self._wide_body(ctx, qkv, lambda i, grouped: self._attend(ctx, i, grouped), None)
 
     def _step_torch_paged(self, ctx):
         cfg = self.cfg
         b = ctx["token"].shape[0]
-        kv, table, pos = ctx["kv"], ctx["table"], ctx["pos"]
+        pos = ctx["pos"]
         hidden = F.embedding(ctx["token"], self.w["embed"]).view(b, 1, cfg.hidden)
         cos, sin = cos_sin(pos, self.inv_freq)
-        for layer, (kp, vp) in zip(self.w["layers"], kv.pools):
+        for i, layer in enumerate(self.w["layers"]):
             residual = hidden
             q, k, v = self._qkv(self._rms(hidden, layer["input_norm"]), layer)
-            q_rot = paged.rope_append_paged(q, k, v, cos, sin, kp, vp, table, pos)
+            q_rot = paged.rope_append_paged(q, k, v, cos, sin, *self._write_to(ctx, i))
             grouped = q_rot.view(b, cfg.kv_heads, cfg.groups, cfg.head_dim)
-            if ctx["prefix"] is not None:
-                att = self._attend_prefix(ctx, grouped, kp, vp)
-            else:
-                att = paged.flash_decode_attention_paged(grouped, kp, vp, table, None, ctx["flash"],
-                                                         kv_last=pos, scale=self.scale,
-                                                         share_rows=ctx["share_rows"])
+            att = self._attend(ctx, i, grouped)
             hidden = residual + F.linear(att.reshape(b, 1, cfg.hidden), layer["o_weight"])
             residual = hidden
             hidden = residual + self._mlp(self._rms(hidden, layer["post_norm"]), layer)
@@ -335,15 +392,16 @@ class PagedDecodeEngine(DecodeEngine):
     # ------------------------------------------------------------------ generation
     @torch.no_grad()
     def generate_paged(self, prompts, max_new_tokens: int, page_size: int = 64,
-                       timing: dict | None = None):
+                       timing: dict | None = None, kv_code: str | None = None):
         """Greedy ids (B, max_new_tokens) for variable-length prompts, each row
-        holding only the pages of its own prompt + new tokens."""
+        holding only the pages of its own prompt + new tokens: in fp16, or with
+        ``kv_code`` "int8" or "e4m3" in 8 bits (``paged8``)."""
         b = len(prompts)
         lengths = [int(p.numel()) for p in prompts]
         need = [n + max(max_new_tokens - 1, 0) for n in lengths]
         ppr = -(-max(need) // page_size)
         n_pages = sum(-(-n // page_size) for n in need)
-        kv = self.new_paged_cache(b, n_pages, page_size, ppr)
+        kv = self.new_paged_cache(b, n_pages, page_size, ppr, kv_code)
         for r, n in enumerate(need):
             kv.map_row(r, n)
         ev = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
@@ -372,7 +430,7 @@ class PagedDecodeEngine(DecodeEngine):
     @torch.no_grad()
     def generate_drafted(self, prompts, max_new_tokens: int, draft_len: int = 4,
                          temperature: float = 0.0, seed: int = 0, drafter=lookup_drafts,
-                         page_size: int = 64, stats: dict | None = None):
+                         page_size: int = 64, stats: dict | None = None, kv_code: str | None = None):
         """``max_new_tokens`` ids for each of variable-length prompts (B, new), up
         to ``draft_len`` + 1 of them per pass.
 
@@ -383,7 +441,9 @@ class PagedDecodeEngine(DecodeEngine):
         would have said: the argmax at ``temperature`` 0, else tokens distributed
         as softmax(logits / temperature) whatever the drafter proposes, from
         random numbers of a generator seeded with ``seed``.  ``stats`` (optional
-        dict) receives the passes, drafts and accepted drafts.
+        dict) receives the passes, drafts and accepted drafts.  With ``kv_code`` the
+        cache is held in 8 bits; what a block of slots holds then depends a little
+        on the drafts that were written to it, kept or not.
 
         It pays where drafts are mostly kept.  A pass is not captured and runs the
         prompt's kernels: MI355X, Qwen2.5-0.5B shape behind 500 tokens, ms per pass of
@@ -397,7 +457,7 @@ class PagedDecodeEngine(DecodeEngine):
         text = [p.reshape(-1).tolist() for p in prompts]
         ends = [len(t) + max_new_tokens for t in text]
         ppr = -(-max(ends) // page_size)
-        kv = self.new_paged_cache(b, sum(-(-n // page_size) for n in ends), page_size, ppr)
+        kv = self.new_paged_cache(b, sum(-(-n // page_size) for n in ends), page_size, ppr, kv_code)
         for r, n in enumerate(ends):
             kv.map_row(r, n)
 
@@ -440,7 +500,8 @@ class PagedDecodeEngine(DecodeEngine):
 
     @torch.no_grad()
     def serve(self, prompts, max_new_tokens, max_batch: int = 4, page_size: int = 64,
-              n_pages: int | None = None, stats: dict | None = None, prefix=None):
+              n_pages: int | None = None, stats: dict | None = None, prefix=None,
+              kv_code: str | None = None):
         """Continuous batching: greedy ids for every prompt (list of 1-D tensors),
         ``max_new_tokens`` an int or one per prompt.
 
@@ -457,6 +518,10 @@ class PagedDecodeEngine(DecodeEngine):
         The prefix is prefilled once, each request's row forks its pages and
         extends them by the prompt, and the steps read the shared pages once for
         all rows where that is the faster way (``reads_prefix_once``).
+
+        ``kv_code`` "int8" or "e4m3" holds the cache in 8 bits (``paged8``): half the
+        bytes of a step's attention, twice the slots in a pool's memory.  Each row then
+        reads a prefix by itself.
         """
         n_req = len(prompts)
         news = [max_new_tokens] * n_req if isinstance(max_new_tokens, int) else list(max_new_tokens)
@@ -470,13 +535,13 @@ class PagedDecodeEngine(DecodeEngine):
         whole = common // page_size       # pages that rows share
         if n_pages is None:
             n_pages = max_batch * (ppr - whole) + -(-common // page_size)
-        kv = self.new_paged_cache(max_batch + (common > 0), n_pages, page_size, ppr)
+        kv = self.new_paged_cache(max_batch + (common > 0), n_pages, page_size, ppr, kv_code)
         shared = None
         if common:
             # The row behind the batch holds the prefix for as long as the call runs.
             kv.map_row(max_batch, common)
             self.prefill_paged([prefix], kv, [max_batch])
-        if common and self.reads_prefix_once(max_batch, common):
+        if common and kv_code is None and self.reads_prefix_once(max_batch, common):
             i32 = dict(device=self.device, dtype=torch.int32)
             shared = (torch.tensor([0, max_batch], **i32), torch.tensor([common], **i32),
                       kv.table[max_batch:])

@@ -345,3 +345,145 @@ def test_max_slots_bounds_writes_and_reads(dev, code):
         n = min(91 + i, 100)
         want = kv8.attend(x[i, :2].cpu().double().numpy(), kk[:n], vv[:n])
         check(got[i], want, np.abs(vv).max(), i)
+
+
+# --------------------------------------------------------------------------
+# a decoding step: the new token appended by the launch that attends
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("case", [1, 2, 3, 4, 6, 8, 9])
+def test_step_is_append_then_attend(dev, case, code):
+    """Bit for bit, at every place in a block, parked rows left alone."""
+    gen = torch.Generator().manual_seed(400 + case)
+    rows, layer, table, host, q, last = decode_case(gen, case, code, dev)
+    b, kvh, g, _ = q.shape
+    other = tuple(t.clone() for t in layer)
+    kv = (torch.randn(b, 3, kvh, D, generator=gen) * 2.0 ** torch.randint(-3, 4, (b, 1, 1, 1), generator=gen)).half()
+    kv = kv.to(dev)
+    key, value = kv[:, 0], kv[:, 2]
+    cu = torch.arange(b + 1, dtype=torch.int32, device=dev)
+    paged8.append_paged8(key, value, cu, 1, last, None, None, other, table)
+    want = paged8.flash_decode_attention_paged8(q, other, table, last)
+    got = paged8.flash_decode_attention_paged8(q, layer, table, last, key=key, value=value)
+    assert torch.equal(got, want)
+    for a, c in zip(layer, other):
+        assert torch.equal(a.view(torch.uint8), c.view(torch.uint8))
+    flash = ops.make_flash_scratch(b, kvh, g, table.shape[1] * layer[0].shape[2], dev, splits=5, fused=False)
+    fresh = tuple(t.clone() for t in layer)
+    paged8.flash_decode_split_paged8(q, fresh, table, flash, last, key=key * 3, value=value)
+    paged8.append_paged8(key * 3, value, cu, 1, last, None, None, other, table)
+    for a, c in zip(fresh, other):
+        assert torch.equal(a.view(torch.uint8), c.view(torch.uint8))
+
+
+def test_step_at_a_slot_without_a_page(dev):
+    """Past the row's pages nothing is written and the row attends to all it has; an unmapped page is skipped."""
+    gen = torch.Generator().manual_seed(71)
+    layer = tuple(t[0] for t in make_pools(gen, 5, 2, 64, "int8", dev))
+    table, host = make_table(gen, [128, 64], 64, 5, 2, dev)
+    fill_rows(gen, layer, table, [128, 64], dev)
+    before = tuple(t.clone() for t in layer)
+    q = torch.randn(2, 2, 7, D, generator=gen).half().to(dev)
+    new = torch.randn(2, 2, D, generator=gen).half().to(dev)
+    got = paged8.flash_decode_attention_paged8(q, layer, table, torch.tensor([128, 70], device=dev), key=new, value=new)
+    for a, c in zip(layer, before):
+        assert torch.equal(a.view(torch.uint8), c.view(torch.uint8))
+    want = paged8.flash_decode_attention_paged8(q, layer, table, torch.tensor([127, 70], device=dev))
+    assert torch.equal(got[0], want[0])
+
+
+# --------------------------------------------------------------------------
+# graphs, streams, far pages
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_captured_steps_replay(dev, code):
+    """Two graphs over one cache, replayed in turn with eager calls between: each replay is the eager step's."""
+    gen = torch.Generator().manual_seed(73)
+    rows = [100, 0, 1100, 15]
+    layer = tuple(t[0] for t in make_pools(gen, 60, 2, 64, code, dev))
+    table, host = make_table(gen, [n + 40 for n in rows], 64, 60, 20, dev)
+    fill_rows(gen, layer, table, rows, dev)
+    mirror = tuple(t.clone() for t in layer)
+    q = torch.zeros(4, 2, 7, D, device=dev, dtype=torch.float16)
+    new = torch.zeros(2, 4, 2, D, device=dev, dtype=torch.float16)
+    last = torch.tensor([n if n else -1 for n in rows], device=dev)
+    cu = torch.arange(5, dtype=torch.int32, device=dev)
+
+    def step(pools):
+        return paged8.flash_decode_attention_paged8(q, pools, table, last, key=new[0], value=new[1])
+
+    def long_step(pools):
+        out = paged8.prefill_extend_paged8(q.view(4, 14, D), new[0], new[1], cu, 1, last, None, None, pools, table,
+                                           lengths=[1, 1, 1, 1])
+        return out, paged8.read_paged8(pools, table, cu, 1, last, lengths=[1, 1, 1, 1])
+
+    graphs = []
+    for fn in (step, long_step):
+        pools = tuple(t.clone() for t in layer)
+        fn(pools)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = fn(layer)
+        graphs.append((g, out))
+    for i in range(6):
+        q.copy_(torch.randn(q.shape, generator=gen))
+        new.copy_(torch.randn(new.shape, generator=gen))
+        graphs[i % 2][0].replay()
+        got = graphs[i % 2][1]
+        torch.cuda.synchronize()
+        want = (step, long_step)[i % 2](mirror)
+        flat = lambda x: [x] if isinstance(x, torch.Tensor) else [x[0], *x[1]]  # noqa: E731
+        for a, c in zip(flat(got), flat(want)):
+            assert torch.equal(a, c), i
+        for a, c in zip(layer, mirror):
+            assert torch.equal(a.view(torch.uint8), c.view(torch.uint8)), i
+        last += (last >= 0).long()
+
+
+def test_two_streams_at_once(dev):
+    """Calls on two streams over one cache: workspaces are each call's own."""
+    gen = torch.Generator().manual_seed(79)
+    rows, layer, table, host, q, last = decode_case(gen, 4, "int8", dev)
+    qs = [torch.randn(q.shape, generator=gen).half().to(dev) for _ in range(8)]
+    want = [paged8.flash_decode_attention_paged8(x, layer, table, last) for x in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    got = []
+    for i, x in enumerate(qs):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(paged8.flash_decode_attention_paged8(x, layer, table, last))
+    torch.cuda.synchronize()
+    for a, c in zip(got, want):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_pages_past_four_gigabytes(dev, code):
+    """A pool of 6 GB: pages whose offsets pass 32 bits are written, read and attended as the first ones are."""
+    kvh, page, n_pages = 2, 256, 90000
+    kv = paged8.PagedKv8Cache(1, kvh, n_pages, page, 2, 6, dev, code)
+    gen = torch.Generator().manual_seed(83)
+    far = [n_pages - 1, 70000, 66000, n_pages - 7, 69999]
+    near = [0, 5, 2, 9, 1]
+    n = 1111
+    x = torch.randn(n, 4, D, generator=gen).half().to(dev)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    zero = torch.zeros(1, dtype=torch.int64, device=dev)
+    q = torch.randn(1, 2, 7, D, generator=gen).half().to(dev)
+    got = []
+    for r, pages in enumerate((near, far)):
+        kv.table[r, :5] = torch.tensor(pages, dtype=torch.int32)
+        t = kv.table[r:r + 1]
+        paged8.append_paged8(x[:, :2], x[:, 2:], cu, n, zero, None, None, kv.pools[0], t)
+        got.append((*paged8.read_paged8(kv.pools[0], t, cu, n, zero),
+                    paged8.flash_decode_attention_paged8(q, kv.pools[0], t, torch.tensor([n - 1], device=dev))))
+    for a, c in zip(*got):
+        assert torch.equal(a, c)
+    k, v = (t.double().cpu().numpy() for t in got[1][:2])
+    check(got[1][2].reshape(-1, D), kv8.attend(q.reshape(-1, D).cpu().double().numpy(), k, v), np.abs(v).max(), "far")
+    # Page copies over the same distance.
+    paged8.copy_pages8(kv.store, far, [20, 21, 22, 23, 24])
+    assert torch.equal(kv.store[0, 20:25], kv.store[0, far])
