@@ -132,13 +132,13 @@ struct State {
   f32x4 o[kNC][4];
 };
 
-// The unit's queries; what each sees is set_limits'.
+// The unit's query rows from `first` on; what each sees is set_limits'.
 template <int kNC, bool kDecode>
-__device__ __forceinline__ void load_queries(State<kNC>& s, const AttnArgs& a, const Unit& u) {
+__device__ __forceinline__ void load_queries(State<kNC>& s, const AttnArgs& a, const Unit& u, int first) {
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int b = 0; b < kNC; ++b) {
-    const int rr = min(u.r0 + 16 * b + col, u.rows - 1);
+    const int rr = min(first + 16 * b + col, u.rows - 1);
     const int token = kDecode ? u.tok0 : u.tok0 + rr / a.G, h = kDecode ? rr : rr % a.G;
     const f16* qp = a.q + token * a.q_st + u.hk * a.q_sh + h * a.q_sg + 16 * g;
 #pragma unroll
@@ -164,14 +164,14 @@ __device__ __forceinline__ void load_queries(State<kNC>& s, const AttnArgs& a, c
 }
 
 template <int kNC, bool kDecode>
-__device__ __forceinline__ void set_limits(State<kNC>& s, const AttnArgs& a, const Unit& u) {
+__device__ __forceinline__ void set_limits(State<kNC>& s, const AttnArgs& a, const Unit& u, int first) {
   const int col = threadIdx.x & 15;
   int least = u.k1;
 #pragma unroll
   for (int b = 0; b < kNC; ++b) {
     s.lim[b] = u.k1;
     if (!kDecode) {
-      const int r = u.r0 + 16 * b + col;
+      const int r = first + 16 * b + col;
       if (r < u.rows) s.lim[b] = min(u.ctx + r / a.G + 1, u.k1);
       least = min(least, s.lim[b]);
     }
@@ -183,61 +183,45 @@ __device__ __forceinline__ void set_limits(State<kNC>& s, const AttnArgs& a, con
   s.seen = least;
 }
 
-// Scores, online softmax and PV product of the tile at key0.  `next` loads what
-// comes after it, once the tile's codes are in fp16.
-template <bool kE4m3, int kNC, typename Next>
-__device__ __forceinline__ void tile_step(State<kNC>& s, Raw& r, int key0, int k1, float scale_log2,
-                                          Next&& next) {
+// What a tile's scales mean for a lane's 16 slots: the scores' factor, the values' scale
+// (1 where the lane has no slot below k1), and whether they read as NaN.
+struct Block {
+  float ks2, vs;
+  bool bad;
+};
+
+__device__ __forceinline__ Block block_scales(float ks, float vs, int have, float scale_log2) {
+  Block r;
+  r.ks2 = ks * scale_log2;
+  r.vs = have <= 0 ? 1.f : vs;
+  r.bad = !(r.vs == r.vs);
+  if (r.bad) r.vs = 0.f;   // zeros, and NaN probabilities for who sees them
+  return r;
+}
+
+// Slots behind the last one may hold anything: of the lane's 16 the first `have` keep
+// their codes, the others become zeros.
+__device__ __forceinline__ u32x4 keep_slots(u32x4 w, int have) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = min(max(have - 4 * i, 0), 4);
+    w[i] &= n == 4 ? ~0u : (1u << (8 * n)) - 1u;
+  }
+  return w;
+}
+
+// Online softmax and PV product from a tile's scores; `values` gives operand (t, u) of
+// V^T.  `left`: how many of the lane's 16 slots, from the first on, a column sees.
+template <int kNC, typename Values>
+__device__ __forceinline__ void attend_tile(State<kNC>& s, f32x4 (&sc)[kNC][4], const Block& blk, int key0,
+                                            Values&& values) {
   const int g = (threadIdx.x & 63) >> 4;
   const bool masked = key0 + kTile > s.seen;
-  float vs = r.vs;
-  const float ks2 = r.ks * scale_log2;
-  if (key0 + kTile > k1) {
-    // Slots behind the last one may hold anything: their values become zeros.
-    const int have = k1 - key0 - 16 * g;  // of the lane's 16
-    if (have <= 0) vs = 1.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = min(max(have - 4 * i, 0), 4);
-      const unsigned keep = n == 4 ? ~0u : (1u << (8 * n)) - 1u;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) r.v[t][i] &= keep;
-    }
-  }
-  // A block that reads as NaN: zeros here, and NaN probabilities for who sees it.
-  const bool bad = !(vs == vs);
-  if (bad) vs = 0.f;
-  f16x8 k[4][2], v[4][2];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) k[i][h] = codes8<kE4m3>(r.k[i][2 * h], r.k[i][2 * h + 1], 1.f);
-  if (kE4m3 || !__any(vs > kAffineMost)) {
-    const Affine f = affine(vs);
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) v[t][h] = values8<kE4m3>(r.v[t][2 * h], r.v[t][2 * h + 1], vs, f);
-  } else {
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) v[t][h] = values8<kE4m3>(r.v[t][2 * h], r.v[t][2 * h + 1], vs);
-  }
-  next();
-  f32x4 sc[kNC][4];
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int b = 0; b < kNC; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sc[b][i] = mfma16x16x32(k[i][h], s.q[b][h], h == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[b][i]);
   float f[kNC], mx[kNC];
   bool grew = false;
 #pragma unroll
   for (int b = 0; b < kNC; ++b) {
-    f[b] = ks2;
+    f[b] = blk.ks2;
     if (masked) {
       const int left = s.lim[b] - key0 - 16 * g;
       if (left <= 0) f[b] = 1.f;   // whatever scale an unseen block has
@@ -261,9 +245,12 @@ __device__ __forceinline__ void tile_step(State<kNC>& s, Raw& r, int key0, int k
       s.m[b] = m_new;
     }
   }
-  f16x8 p[kNC][2];
   const f16x8 ones = {(f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f};
-  const auto weights = [&](int b) {
+  f16x8 p[kNC][2];
+#pragma unroll
+  for (int b = 0; b < kNC; ++b) {
+    // p is rounded to fp16 for the matrix cores (2^-12 of it at most, as much as the
+    // output's own rounding), and the sum adds the rounded ones: the weights add to one.
     const float neg_m = s.m[b] == kNegInf ? 0.f : -s.m[b];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -272,37 +259,69 @@ __device__ __forceinline__ void tile_step(State<kNC>& s, Raw& r, int key0, int k
       for (int e = 0; e < 8; ++e) x[e] = fast_exp2(__builtin_fmaf(sc[b][2 * u + e / 4][e % 4], f[b], neg_m));
       p[b][u] = __builtin_convertvector(x, f16x8);
     }
-  };
-  const auto products = [&](int b) {
+  }
+  if (__any(blk.bad)) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      // The sum adds the rounded p, so that the weights add to one.
-      s.l[b] = mfma16x16x32(ones, p[b][u], s.l[b]);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) s.o[b][t] = mfma16x16x32(v[t][u], p[b][u], s.o[b][t]);
-    }
-  };
-  if (__any(bad)) {
-#pragma unroll
-    for (int b = 0; b < kNC; ++b) {
-      weights(b);
+    for (int b = 0; b < kNC; ++b)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (bad && s.lim[b] > key0 + 16 * g) p[b][u][e] = (f16)__builtin_nanf("");
-      products(b);
-    }
-    return;
+          if (blk.bad && s.lim[b] > key0 + 16 * g) p[b][u][e] = (f16)__builtin_nanf("");
   }
-  weights(0);
 #pragma unroll
-  for (int b = 0; b < kNC; ++b) {
-    products(b);
-    if (b + 1 < kNC) {
-      weights(b + 1);
+  for (int b = 0; b < kNC; ++b)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) s.l[b] = mfma16x16x32(ones, p[b][u], s.l[b]);
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const f16x8 v = values(t, u);
+#pragma unroll
+      for (int b = 0; b < kNC; ++b) s.o[b][t] = mfma16x16x32(v, p[b][u], s.o[b][t]);
     }
+}
+
+// Scores, softmax and PV product of the tile at key0.  `next` loads what comes after
+// it, once the tile's codes are in fp16.
+template <bool kE4m3, int kNC, typename Next>
+__device__ __forceinline__ void tile_step(State<kNC>& s, Raw& r, int key0, int k1, float scale_log2,
+                                          Next&& next) {
+  const int g = (threadIdx.x & 63) >> 4;
+  const int have = k1 - key0 - 16 * g;  // of the lane's 16 slots
+  const Block blk = block_scales(r.ks, r.vs, have, scale_log2);
+  if (key0 + kTile > k1) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) r.v[t] = keep_slots(r.v[t], have);
   }
+  f16x8 k[4][2], v[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) k[i][h] = codes8<kE4m3>(r.k[i][2 * h], r.k[i][2 * h + 1], 1.f);
+  if (kE4m3 || !__any(blk.vs > kAffineMost)) {
+    const Affine f = affine(blk.vs);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) v[t][u] = values8<kE4m3>(r.v[t][2 * u], r.v[t][2 * u + 1], blk.vs, f);
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) v[t][u] = values8<kE4m3>(r.v[t][2 * u], r.v[t][2 * u + 1], blk.vs);
+  }
+  next();
+  f32x4 sc[kNC][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int b = 0; b < kNC; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sc[b][i] = mfma16x16x32(k[i][h], s.q[b][h], h == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[b][i]);
+  attend_tile<kNC>(s, sc, blk, key0, [&](int t, int u) { return v[t][u]; });
 }
 
 __device__ __forceinline__ void store_out(const AttnArgs& a, int token, int hk, int g, int d, f32x4 o,
@@ -375,7 +394,7 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Unit& u, Sourc
     Raw r0, r1;
     load_tile<kDecode>(r0, src, slot(0), 0 < mine);
     load_tile<kDecode>(r1, src, slot(1), 1 < mine);
-    set_limits<kNC, kDecode>(s, a, u);
+    set_limits<kNC, kDecode>(s, a, u, u.r0);
     int j = 0;
     for (; j + 2 <= mine; j += 2) {
       tile_step<kE4m3, kNC>(s, r0, slot(j), u.k1, a.scale_log2,
@@ -387,7 +406,7 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Unit& u, Sourc
   } else {
     Raw r;
     load_tile<kDecode>(r, src, slot(0), 0 < mine);
-    set_limits<kNC, kDecode>(s, a, u);
+    set_limits<kNC, kDecode>(s, a, u, u.r0);
     for (int j = 0; j < mine; ++j)
       tile_step<kE4m3, kNC>(s, r, slot(j), u.k1, a.scale_log2,
                             [&] { load_tile<kDecode>(r, src, slot(j + 1), j + 1 < mine); });
@@ -446,7 +465,7 @@ __global__ __launch_bounds__(512, 2) void decode_kernel(AttnArgs a) {
   const int64_t last = a.last[u.row * a.last_sb];
   Source src = make_source(a, u);
   State<1> s;
-  load_queries<1, true>(s, a, u);
+  load_queries<1, true>(s, a, u, 0);
   cut(clampi(last, -1, a.cap - 1) + 1, u.split, a.splits, u.k0, u.k1);
   if (a.kn != nullptr && last >= u.k0 && last < u.k1) {
     // The unit that sees the new token writes it; its block is in no other unit.  The
@@ -464,18 +483,17 @@ __global__ __launch_bounds__(512, 2) void decode_kernel(AttnArgs a) {
   run_unit<kE4m3, 1, true>(a, u, src, s, lds);
 }
 
-template <bool kE4m3, int kNC>
-__global__ __launch_bounds__(256, 2) void extend_kernel(AttnArgs a) {
-  extern __shared__ f32x4 lds[];
+// The extension's unit of this workgroup, of kRows query rows; false: none.
+template <int kRows>
+__device__ __forceinline__ bool extend_unit(const AttnArgs& a, Unit& u) {
   // Query tiles that read the same slots share an XCD (workgroups go to the XCDs in
   // turn) and its L2, where there are XCDs enough.
   const int groups = a.B * a.p.kvh * a.splits;
   int id = blockIdx.x;
   if (groups >= 8) id = (id / (8 * a.n_tiles) * 8 + id % 8) * a.n_tiles + id / 8 % a.n_tiles;
-  Unit u;
   const int tile = id % a.n_tiles;
   id /= a.n_tiles;
-  if (id >= groups) return;
+  if (id >= groups) return false;
   u.split = id % a.splits;
   id /= a.splits;
   u.hk = id % a.p.kvh;
@@ -483,20 +501,144 @@ __global__ __launch_bounds__(256, 2) void extend_kernel(AttnArgs a) {
   const int lo = clampi(a.cu[u.row], 0, a.tokens), hi = clampi(a.cu[u.row + 1], lo, a.tokens);
   u.tok0 = lo;
   u.rows = (hi - lo) * a.G;
-  u.r0 = tile * 16 * kNC;
-  if (u.r0 >= u.rows) return;
+  u.r0 = tile * kRows;
+  if (u.r0 >= u.rows) return false;
   u.ctx = clampi(a.last[u.row * a.last_sb], -1, a.cap);
   // All tiles of a row are cut alike; a tile stops where its newest token does.
   const int end = u.ctx < 0 ? 0 : min(u.ctx + hi - lo, a.cap);
   cut(end, u.split, a.splits, u.k0, u.k1);
   if (u.ctx >= 0) {
-    const int newest = (min(u.r0 + 16 * kNC, u.rows) - 1) / a.G;
+    const int newest = (min(u.r0 + kRows, u.rows) - 1) / a.G;
     u.k1 = min(u.k1, min(u.ctx + newest + 1, a.cap));
   }
+  return true;
+}
+
+// Few query rows: the waves take the tiles in turn.
+template <bool kE4m3, int kNC>
+__global__ __launch_bounds__(512, 2) void extend_kernel(AttnArgs a) {
+  extern __shared__ f32x4 lds[];
+  Unit u;
+  if (!extend_unit<16 * kNC>(a, u)) return;
   Source src = make_source(a, u);
   State<kNC> s;
-  load_queries<kNC, false>(s, a, u);
+  load_queries<kNC, false>(s, a, u, u.r0);
   run_unit<kE4m3, kNC, false>(a, u, src, s, lds);
+}
+
+// Many query rows: the waves take 32 of them each and share the tiles.  A wave
+// turns a quarter of each tile's codes into operands, in LDS, a tile ahead of their
+// use: a quarter of the conversions that a wave by itself has for as many queries.
+template <bool kE4m3>
+__global__ __launch_bounds__(256, 3) void extend_wide_kernel(AttnArgs a) {
+  constexpr int kWaves = 4, kQB = 2;
+  // [stage][operand: K (i, h), then V (t, u)][lane]
+  __shared__ f16x8 lds[2][16][64];
+  Unit u;
+  if (!extend_unit<16 * kQB * kWaves>(a, u)) return;
+  if (u.k1 <= u.k0) {
+    empty_unit(a, u, 16 * kQB * kWaves);
+    return;
+  }
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  Source src = make_source(a, u);
+  src.koff += w * 4 * kD;
+  src.voff += w * 16 * kTile;
+  const int n = (u.k1 - u.k0 + kTile - 1) / kTile;
+  struct Part {
+    u32x4 k, v;
+    float ks, vs;
+  };
+  const auto load = [&](Part& r, int i) {
+    const bool valid = i < n;
+    const int slot0 = u.k0 + i * kTile;
+    const int lp = valid ? slot0 >> src.log2p : src.pwin;
+    if (lp - src.pwin >= 64) load_pids(src, lp);
+    const int64_t page = __builtin_amdgcn_readlane(src.pid, lp - src.pwin);
+    const int in_page = slot0 & ((1 << src.log2p) - 1);
+    const int64_t at = page * src.sp + in_page * kD, sat = page * src.ssp + (in_page >> 4);
+    r.k = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+        buffer_rsrc(src.k + at, valid ? kTile * kD : 0), src.koff, 0, 0));
+    r.v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+        buffer_rsrc(src.v + at, valid ? kTile * kD : 0), src.voff, 0, 0));
+    r.ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+        buffer_rsrc(src.ks + sat, valid ? 16 : 0), 4 * g, 0, 0));
+    r.vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+        buffer_rsrc(src.vs + sat, valid ? 16 : 0), 4 * g, 0, 0));
+  };
+  // Tile i's part into its stage; returns the scales' meaning for the lane.
+  const auto convert = [&](const Part& r, int i) {
+    const int key0 = u.k0 + i * kTile, have = u.k1 - key0 - 16 * g;
+    const Block blk = block_scales(r.ks, r.vs, have, a.scale_log2);
+    const u32x4 vw = key0 + kTile > u.k1 ? keep_slots(r.v, have) : r.v;
+    f16x8(&to)[16][64] = lds[i & 1];
+    to[2 * w][lane] = codes8<kE4m3>(r.k[0], r.k[1], 1.f);
+    to[2 * w + 1][lane] = codes8<kE4m3>(r.k[2], r.k[3], 1.f);
+    to[8 + 2 * w][lane] = values8<kE4m3>(vw[0], vw[1], blk.vs);
+    to[9 + 2 * w][lane] = values8<kE4m3>(vw[2], vw[3], blk.vs);
+    return blk;
+  };
+  // Every wave's LDS writes are there, and its reads done; loads from memory go on.
+  const auto meet = [] {
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  };
+  Part r0, r1;
+  load(r0, 0);
+  load(r1, 1);
+  State<kQB> s;
+  const int first = u.r0 + w * 16 * kQB;
+  load_queries<kQB, false>(s, a, u, first);
+  set_limits<kQB, false>(s, a, u, first);
+  Block blk = convert(r0, 0);
+  load(r0, 2);
+  meet();
+  const auto step = [&](int i, Part& r) {
+    const f16x8(&at)[16][64] = lds[i & 1];
+    f16x8 k[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) k[j][h] = at[2 * j + h][lane];
+    // Past the last tile: zeros that nobody reads.
+    const Block next = convert(r, i + 1);
+    load(r, i + 3);
+    f32x4 sc[kQB][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int b = 0; b < kQB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sc[b][j] = mfma16x16x32(k[j][h], s.q[b][h], h == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[b][j]);
+    attend_tile<kQB>(s, sc, blk, u.k0 + i * kTile, [&](int t, int e) { return at[8 + 2 * t + e][lane]; });
+    blk = next;
+    meet();
+  };
+  for (int i = 0; i < n; i += 2) {
+    step(i, r1);
+    if (i + 1 < n) step(i + 1, r0);
+  }
+#pragma unroll
+  for (int b = 0; b < kQB; ++b) {
+    const int rr = first + 16 * b + col;
+    if (rr >= u.rows) continue;
+    const int token = u.tok0 + rr / a.G, h = rr % a.G;
+    const float l = s.l[b][0];
+    const int64_t p = part_index(a, u, token, h);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (a.splits == 1) store_out(a, token, u.hk, h, 16 * t + 4 * g, s.o[b][t], l, true);
+      else *reinterpret_cast<f32x4*>(a.acc + p * kD + 16 * t + 4 * g) = s.o[b][t];
+    }
+    if (a.splits > 1 && g == 0) {
+      a.m[p] = s.m[b];
+      a.l[p] = l;
+    }
+  }
 }
 
 // Joins the at most kSubs * kEach partials of each (token, kv head, query head).  kSubs
@@ -575,7 +717,8 @@ constexpr int kCus = 256;
 int64_t part_bytes(int64_t queries, int n) { return n <= 1 ? 0 : queries * n * (kD + 2) * 4; }
 
 struct Plan {
-  int waves, splits, cols, n_tiles;
+  int waves, splits, cols, n_tiles;   // cols: blocks of 16 query rows of a unit
+  bool wide;
 };
 
 // Rows of at most 1024 slots whole, by one launch; longer ones in ranges of at least a
@@ -589,21 +732,44 @@ struct Plan {
 // four take 6.1, but 200 rows of 1024 in 17.6 where those take 15.7.
 Plan decode_plan(int B, int KVH, int cap) {
   const int64_t pairs = (int64_t)B * KVH, tiles = ((int64_t)cap + kTile - 1) / kTile;
-  if (tiles <= 16) return {pairs <= kCus / 2 ? 8 : 4, 1, 1, 1};
+  if (tiles <= 16) return {pairs <= kCus / 2 ? 8 : 4, 1, 1, 1, false};
   const int64_t fill = std::max<int64_t>(2 * kCus / pairs, tiles >= 64 ? 2 : 1);
-  return {4, (int)std::min<int64_t>({(tiles + 3) / 4, fill, kMaxSplits}), 1, 1};
+  return {4, (int)std::min<int64_t>({(tiles + 3) / 4, fill, kMaxSplits}), 1, 1, false};
 }
 
-// As many splits as let two workgroups a CU run at once.
+// Three forms: a workgroup of 128 query rows whose waves share the tiles (wide), or of
+// 16 cols query rows whose waves take the tiles in turn.  MI355X, 7 queries to each of 2
+// kv heads, us in a replayed graph, int8:
+// - wide where its units give most CUs two workgroups or more, if need be cut along
+//   slots as long as each piece keeps 90 tiles: 4 rows of 2048 tokens 73, 89 with two
+//   column blocks and 82 with three; 32 of 100 behind 500 slots 30, 36 and 34; 2048
+//   tokens behind 16384 slots in three pieces 199, 232 and 236; but 2 rows of 1024
+//   behind 8000 in one piece 170, 133 and 129, 16 of 9 to 301 behind 2048 65, 57, 55;
+// - three column blocks, for which a wave turns codes into halves once, where there are
+//   units enough and most slots are old ones: 8 rows of 512 behind 4000 slots 110, with
+//   two 120; but 2048 tokens from slot 0 on 40 and 35, one row of 300 behind 2000 25, 21;
+// - one for a single token's heads and for short rows of up to 64 (4 rows of 5 tokens
+//   behind 1000 slots 12.9, with two 14.3; behind 8000 in 16 pieces 17.5 and 17.1).
+// Rows of at most 2048 slots whole.  Longer ones in as many pieces as let two workgroups a
+// CU run at once; of 32 tiles at least where there are 64 units, whose partials are many.
+// Eight waves where a piece is all of a row and units are few (one row of 300 behind
+// 2000 slots 18.4, with four waves 21.1; 4 rows 43 and 38).
 Plan extend_plan(int B, int KVH, int G, int total, int max_seqlen, int cap) {
-  Plan p = {4, 1, 1, 1};
-  const int64_t rows = (int64_t)max_seqlen * G;
-  p.cols = rows <= 16 ? 1 : 2;
-  p.n_tiles = (int)((rows + 16 * p.cols - 1) / (16 * p.cols));
-  const int64_t units = (int64_t)KVH * std::min<int64_t>((int64_t)B * p.n_tiles,
-                                                         (int64_t)total * G / (16 * p.cols) + B);
-  const int64_t tiles = ((int64_t)cap + kTile - 1) / kTile;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, (tiles + 3) / 4, 2 * kCus / units}));
+  const int64_t rows = (int64_t)max_seqlen * G, tiles = ((int64_t)cap + kTile - 1) / kTile;
+  const auto units = [&](int64_t tr) {   // of tr query rows, at most
+    return KVH * std::min<int64_t>(B * ((rows + tr - 1) / tr), (int64_t)total * G / tr + B);
+  };
+  const auto plan = [&](int cols, int64_t splits, bool wide) {
+    return Plan{4, (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)), cols,
+                (int)((rows + 16 * cols - 1) / (16 * cols)), wide};
+  };
+  const int64_t wide_units = units(128), pieces = std::min<int64_t>(3 * kCus / wide_units, tiles / 90);
+  if (rows > 64 && wide_units * std::max<int64_t>(pieces, 1) >= 3 * kCus / 2) return plan(8, pieces, true);
+  const int cols = rows <= 16 || (rows <= 64 && tiles <= 64) ? 1
+                   : units(48) >= kCus && cap >= 4 * (int64_t)max_seqlen ? 3 : 2;
+  const int64_t n = units(16 * cols);
+  Plan p = plan(cols, tiles <= 32 ? 1 : std::min<int64_t>(tiles / (n >= 64 ? 32 : 4), 2 * kCus / n), false);
+  if (p.splits == 1 && n <= kCus) p.waves = 8;
   return p;
 }
 
@@ -628,13 +794,15 @@ int launch_decode(const AttnArgs& a, int code, int waves, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-template <int kNC>
-int launch_extend(const AttnArgs& a, int code, int waves, hipStream_t st) {
+template <bool kE4m3>
+int launch_extend(const AttnArgs& a, const Plan& p, hipStream_t st) {
   const int64_t grid = (((int64_t)a.B * a.p.kvh * a.splits + 7) & ~(int64_t)7) * a.n_tiles;
   if (grid > 0x7fffffff) return QF_ERR_UNSUPPORTED;
-  const dim3 g((unsigned)grid), b(64 * waves);
-  if (code == QF_CODE_E4M3) hipLaunchKernelGGL((extend_kernel<true, kNC>), g, b, lds_bytes(waves), st, a);
-  else hipLaunchKernelGGL((extend_kernel<false, kNC>), g, b, lds_bytes(waves), st, a);
+  const dim3 g((unsigned)grid), b(64 * p.waves);
+  if (p.wide) hipLaunchKernelGGL(extend_wide_kernel<kE4m3>, g, b, 0, st, a);
+  else if (p.cols == 1) hipLaunchKernelGGL((extend_kernel<kE4m3, 1>), g, b, lds_bytes(p.waves), st, a);
+  else if (p.cols == 3) hipLaunchKernelGGL((extend_kernel<kE4m3, 3>), g, b, lds_bytes(p.waves), st, a);
+  else hipLaunchKernelGGL((extend_kernel<kE4m3, 2>), g, b, lds_bytes(p.waves), st, a);
   return (int)hipGetLastError();
 }
 
@@ -777,7 +945,6 @@ extern "C" int qf_prefill_extend_paged8(const QfExtend8* h, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   rc = append(r, a.cap, st);
   if (rc != QF_OK) return rc;
-  const int code = (int)r.pool.code;
-  rc = p.cols == 1 ? launch_extend<1>(a, code, p.waves, st) : launch_extend<2>(a, code, p.waves, st);
+  rc = r.pool.code == QF_CODE_E4M3 ? launch_extend<true>(a, p, st) : launch_extend<false>(a, p, st);
   return rc == 0 && a.splits > 1 ? launch_merge<false>(a, st) : rc;
 }

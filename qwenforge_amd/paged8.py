@@ -34,8 +34,8 @@ import struct
 import torch
 
 from . import _lib, paged
-from .ops import HEAD_DIM, _scratch_args
-from .paged import MAX_PAGE, _check_page_size, _check_rows, _half, _int_rows, _page_list
+from .ops import HEAD_DIM, _require_cuda_fp16, _scratch_args
+from .paged import MAX_PAGE, _check_page_size, _check_rows, _int_rows, _page_list
 
 BLOCK = 16
 CODES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
@@ -132,39 +132,46 @@ def _pools8(pools, block_table, batch: int, index: int, lead: int = 0):
     try:
         k, v, ks, vs = pools
         shape, strides, scale_strides = k.shape, k.stride(), ks.stride()
-        *_, n_pages, kvh, page, d = shape
-        kind = _KINDS[k.dtype]
-        ok = (len(shape) == 4 + lead and d == HEAD_DIM and n_pages * kvh > 0 and shape[0] > 0
+        if lead:
+            layers, n_pages, kvh, page, d = shape
+            head, outer, scale_outer = (layers, n_pages, kvh), strides[:3], scale_strides[:3]
+        else:
+            n_pages, kvh, page, d = shape
+            layers, head, outer, scale_outer = 1, (n_pages, kvh), strides[:2], scale_strides[:2]
+        dtype, scale_shape = k.dtype, (*head, page // BLOCK)
+        kind = _KINDS[dtype]
+        ok = (d == HEAD_DIM and n_pages > 0 and kvh > 0 and layers > 0
               and 64 <= page <= MAX_PAGE and not page & (page - 1)
-              and v.shape == (*shape[:-2], page // 64, HEAD_DIM, 64) and ks.shape == (*shape[:-2], page // BLOCK)
-              and vs.shape == ks.shape
-              and v.stride() == (*strides[:-2], 4096, 64, 1) and strides[-2:] == (64, 1)
-              and vs.stride() == scale_strides and scale_strides[-1] == 1
-              and v.dtype is k.dtype and ks.dtype is torch.float32 and vs.dtype is torch.float32
+              and v.shape == (*head, page // 64, HEAD_DIM, 64) and ks.shape == scale_shape
+              and vs.shape == scale_shape and v.dtype is dtype
+              and ks.dtype is torch.float32 and vs.dtype is torch.float32
+              and strides == (*outer, 64, 1) and v.stride() == (*outer, 4096, 64, 1)
+              and scale_strides == (*scale_outer, 1) and vs.stride() == scale_strides
               and k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == index >= 0)
     except (AttributeError, KeyError, TypeError, ValueError):
         ok = False
     if not ok:
         _explain_pools(pools, index, lead)
-    if (not isinstance(block_table, torch.Tensor) or block_table.dtype is not torch.int32
-            or block_table.get_device() != index):
-        raise TypeError(f"block_table must be an int32 tensor on cuda:{index}")
-    table_shape, table_strides = block_table.shape, block_table.stride()
-    if len(table_shape) != 2 or table_shape[0] != batch or table_strides[1] != 1:
+    try:
+        (rows, ppr), (table_sb, unit) = block_table.shape, block_table.stride()
+        if block_table.dtype is not torch.int32 or block_table.get_device() != index:
+            raise TypeError(f"block_table must be an int32 tensor on cuda:{index}")
+    except AttributeError:
+        raise TypeError(f"block_table must be an int32 tensor on cuda:{index}") from None
+    except ValueError:
+        rows = unit = -1
+    if rows != batch or unit != 1:
         raise ValueError(f"block_table must be (B={batch}, pages_per_row) with unit inner stride")
-    ppr = table_shape[1]
-    if lead:
-        outer = (*strides[:3], *scale_strides[:3])
-    else:
-        outer = (0, *strides[:2], 0, *scale_strides[:2])
-    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), *outer, block_table.data_ptr(),
-            table_strides[0], ppr, n_pages, page, shape[0] if lead else 1, kvh, kind), kvh, ppr * page
+    if not lead:
+        outer, scale_outer = (0, *outer), (0, *scale_outer)
+    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), *outer, *scale_outer,
+            block_table.data_ptr(), table_sb, ppr, n_pages, page, layers, kvh, kind), kvh, ppr * page
 
 
 def _call8(name: str, index: int, *args) -> None:
     """Entry point ``name`` on GPU ``index`` and its current stream."""
     fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -185,14 +192,42 @@ def _scratch(need: int, device):
     return torch.empty(need, device=device, dtype=torch.uint8) if need else None
 
 
+def _half8(name: str, t, ndim: int):
+    """Shape and strides of an fp16 device tensor of ``ndim`` dimensions with 64 contiguous
+    values in the last, or raises."""
+    try:
+        shape, strides = t.shape, t.stride()
+        if t.dtype is torch.float16 and len(shape) == ndim and shape[-1] == HEAD_DIM and strides[-1] == 1 \
+                and t.get_device() >= 0:
+            return shape, strides
+    except (AttributeError, IndexError):
+        pass
+    _require_cuda_fp16(name, t, ndim)
+    raise RuntimeError(f"{name} must be a HIP device tensor")
+
+
+def _ints8(name: str, t, n: int, dtype, index: int) -> int:
+    """Stride of an ``(n,)`` tensor of ``dtype`` on GPU ``index``, or raises."""
+    try:
+        if t.dtype is dtype and t.shape == (n,) and t.get_device() == index:
+            return t.stride()[0]
+    except AttributeError:
+        pass
+    return _int_rows(name, t, n, dtype, index)
+
+
 def _packed(cu_seqlens, total: int, max_seqlen: int, first, name: str, index: int, lengths):
     """Rows of packed tokens and each one's first slot: their number and first's stride."""
-    b = cu_seqlens.shape[0] - 1 if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.dim() == 1 else 0
+    try:
+        (b,) = cu_seqlens.shape
+        b -= 1
+    except (AttributeError, ValueError):
+        b = 0
     if b < 1 or not 1 <= max_seqlen <= total:
         raise ValueError(f"need B >= 1 rows and 1 <= max_seqlen <= T (got {b}, {max_seqlen})")
-    if _int_rows("cu_seqlens", cu_seqlens, b + 1, torch.int32, index) != 1:
+    if _ints8("cu_seqlens", cu_seqlens, b + 1, torch.int32, index) != 1:
         raise ValueError("cu_seqlens must be contiguous")
-    stride = _int_rows(name, first, b, torch.int64, index)
+    stride = _ints8(name, first, b, torch.int64, index)
     _check_rows(cu_seqlens, total, max_seqlen, lengths)
     return b, stride
 
@@ -204,7 +239,7 @@ def _rope(cos, sin, total: int, index: int):
     if cos is None:
         return None, None, 0
     for n, t in (("cos", cos), ("sin", sin)):
-        _half(n, t, 2)
+        _half8(n, t, 2)
         if t.shape[0] != total or t.get_device() != index:
             raise ValueError(f"{n} must be (T={total}, 64) on cuda:{index}")
     if cos.stride(0) != sin.stride(0):
@@ -241,12 +276,11 @@ def append_paged8(key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tens
     the first slot is written again.  Pages written to must be the row's own.
     """
     lead = 1 if isinstance(key, torch.Tensor) and key.dim() == 4 else 0
-    _half("key", key, 3 + lead)
-    _half("value", value, 3 + lead)
-    index, shape = key.get_device(), key.shape
-    total, kvh = shape[lead], shape[lead + 1]
-    if value.shape != shape or value.get_device() != index:
-        raise ValueError(f"key and value must be alike (got {tuple(shape)}, {tuple(value.shape)})")
+    shape, ks = _half8("key", key, 3 + lead)
+    other, vs = _half8("value", value, 3 + lead)
+    index, total, kvh = key.get_device(), shape[lead], shape[lead + 1]
+    if other != shape or value.get_device() != index:
+        raise ValueError(f"key and value must be alike (got {tuple(shape)}, {tuple(other)})")
     b, ctx_sb = _packed(cu_seqlens, total, max_seqlen, context, "context", index, lengths)
     pool, heads, cap = _pools8(pools, block_table, b, index, lead)
     if heads != kvh or (lead and pool[15] != shape[0]):
@@ -254,7 +288,6 @@ def append_paged8(key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tens
     if max_seqlen > cap:
         raise ValueError(f"max_seqlen exceeds the row capacity {cap}")
     cos, sin, cs_sn = _rope(cos, sin, total, index)
-    ks, vs = key.stride(), value.stride()
     _call8("qf_append_paged8", index, _ROWS.pack(
         *pool, key.data_ptr(), ks[0] if lead else 0, ks[lead + 1], ks[lead], value.data_ptr(),
         vs[0] if lead else 0, vs[lead + 1], vs[lead], cu_seqlens.data_ptr(), total, max_seqlen,
@@ -327,21 +360,22 @@ def copy_pages8(store: torch.Tensor, src, dst) -> None:
 def _decode_args(grouped, pools, block_table, kv_last, key, value):
     """``QfDecode8``'s fields up to kv_last's, the call's GPU, shape and capacity, and
     the fields of the new tokens."""
-    _half("grouped", grouped, 4)
-    shape, index = grouped.shape, grouped.get_device()
+    shape, strides = _half8("grouped", grouped, 4)
+    index = grouped.get_device()
     pool, kvh, cap = _pools8(pools, block_table, shape[0], index)
     if kvh != shape[1]:
         raise ValueError(f"pools hold {kvh} kv heads, grouped {shape[1]}")
-    last_sb = _int_rows("kv_last", kv_last, shape[0], torch.int64, index)
-    strides, new = grouped.stride(), (0, 0, 0, 0, 0, 0)
+    last_sb = _ints8("kv_last", kv_last, shape[0], torch.int64, index)
+    new = (0, 0, 0, 0, 0, 0)
     if (key is None) != (value is None):
         raise ValueError("key and value go together")
     if key is not None:
-        for name, t in (("key", key), ("value", value)):
-            _half(name, t, 3)
-            if t.shape != (shape[0], kvh, HEAD_DIM) or t.get_device() != index:
-                raise ValueError(f"{name} must be {(shape[0], kvh, HEAD_DIM)} on cuda:{index}")
-        new = (key.data_ptr(), *key.stride()[:2], value.data_ptr(), *value.stride()[:2])
+        k_shape, k_strides = _half8("key", key, 3)
+        v_shape, v_strides = _half8("value", value, 3)
+        if k_shape != (shape[0], kvh, HEAD_DIM) or v_shape != k_shape or not (
+                key.get_device() == value.get_device() == index):
+            raise ValueError(f"key and value must be {(shape[0], kvh, HEAD_DIM)} on cuda:{index}")
+        new = (key.data_ptr(), k_strides[0], k_strides[1], value.data_ptr(), v_strides[0], v_strides[1])
     return (*pool, grouped.data_ptr(), strides[0], strides[1], strides[2], kv_last.data_ptr(),
             last_sb), index, shape, cap, new
 
@@ -363,15 +397,16 @@ def flash_decode_attention_paged8(grouped: torch.Tensor, pools, block_table: tor
     """
     head, index, shape, cap, new = _decode_args(grouped, pools, block_table, kv_last, key, value)
     b, kvh, g, d = shape
+    device = grouped.device
     if out is None:
-        out = torch.empty(shape, device=grouped.device, dtype=torch.float16)
+        out = torch.empty(shape, device=device, dtype=torch.float16)
+        strides = (kvh * g * d, g * d, d)
     else:
-        _half("out", out, 4)
-        if out.shape != shape or out.get_device() != index:
-            raise ValueError(f"out must be {tuple(shape)} on {grouped.device}")
+        o_shape, strides = _half8("out", out, 4)
+        if o_shape != shape or out.get_device() != index:
+            raise ValueError(f"out must be {tuple(shape)} on {device}")
     need = _workspace_bytes("qf_decode_attn_paged8_workspace", b, kvh, g, cap)
-    ws = _scratch(need, grouped.device)
-    strides = out.stride()
+    ws = _scratch(need, device)
     _call8("qf_decode_attn_paged8", index, _DECODE.pack(
         *head, out.data_ptr(), strides[0], strides[1], strides[2], _address(ws), need, b, g, d, *new,
         d ** -0.5 if scale is None else scale))
@@ -407,12 +442,11 @@ def prefill_extend_paged8(query: torch.Tensor, key: torch.Tensor, value: torch.T
     is split by it, and slots past it are neither written nor read.  A parked row
     (negative context) gets zeros.  Returns (T, QH, 64).
     """
-    _half("query", query, 3)
-    _half("key", key, 3)
-    _half("value", value, 3)
-    (total, qh, d), shape = query.shape, key.shape
+    (total, qh, d), qs = _half8("query", query, 3)
+    shape, ks = _half8("key", key, 3)
+    v_shape, vs = _half8("value", value, 3)
     kvh = shape[1]
-    if shape[0] != total or value.shape != shape or kvh < 1 or qh % kvh != 0:
+    if shape[0] != total or v_shape != shape or kvh < 1 or qh % kvh != 0:
         raise ValueError("packed extension shapes: query (T, QH, D), key/value (T, KVH, D)")
     index = query.get_device()
     if key.get_device() != index or value.get_device() != index:
@@ -428,10 +462,10 @@ def prefill_extend_paged8(query: torch.Tensor, key: torch.Tensor, value: torch.T
     elif max_seqlen > cap:
         raise ValueError(f"max_seqlen exceeds the row capacity {cap}")
     cos, sin, cs_sn = _rope(cos, sin, total, index)
-    out = torch.empty((total, qh, d), device=query.device, dtype=torch.float16)
+    device = query.device
+    out = torch.empty((total, qh, d), device=device, dtype=torch.float16)
     need = _workspace_bytes("qf_prefill_extend_paged8_workspace", b, qh, kvh, total, max_seqlen, cap)
-    ws = _scratch(need, query.device)
-    qs, ks, vs = query.stride(), key.stride(), value.stride()
+    ws = _scratch(need, device)
     _call8("qf_prefill_extend_paged8", index, _EXTEND.pack(
         *pool, key.data_ptr(), 0, ks[1], ks[0], value.data_ptr(), 0, vs[1], vs[0], cu_seqlens.data_ptr(), total,
         max_seqlen, context.data_ptr(), ctx_sb, _address(cos), _address(sin), cs_sn, b, d, query.data_ptr(), qs[1],

@@ -487,3 +487,78 @@ def test_pages_past_four_gigabytes(dev, code):
     # Page copies over the same distance.
     paged8.copy_pages8(kv.store, far, [20, 21, 22, 23, 24])
     assert torch.equal(kv.store[0, 20:25], kv.store[0, far])
+
+
+# --------------------------------------------------------------------------
+# every form of the extension, past its loops' first rounds
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("lens,ctx,kvh,g,cap", [
+    ([700, 0, 513, 640], [0, 3, 100, 33], 4, 7, None),              # 128 query rows a workgroup, from an odd slot on
+    ([400] * 6, [0, 64, 1, 15, 300, 17], 4, 8, None),
+    ([129, 128, 127, 1], [0, 0, 0, 1], 64, 1, None),
+    ([200], [5900], 16, 16, None),
+    ([200], [12801], 8, 16, None),                                  # the same, cut along slots
+    ([300, 250], [3000, 2500], 8, 7, None),                         # 48 query rows
+    ([70], [2500], 2, 7, None),                                     # 32, in pieces
+    ([2, 1], [4500, 4300], 1, 2, None),                             # 16, in pieces
+    ([60], [10], 2, 7, 65536),                                      # a bound far above what is there
+])
+def test_extension_forms(dev, lens, ctx, kvh, g, cap, code):
+    """Sampled queries of long rows: the first and last of each, those around block, tile and workgroup edges."""
+    gen = torch.Generator().manual_seed(500 + lens[0] + kvh)
+    page = 128
+    need = [c + n for n, c in zip(lens, ctx)]
+    n_pages = sum(-(-n // page) for n in need) + 1
+    layer = tuple(t[0] for t in make_pools(gen, n_pages, kvh, page, code, dev))
+    ppr = -(-(cap or max(need)) // page)
+    table, host = make_table(gen, need, page, n_pages, ppr, dev)
+    fill_rows(gen, layer, table, ctx, dev)
+    total = sum(lens)
+    qkv = torch.randn(total, (g + 2) * kvh, D, generator=gen).half().to(dev)
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=dev)
+    got = paged8.prefill_extend_paged8(qkv[:, :g * kvh], qkv[:, g * kvh:(g + 1) * kvh], qkv[:, (g + 1) * kvh:], cu,
+                                       max(lens), torch.tensor(ctx, device=dev), None, None, layer, table, lengths=lens,
+                                       max_slots=cap or max(need))
+    assert torch.isfinite(got).all()
+    for r, (n, c) in enumerate(zip(lens, ctx)):
+        if n == 0:
+            continue
+        k, v = values_of(layer, host[r], c + n)
+        edges = {0, 1, n - 1, n - 2, n // 2} | {128 // g * j + e for j in range(1, 9) for e in (-1, 0, 1)} \
+            | {64 * j - c % 64 + e for j in range(1, 6) for e in (-1, 0)}
+        for i in sorted(e for e in edges if 0 <= e < n):
+            q = qkv[sum(lens[:r]) + i, :g * kvh].cpu().double().numpy()
+            check(got[sum(lens[:r]) + i], kv8.attend(q, k[:c + i + 1], v[:c + i + 1]), np.abs(v).max(), (r, i))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_wide_extension_with_nan_blocks_and_junk(dev, code):
+    """As the narrow form: NaN tokens reach their block's and later queries, slots behind the row hold anything."""
+    gen = torch.Generator().manual_seed(89)
+    kvh, n, c, b = 8, 300, 20, 6
+    layer = tuple(t[0] for t in make_pools(gen, 40, kvh, 64, code, dev))
+    table, host = make_table(gen, [n + c] * b, 64, 40, 6, dev)
+    fill_rows(gen, layer, table, [c] * b, dev)
+    # Behind the rows: NaN codes and scales.
+    for r in range(b):
+        page = int(host[r, (n + c) // 64])
+        for t, x in ((layer[0], 0x7F), (layer[1], 0xFF)):
+            t.view(torch.uint8)[page] = x
+        for t in layer[2:]:
+            t[page, :, (n + c) % 64 // 16 + 1:] = float("nan")
+    x = torch.randn(2, b * n, kvh, D, generator=gen).half()
+    x[0, 100, 1, 3] = float("nan")                    # row 0, slot 120 (block 112 .. 127), head 1: K
+    x[1, 2 * n + 5, 2, 7] = float("inf")              # row 2, slot 25 (block 16 .. 31), head 2: V
+    q = torch.randn(b * n, kvh * 7, D, generator=gen).half().to(dev)
+    cu = torch.arange(0, (b + 1) * n, n, dtype=torch.int32, device=dev)
+    ctx = torch.tensor([c, c, c, -1, c, c], device=dev)
+    got = paged8.prefill_extend_paged8(q, x[0].to(dev), x[1].to(dev), cu, n, ctx, None, None, layer, table)
+    bad = torch.isnan(got).view(b, n, kvh, 7 * D).all(-1).cpu()
+    assert torch.equal(bad, ~torch.isfinite(got).view(b, n, kvh, 7 * D).all(-1).cpu())
+    want = torch.zeros(b, n, kvh, dtype=torch.bool)
+    want[0, 112 - c:, 1] = True
+    want[2, 0:, 2] = True                             # slots 16 .. 19 of that block are older ones: all see it
+    assert torch.equal(bad, want)
+    assert not got[3 * n:4 * n].any()

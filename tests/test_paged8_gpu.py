@@ -311,3 +311,102 @@ def test_forked_rows_and_compaction(dev, code):
         for a, b in zip(kv.gather(i, 3, 140), want[i]):
             assert torch.equal(a, b[:, :140])
     assert sorted(kv.row_pages(3)) == [0, 1, 2]
+
+
+def test_refusals(dev):
+    """Arguments that the calls refuse, each with one thing wrong."""
+    kv = paged8.PagedKv8Cache(2, 2, 4, 64, 2, 2, dev, "int8")
+    kv.map_row(0, 100)
+    pools, table = kv.pools[0], kv.table
+    x = torch.zeros(9, 2, D, device=dev, dtype=torch.float16)
+    q = torch.zeros(9, 14, D, device=dev, dtype=torch.float16)
+    g = torch.zeros(2, 2, 7, D, device=dev, dtype=torch.float16)
+    cu = torch.tensor([0, 5, 9], dtype=torch.int32, device=dev)
+    ctx = torch.zeros(2, dtype=torch.int64, device=dev)
+    e4m3 = pools[0].view(torch.float8_e4m3fn)
+
+    def append(key=x, value=x, cu=cu, longest=5, ctx=ctx, cos=None, sin=None, pools=pools, table=table, **kw):
+        paged8.append_paged8(key, value, cu, longest, ctx, cos, sin, pools, table, **kw)
+
+    def extend(query=q, key=x, value=x, cu=cu, longest=5, ctx=ctx, cos=None, sin=None, pools=pools, table=table, **kw):
+        paged8.prefill_extend_paged8(query, key, value, cu, longest, ctx, cos, sin, pools, table, **kw)
+
+    def read(pools=pools, table=table, cu=cu, longest=5, ctx=ctx, **kw):
+        paged8.read_paged8(pools, table, cu, longest, ctx, **kw)
+
+    def decode(grouped=g, pools=pools, table=table, ctx=ctx, **kw):
+        paged8.flash_decode_attention_paged8(grouped, pools, table, ctx, **kw)
+
+    k, v, ks, vs = pools
+    bad_pools = [(k, v, ks), (k.float(), v, ks, vs), (k, v.view(torch.uint8), ks, vs), (k, v.view(torch.float8_e4m3fn), ks, vs),
+                 (k, v, ks.half(), vs), (k, v.transpose(3, 4), ks, vs), (k, v, ks[:, :, :2], vs),
+                 (k, v.contiguous(), ks, vs), (k, v, ks.contiguous(), vs), (k[..., :32], v, ks, vs), (k[:, :, :32], v, ks, vs),
+                 (k, v, ks, vs.cpu()), (k[:0], v[:0], ks[:0], vs[:0]), kv.all_pools, (e4m3, v, ks, vs), None]
+    for call in (append, extend, read, decode):
+        for p in bad_pools:
+            if call is read and p is kv.all_pools:
+                continue
+            with pytest.raises((TypeError, ValueError, RuntimeError)):
+                call(pools=p)
+        for t in (table.long(), table.cpu(), table[:1], table.t(), table[0], None):
+            with pytest.raises((TypeError, ValueError)):
+                call(table=t)
+        for c in (ctx.int(), ctx.cpu(), ctx[:1], ctx.view(1, 2), None):
+            with pytest.raises((TypeError, ValueError)):
+                call(ctx=c)
+    for call in (append, extend, read):
+        for c in (cu.long(), cu.cpu(), cu[:1], cu.view(1, 3), cu + 1, cu.flip(0), cu.repeat_interleave(2)[::2], None):
+            with pytest.raises((TypeError, ValueError)):
+                call(cu=c)
+        for n in (0, 4, 10):
+            with pytest.raises(ValueError):
+                call(longest=n)
+        # (The read's total is the sum of lengths: 5 and 5 would be rows of another cu_seqlens.)
+        for n in ([9], [5, 4, 0], [10, -1]) + (() if call is read else ([5, 5],)):
+            with pytest.raises(ValueError):
+                call(lengths=n)
+    for call in (append, extend):
+        for t in (x.float(), x.cpu(), x[..., :32], x[:, :1], x[:8], x[:, 0], x.transpose(0, 2), None):
+            with pytest.raises((TypeError, ValueError, RuntimeError)):
+                call(key=t)
+            with pytest.raises((TypeError, ValueError, RuntimeError)):
+                call(value=t)
+        with pytest.raises(ValueError):
+            call(cos=x[:, 0].contiguous())
+        with pytest.raises(ValueError):
+            call(cos=x[:8, 0].contiguous(), sin=x[:8, 0].contiguous())
+        with pytest.raises((TypeError, RuntimeError)):
+            call(cos=x[:, 0].float(), sin=x[:, 0].float())
+    with pytest.raises(ValueError):
+        append(key=x[None], value=x[None], pools=kv.all_pools)        # one layer's tokens, two layers' pools
+    for t in (q.float(), q[:8], q[:, :13], q[:, :, :32], q[0], None):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            extend(query=t)
+    with pytest.raises((ValueError, RuntimeError)):
+        extend(query=torch.zeros(9, 34, D, device=dev, dtype=torch.float16))   # 17 heads of a kv head
+    for n in (4, 129):
+        with pytest.raises(ValueError):
+            extend(max_slots=n)
+    for kw in (dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan"))):
+        for call in (extend, decode):
+            with pytest.raises(RuntimeError, match="invalid"):
+                call(**kw)
+    for t in (g.float(), g[:1], g[:, :1], g[..., :32], g[0], None):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            decode(grouped=t)
+    new = x[:2]
+    for kw in (dict(out=g.float()), dict(out=g[:1]), dict(out=g.cpu()), dict(key=new), dict(value=new),
+               dict(key=new, value=x[:1]), dict(key=new.float(), value=new), dict(key=new[:, :1], value=new[:, :1])):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            decode(**kw)
+    big = torch.zeros(200, 2, D, device=dev, dtype=torch.float16)
+    with pytest.raises(ValueError, match="capacity"):
+        append(key=big, value=big, cu=torch.tensor([0, 200, 200], dtype=torch.int32, device=dev), longest=200)
+    for src, dst in (([0], [0]), ([0, 1], [2, 2]), ([4], [0]), ([-1], [0]), ([0], [1, 2]), ([0.5], [1])):
+        with pytest.raises((ValueError, TypeError)):
+            paged8.copy_pages8(kv.store, src, dst)
+    for store in (kv.store.view(torch.int8), kv.store[:, :2], kv.store[0], kv.store.cpu()):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            paged8.copy_pages8(store, [0], [1])
+    for call in (append, extend, read, decode):
+        call()                                                       # and as they are
