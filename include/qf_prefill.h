@@ -14,6 +14,7 @@
 #include <stdint.h>
 
 #include "qf_attn.h"
+#include "qf_paged8.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -69,6 +70,17 @@ int qf_extend_layers(const QfPrefillLayer* layers, int n_layers, void* hidden, i
                      const float* inv_freq, const int32_t* block_table, int64_t bt_sb,
                      int pages_per_row, int n_pages, int page_size, void* ws, int64_t ws_bytes,
                      float eps, int hidden_size, int QH, int KVH, int D, int I, void* stream);
+
+/* qf_extend_layers over caches held in 8 bits (qf_prefill_extend_paged8: cu, context,
+ * ctx_sb, max_seqlen and cap as there): layer i's keys and values go to pools[i], HOST
+ * structs of one layer each; the caches of `layers` are not used. */
+int64_t qf_extend_layers_paged8_workspace(int T, int hidden, int QH, int KVH, int D, int I, int B,
+                                          int max_seqlen, int cap);
+
+int qf_extend_layers_paged8(const QfPrefillLayer* layers, const QfPool8* pools, int n_layers, void* hidden,
+                            int T, int B, int max_seqlen, const int32_t* cu, const int64_t* context,
+                            int64_t ctx_sb, int cap, const float* inv_freq, void* ws, int64_t ws_bytes,
+                            float eps, int hidden_size, int QH, int KVH, int D, int I, void* stream);
 
 #ifdef __cplusplus
 }

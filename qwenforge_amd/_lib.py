@@ -270,6 +270,15 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32, _i32,   # hidden_size, QH, KVH, D, I
         _vp,                            # stream
     ],
+    "qf_extend_layers_paged8_workspace": [_i32] * 9,  # T, hidden, QH, KVH, D, I, B, max_seqlen, cap
+    "qf_extend_layers_paged8": [
+        _vp, C.c_char_p, _i32, _vp,     # layers, pools, n_layers, hidden
+        _i32, _i32, _i32,               # T, B, max_seqlen
+        _vp, _vp, _i64, _i32, _vp,      # cu, context, ctx_sb, cap, inv_freq
+        _vp, _i64, _f32,                # ws, ws_bytes, eps
+        _i32, _i32, _i32, _i32, _i32,   # hidden_size, QH, KVH, D, I
+        _vp,                            # stream
+    ],
     "qf_prefill_layers": [
         _vp, _i32, _vp, _i32, _i32, _i32,  # layers, n_layers, hidden, T, B, S
         _vp, _vp,                       # cu, inv_freq
@@ -360,7 +369,7 @@ for _name in ("qf_decode_attn", "qf_decode_attn_paged"):
 RESTYPES = {"qf_error_string": C.c_char_p, "qf_prefill_layers_workspace": _i64,
             "qf_decode_attn_prefix_workspace": _i64, "qf_prefill_extend_workspace": _i64,
             "qf_extend_layers_workspace": _i64, "qf_verify_workspace": _i64,
-            "qf_decode_attn_paged8_workspace": _i64, "qf_prefill_extend_paged8_workspace": _i64}
+            "qf_extend_layers_paged8_workspace": _i64, "qf_decode_attn_paged8_workspace": _i64, "qf_prefill_extend_paged8_workspace": _i64}
 
 _lock = threading.Lock()
 _lib: C.CDLL | None = None

@@ -20,6 +20,7 @@
 
 #include "extend.h"
 #include "step_common.h"
+#include "../../include/qf_paged8.h"
 #include "../../include/qf_prefill.h"
 #include "../../include/qf_prefix.h"
 
@@ -455,7 +456,7 @@ __global__ __launch_bounds__(256) void prefill_tokens_kernel(const int* cu, int 
                                                              const int32_t* table, int64_t t_sb,
                                                              int log2p, int ppr, int n_pages,
                                                              const int64_t* context, int64_t ctx_sb,
-                                                             int cap, f16* cs, int2* info) {
+                                                             int cap, f16* cs, int2* info, bool append) {
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5), i = threadIdx.x & 31;
   if (t >= T) return;
   int b, pos;
@@ -484,7 +485,7 @@ __global__ __launch_bounds__(256) void prefill_tokens_kernel(const int* cu, int 
   cs[64 * t + i] = (f16)cosf(ang);
   cs[64 * t + 32 + i] = (f16)sinf(ang);
   if (i == 0) {
-    int2 at = make_int2(pos < S ? b : -1, pos);
+    int2 at = make_int2(append && pos < S ? b : -1, pos);
     if (table != nullptr) {
       const int lp = pos >> log2p;
       const int page = pos < S && lp < ppr ? table[b * t_sb + lp] : -1;
@@ -664,12 +665,14 @@ extern "C" int64_t qf_prefill_layers_workspace(int T, int hidden, int QH, int KV
 }
 
 // Every layer of a prompt pass, or with `context` of an extension (then with cu
-// and block_table; `cap` as there).
+// and block_table; `cap` as there), over the layers' `pools` in 8 bits if given (then
+// without block_table, S the longest row).
 static int run_layers(const QfPrefillLayer* layers, int n_layers, void* hidden_p, int T, int B, int S,
                       const int32_t* cu, const int64_t* context, int64_t ctx_sb, int cap,
                       const float* inv_freq, const int32_t* block_table, int64_t bt_sb,
                       int pages_per_row, int n_pages, int page_size, void* ws, int64_t ws_bytes,
-                      float eps, int H, int QH, int KVH, int D, int I, void* stream) {
+                      float eps, int H, int QH, int KVH, int D, int I, void* stream,
+                      const QfPool8* pools = nullptr) {
   if (!shapes_ok(T, H, QH, KVH, D, I)) return QF_ERR_UNSUPPORTED;
   if (!layers || n_layers < 1 || !hidden_p || !inv_freq || !ws || B < 1 || S < 1)
     return QF_ERR_INVALID_ARG;
@@ -680,7 +683,8 @@ static int run_layers(const QfPrefillLayer* layers, int n_layers, void* hidden_p
   const Workspace w = workspace(T, H, QH, KVH, I);
   int64_t spans = 0;  // the extension's attention scratch, behind the rest
   if (context != nullptr) {
-    spans = qf_prefill_extend_workspace(B, QH, KVH, T, cap);
+    spans = pools != nullptr ? qf_prefill_extend_paged8_workspace(B, QH, KVH, T, S, cap)
+                             : qf_prefill_extend_workspace(B, QH, KVH, T, cap);
     if (spans < 0) return (int)spans;
   }
   if (ws_bytes < w.bytes + spans) return QF_ERR_SCRATCH_LIMIT;
@@ -692,8 +696,8 @@ static int run_layers(const QfPrefillLayer* layers, int n_layers, void* hidden_p
   }
   for (int i = 0; i < n_layers; ++i) {
     const QfPrefillLayer& y = layers[i];
-    if (!y.norm1 || !y.w_qkv || !y.w_o || !y.norm2 || !y.w_gate_up || !y.w_down || !y.k_cache ||
-        !y.v_cache)
+    if (!y.norm1 || !y.w_qkv || !y.w_o || !y.norm2 || !y.w_gate_up || !y.w_down ||
+        (pools == nullptr && (!y.k_cache || !y.v_cache)))
       return QF_ERR_INVALID_ARG;
     if (!al16(y.norm1) || !al16(y.w_qkv) || !al16(y.w_o) || !al16(y.norm2) || !al16(y.w_gate_up) ||
         !al16(y.w_down) || !al16(y.k_cache) || !al16(y.v_cache) || !al16(y.b_qkv))
@@ -723,7 +727,7 @@ static int run_layers(const QfPrefillLayer* layers, int n_layers, void* hidden_p
   };
   hipLaunchKernelGGL(prefill_tokens_kernel, dim3((T + 7) / 8), dim3(256), 0, st, cu, B, S, T,
                      inv_freq, block_table, bt_sb, l2, pages_per_row, n_pages, context, ctx_sb, cap, cs,
-                     info);
+                     info, pools == nullptr);
   int rc = (int)hipGetLastError();
   for (int i = 0; i < n_layers && rc == 0; ++i) {
     const QfPrefillLayer& y = layers[i];
@@ -748,7 +752,30 @@ static int run_layers(const QfPrefillLayer* layers, int n_layers, void* hidden_p
     gq.N = W; gq.K = H;
     rc = launch<kEpiQkv>(gq, cus, st);
     if (rc) break;
-    if (context != nullptr) {
+    if (pools != nullptr) {
+      // The projection left the rotated K and V behind Q; they go to the pages from there.
+      QfExtend8 e = {};
+      e.rows.pool = pools[i];
+      e.rows.k = qkv + A;
+      e.rows.v = qkv + A + KVH * 64;
+      e.rows.k_sh = e.rows.v_sh = 64;
+      e.rows.k_sn = e.rows.v_sn = W;
+      e.rows.cu_seqlens = cu;
+      e.rows.total = T; e.rows.max_seqlen = S;
+      e.rows.first = context;
+      e.rows.first_sb = ctx_sb;
+      e.rows.B = B; e.rows.D = D;
+      e.q = qkv;
+      e.q_sh = 64; e.q_sn = W;
+      e.out = att;
+      e.o_sh = 64; e.o_sn = A;
+      e.cap = cap;
+      e.ws = base + w.bytes;
+      e.ws_bytes = spans;
+      e.QH = QH;
+      e.scale = 0.125;
+      rc = qf_prefill_extend_paged8(&e, stream);
+    } else if (context != nullptr) {
       const ExtendCall c = {cu, context, ctx_sb, block_table, bt_sb, pages_per_row, n_pages, page_size,
                             cap, B, T, QH, KVH};
       rc = extend_attention(c, qkv, 64, W, att, 64, A, y.k_cache, y.kc_sb, y.kc_sh, y.kc_sn, y.v_cache,
@@ -817,4 +844,29 @@ extern "C" int qf_extend_layers(const QfPrefillLayer* layers, int n_layers, void
   return run_layers(layers, n_layers, hidden_p, T, B, 1, cu, context, ctx_sb, cap, inv_freq,
                     block_table, bt_sb, pages_per_row, n_pages, page_size, ws, ws_bytes, eps, H, QH,
                     KVH, D, I, stream);
+}
+
+extern "C" int64_t qf_extend_layers_paged8_workspace(int T, int hidden, int QH, int KVH, int D, int I,
+                                                     int B, int max_seqlen, int cap) {
+  const int64_t bytes = qf_prefill_layers_workspace(T, hidden, QH, KVH, D, I);
+  const int64_t spans =
+      bytes < 0 ? bytes : qf_prefill_extend_paged8_workspace(B, QH, KVH, T, max_seqlen, cap);
+  return spans < 0 ? spans : bytes + spans;
+}
+
+extern "C" int qf_extend_layers_paged8(const QfPrefillLayer* layers, const QfPool8* pools, int n_layers,
+                                       void* hidden_p, int T, int B, int max_seqlen, const int32_t* cu,
+                                       const int64_t* context, int64_t ctx_sb, int cap,
+                                       const float* inv_freq, void* ws, int64_t ws_bytes, float eps, int H,
+                                       int QH, int KVH, int D, int I, void* stream) {
+  if (!pools || !cu || !context || B < 1 || cap < 1 || T < 1 || max_seqlen < 1 || max_seqlen > T || n_layers < 1)
+    return QF_ERR_INVALID_ARG;
+  if ((int64_t)cap + T > 0x7fffffff) return QF_ERR_UNSUPPORTED;
+  for (int i = 0; i < n_layers; ++i)
+    if (pools[i].KVH != KVH || pools[i].layers != 1 || pools[i].page_size < 1 ||
+        pools[i].page_size > 4096 || pools[i].pages_per_row < 1 || pools[i].pages_per_row > 0x7fffffff ||
+        cap > pools[i].pages_per_row * pools[i].page_size)
+      return QF_ERR_INVALID_ARG;
+  return run_layers(layers, n_layers, hidden_p, T, B, max_seqlen, cu, context, ctx_sb, cap, inv_freq, nullptr, 0,
+                    0, 0, 0, ws, ws_bytes, eps, H, QH, KVH, D, I, stream, pools);
 }

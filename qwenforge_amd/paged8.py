@@ -95,6 +95,7 @@ class PagedKv8Cache(paged.PagedKvCache):
 
 # The structs of the C ABI, all of 8-byte fields: packed here in one go, where
 # handing that many arguments to ctypes would take longer than the launch.
+POOL = struct.Struct("=18q")
 _ROWS = struct.Struct("=36q")         # QfPool8 (18), then QfRows8's own
 _DECODE = struct.Struct("=39qd")      # QfPool8, then QfDecode8's own
 _EXTEND = struct.Struct("=46qd")      # QfRows8, then QfExtend8's own

@@ -136,8 +136,7 @@ class PagedDecodeEngine(DecodeEngine):
         after every token (packed) without ``last_only``.
 
         The slots must be mapped; pages of theirs that another row holds too are
-        copied first (``PagedKvCache.own_slots``).  Over a cache in 8 bits the
-        projections are torch's."""
+        copied first (``PagedKvCache.own_slots``)."""
         cfg, dev = self.cfg, self.device
         rows, contexts = list(rows), [int(c) for c in contexts]
         lengths = [int(c.numel()) for c in chunks]
@@ -156,7 +155,7 @@ class PagedDecodeEngine(DecodeEngine):
         cu = torch.tensor(starts, dtype=torch.int32, device=dev)
         ctx = torch.tensor(contexts, dtype=torch.int64, device=dev)
         hidden = F.embedding(ids, self.w["embed"])
-        if not self._native_extension(hidden, kv, cu, ctx, most, table):
+        if not self._native_extension(hidden, kv, cu, max(lengths), ctx, most, table):
             pos = torch.cat([torch.arange(c, c + n, device=dev) for c, n in zip(contexts, lengths)])
             cos, sin = cos_sin(pos, self.inv_freq)
             qh, kvh, d = cfg.heads, cfg.kv_heads, cfg.head_dim
@@ -173,13 +172,20 @@ class PagedDecodeEngine(DecodeEngine):
                 hidden = hidden + self._mlp(self._rms(hidden, layer["post_norm"]), layer)
         return self._last_logits(hidden[cu[1:].long() - 1] if last_only else hidden)
 
-    def _native_extension(self, hidden, kv, cu, ctx, most: int, table) -> bool:
+    def _native_extension(self, hidden, kv, cu, longest: int, ctx, most: int, table) -> bool:
         """Every layer of an extension in one native call, or False where the
         model's or the caches' layout is one it does not take."""
         cfg = self.cfg
-        if (isinstance(kv, paged8.PagedKv8Cache) or hidden.dtype != torch.float16 or not hidden.is_cuda
+        if (hidden.dtype != torch.float16 or not hidden.is_cuda
                 or prefill_ops.workspace_bytes(cfg, hidden.shape[0]) < 0):
             return False
+        if isinstance(kv, paged8.PagedKv8Cache):
+            layers = prefill_ops.layer_table(cfg, self.w["layers"], None, hidden.device, None)
+            if layers is None:
+                return False
+            prefill_ops.extend_layers_paged8(cfg, layers, kv.pools, hidden, cu, longest, ctx, most,
+                                             self.inv_freq, table)
+            return True
         layers = prefill_ops.layer_table(cfg, self.w["layers"], kv.pools, hidden.device,
                                          (kv.n_pages, kv.kv_heads, kv.page_size, cfg.head_dim))
         if layers is None:

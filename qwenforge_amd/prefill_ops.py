@@ -5,7 +5,7 @@ o_proj + residual, rms_norm, gate/up + SwiGLU and down_proj + residual of all
 layers (SE:679-737, SE:1162-1204).  ``layer_table`` says whether a model and its
 caches have the layouts it takes; the engine keeps the torch projections
 otherwise.  ``extend_layers`` is the same pass for new tokens of rows that hold
-cached slots already.
+cached slots already, ``extend_layers_paged8`` over caches held in 8 bits.
 """
 
 from __future__ import annotations
@@ -14,7 +14,7 @@ import ctypes as C
 
 import torch
 
-from . import _lib
+from . import _lib, paged8
 from .ops import _ptr, _stream
 
 
@@ -31,11 +31,13 @@ def layer_table(cfg, layers, caches, device, shape):
     any of them has another type, device, layout or size.  ``shape`` is the
     caches' (rows or pages, kv heads, least slots, 64).  Built for each call:
     no pointer outlives it.  ``rows`` and ``slots`` of the result are what every
-    cache holds."""
+    cache holds.  Without ``caches`` (None) the weights alone."""
     h, width = cfg.hidden, cfg.qkv_width
     want = (("input_norm", (h,)), ("qkv_weight", (width, h)), ("qkv_bias", (width,)),
             ("o_weight", (h, cfg.heads * cfg.head_dim)), ("post_norm", (h,)),
             ("gate_up_weight", (2 * cfg.intermediate, h)), ("down_weight", (h, cfg.intermediate)))
+    if caches is None:
+        caches, shape = [()] * len(layers), (0, 0, 0, 0)
     if cfg.heads * cfg.head_dim != h or len(layers) != len(caches):
         return None
     table = (Layer * len(layers))()
@@ -62,6 +64,8 @@ def layer_table(cfg, layers, caches, device, shape):
                 return None
             ptrs.append(ptr)
             strides += stride[:3]
+        if not pair:
+            ptrs, strides = ptrs + [None, None], [0] * 6
         (entry.norm1, entry.w_qkv, entry.b_qkv, entry.w_o, entry.norm2, entry.w_gate_up,
          entry.w_down, entry.k_cache, entry.v_cache) = ptrs
         (entry.kc_sb, entry.kc_sh, entry.kc_sn, entry.vc_sb, entry.vc_sh, entry.vc_sn) = strides
@@ -151,3 +155,36 @@ def extend_layers(cfg, table, hidden: torch.Tensor, cu: torch.Tensor, context: t
             block_table.shape[1], n_pages, page_size, ws.data_ptr(), need, float(cfg.rms_eps),
             cfg.hidden, cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.intermediate, _stream(dev))
     _lib.check(rc, "qf_extend_layers")
+
+
+def extend_layers_paged8(cfg, table, pools, hidden: torch.Tensor, cu: torch.Tensor, max_seqlen: int,
+                         context: torch.Tensor, max_slots: int, inv_freq: torch.Tensor,
+                         block_table: torch.Tensor) -> None:
+    """``extend_layers`` over caches held in 8 bits: ``pools`` are every layer's
+    (``paged8.PagedKv8Cache.pools``), ``table`` a ``layer_table`` without caches, and
+    no row has more than ``max_seqlen`` new tokens."""
+    rows, tokens = context.numel(), hidden.numel() // cfg.hidden
+    dev = hidden.device
+    if hidden.dtype != torch.float16 or dev.type != "cuda" or not hidden.is_contiguous():
+        raise ValueError("hidden must be a contiguous fp16 device tensor")
+    if len(pools) != len(table):
+        raise ValueError(f"{len(table)} layers need as many pools (got {len(pools)})")
+    for name, t, dtype, shape in (("cu", cu, torch.int32, (rows + 1,)),
+                                  ("context", context, torch.int64, (rows,)),
+                                  ("inv_freq", inv_freq, torch.float32, (cfg.head_dim // 2,))):
+        if t.dtype != dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {shape} {str(dtype)[6:]} on hidden's device")
+    index = hidden.get_device()
+    packed = b"".join(paged8.POOL.pack(*paged8._pools8(p, block_table, rows, index)[0]) for p in pools)
+    sizes = (tokens, cfg.hidden, cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.intermediate, rows, int(max_seqlen),
+             int(max_slots))
+    lib = _lib.load()
+    need = lib.qf_extend_layers_paged8_workspace(*sizes)
+    _lib.check(min(need, 0), "qf_extend_layers_paged8_workspace")
+    with torch.cuda.device(dev):
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        rc = lib.qf_extend_layers_paged8(
+            table, packed, len(table), hidden.data_ptr(), tokens, rows, int(max_seqlen), cu.data_ptr(),
+            context.data_ptr(), 1, int(max_slots), inv_freq.data_ptr(), ws.data_ptr(), need, float(cfg.rms_eps),
+            cfg.hidden, cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.intermediate, _stream(dev))
+    _lib.check(rc, "qf_extend_layers_paged8")

@@ -99,11 +99,15 @@ def test_steps_match_the_oracle_over_the_same_pages(dev, batch, tiles, code):
     assert ctx["pos"].cpu().tolist() == [n + 4 for n in lengths]
 
 
+@pytest.mark.parametrize("native", [True, False])
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
-def test_extension_matches_the_oracle_over_the_same_pages(dev, code):
+def test_extension_matches_the_oracle_over_the_same_pages(dev, code, native, monkeypatch):
+    """All layers in one native call, and with torch's projections."""
     cfg = Qwen2Config(layers=2, vocab=4096)
     w_cpu = init_weights(cfg, "cpu", seed=18)
     eng = PagedDecodeEngine(cfg, weights_to(w_cpu, dev), dev)
+    if not native:
+        monkeypatch.setattr(eng, "_native_extension", lambda *args: False)
     gen = torch.Generator().manual_seed(23)
     prompts = [torch.randint(0, cfg.vocab, (n,), generator=gen) for n in (40, 70)]
     chunks = [torch.randint(0, cfg.vocab, (n,), generator=gen) for n in (5, 3)]
@@ -114,6 +118,8 @@ def test_extension_matches_the_oracle_over_the_same_pages(dev, code):
     got = eng.extend_paged([c.to(dev) for c in chunks], kv, [0, 1], [40, 70], last_only=False).float().cpu()
     first = 0
     for r, (p, c) in enumerate(zip(prompts, chunks)):
+        before = [[x.cpu() for x in kv.gather(layer, r, len(p))] for layer in range(cfg.layers)]
+        assert all(torch.isfinite(x).all() and x.any() for pair in before for x in pair)
         for i, token in enumerate(c):
             pos = len(p) + i
             caches = [tuple(x.cpu() for x in kv.gather(layer, r, pos + 1)) for layer in range(cfg.layers)]
@@ -159,3 +165,29 @@ def test_generation_and_drafts(dev, code):
     assert out.shape == (3, 10) and stats["drafted"] > 0
     with pytest.raises(ValueError, match="code must be"):
         eng.generate_paged(prompts, 2, kv_code="int4")
+
+
+def test_native_extension_s_refusals(dev):
+    from qwenforge_amd import prefill_ops
+
+    cfg = Qwen2Config(layers=2, vocab=4096)
+    eng = PagedDecodeEngine(cfg, init_weights(cfg, dev, seed=5), dev)
+    kv = eng.new_paged_cache(2, 4, 64, 2, "int8")
+    kv.map_row(0, 100)
+    table = prefill_ops.layer_table(cfg, eng.w["layers"], None, dev, None)
+    hidden = torch.zeros(7, cfg.hidden, device=dev, dtype=torch.float16)
+    cu = torch.tensor([0, 5, 7], dtype=torch.int32, device=dev)
+    ctx = torch.zeros(2, dtype=torch.int64, device=dev)
+
+    def call(pools=kv.pools, hidden=hidden, cu=cu, longest=5, ctx=ctx, most=128, freq=eng.inv_freq, blocks=kv.table):
+        prefill_ops.extend_layers_paged8(cfg, table, pools, hidden, cu, longest, ctx, most, freq, blocks)
+
+    for kw in (dict(pools=kv.pools[:1]), dict(pools=[kv.pools[0], kv.all_pools]), dict(hidden=hidden.float()),
+               dict(hidden=hidden.t().contiguous().t()), dict(cu=cu.long()), dict(cu=cu[:2]), dict(ctx=ctx.int()),
+               dict(freq=eng.inv_freq.half()), dict(blocks=kv.table[:1]), dict(blocks=kv.table.long())):
+        with pytest.raises((ValueError, TypeError)):
+            call(**kw)
+    for kw in (dict(longest=0), dict(longest=8), dict(most=0), dict(most=129)):
+        with pytest.raises(RuntimeError):
+            call(**kw)
+    call()
