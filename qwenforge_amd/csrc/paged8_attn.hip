@@ -38,6 +38,7 @@ struct AttnArgs {
   const int64_t* last;                       // decode: last slot; extension: cached slots
   int64_t last_sb;
   int B, tokens, G, cap;
+  int longest;                               // extension: tokens of a row that get an output
   int n_tiles, splits;                       // query tiles of a row, splits of a row's slots
   float* acc;                                // (token, kv head, split, query head, 64)
   float* m;                                  // (token, kv head, split, query head), times m_unit
@@ -498,14 +499,15 @@ __device__ __forceinline__ bool extend_unit(const AttnArgs& a, Unit& u) {
   id /= a.splits;
   u.hk = id % a.p.kvh;
   u.row = id / a.p.kvh;
-  const int lo = clampi(a.cu[u.row], 0, a.tokens), hi = clampi(a.cu[u.row + 1], lo, a.tokens);
+  const int lo = clampi(a.cu[u.row], 0, a.tokens);
+  const int new_tokens = min(clampi(a.cu[u.row + 1], lo, a.tokens) - lo, a.longest);
   u.tok0 = lo;
-  u.rows = (hi - lo) * a.G;
+  u.rows = new_tokens * a.G;
   u.r0 = tile * kRows;
   if (u.r0 >= u.rows) return false;
   u.ctx = clampi(a.last[u.row * a.last_sb], -1, a.cap);
   // All tiles of a row are cut alike; a tile stops where its newest token does.
-  const int end = u.ctx < 0 ? 0 : min(u.ctx + hi - lo, a.cap);
+  const int end = u.ctx < 0 ? 0 : min(u.ctx + new_tokens, a.cap);
   cut(end, u.split, a.splits, u.k0, u.k1);
   if (u.ctx >= 0) {
     const int newest = (min(u.r0 + kRows, u.rows) - 1) / a.G;
@@ -665,10 +667,11 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a) {
       if (a.cu[mid] <= token) lo = mid;
       else hi = mid;
     }
-    const int t0 = clampi(a.cu[lo], 0, a.tokens), t1 = clampi(a.cu[lo + 1], t0, a.tokens);
-    mine = mine && token >= t0 && token < t1;
+    const int t0 = clampi(a.cu[lo], 0, a.tokens);
+    const int new_tokens = min(clampi(a.cu[lo + 1], t0, a.tokens) - t0, a.longest);
+    mine = mine && token >= t0 && token < t0 + new_tokens;
     const int ctx = clampi(a.last[lo * a.last_sb], -1, a.cap);
-    end = ctx < 0 ? 0 : min(ctx + t1 - t0, a.cap);
+    end = ctx < 0 ? 0 : min(ctx + new_tokens, a.cap);
     lim = ctx < 0 ? 0 : min(ctx + token - t0 + 1, a.cap);
   }
   int n = 0;   // splits that hold a slot below lim
@@ -940,6 +943,7 @@ extern "C" int qf_prefill_extend_paged8(const QfExtend8* h, void* stream) {
   const Plan p = extend_plan(a.B, a.p.kvh, a.G, a.tokens, (int)r.max_seqlen, a.cap);
   a.splits = p.splits;
   a.n_tiles = p.n_tiles;
+  a.longest = (int)r.max_seqlen;
   rc = set_parts(a, h->ws, h->ws_bytes);
   if (rc != QF_OK) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -562,3 +562,38 @@ def test_wide_extension_with_nan_blocks_and_junk(dev, code):
     want[2, 0:, 2] = True                             # slots 16 .. 19 of that block are older ones: all see it
     assert torch.equal(bad, want)
     assert not got[3 * n:4 * n].any()
+
+
+def test_wild_device_arrays_stay_in_bounds(dev):
+    """Offsets, slots, tables and contexts of any contents: nothing outside is touched, the call comes back, and rows
+    that are right are right.  (Offsets can only be wrong where they are not read on the host: with ``lengths``.)"""
+    gen = torch.Generator().manual_seed(97)
+    for code in ("int8", "e4m3"):
+        pools = make_pools(gen, 8, 2, 64, code, dev)
+        layer = tuple(t[0] for t in pools)
+        table, host = make_table(gen, [200, 150], 64, 8, 4, dev)
+        fill_rows(gen, layer, table, [200, 150], dev)
+        kv = torch.randn(9, 4, D, generator=gen).half().to(dev)
+        q = torch.randn(9, 14, D, generator=gen).half().to(dev)
+        lengths = [5, 4]
+        big = [2 ** 63 - 1, 2 ** 40 + 5, 2 ** 31, 10 ** 6, -2 ** 63]
+        for cu in ([0, 5, 9], [0, 9, 0], [7, 3, 20], [-4, 100, 2 ** 31 - 1], [2 ** 31 - 1, -2 ** 31, 5]):
+            cu = torch.tensor(cu, dtype=torch.int32, device=dev)
+            for a in big + [100]:
+                for wild in (table, torch.full_like(table, 2 ** 31 - 1), torch.full_like(table, -2 ** 31)):
+                    ctx = torch.tensor([a, 100], device=dev)
+                    work = tuple(t.clone() for t in layer)
+                    paged8.append_paged8(kv[:, :2], kv[:, 2:], cu, 5, ctx, None, None, work, wild, lengths=lengths)
+                    paged8.read_paged8(work, wild, cu, 5, ctx, lengths=lengths)
+                    paged8.prefill_extend_paged8(q, kv[:, :2], kv[:, 2:], cu, 5, ctx, None, None, work, wild,
+                                                 lengths=lengths)
+                    g = q[:2].view(2, 2, 7, D)
+                    paged8.flash_decode_attention_paged8(g, work, wild, ctx, key=kv[:2, :2], value=kv[:2, 2:])
+                    torch.cuda.synchronize()
+    cu = torch.tensor([0, 5, 9], dtype=torch.int32, device=dev)
+    ctx = torch.tensor([2 ** 40, 100], device=dev)
+    work = tuple(t.clone() for t in layer)
+    got = paged8.prefill_extend_paged8(q, kv[:, :2], kv[:, 2:], cu, 5, ctx, None, None, work, table, lengths=lengths)
+    k, v = values_of(work, host[1], 104)
+    for i in range(4):
+        check(got[5 + i], kv8.attend(q[5 + i].cpu().double().numpy(), k[:101 + i], v[:101 + i]), np.abs(v).max(), i)
