@@ -118,6 +118,9 @@ inline int make_pool(const QfPool8& h, Pool& p) {
 
 inline int row_cap(const Pool& p) { return p.ppr << p.log2p; }
 
+// What a call has to say about packed tokens, but for its pool (paged8.hip).
+int check_rows(const QfRows8& rows);
+
 // qf_append_paged8 into the rows' slots below cap (paged8.hip).
 int append(const QfRows8& rows, int cap, hipStream_t st);
 

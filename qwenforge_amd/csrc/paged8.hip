@@ -202,16 +202,10 @@ __global__ __launch_bounds__(kCopyThreads) void copy_kernel(uint8_t* store, int6
 // Checks and fills what the append and the read share; `blocks`: how many the tokens may
 // touch.
 int make_rows(RowsArgs& a, int64_t& blocks, const QfRows8& h) {
-  if (h.D != kD) return QF_ERR_UNSUPPORTED;
-  if (!h.k || !h.v || !h.cu_seqlens || !h.first || h.B < 1 || h.total < 1 || h.max_seqlen < 1 ||
-      h.max_seqlen > h.total)
-    return QF_ERR_INVALID_ARG;
-  if (((reinterpret_cast<uintptr_t>(h.k) | reinterpret_cast<uintptr_t>(h.v)) & 15u) != 0 ||
-      ((h.k_sl | h.k_sh | h.k_sn | h.v_sl | h.v_sh | h.v_sn) & 7) != 0)
-    return QF_ERR_INVALID_ARG;
-  if (h.B > 0x3fffffff || h.total > 0x3fffffff) return QF_ERR_UNSUPPORTED;
+  int rc = check_rows(h);
+  if (rc != QF_OK) return rc;
   a = RowsArgs{};
-  const int rc = make_pool(h.pool, a.p);
+  rc = make_pool(h.pool, a.p);
   if (rc != QF_OK) return rc;
   a.k = static_cast<f16*>(h.k);
   a.k_sl = h.k_sl; a.k_sh = h.k_sh; a.k_sn = h.k_sn;
@@ -231,15 +225,27 @@ int make_rows(RowsArgs& a, int64_t& blocks, const QfRows8& h) {
 }  // namespace kv8
 }  // namespace qf
 
+int qf::kv8::check_rows(const QfRows8& h) {
+  if (h.D != kD) return QF_ERR_UNSUPPORTED;
+  if (!h.k || !h.v || !h.cu_seqlens || !h.first || h.B < 1 || h.total < 1 || h.max_seqlen < 1 ||
+      h.max_seqlen > h.total)
+    return QF_ERR_INVALID_ARG;
+  if (((reinterpret_cast<uintptr_t>(h.k) | reinterpret_cast<uintptr_t>(h.v)) & 15u) != 0 ||
+      ((h.k_sl | h.k_sh | h.k_sn | h.v_sl | h.v_sh | h.v_sn) & 7) != 0)
+    return QF_ERR_INVALID_ARG;
+  if (h.B > 0x3fffffff || h.total > 0x3fffffff) return QF_ERR_UNSUPPORTED;
+  if ((h.cos == nullptr) != (h.sin == nullptr) ||
+      ((reinterpret_cast<uintptr_t>(h.cos) | reinterpret_cast<uintptr_t>(h.sin)) & 15u) != 0 ||
+      (h.cos != nullptr && (h.cs_sn & 7) != 0))
+    return QF_ERR_INVALID_ARG;
+  return QF_OK;
+}
+
 int qf::kv8::append(const QfRows8& h, int cap, hipStream_t st) {
   RowsArgs a;
   int64_t blocks;
   const int rc = make_rows(a, blocks, h);
   if (rc != QF_OK) return rc;
-  if ((h.cos == nullptr) != (h.sin == nullptr) ||
-      ((reinterpret_cast<uintptr_t>(h.cos) | reinterpret_cast<uintptr_t>(h.sin)) & 15u) != 0 ||
-      (h.cos != nullptr && (h.cs_sn & 7) != 0))
-    return QF_ERR_INVALID_ARG;
   a.cos = static_cast<const f16*>(h.cos);
   a.sin = static_cast<const f16*>(h.sin);
   a.cs_sn = h.cs_sn;

@@ -51,10 +51,12 @@ struct AttnArgs {
   const f16* cos;
   const f16* sin;
   int64_t cs_sn;
-  const f16* kn;                             // decode: the token of slot `last`, appended
-  int64_t kn_sb, kn_sh;
+  // New tokens that the attention itself appends, or null.  Decode: a row's for its slot
+  // `last`.  Extension: the packed ones, where a unit has all of a row's queries.
+  const f16* kn;
+  int64_t kn_st, kn_sh;
   const f16* vn;
-  int64_t vn_sb, vn_sh;
+  int64_t vn_st, vn_sh;
 };
 
 // Slots [k0, k1) of split s of [0, end): cut at multiples of `least` and 64.
@@ -450,6 +452,26 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Unit& u, Sourc
   }
 }
 
+// The unit's row's new tokens into its slots [first, end), a wave a block.  The waves of
+// a workgroup share a first-level cache: past the barrier they see what was written.
+template <bool kE4m3, bool kDecode>
+__device__ __forceinline__ void append_tokens(const AttnArgs& a, const Unit& u, const Source& src, int first,
+                                              int end) {
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+  for (int s0 = (first / kBlock + w) * kBlock; s0 < end; s0 += nw * kBlock) {
+    const int from = max(s0, first);
+    const int64_t token = u.tok0 + from - first;
+    const bool turn = !kDecode && a.cos != nullptr;
+    const Tokens t = {a.kn + token * a.kn_st + u.hk * a.kn_sh, a.kn_st, a.vn + token * a.vn_st + u.hk * a.vn_sh,
+                      a.vn_st, turn ? a.cos + token * a.cs_sn : nullptr, turn ? a.sin + token * a.cs_sn : nullptr,
+                      a.cs_sn};
+    append_block<kE4m3>(a.p, 0, u.hk, src.row[s0 >> a.p.log2p], s0, from - s0, min(end - s0, kBlock), t);
+  }
+  s_waitcnt_vm(0);
+  __threadfence_block();
+  __syncthreads();
+}
+
 template <bool kE4m3>
 __global__ __launch_bounds__(512, 2) void decode_kernel(AttnArgs a) {
   extern __shared__ f32x4 lds[];
@@ -469,17 +491,8 @@ __global__ __launch_bounds__(512, 2) void decode_kernel(AttnArgs a) {
   load_queries<1, true>(s, a, u, 0);
   cut(clampi(last, -1, a.cap - 1) + 1, u.split, a.splits, u.k0, u.k1);
   if (a.kn != nullptr && last >= u.k0 && last < u.k1) {
-    // The unit that sees the new token writes it; its block is in no other unit.  The
-    // waves of a workgroup share a first-level cache, so they see it past the barrier.
-    if (threadIdx.x < 64) {
-      const int slot = (int)last, lo = slot % kBlock;
-      const Tokens t = {a.kn + u.row * a.kn_sb + u.hk * a.kn_sh, 0, a.vn + u.row * a.vn_sb + u.hk * a.vn_sh,
-                        0, nullptr, nullptr, 0};
-      append_block<kE4m3>(a.p, 0, u.hk, src.row[slot >> a.p.log2p], slot - lo, lo, lo + 1, t);
-      s_waitcnt_vm(0);
-    }
-    __threadfence_block();
-    __syncthreads();
+    // The unit that sees the new token writes it; its block is in no other unit.
+    append_tokens<kE4m3, true>(a, u, src, (int)last, (int)last + 1);
   }
   run_unit<kE4m3, 1, true>(a, u, src, s, lds);
 }
@@ -525,6 +538,7 @@ __global__ __launch_bounds__(512, 2) void extend_kernel(AttnArgs a) {
   Source src = make_source(a, u);
   State<kNC> s;
   load_queries<kNC, false>(s, a, u, u.r0);
+  if (a.kn != nullptr && u.ctx >= 0) append_tokens<kE4m3, false>(a, u, src, u.ctx, u.k1);
   run_unit<kE4m3, kNC, false>(a, u, src, s, lds);
 }
 
@@ -721,7 +735,7 @@ int64_t part_bytes(int64_t queries, int n) { return n <= 1 ? 0 : queries * n * (
 
 struct Plan {
   int waves, splits, cols, n_tiles;   // cols: blocks of 16 query rows of a unit
-  bool wide;
+  bool wide, appends;                // appends: the attention writes the new tokens
 };
 
 // Rows of at most 1024 slots whole, by one launch; longer ones in ranges of at least a
@@ -735,14 +749,19 @@ struct Plan {
 // four take 6.1, but 200 rows of 1024 in 17.6 where those take 15.7.
 Plan decode_plan(int B, int KVH, int cap) {
   const int64_t pairs = (int64_t)B * KVH, tiles = ((int64_t)cap + kTile - 1) / kTile;
-  if (tiles <= 16) return {pairs <= kCus / 2 ? 8 : 4, 1, 1, 1, false};
+  if (tiles <= 16) return {pairs <= kCus / 2 ? 8 : 4, 1, 1, 1, false, false};
   const int64_t fill = std::max<int64_t>(2 * kCus / pairs, tiles >= 64 ? 2 : 1);
-  return {4, (int)std::min<int64_t>({(tiles + 3) / 4, fill, kMaxSplits}), 1, 1, false};
+  return {4, (int)std::min<int64_t>({(tiles + 3) / 4, fill, kMaxSplits}), 1, 1, false, false};
 }
 
-// Three forms: a workgroup of 128 query rows whose waves share the tiles (wide), or of
-// 16 cols query rows whose waves take the tiles in turn.  MI355X, 7 queries to each of 2
-// kv heads, us in a replayed graph, int8:
+// A workgroup has 128 query rows and its waves share the tiles (wide), or 16 cols query
+// rows and its waves take the tiles in turn.  MI355X, 7 queries to each of 2 kv heads, us
+// in a replayed graph, int8:
+// - where one unit of up to 32 query rows has all of a short row's queries, it appends the
+//   row's tokens too: 4 rows of 3 tokens behind 1000 slots 12.0, by a launch of its own
+//   13.0 (calls from Python 12.4 and 15.3); 32 of 2 behind 2000 15.3 and 17.8.  48 query
+//   rows take a wave longer than the launch unless the units fill the CUs: 4 of 5 behind
+//   2000 18.8 and 15.9, 64 of 5 behind 1000 16.2 and 18.6;
 // - wide where its units give most CUs two workgroups or more, if need be cut along
 //   slots as long as each piece keeps 90 tiles: 4 rows of 2048 tokens 73, 89 with two
 //   column blocks and 82 with three; 32 of 100 behind 500 slots 30, 36 and 34; 2048
@@ -764,12 +783,18 @@ Plan extend_plan(int B, int KVH, int G, int total, int max_seqlen, int cap) {
   };
   const auto plan = [&](int cols, int64_t splits, bool wide) {
     return Plan{4, (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)), cols,
-                (int)((rows + 16 * cols - 1) / (16 * cols)), wide};
+                (int)((rows + 16 * cols - 1) / (16 * cols)), wide, false};
   };
   const int64_t wide_units = units(128), pieces = std::min<int64_t>(3 * kCus / wide_units, tiles / 90);
   if (rows > 64 && wide_units * std::max<int64_t>(pieces, 1) >= 3 * kCus / 2) return plan(8, pieces, true);
   const int cols = rows <= 16 || (rows <= 64 && tiles <= 64) ? 1
                    : units(48) >= kCus && cap >= 4 * (int64_t)max_seqlen ? 3 : 2;
+  if (tiles <= 32 && (rows <= 32 || (rows <= 48 && (int64_t)B * KVH >= kCus / 2))) {
+    Plan p = plan((int)((rows + 15) / 16), 1, false);
+    p.appends = true;
+    p.waves = 8;
+    return p;
+  }
   const int64_t n = units(16 * cols);
   Plan p = plan(cols, tiles <= 32 ? 1 : std::min<int64_t>(tiles / (n >= 64 ? 32 : 4), 2 * kCus / n), false);
   if (p.splits == 1 && n <= kCus) p.waves = 8;
@@ -858,9 +883,9 @@ int decode_args(AttnArgs& a, const QfDecode8* h) {
       (h->k_new != nullptr && ((h->kn_sb | h->kn_sh | h->vn_sb | h->vn_sh) & 7) != 0))
     return QF_ERR_INVALID_ARG;
   a.kn = static_cast<const f16*>(h->k_new);
-  a.kn_sb = h->kn_sb; a.kn_sh = h->kn_sh;
+  a.kn_st = h->kn_sb; a.kn_sh = h->kn_sh;
   a.vn = static_cast<const f16*>(h->v_new);
-  a.vn_sb = h->vn_sb; a.vn_sh = h->vn_sh;
+  a.vn_st = h->vn_sb; a.vn_sh = h->vn_sh;
   return QF_OK;
 }
 
@@ -947,7 +972,15 @@ extern "C" int qf_prefill_extend_paged8(const QfExtend8* h, void* stream) {
   rc = set_parts(a, h->ws, h->ws_bytes);
   if (rc != QF_OK) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  rc = append(r, a.cap, st);
+  if (p.appends) {
+    rc = check_rows(r);
+    a.kn = static_cast<const f16*>(r.k);
+    a.kn_st = r.k_sn; a.kn_sh = r.k_sh;
+    a.vn = static_cast<const f16*>(r.v);
+    a.vn_st = r.v_sn; a.vn_sh = r.v_sh;
+  } else {
+    rc = append(r, a.cap, st);
+  }
   if (rc != QF_OK) return rc;
   rc = r.pool.code == QF_CODE_E4M3 ? launch_extend<true>(a, p, st) : launch_extend<false>(a, p, st);
   return rc == 0 && a.splits > 1 ? launch_merge<false>(a, st) : rc;

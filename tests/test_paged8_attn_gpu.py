@@ -18,7 +18,7 @@ import torch
 
 from oracle import kv8
 from qwenforge_amd import ops, paged8
-from test_paged8_gpu import make_pools, make_table, row_state
+from test_paged8_gpu import make_pools, make_table, row_state, spread
 
 pytestmark = pytest.mark.gpu
 TOL = 3.1 * 2.0 ** -11
@@ -597,3 +597,48 @@ def test_wild_device_arrays_stay_in_bounds(dev):
     k, v = values_of(work, host[1], 104)
     for i in range(4):
         check(got[5 + i], kv8.attend(q[5 + i].cpu().double().numpy(), k[:101 + i], v[:101 + i]), np.abs(v).max(), i)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("lens,ctx,kvh,g", [
+    ([1, 2, 4, 3], [14, 15, 30, 2000], 2, 7),                       # appended by the attention's own launch
+    ([32, 16, 1, 0, 31], [0, 1, 17, 5, 16], 3, 1),
+    ([2, 1, 2], [100, -1, 63], 1, 16),
+    ([6] * 70, [i * 9 % 400 for i in range(70)], 2, 7),             # 42 query rows, units enough
+    ([33, 2], [40, 100], 2, 1),                                     # one query row more: by a launch of its own
+])
+def test_short_extensions_append_as_the_append_does(dev, lens, ctx, kvh, g, code):
+    """Bit for bit in the pages, rotated keys too; the attention is over them."""
+    gen = torch.Generator().manual_seed(700 + len(lens) + g)
+    need = [max(c, 0) + n for n, c in zip(lens, ctx)]
+    n_pages = sum(-(-n // 64) for n in need) + 2
+    layer = tuple(t[0] for t in make_pools(gen, n_pages, kvh, 64, code, dev))
+    table, host = make_table(gen, need, 64, n_pages, 32, dev)
+    fill_rows(gen, layer, table, ctx, dev)
+    total = sum(lens)
+    qkv = spread(gen, total, (g + 2) * kvh, D).to(dev)
+    q, k, v = qkv[:, :g * kvh], qkv[:, g * kvh:(g + 1) * kvh], qkv[:, (g + 1) * kvh:]
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=dev)
+    ang = torch.rand(total, 32, generator=gen) * 6
+    cos, sin = (torch.cat([f(ang), f(ang)], dim=1).half().to(dev) for f in (torch.cos, torch.sin))
+    context = torch.tensor(ctx, device=dev)
+    for turn in ((None, None), (cos, sin)):
+        a, c = tuple(t.clone() for t in layer), tuple(t.clone() for t in layer)
+        paged8.append_paged8(k, v, cu, max(lens), context, *turn, a, table, lengths=lens)
+        got = paged8.prefill_extend_paged8(q, k, v, cu, max(lens), context, *turn, c, table, lengths=lens)
+        for x, y in zip(a, c):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    for r, (n, c0) in enumerate(zip(lens, ctx)):
+        lo = sum(lens[:r])
+        if c0 < 0:
+            assert not got[lo:lo + n].any()
+        elif n:
+            kk, vv = values_of(c, host[r], c0 + n)
+            state = paged8.prefill_extend_paged8(q, k, v, cu, max(lens), context, None, None,
+                                                 tuple(t.clone() for t in layer), table, lengths=lens)
+            plain = tuple(t.clone() for t in layer)
+            paged8.append_paged8(k, v, cu, max(lens), context, None, None, plain, table, lengths=lens)
+            kk, vv = values_of(plain, host[r], c0 + n)
+            for i in {0, n - 1}:
+                want = kv8.attend(q[lo + i].cpu().double().numpy(), kk[:c0 + i + 1], vv[:c0 + i + 1])
+                check(state[lo + i], want, np.abs(vv).max(), (r, i))
