@@ -8,7 +8,6 @@ namespace qf {
 namespace kv8 {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kD = 64;
 constexpr int kBlock = QF_BLOCK8;
@@ -123,6 +122,16 @@ int check_rows(const QfRows8& rows);
 
 // qf_append_paged8 into the rows' slots below cap (paged8.hip).
 int append(const QfRows8& rows, int cap, hipStream_t st);
+
+// The sum of x over the lanes up to this one.
+__device__ __forceinline__ int scan_sum(int x) {
+  const int lane = threadIdx.x & 63;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
 
 __device__ __forceinline__ int clampi(int64_t x, int lo, int hi) {
   return (int)(x < lo ? lo : x > hi ? hi : x);

@@ -2,10 +2,11 @@
 // single tokens of a batch, and new tokens behind cached ones.
 //
 // softmax(q K^T) V over slots [0, lim) of a row's pages, lim differing by query, is
-// cut into units: up to 16 kNC query rows (token, query head of one kv head) times
-// a range of slots.  The waves of a unit's workgroup take tiles of 64 slots in turn and
-// join their states in LDS; what several ranges of a query leave is joined by
-// merge_kernel.
+// cut into units: query rows (token, query head of one kv head) times a range of slots.
+// With few query rows, 16 kNC of them, the waves of a unit's workgroup take tiles of 64
+// slots in turn and join their states in LDS (decode_kernel, extend_kernel); with many,
+// 128, each wave has 32 of its own and the tiles are shared (extend_wide_kernel).
+// What several ranges of a query leave is joined by merge_kernel.
 //
 // A tile is 8 KB of codes, K and V both loaded straight into matrix-core operands,
 // 16 bytes a lane: with lane group g = lane / 16,
@@ -16,10 +17,16 @@
 //      dim-major pages hold side by side: no transposition anywhere.
 // So all 16 slots whose scores and values a lane has are one block of the cache, and a
 // tile's scales are two floats a lane.  K's scale goes into the factor that the scores
-// have anyway; V's into the conversion of its codes to fp16, which is exact.
+// have anyway; V's into the conversion of its codes to fp16, which is exact (taken into
+// P instead it would round small P below fp16's normal range).
+//
+// New tokens are appended by the attention itself where one workgroup has all that a
+// row and kv head attend with: in decoding the unit that sees the token's slot, in short
+// extensions the row's only one.  A launch less is 1 to 3 us less.
 #include <algorithm>
 
 #include "kv8_block.h"
+#include "kv8_pieces.h"
 #include "lds_tile.h"
 
 namespace qf {
@@ -29,6 +36,12 @@ constexpr int kTile = 64;                    // slots
 constexpr int kMaxSplits = 64;
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// A unit of 128 query rows that pieces have to be joined for: `more` partials behind the
+// first; 0: none.
+struct Join {
+  int more, tok0, rows, r0, hk, pad[3];
+};
 
 struct AttnArgs {
   Pool p;
@@ -40,6 +53,8 @@ struct AttnArgs {
   int B, tokens, G, cap;
   int longest;                               // extension: tokens of a row that get an output
   int n_tiles, splits;                       // query tiles of a row, splits of a row's slots
+  int pieces, shift;                         // even pieces: how many, and the costs' quantum
+  Join* joins;                               // even pieces: one for each
   float* acc;                                // (token, kv head, split, query head, 64)
   float* m;                                  // (token, kv head, split, query head), times m_unit
   float* l;
@@ -59,7 +74,8 @@ struct AttnArgs {
   int64_t vn_st, vn_sh;
 };
 
-// Slots [k0, k1) of split s of [0, end): cut at multiples of `least` and 64.
+// Slots [k0, k1) of split s of n of [0, end): n ranges of whole tiles, the last ones shorter
+// or empty.
 __device__ __forceinline__ void cut(int end, int s, int n, int& k0, int& k1) {
   const int tiles = (end + kTile - 1) / kTile;
   const int len = (tiles + n - 1) / n * kTile;
@@ -214,7 +230,7 @@ __device__ __forceinline__ u32x4 keep_slots(u32x4 w, int have) {
 }
 
 // Online softmax and PV product from a tile's scores; `values` gives operand (t, u) of
-// V^T.  `left`: how many of the lane's 16 slots, from the first on, a column sees.
+// V^T.
 template <int kNC, typename Values>
 __device__ __forceinline__ void attend_tile(State<kNC>& s, f32x4 (&sc)[kNC][4], const Block& blk, int key0,
                                             Values&& values) {
@@ -226,7 +242,7 @@ __device__ __forceinline__ void attend_tile(State<kNC>& s, f32x4 (&sc)[kNC][4], 
   for (int b = 0; b < kNC; ++b) {
     f[b] = blk.ks2;
     if (masked) {
-      const int left = s.lim[b] - key0 - 16 * g;
+      const int left = s.lim[b] - key0 - 16 * g;   // of the lane's 16 slots, what the column sees
       if (left <= 0) f[b] = 1.f;   // whatever scale an unseen block has
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -252,8 +268,8 @@ __device__ __forceinline__ void attend_tile(State<kNC>& s, f32x4 (&sc)[kNC][4], 
   f16x8 p[kNC][2];
 #pragma unroll
   for (int b = 0; b < kNC; ++b) {
-    // p is rounded to fp16 for the matrix cores (2^-12 of it at most, as much as the
-    // output's own rounding), and the sum adds the rounded ones: the weights add to one.
+    // p is rounded to fp16 for the matrix cores (off by 2^-11 of it at most, as the output
+    // is by its own rounding), and the sum adds the rounded ones: the weights add to one.
     const float neg_m = s.m[b] == kNegInf ? 0.f : -s.m[b];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -472,6 +488,10 @@ __device__ __forceinline__ void append_tokens(const AttnArgs& a, const Unit& u, 
   __syncthreads();
 }
 
+// One unit a workgroup: a row's queries of a kv head over a range of its slots.  Long rows
+// are bound by memory (64 rows of some 31400 slots, 516 MB, in 87 us: 5.9 TB/s), short ones
+// by three loads that wait for each other and some 1 us a tile (one row of 1024 slots, 16
+// tiles on 8 waves, 7.0 us).
 template <bool kE4m3>
 __global__ __launch_bounds__(512, 2) void decode_kernel(AttnArgs a) {
   extern __shared__ f32x4 lds[];
@@ -529,7 +549,9 @@ __device__ __forceinline__ bool extend_unit(const AttnArgs& a, Unit& u) {
   return true;
 }
 
-// Few query rows: the waves take the tiles in turn.
+// Few query rows: the waves take the tiles in turn.  Bound by the vector unit and by
+// latency: 16 rows of 9 to 301 tokens behind 2048 slots, in e4m3, issue it 37% of the time
+// with 1.1 waves a SIMD on average (48 us; their products alone 16), as rows end unevenly.
 template <bool kE4m3, int kNC>
 __global__ __launch_bounds__(512, 2) void extend_kernel(AttnArgs a) {
   extern __shared__ f32x4 lds[];
@@ -542,22 +564,118 @@ __global__ __launch_bounds__(512, 2) void extend_kernel(AttnArgs a) {
   run_unit<kE4m3, kNC, false>(a, u, src, s, lds);
 }
 
-// Many query rows: the waves take 32 of them each and share the tiles.  A wave
-// turns a quarter of each tile's codes into operands, in LDS, a tile ahead of their
-// use: a quarter of the conversions that a wave by itself has for as many queries.
-template <bool kE4m3>
-__global__ __launch_bounds__(256, 3) void extend_wide_kernel(AttnArgs a) {
-  constexpr int kWaves = 4, kQB = 2;
-  // [stage][operand: K (i, h), then V (t, u)][lane]
-  __shared__ f16x8 lds[2][16][64];
-  Unit u;
-  if (!extend_unit<16 * kQB * kWaves>(a, u)) return;
-  if (u.k1 <= u.k0) {
-    empty_unit(a, u, 16 * kQB * kWaves);
-    return;
+// ---- many query rows: even pieces of units of 128 (kv8_pieces.h)
+
+// What all lanes have alike, in scalar registers, where the loop over a piece's units is to
+// keep its state.
+__device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+__device__ __forceinline__ RowUnits load_units(const AttnArgs& a, int r) {
+  return row_units(a.cu[r], a.cu[r + 1], a.last[r * a.last_sb], a.G, a.tokens, a.longest, a.cap, a.shift);
+}
+
+__device__ __forceinline__ RowUnits of_lane(const RowUnits& w, int lane) {
+  const auto get = [&](int x) { return __builtin_amdgcn_readlane(x, lane); };
+  return {get(w.tok0), get(w.rows), get(w.ctx), get(w.n), get(w.first), get(w.step)};
+}
+
+// A unit and its part of the line.
+struct Place {
+  RowUnits w;
+  int r, hk, q, seen, x0, x1;
+};
+
+__device__ __forceinline__ void set_place(const AttnArgs& a, Place& u, int x0) {
+  u.x0 = x0;
+  u.x1 = x0 + u.w.first + u.w.step * u.q;
+  u.seen = same(slots_seen(u.w, u.q, a.G, a.cap));
+}
+
+// Finds the piece's part [x, end) of the line and the unit that has x; false: none.
+__device__ __forceinline__ bool find_piece(const AttnArgs& a, int& piece, int& x, int& end, int& len, Place& u) {
+  const int lane = threadIdx.x & 63;
+  // 64 rows at a time; with no more of them all is there after one pass.
+  RowUnits w;
+  int mine, upto;
+  const auto rows_from = [&](int i0) {
+    w = load_units(a, min(i0 + lane, a.B - 1));
+    mine = i0 + lane < a.B ? cost_before(w, w.n) * a.p.kvh : 0;
+    upto = scan_sum(mine);
+    return __builtin_amdgcn_readlane(upto, 63);
+  };
+  int work = rows_from(0);
+  for (int i0 = 64; i0 < a.B; i0 += 64) work += rows_from(i0);
+  len = same(piece_length(work, a.pieces, a.G, a.shift));
+  // Neighbouring pieces share an XCD (workgroups go to the XCDs in turn) and its L2; those
+  // that have work are spread over all XCDs.
+  const int eighth = same((int)((unsigned)((work + len - 1) / len + 7) / 8u)), nth = blockIdx.x / 8;
+  piece = nth < eighth ? blockIdx.x % 8 * eighth + nth : 8 * eighth + blockIdx.x % 8 * (a.pieces / 8 - eighth) + nth - eighth;
+  x = piece * len;
+  end = min(x + len, work);
+  if (x >= work) return false;
+  int before = 0, i0 = 0;
+  if (a.B > 64) rows_from(0);
+  for (;;) {
+    const uint64_t hit = __ballot(x < before + upto);
+    if (hit != 0) {
+      const int j = __builtin_ctzll(hit);
+      int base = before + __builtin_amdgcn_readlane(upto - mine, j);
+      u.r = i0 + j;
+      u.w = of_lane(w, j);
+      const int row = cost_before(u.w, u.w.n);
+      u.hk = same((int)min((unsigned)(x - base) / (unsigned)row, (unsigned)a.p.kvh - 1u));
+      base += u.hk * row;
+      u.q = unit_at(u.w, x - base);
+      set_place(a, u, base + cost_before(u.w, u.q));
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+    i0 += 64;
+    if (i0 >= a.B) return false;
+    rows_from(i0);
   }
+}
+
+// The unit behind u; false: none.
+__device__ __forceinline__ bool next_place(const AttnArgs& a, Place& u) {
+  if (++u.q >= u.w.n) {
+    u.q = 0;
+    if (++u.hk >= a.p.kvh) {
+      u.hk = 0;
+      do {
+        if (++u.r >= a.B) return false;
+        u.w = of_lane(load_units(a, u.r), 0);
+      } while (u.w.n == 0);
+    }
+  }
+  set_place(a, u, u.x1);
+  return true;
+}
+
+// Tiles that a workgroup has done, of about how many, and when its priority changes next.
+struct Progress {
+  int done, tiles, quarter, level;
+};
+
+// The waves take 32 query rows of a unit each and share its tiles.  A wave turns a
+// quarter of each tile's codes into operands, in LDS, a tile ahead of their use: a
+// quarter of the conversions that a wave by itself has for as many queries.  lds:
+// [stage][operand: K (i, h), then V (t, u)][lane].  The result goes to the output, or to
+// partial `part` if that is one.
+//
+// What bounds it: a wave-step (32 query rows x 64 slots) is 36 matrix instructions of 16
+// cycles and some 180 vector ones, 32 of them exponentials; with three waves a SIMD the
+// vector unit issues 56% of the time, the matrix cores run 32% of it, and the clock is
+// lowered (2.0 GHz with int8 codes, 2.4 without load).  2048 tokens behind 16384 slots:
+// 620 to 660 TF/s in int8, 730 in e4m3.
+template <bool kE4m3, bool kEven>
+__device__ __forceinline__ void wide_unit(const AttnArgs& a, const Unit& u, int part, Progress& pr,
+                                          f16x8 (&lds)[2][16][64]) {
+  constexpr int kQB = 2;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  int lane = threadIdx.x & 63;
+  if (kEven) asm volatile("" : "+v"(lane));   // what hangs on it is not kept from one unit to the next
+  const int col = lane & 15, g = lane >> 4;
   Source src = make_source(a, u);
   src.koff += w * 4 * kD;
   src.voff += w * 16 * kTile;
@@ -566,12 +684,19 @@ __global__ __launch_bounds__(256, 3) void extend_wide_kernel(AttnArgs a) {
     u32x4 k, v;
     float ks, vs;
   };
+  // Tiles are loaded in order; a tile's page is fetched, into a scalar register, while the
+  // one before it is loaded.
+  typedef const __attribute__((address_space(4))) int32_t* Table;
+  const auto fetch = [&](int i) {
+    const int lp = min((u.k0 + i * kTile) >> src.log2p, src.ppr - 1);
+    return ((Table)src.row)[lp];
+  };
+  int pid = fetch(0);
   const auto load = [&](Part& r, int i) {
     const bool valid = i < n;
     const int slot0 = u.k0 + i * kTile;
-    const int lp = valid ? slot0 >> src.log2p : src.pwin;
-    if (lp - src.pwin >= 64) load_pids(src, lp);
-    const int64_t page = __builtin_amdgcn_readlane(src.pid, lp - src.pwin);
+    const int64_t page = min(max(pid, 0), src.n_pages - 1);
+    pid = fetch(min(i + 1, n - 1));
     const int in_page = slot0 & ((1 << src.log2p) - 1);
     const int64_t at = page * src.sp + in_page * kD, sat = page * src.ssp + (in_page >> 4);
     r.k = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
@@ -635,26 +760,147 @@ __global__ __launch_bounds__(256, 3) void extend_wide_kernel(AttnArgs a) {
     meet();
   };
   for (int i = 0; i < n; i += 2) {
+    if (kEven && pr.done + i >= pr.quarter) {
+      // Of the three waves of a SIMD the eldest goes first, so the workgroups of a CU would end
+      // one after the other (115 to 195 us where the mean is 155), the last with the CU for
+      // itself: the further a piece is, the lower its priority (121 to 179; 2048 tokens
+      // behind 16384 slots 216 -> 205 us).
+      if (pr.level == 0) __builtin_amdgcn_s_setprio(2);
+      else if (pr.level == 1) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
+      ++pr.level;
+      pr.quarter += pr.tiles / 4 + 1;
+    }
     step(i, r1);
     if (i + 1 < n) step(i + 1, r0);
   }
+  if (kEven) pr.done += n;
 #pragma unroll
   for (int b = 0; b < kQB; ++b) {
     const int rr = first + 16 * b + col;
     if (rr >= u.rows) continue;
-    const int token = u.tok0 + rr / a.G, h = rr % a.G;
     const float l = s.l[b][0];
-    const int64_t p = part_index(a, u, token, h);
+    if (part < 0) {
+      const int token = u.tok0 + rr / a.G, h = rr % a.G;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if (a.splits == 1) store_out(a, token, u.hk, h, 16 * t + 4 * g, s.o[b][t], l, true);
-      else *reinterpret_cast<f32x4*>(a.acc + p * kD + 16 * t + 4 * g) = s.o[b][t];
-    }
-    if (a.splits > 1 && g == 0) {
-      a.m[p] = s.m[b];
-      a.l[p] = l;
+      for (int t = 0; t < 4; ++t) store_out(a, token, u.hk, h, 16 * t + 4 * g, s.o[b][t], l, true);
+    } else {
+      const int64_t p = (int64_t)part * kUnitRows + rr - u.r0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(a.acc + p * kD + 16 * t + 4 * g) = s.o[b][t];
+      if (g == 0) {
+        a.m[p] = s.m[b];
+        a.l[p] = l;
+      }
     }
   }
+}
+
+// A unit to a workgroup.
+template <bool kE4m3>
+__global__ __launch_bounds__(256, 3) void extend_wide_kernel(AttnArgs a) {
+  __shared__ f16x8 lds[2][16][64];
+  Unit u;
+  if (!extend_unit<kUnitRows>(a, u)) return;
+  Progress none;
+  if (u.k1 > u.k0) wide_unit<kE4m3, false>(a, u, -1, none, lds);
+  else empty_unit(a, u, kUnitRows);
+}
+
+// The kernel's arguments, loaded again: nothing of them is kept in registers from one unit
+// to the next.
+__device__ __forceinline__ AttnArgs arguments() {
+  typedef const __attribute__((address_space(4))) AttnArgs* Pointer;
+  Pointer p = (Pointer)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttnArgs*)p;
+}
+
+// A piece to a workgroup.  Piece p leaves at most two partials: 2 p of the unit that it takes up
+// inside, 2 p + 1 of one that it begins and does not end.  Finding the piece takes 2 us.
+template <bool kE4m3>
+__global__ __launch_bounds__(256, 3) void extend_even_kernel(AttnArgs a) {
+  __shared__ f16x8 lds[2][16][64];
+  __shared__ Place held;
+  int piece, x, end, len, k0 = 0;
+  Place at;
+  Join join = {};
+  const bool any = find_piece(a, piece, x, end, len, at);
+  if (any) {
+    const auto cut_at = [&](int y) { return same(cut_slot(y - at.x0, at.seen, a.G, a.shift)); };
+    k0 = cut_at(x);
+    if (k0 > 0 && k0 < at.seen && (x - len < at.x0 || cut_at(x - len) == 0)) {
+      // The unit's first cut.
+      join = {1, at.w.tok0, at.w.rows, at.q * kUnitRows, at.hk};
+      for (int y = x + len; join.more < a.pieces - piece && y < at.x1 && cut_at(y) < at.seen; y += len) ++join.more;
+    }
+  }
+  if (threadIdx.x == 0) a.joins[piece] = join;
+  if (!any) return;
+  Progress progress = {0, len / a.G, len / a.G / 4, 0};
+  __builtin_amdgcn_s_setprio(3);
+  for (;;) {
+    const int k1 = end >= at.x1 ? at.seen : same(cut_slot(end - at.x0, at.seen, a.G, a.shift));
+    const bool more = at.x1 < end;
+    if (threadIdx.x == 0) held = at;
+    {
+      const AttnArgs b = arguments();
+      const Unit u = {at.w.tok0, at.w.rows, at.q * kUnitRows, at.r, at.hk, 0, at.w.ctx, k0, k1};
+      const bool whole = k0 == 0 && k1 == at.seen;
+      if (k1 > k0) wide_unit<kE4m3, true>(b, u, whole ? -1 : 2 * piece + (k0 == 0), progress, lds);
+      else if (at.seen == 0) empty_unit(b, u, kUnitRows);
+    }
+    if (!more) return;
+    __syncthreads();
+    at.w = of_lane(held.w, 0);
+    at.r = same(held.r);
+    at.hk = same(held.hk);
+    at.q = same(held.q);
+    at.x1 = same(held.x1);
+    __syncthreads();
+    if (!next_place(arguments(), at)) return;
+    k0 = 0;
+  }
+}
+
+// Joins the partials of the unit that piece blockIdx.x + 1 cuts first; 16 lanes, 4 dims
+// each, share a query row.  7 us behind 224 units in 768 pieces (the pieces leave the
+// places: finding them here again took 30).
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+  const int piece = blockIdx.x + 1;
+  const Join u = a.joins[piece];
+  const int more = u.more;
+  const int rr = blockIdx.y * 16 + (threadIdx.x >> 4), d0 = 4 * (threadIdx.x & 15), r = u.r0 + rr;
+  if (more == 0 || r >= u.rows) return;
+  constexpr int kEach = 6;
+  float top = kNegInf, sum = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0; j0 <= more; j0 += kEach) {
+    float mv[kEach], lv[kEach], t = top;
+    f32x4 acc[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int j = min(j0 + e, more);
+      const int64_t p = (int64_t)(j == 0 ? 2 * piece - 1 : 2 * (piece + j - 1)) * kUnitRows + rr;
+      mv[e] = a.m[p];
+      lv[e] = a.l[p];
+      acc[e] = *reinterpret_cast<const f32x4*>(a.acc + p * kD + d0);
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) t = fmaxf(t, mv[e]);
+    const float c = top == t ? 1.f : fast_exp2(top - t);
+    sum *= c;
+    o *= c;
+    top = t;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (j0 + e > more) continue;
+      const float f = mv[e] == top ? 1.f : fast_exp2(mv[e] - top);
+      sum += lv[e] * f;
+      o += acc[e] * f;
+    }
+  }
+  store_out(a, u.tok0 + r / a.G, u.hk, r % a.G, d0, o, sum, true);
 }
 
 // Joins the at most kSubs * kEach partials of each (token, kv head, query head).  kSubs
@@ -729,13 +975,19 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------
 // host side
 
-constexpr int kCus = 256;
+constexpr int kCus = 256, kPieces = 3 * kCus;   // as many as run at once
 
-int64_t part_bytes(int64_t queries, int n) { return n <= 1 ? 0 : queries * n * (kD + 2) * 4; }
+// Partials of a plan's call.
+int64_t part_rows(int64_t queries, int splits, int pieces) {
+  return pieces > 0 ? 2 * (int64_t)pieces * kUnitRows : splits <= 1 ? 0 : queries * splits;
+}
+
+int64_t part_bytes(int64_t rows, int pieces) { return rows * (kD + 2) * 4 + pieces * (int64_t)sizeof(Join); }
 
 struct Plan {
-  int waves, splits, cols, n_tiles;   // cols: blocks of 16 query rows of a unit
-  bool wide, appends;                // appends: the attention writes the new tokens
+  int waves, splits, cols, n_tiles;   // cols: blocks of 16 query rows of a unit, 8: wide
+  int pieces, shift;                 // of a wide extension in even pieces, else 0
+  bool appends;                      // the attention writes the new tokens
 };
 
 // Rows of at most 1024 slots whole, by one launch; longer ones in ranges of at least a
@@ -749,24 +1001,28 @@ struct Plan {
 // four take 6.1, but 200 rows of 1024 in 17.6 where those take 15.7.
 Plan decode_plan(int B, int KVH, int cap) {
   const int64_t pairs = (int64_t)B * KVH, tiles = ((int64_t)cap + kTile - 1) / kTile;
-  if (tiles <= 16) return {pairs <= kCus / 2 ? 8 : 4, 1, 1, 1, false, false};
+  if (tiles <= 16) return {pairs <= kCus / 2 ? 8 : 4, 1, 1, 1, 0, 0, false};
   const int64_t fill = std::max<int64_t>(2 * kCus / pairs, tiles >= 64 ? 2 : 1);
-  return {4, (int)std::min<int64_t>({(tiles + 3) / 4, fill, kMaxSplits}), 1, 1, false, false};
+  return {4, (int)std::min<int64_t>({(tiles + 3) / 4, fill, kMaxSplits}), 1, 1, 0, 0, false};
 }
 
-// A workgroup has 128 query rows and its waves share the tiles (wide), or 16 cols query
-// rows and its waves take the tiles in turn.  MI355X, 7 queries to each of 2 kv heads, us
-// in a replayed graph, int8:
+// A workgroup has 128 query rows and its waves share the tiles (wide, cols 8), or 16 cols
+// query rows and its waves take the tiles in turn.  MI355X, 7 queries to each of 2 kv
+// heads, us in a replayed graph, int8:
 // - where one unit of up to 32 query rows has all of a short row's queries, it appends the
 //   row's tokens too: 4 rows of 3 tokens behind 1000 slots 12.0, by a launch of its own
 //   13.0 (calls from Python 12.4 and 15.3); 32 of 2 behind 2000 15.3 and 17.8.  48 query
 //   rows take a wave longer than the launch unless the units fill the CUs: 4 of 5 behind
 //   2000 18.8 and 15.9, 64 of 5 behind 1000 16.2 and 18.6;
-// - wide where its units give most CUs two workgroups or more, if need be cut along
-//   slots as long as each piece keeps 90 tiles: 4 rows of 2048 tokens 73, 89 with two
-//   column blocks and 82 with three; 32 of 100 behind 500 slots 30, 36 and 34; 2048
-//   tokens behind 16384 slots in three pieces 199, 232 and 236; but 2 rows of 1024
-//   behind 8000 in one piece 170, 133 and 129, 16 of 9 to 301 behind 2048 65, 57, 55;
+// - wide, in even pieces of all units (kv8_pieces.h), where those have 48 tiles or more:
+//   2048 tokens behind 16384 slots 205, with each unit in as many equal ranges as fill the
+//   CUs once 214; 1750 tokens 169 and 193, 2400 218 and 289, 1024 behind 65536 343 and 477;
+//   but one row of 512 behind 16000 83 and with two column blocks 73, 8 of 512 behind 4000
+//   129 and with three 121;
+// - wide, a workgroup a unit, where there are units for most CUs and a half: 4 rows of 2048
+//   tokens 71, in even pieces 89, with two column blocks 89 and with three 82; 32 of 100
+//   behind 500 slots 30, 49, 36 and 34; but 2 rows of 1024 behind 8000 170, 133 and 129 with
+//   two and three column blocks, 16 of 9 to 301 behind 2048 65, 57, 55;
 // - three column blocks, for which a wave turns codes into halves once, where there are
 //   units enough and most slots are old ones: 8 rows of 512 behind 4000 slots 110, with
 //   two 120; but 2048 tokens from slot 0 on 40 and 35, one row of 300 behind 2000 25, 21;
@@ -781,22 +1037,28 @@ Plan extend_plan(int B, int KVH, int G, int total, int max_seqlen, int cap) {
   const auto units = [&](int64_t tr) {   // of tr query rows, at most
     return KVH * std::min<int64_t>(B * ((rows + tr - 1) / tr), (int64_t)total * G / tr + B);
   };
-  const auto plan = [&](int cols, int64_t splits, bool wide) {
+  const auto plan = [&](int cols, int64_t splits) {
     return Plan{4, (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)), cols,
-                (int)((rows + 16 * cols - 1) / (16 * cols)), wide, false};
+                (int)((rows + 16 * cols - 1) / (16 * cols)), 0, 0, false};
   };
-  const int64_t wide_units = units(128), pieces = std::min<int64_t>(3 * kCus / wide_units, tiles / 90);
-  if (rows > 64 && wide_units * std::max<int64_t>(pieces, 1) >= 3 * kCus / 2) return plan(8, pieces, true);
+  const int64_t n_units = units(kUnitRows);
+  if (rows > 64 && n_units * tiles >= 48 * kPieces) {
+    Plan p = plan(8, 1);
+    p.pieces = kPieces;
+    while (p.shift < 20 && most_cost(n_units, G, cap, max_seqlen, p.shift) >= 1 << 30) ++p.shift;
+    if (p.shift < 20) return p;
+  }
+  if (rows > 64 && n_units >= 3 * kCus / 2) return plan(8, 1);
   const int cols = rows <= 16 || (rows <= 64 && tiles <= 64) ? 1
                    : units(48) >= kCus && cap >= 4 * (int64_t)max_seqlen ? 3 : 2;
   if (tiles <= 32 && (rows <= 32 || (rows <= 48 && (int64_t)B * KVH >= kCus / 2))) {
-    Plan p = plan((int)((rows + 15) / 16), 1, false);
+    Plan p = plan((int)((rows + 15) / 16), 1);
     p.appends = true;
     p.waves = 8;
     return p;
   }
   const int64_t n = units(16 * cols);
-  Plan p = plan(cols, tiles <= 32 ? 1 : std::min<int64_t>(tiles / (n >= 64 ? 32 : 4), 2 * kCus / n), false);
+  Plan p = plan(cols, tiles <= 32 ? 1 : std::min<int64_t>(tiles / (n >= 64 ? 32 : 4), 2 * kCus / n));
   if (p.splits == 1 && n <= kCus) p.waves = 8;
   return p;
 }
@@ -824,10 +1086,17 @@ int launch_decode(const AttnArgs& a, int code, int waves, hipStream_t st) {
 
 template <bool kE4m3>
 int launch_extend(const AttnArgs& a, const Plan& p, hipStream_t st) {
+  if (p.pieces > 0) {
+    hipLaunchKernelGGL(extend_even_kernel<kE4m3>, dim3(p.pieces), dim3(256), 0, st, a);
+    const int rc = (int)hipGetLastError();
+    if (rc != 0) return rc;
+    hipLaunchKernelGGL(join_kernel, dim3(p.pieces - 1, kUnitRows / 16), dim3(256), 0, st, a);
+    return (int)hipGetLastError();
+  }
   const int64_t grid = (((int64_t)a.B * a.p.kvh * a.splits + 7) & ~(int64_t)7) * a.n_tiles;
   if (grid > 0x7fffffff) return QF_ERR_UNSUPPORTED;
   const dim3 g((unsigned)grid), b(64 * p.waves);
-  if (p.wide) hipLaunchKernelGGL(extend_wide_kernel<kE4m3>, g, b, 0, st, a);
+  if (p.cols == 8) hipLaunchKernelGGL(extend_wide_kernel<kE4m3>, g, b, 0, st, a);
   else if (p.cols == 1) hipLaunchKernelGGL((extend_kernel<kE4m3, 1>), g, b, lds_bytes(p.waves), st, a);
   else if (p.cols == 3) hipLaunchKernelGGL((extend_kernel<kE4m3, 3>), g, b, lds_bytes(p.waves), st, a);
   else hipLaunchKernelGGL((extend_kernel<kE4m3, 2>), g, b, lds_bytes(p.waves), st, a);
@@ -861,14 +1130,18 @@ bool bad_out(const void* out, int64_t st, int64_t sh, int64_t sg) {
   return !out || (reinterpret_cast<uintptr_t>(out) & 7u) != 0 || ((st | sh | sg) & 3) != 0;
 }
 
-int set_parts(AttnArgs& a, void* ws, int64_t ws_bytes) {
-  if (a.splits <= 1) return QF_OK;
-  const int64_t queries = (int64_t)a.tokens * a.p.kvh * a.G;
+int set_parts(AttnArgs& a, const Plan& p, void* ws, int64_t ws_bytes) {
+  a.splits = p.splits;
+  a.pieces = p.pieces;
+  a.shift = p.shift;
+  const int64_t rows = part_rows((int64_t)a.tokens * a.p.kvh * a.G, p.splits, p.pieces);
+  if (rows == 0) return QF_OK;
   if (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u) != 0) return QF_ERR_INVALID_ARG;
-  if (ws_bytes < part_bytes(queries, a.splits)) return QF_ERR_SCRATCH_LIMIT;
+  if (ws_bytes < part_bytes(rows, p.pieces)) return QF_ERR_SCRATCH_LIMIT;
   a.acc = static_cast<float*>(ws);
-  a.m = a.acc + queries * a.splits * kD;
-  a.l = a.m + queries * a.splits;
+  a.m = a.acc + rows * kD;
+  a.l = a.m + rows;
+  a.joins = reinterpret_cast<Join*>(a.l + rows);
   return QF_OK;
 }
 
@@ -896,7 +1169,7 @@ extern "C" int64_t qf_decode_attn_paged8_workspace(int B, int KVH, int G, int ca
   using namespace qf::kv8;
   if (B < 1 || KVH < 1 || cap < 1) return QF_ERR_INVALID_ARG;
   if (G < 1 || G > 16 || (int64_t)B * KVH * G > 0x7fffffff) return QF_ERR_UNSUPPORTED;
-  return part_bytes((int64_t)B * KVH * G, decode_plan(B, KVH, cap).splits);
+  return part_bytes(part_rows((int64_t)B * KVH * G, decode_plan(B, KVH, cap).splits, 0), 0);
 }
 
 extern "C" int qf_decode_attn_paged8(const QfDecode8* h, void* stream) {
@@ -909,8 +1182,7 @@ extern "C" int qf_decode_attn_paged8(const QfDecode8* h, void* stream) {
   a.out = static_cast<f16*>(h->out);
   a.o_st = h->o_sb; a.o_sh = h->o_sh; a.o_sg = h->o_sg;
   const Plan p = decode_plan(a.B, a.p.kvh, a.cap);
-  a.splits = p.splits;
-  rc = set_parts(a, h->ws, h->ws_bytes);
+  rc = set_parts(a, p, h->ws, h->ws_bytes);
   if (rc != QF_OK) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   rc = launch_decode(a, (int)h->pool.code, p.waves, st);
@@ -941,7 +1213,8 @@ extern "C" int64_t qf_prefill_extend_paged8_workspace(int B, int QH, int KVH, in
   if (B < 1 || KVH < 1 || QH < KVH || QH % KVH != 0 || total < 1 || max_seqlen < 1 || cap < 1)
     return QF_ERR_INVALID_ARG;
   if (QH / KVH > 16 || (int64_t)total * QH > 0x7fffffff || B > 0x3fffffff) return QF_ERR_UNSUPPORTED;
-  return part_bytes((int64_t)total * QH, extend_plan(B, KVH, QH / KVH, total, max_seqlen, cap).splits);
+  const Plan p = extend_plan(B, KVH, QH / KVH, total, max_seqlen, cap);
+  return part_bytes(part_rows((int64_t)total * QH, p.splits, p.pieces), p.pieces);
 }
 
 extern "C" int qf_prefill_extend_paged8(const QfExtend8* h, void* stream) {
@@ -966,10 +1239,9 @@ extern "C" int qf_prefill_extend_paged8(const QfExtend8* h, void* stream) {
   a.sin = static_cast<const f16*>(r.sin);
   a.cs_sn = r.cs_sn;
   const Plan p = extend_plan(a.B, a.p.kvh, a.G, a.tokens, (int)r.max_seqlen, a.cap);
-  a.splits = p.splits;
   a.n_tiles = p.n_tiles;
   a.longest = (int)r.max_seqlen;
-  rc = set_parts(a, h->ws, h->ws_bytes);
+  rc = set_parts(a, p, h->ws, h->ws_bytes);
   if (rc != QF_OK) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p.appends) {

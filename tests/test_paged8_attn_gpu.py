@@ -642,3 +642,127 @@ def test_short_extensions_append_as_the_append_does(dev, lens, ctx, kvh, g, code
             for i in {0, n - 1}:
                 want = kv8.attend(q[lo + i].cpu().double().numpy(), kk[:c0 + i + 1], vv[:c0 + i + 1])
                 check(state[lo + i], want, np.abs(vv).max(), (r, i))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("lens,ctx,kvh", [
+    ([150, 400, 0, 333], [64, 5, 7, 90], 8),                        # shared tiles
+    ([600], [9000], 8),                                             # the same, in pieces that are joined
+    ([20, 9], [2500, 2100], 2),                                     # the waves' own tiles, in pieces
+])
+def test_captured_chunks_replay(dev, lens, ctx, kvh, code):
+    """A captured extension's replays, on a stream of its own, are the eager calls' on another, both running."""
+    gen = torch.Generator().manual_seed(800 + kvh + len(lens))
+    rounds = 3
+    need = [c + rounds * n for n, c in zip(lens, ctx)]
+    n_pages = sum(-(-n // 64) for n in need) + 1
+    layer = tuple(t[0] for t in make_pools(gen, n_pages, kvh, 64, code, dev))
+    table, host = make_table(gen, need, 64, n_pages, -(-max(need) // 64), dev)
+    fill_rows(gen, layer, table, ctx, dev)
+    mirror = tuple(t.clone() for t in layer)
+    total = sum(lens)
+    qkv = torch.zeros(total, 9 * kvh, D, device=dev, dtype=torch.float16)
+    at = torch.tensor(ctx, device=dev)
+    step = torch.tensor(lens, device=dev)
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=dev)
+
+    def chunk(x, pools, at):
+        return paged8.prefill_extend_paged8(x[:, :7 * kvh], x[:, 7 * kvh:8 * kvh], x[:, 8 * kvh:], cu, max(lens), at, None,
+                                            None, pools, table, lengths=lens, max_slots=max(need))
+
+    chunk(qkv, tuple(t.clone() for t in layer), at)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chunk(qkv, layer, at)
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    for i in range(rounds):
+        x = torch.randn(qkv.shape, generator=gen).half().to(dev)
+        qkv.copy_(x)
+        here = at.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[0]):
+            graph.replay()
+        with torch.cuda.stream(streams[1]):
+            want = chunk(x, mirror, here)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        for a, c in zip(layer, mirror):
+            assert torch.equal(a.view(torch.uint8), c.view(torch.uint8)), i
+        at += step
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("lens,ctx,kvh,g,cap", [
+    ([300, 0, 250, 128], [6000, 3, 1000, 9000], 8, 7, None),
+    ([300, 40, 250, 128], [6000, -1, 1000, 9000], 8, 7, None),      # a parked row inside the line
+    ([6] * 70, [i * 9 % 400 for i in range(70)], 2, 16, 65536),     # more rows than lanes, little work for each
+    ([300, 280], [700, 900], 8, 16, 1 << 23),                       # costs in coarser quanta
+    ([1500], [7000], 2, 7, 1 << 15),
+])
+def test_extension_in_even_pieces(dev, lens, ctx, kvh, g, cap, code):
+    """Pieces that begin and end inside units, that hold several, and none; as the definition, and as the rows one
+    by one."""
+    gen = torch.Generator().manual_seed(900 + len(lens) + kvh)
+    page = 4096 if cap and cap > 1 << 20 else 128
+    need = [max(c, 0) + n for n, c in zip(lens, ctx)]
+    n_pages = sum(-(-n // page) for n in need) + 1
+    layer = tuple(t[0] for t in make_pools(gen, n_pages, kvh, page, code, dev))
+    ppr = -(-(cap or max(need)) // page)
+    table, host = make_table(gen, need, page, n_pages, ppr, dev)
+    fill_rows(gen, layer, table, ctx, dev)
+    total = sum(lens)
+    qkv = torch.randn(total, (g + 2) * kvh, D, generator=gen).half().to(dev)
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=dev)
+    q, k, v = qkv[:, :g * kvh], qkv[:, g * kvh:(g + 1) * kvh], qkv[:, (g + 1) * kvh:]
+    got = paged8.prefill_extend_paged8(q, k, v, cu, max(lens), torch.tensor(ctx, device=dev), None, None, layer, table,
+                                       lengths=lens, max_slots=cap or max(need))
+    assert torch.isfinite(got).all()
+    for r in range(0, len(lens), max(1, len(lens) // 8)):
+        n, c, lo = lens[r], ctx[r], sum(lens[:r])
+        if n == 0 or c < 0:
+            assert not got[lo:lo + n].any()
+            continue
+        kk, vv = values_of(layer, host[r], c + n)
+        edges = {0, 1, n - 1, n // 2} | {128 // g * j + e for j in range(1, 5) for e in (-1, 0, 1)}
+        for i in sorted(e for e in edges if 0 <= e < n):
+            check(got[lo + i], kv8.attend(qkv[lo + i, :g * kvh].cpu().double().numpy(), kk[:c + i + 1], vv[:c + i + 1]),
+                  np.abs(vv).max(), (r, i))
+        # Every token: the row by itself, whose units are cut elsewhere or not at all.
+        alone = paged8.prefill_extend_paged8(q[lo:lo + n], k[lo:lo + n], v[lo:lo + n],
+                                             torch.tensor([0, n], dtype=torch.int32, device=dev), n,
+                                             torch.tensor([c], device=dev), None, None,
+                                             tuple(t.clone() for t in layer), table[r:r + 1], max_slots=c + n)
+        check(got[lo:lo + n], alone.cpu().double().numpy(), np.abs(vv).max(), r)
+
+
+def test_wild_device_arrays_in_long_extensions(dev):
+    """As for short ones: workgroups that find their work from such arrays come back, and touch nothing outside."""
+    gen = torch.Generator().manual_seed(101)
+    kvh, g, total = 8, 7, 600
+    layer = tuple(t[0] for t in make_pools(gen, 90, kvh, 64, "int8", dev))
+    table, host = make_table(gen, [2000, 1500, 700], 64, 90, 60, dev)
+    fill_rows(gen, layer, table, [1800, 1200, 500], dev)
+    x = torch.randn(total, (g + 2) * kvh, D, generator=gen).half().to(dev)
+    q, k, v = x[:, :g * kvh], x[:, g * kvh:(g + 1) * kvh], x[:, (g + 1) * kvh:]
+    for rows, most in ((3, 1024), (3, None), (2, None)):
+        lengths = [total // rows] * rows
+        for cu in ([0, 200, 400, 600], [0, 600, 0, 600], [500, 3, 20, -7], [-4, 100, 2 ** 31 - 1, 5],
+                   [2 ** 31 - 1, -2 ** 31, 5, 600]):
+            cu = torch.tensor(cu[:rows + 1], dtype=torch.int32, device=dev)
+            for a in (2 ** 63 - 1, 2 ** 40 + 5, 2 ** 31, 10 ** 6, -2 ** 63, 100):
+                ctx = torch.tensor([a, 100, a][:rows], device=dev)
+                for wild in (table, torch.full_like(table, 2 ** 31 - 1)):
+                    out = paged8.prefill_extend_paged8(q, k, v, cu, lengths[0], ctx, None, None,
+                                                       tuple(t.clone() for t in layer), wild[:rows], lengths=lengths,
+                                                       max_slots=most)
+                    torch.cuda.synchronize()
+                    assert out.shape == q.shape
+    cu = torch.tensor([0, 200, 400, 600], dtype=torch.int32, device=dev)
+    ctx = torch.tensor([2 ** 40, 1200, -5], device=dev)
+    got = paged8.prefill_extend_paged8(q, k, v, cu, 200, ctx, None, None, layer, table, lengths=[200] * 3)
+    kk, vv = values_of(layer, host[1], 1400)
+    for i in (0, 1, 17, 18, 100, 198, 199):
+        check(got[200 + i], kv8.attend(q[200 + i].cpu().double().numpy(), kk[:1201 + i], vv[:1201 + i]),
+              np.abs(vv).max(), i)
+    assert not got[400:].any()
