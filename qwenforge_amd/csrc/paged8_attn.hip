@@ -53,6 +53,7 @@ struct AttnArgs {
   int B, tokens, G, cap;
   int longest;                               // extension: tokens of a row that get an output
   int n_tiles, splits;                       // query tiles of a row, splits of a row's slots
+  int share;                                 // query tiles that read the same slots share an XCD
   int pieces, shift;                         // even pieces: how many, and the costs' quantum
   Join* joins;                               // even pieces: one for each
   float* acc;                                // (token, kv head, split, query head, 64)
@@ -520,11 +521,11 @@ __global__ __launch_bounds__(512, 2) void decode_kernel(AttnArgs a) {
 // The extension's unit of this workgroup, of kRows query rows; false: none.
 template <int kRows>
 __device__ __forceinline__ bool extend_unit(const AttnArgs& a, Unit& u) {
-  // Query tiles that read the same slots share an XCD (workgroups go to the XCDs in
-  // turn) and its L2, where there are XCDs enough.
+  // Workgroups go to the XCDs in turn: neighbouring tiles to all of them, or with `share` the
+  // tiles that read the same slots to one, and its L2.
   const int groups = a.B * a.p.kvh * a.splits;
   int id = blockIdx.x;
-  if (groups >= 8) id = (id / (8 * a.n_tiles) * 8 + id % 8) * a.n_tiles + id / 8 % a.n_tiles;
+  if (a.share) id = (id / (8 * a.n_tiles) * 8 + id % 8) * a.n_tiles + id / 8 % a.n_tiles;
   const int tile = id % a.n_tiles;
   id /= a.n_tiles;
   if (id >= groups) return false;
@@ -1063,6 +1064,15 @@ Plan extend_plan(int B, int KVH, int G, int total, int max_seqlen, int cap) {
   return p;
 }
 
+// Whether the query tiles of a row, kv head and split go to one XCD: where those are eight or
+// more and must be of like size, as rows are one or have about as many new tokens and no
+// more old ones.  MI355X, us in a replayed graph: 4 rows of 2048 tokens 72, spread 78; 16
+// of 301 behind 2048 slots 80 and 83; but 5 rows of 9 to 301 behind 16000 slots 140 and 98.
+bool share_xcd(const AttnArgs& a, int splits, int max_seqlen) {
+  return (int64_t)a.B * a.p.kvh * splits >= 8 &&
+         (a.B == 1 || ((int64_t)a.tokens * 4 >= (int64_t)a.B * max_seqlen * 3 && a.cap <= 2 * (int64_t)max_seqlen));
+}
+
 size_t lds_bytes(int waves) { return waves * (256 * sizeof(f32x4) + 16 * sizeof(float2)); }
 
 template <bool kDecode>
@@ -1240,6 +1250,7 @@ extern "C" int qf_prefill_extend_paged8(const QfExtend8* h, void* stream) {
   a.cs_sn = r.cs_sn;
   const Plan p = extend_plan(a.B, a.p.kvh, a.G, a.tokens, (int)r.max_seqlen, a.cap);
   a.n_tiles = p.n_tiles;
+  a.share = share_xcd(a, p.splits, (int)r.max_seqlen);
   a.longest = (int)r.max_seqlen;
   rc = set_parts(a, p, h->ws, h->ws_bytes);
   if (rc != QF_OK) return rc;
