@@ -33,6 +33,9 @@ make the restatement trustworthy live in ``tests/test_oracle_*.py``:
 * ``pages_to_dense`` / ``dense_to_pages`` / ``paged_location``: the identity
   block table reduces to a reshape of the dense cache (closed form), and the
   two are inverse on random tables.
+* ``kv8`` (caches held in 8 bits; the reference has none): e4m3's levels and the
+  nearest of them against torch's casts, the least scale by trying them all, values
+  within fp16, the error of one write.
 
 No function is "parity unpinned".
 """
