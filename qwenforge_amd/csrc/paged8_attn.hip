@@ -1015,11 +1015,12 @@ Plan decode_plan(int B, int KVH, int cap) {
 //   13.0 (calls from Python 12.4 and 15.3); 32 of 2 behind 2000 15.3 and 17.8.  48 query
 //   rows take a wave longer than the launch unless the units fill the CUs: 4 of 5 behind
 //   2000 18.8 and 15.9, 64 of 5 behind 1000 16.2 and 18.6;
-// - wide, in even pieces of all units (kv8_pieces.h), where those have 48 tiles or more:
-//   2048 tokens behind 16384 slots 205, with each unit in as many equal ranges as fill the
-//   CUs once 214; 1750 tokens 169 and 193, 2400 218 and 289, 1024 behind 65536 343 and 477;
-//   but one row of 512 behind 16000 83 and with two column blocks 73, 8 of 512 behind 4000
-//   129 and with three 121;
+// - wide, in even pieces of all units (kv8_pieces.h), where those have 48 tiles or more, or
+//   24 of rows of 120: 2048 tokens behind 16384 slots 205, with each unit in as many equal
+//   ranges as fill the CUs once 214; 1750 tokens 169 and 193, 2400 218 and 289, 1024 behind
+//   65536 343 and 477; with two column blocks one row of 700 behind 16000 91 and 113, of
+//   1024 114 and 150; but of 512 behind 16000 83 and 73, 8 of 512 behind 4000 129 and with
+//   three 124, 4 of 400 71 and 53;
 // - wide, a workgroup a unit, where there are units for most CUs and a half: 4 rows of 2048
 //   tokens 71, in even pieces 89, with two column blocks 89 and with three 82; 32 of 100
 //   behind 500 slots 30, 49, 36 and 34; but 2 rows of 1024 behind 8000 170, 133 and 129 with
@@ -1043,7 +1044,7 @@ Plan extend_plan(int B, int KVH, int G, int total, int max_seqlen, int cap) {
                 (int)((rows + 16 * cols - 1) / (16 * cols)), 0, 0, false};
   };
   const int64_t n_units = units(kUnitRows);
-  if (rows > 64 && n_units * tiles >= 48 * kPieces) {
+  if (rows > 64 && n_units * tiles >= (tiles >= 120 ? 24 : 48) * kPieces) {
     Plan p = plan(8, 1);
     p.pieces = kPieces;
     while (p.shift < 20 && most_cost(n_units, G, cap, max_seqlen, p.shift) >= 1 << 30) ++p.shift;
