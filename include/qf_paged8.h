@@ -114,7 +114,7 @@ int qf_read_paged8(const QfRows8* rows, void* stream);
 int qf_copy_pages8(void* store, int layers, int64_t layer_step, int64_t step, int64_t bytes,
                    const int32_t* src, const int32_t* dst, int n_pairs, int n_pages, void* stream);
 
-/* Queries of single tokens: q and out (B, KVH, G, D), one layer's pool. */
+/* Queries of single tokens: q and out (B, KVH, G, D), G at most 16, one layer's pool. */
 typedef struct {
   QfPool8 pool;
   const void* q;
@@ -160,7 +160,8 @@ int qf_decode_attn_paged8(const QfDecode8* args, void* stream);
 int qf_decode_split_paged8(const QfDecode8* args, float* acc, float* m, float* l, int splits,
                            void* stream);
 
-/* New tokens with their queries: q and out (T, QH, D), QH a multiple of the pool's KVH. */
+/* New tokens with their queries: q and out (T, QH, D), QH a multiple of the pool's KVH, at
+ * most 16 times it. */
 typedef struct {
   QfRows8 rows;              /* k and v appended at first[b] + i, one layer */
   const void* q;

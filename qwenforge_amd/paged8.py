@@ -438,7 +438,8 @@ def prefill_extend_paged8(query: torch.Tensor, key: torch.Tensor, value: torch.T
 
     ``append_paged8`` of key and value, then token i of row b, packed query (T, QH,
     64), attends to slots [0, context[b] + i] as the pages hold them, its own and the
-    call's other tokens among them.  ``cos``/``sin`` rotate query and key.
+    call's other tokens among them.  QH is at most 16 times key's heads.
+    ``cos``/``sin`` rotate query and key.
     ``max_slots`` bounds every row's context + tokens (default: the table's): the work
     is split by it, and slots past it are neither written nor read.  A parked row
     (negative context) gets zeros.  Returns (T, QH, 64).
