@@ -122,95 +122,123 @@ struct Tokens {
   int64_t cs_sn;
 };
 
-// One wave quantises tokens into slots [lo, end) of the block of 16 whose first slot is
-// slot0 of the row, in `page` of the layer; without such a page nothing is written.
-template <bool kE4m3>
+// Where the block of 16 whose first slot is slot0 of a row begins in `page` of the layer.
+struct BlockAt {
+  int64_t code, scale;
+  int in_page;
+};
+
+__device__ __forceinline__ BlockAt block_at(const Pool& p, int layer, int hk, int page, int slot0) {
+  const int in_page = slot0 & ((1 << p.log2p) - 1);
+  return {layer * p.sl + page * p.sp + hk * p.sh, layer * p.ssl + page * p.ssp + hk * p.ssh + (in_page >> 4),
+          in_page};
+}
+
+// One wave quantises tokens into slots [lo, end) of that block, their keys, their values or
+// both; without such a page nothing is written.  All is loaded before any of it is used.
+template <bool kE4m3, bool kKeys, bool kValues>
 __device__ __forceinline__ void append_block(const Pool& p, int layer, int hk, int page, int slot0, int lo,
                                              int end, const Tokens& tokens) {
   const int lane = threadIdx.x & 63;
   const bool begun = lo > 0;
-  // K: slot t, dims 8c and 32 + 8c.
+  // K: slot t, dims c and 32 + c.
   const int t = lane >> 2, c = 8 * (lane & 3);
   const bool fresh = t >= lo && t < end;
   const int64_t tok = fresh ? t - lo : 0;
-  const f16* src = tokens.k + tok * tokens.k_sn + c;
-  f16x8 klo = load16(src), khi = load16(src + 32);
+  f16x8 klo, khi;
+  if (kKeys) {
+    const f16* src = tokens.k + tok * tokens.k_sn + c;
+    klo = load16(src);
+    khi = load16(src + 32);
+  }
   // V: dims 2d and 2d + 1, slots j0 .. j0 + 7.
   const int d = lane & 31, j0 = lane >> 5 << 3;
-  const f16* vsrc = tokens.v + 2 * d;
   unsigned x[8];
+  if (kValues) {
+    const f16* src = tokens.v + 2 * d;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const bool in = j0 + j >= lo && j0 + j < end;
-    x[j] = 0;
-    if (in) x[j] = *reinterpret_cast<const unsigned*>(vsrc + (j0 + j - lo) * tokens.v_sn);
+    for (int j = 0; j < 8; ++j) {
+      const bool in = j0 + j >= lo && j0 + j < end;
+      x[j] = 0;
+      if (in) x[j] = *reinterpret_cast<const unsigned*>(src + (j0 + j - lo) * tokens.v_sn);
+    }
   }
   if (page < 0 || page >= p.n_pages) return;
-  const int in_page = slot0 & ((1 << p.log2p) - 1);
-  const int64_t at = layer * p.sl + page * p.sp + hk * p.sh;
-  const int64_t sat = layer * p.ssl + page * p.ssp + hk * p.ssh + (in_page >> 4);
-  uint8_t* kp = p.k + at + (int64_t)in_page * kD;     // 16 slots x 64
-  uint8_t* vp = p.v + at + (int64_t)(in_page >> 6) * 64 * kD + (in_page & 63) + 128 * d + j0;
-  const float ks_old = p.ks[sat], vs_old = p.vs[sat];
+  const BlockAt at = block_at(p, layer, hk, page, slot0);
+  uint8_t* kp = p.k + at.code + (int64_t)at.in_page * kD + t * kD + c;     // 16 slots x 64
+  uint8_t* vp = p.v + at.code + (int64_t)(at.in_page >> 6) * 64 * kD + (at.in_page & 63) + 128 * d + j0;
+  float ks_old, vs_old;
   u32x2 old_lo = {0, 0}, old_hi = {0, 0}, old_v[2] = {{0, 0}, {0, 0}};
+  if (kKeys) ks_old = p.ks[at.scale];
+  if (kValues) vs_old = p.vs[at.scale];
   if (begun || end < kBlock) {
-    old_lo = *reinterpret_cast<const u32x2*>(kp + t * kD + c);
-    old_hi = *reinterpret_cast<const u32x2*>(kp + t * kD + c + 32);
-    old_v[0] = *reinterpret_cast<const u32x2*>(vp);
-    old_v[1] = *reinterpret_cast<const u32x2*>(vp + 64);
+    if (kKeys) {
+      old_lo = *reinterpret_cast<const u32x2*>(kp);
+      old_hi = *reinterpret_cast<const u32x2*>(kp + 32);
+    }
+    if (kValues) {
+      old_v[0] = *reinterpret_cast<const u32x2*>(vp);
+      old_v[1] = *reinterpret_cast<const u32x2*>(vp + 64);
+    }
   }
-  if (tokens.cos != nullptr) {
-    const int64_t co = tok * tokens.cs_sn + c;
-    rope_pair(klo, khi, load16(tokens.cos + co), load16(tokens.sin + co), load16(tokens.cos + co + 32),
-              load16(tokens.sin + co + 32));
+  Scales ks, vs;
+  if (kKeys) {
+    if (tokens.cos != nullptr) {
+      const int64_t co = tok * tokens.cs_sn + c;
+      rope_pair(klo, khi, load16(tokens.cos + co), load16(tokens.sin + co), load16(tokens.cos + co + 32),
+                load16(tokens.sin + co + 32));
+    }
+    ks = new_scale<kE4m3>(wave_max(fresh ? max(magnitudes(klo), magnitudes(khi)) : 0u), ks_old, begun);
   }
-  const Scales k = new_scale<kE4m3>(
-      wave_max(fresh ? max(magnitudes(klo), magnitudes(khi)) : 0u), ks_old, begun);
-  unsigned vtop = 0;
+  if (kValues) {
+    unsigned top = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) vtop = max(vtop, max(x[j] & 0x7FFFu, (x[j] >> 16) & 0x7FFFu));
-  const Scales v = new_scale<kE4m3>(wave_max(vtop), vs_old, begun);
-
-  if (fresh || (t < lo && k.ratio != 1.f)) {
-    u32x2 out_lo, out_hi;
-    if (fresh) {
+    for (int j = 0; j < 8; ++j) top = max(top, max(x[j] & 0x7FFFu, (x[j] >> 16) & 0x7FFFu));
+    vs = new_scale<kE4m3>(wave_max(top), vs_old, begun);
+  }
+  if (kKeys) {
+    const Scales s = ks;
+    if (fresh || (t < lo && s.ratio != 1.f)) {
+      u32x2 lo8, hi8;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        out_lo[i] = k.bad ? 0u : encode4<kE4m3>(klo[4 * i], klo[4 * i + 1], klo[4 * i + 2], klo[4 * i + 3], k.inv, k.top);
-        out_hi[i] = k.bad ? 0u : encode4<kE4m3>(khi[4 * i], khi[4 * i + 1], khi[4 * i + 2], khi[4 * i + 3], k.inv, k.top);
+        if (fresh) {
+          lo8[i] = s.bad ? 0u : encode4<kE4m3>(klo[4 * i], klo[4 * i + 1], klo[4 * i + 2], klo[4 * i + 3], s.inv, s.top);
+          hi8[i] = s.bad ? 0u : encode4<kE4m3>(khi[4 * i], khi[4 * i + 1], khi[4 * i + 2], khi[4 * i + 3], s.inv, s.top);
+        } else {
+          lo8[i] = recode4<kE4m3>(old_lo[i], s.ratio, s.top);
+          hi8[i] = recode4<kE4m3>(old_hi[i], s.ratio, s.top);
+        }
       }
-    } else {
+      *reinterpret_cast<u32x2*>(kp) = lo8;
+      *reinterpret_cast<u32x2*>(kp + 32) = hi8;
+    }
+  }
+  if (kValues) {
+    const Scales s = vs;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x2 out;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        out_lo[i] = recode4<kE4m3>(old_lo[i], k.ratio, k.top);
-        out_hi[i] = recode4<kE4m3>(old_hi[i], k.ratio, k.top);
+        f16 y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = __builtin_bit_cast(f16, (unsigned short)(x[4 * i + j] >> (16 * h)));
+        const unsigned w = s.bad ? 0u : encode4<kE4m3>(y[0], y[1], y[2], y[3], s.inv, s.top);
+        // Bytes of slots that are new, and of those before them.
+        const int n0 = min(max(lo - j0 - 4 * i, 0), 4), n1 = min(max(end - j0 - 4 * i, 0), 4);
+        const unsigned below = n0 == 4 ? ~0u : (1u << (8 * n0)) - 1u;
+        const unsigned upto = n1 == 4 ? ~0u : (1u << (8 * n1)) - 1u;
+        const unsigned old = old_v[h][i];
+        const unsigned had = s.ratio != 1.f ? recode4<kE4m3>(old, s.ratio, s.top) : old;
+        out[i] = (w & upto & ~below) | (had & below) | (old & ~upto);
       }
+      *reinterpret_cast<u32x2*>(vp + 64 * h) = out;
     }
-    *reinterpret_cast<u32x2*>(kp + t * kD + c) = out_lo;
-    *reinterpret_cast<u32x2*>(kp + t * kD + c + 32) = out_hi;
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    u32x2 out;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      f16 y[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = __builtin_bit_cast(f16, (unsigned short)(x[4 * i + j] >> (16 * h)));
-      const unsigned w = v.bad ? 0u : encode4<kE4m3>(y[0], y[1], y[2], y[3], v.inv, v.top);
-      // Bytes of slots that are new, and of those before them.
-      const int n0 = min(max(lo - j0 - 4 * i, 0), 4), n1 = min(max(end - j0 - 4 * i, 0), 4);
-      const unsigned below = n0 == 4 ? ~0u : (1u << (8 * n0)) - 1u;
-      const unsigned upto = n1 == 4 ? ~0u : (1u << (8 * n1)) - 1u;
-      const unsigned old = old_v[h][i];
-      const unsigned had = v.ratio != 1.f ? recode4<kE4m3>(old, v.ratio, v.top) : old;
-      out[i] = (w & upto & ~below) | (had & below) | (old & ~upto);
-    }
-    *reinterpret_cast<u32x2*>(vp + 64 * h) = out;
   }
   if (lane == 0) {
-    p.ks[sat] = k.s;
-    p.vs[sat] = v.s;
+    if (kKeys) p.ks[at.scale] = ks.s;
+    if (kValues) p.vs[at.scale] = vs.s;
   }
 }
 

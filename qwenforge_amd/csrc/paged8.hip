@@ -1,9 +1,10 @@
 // Tokens quantised into paged caches held in 8 bits, slots read back, pages copied
 // (gfx950; the format is qf_paged8.h's).
 //
-// A wave takes one block of 16 slots of one kv head, K and V (kv8_block.h).  Four waves
-// are a workgroup, so a page's 64-byte lines of V are written on one CU.
+// A wave takes one block of 16 slots of one kv head, K and V or one of them
+// (kv8_block.h).  Four waves are a workgroup.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8_block.h"
 
@@ -11,6 +12,7 @@ namespace qf {
 namespace kv8 {
 
 constexpr int kWaves = 4;
+constexpr int64_t kApartMost = 1500;   // blocks of one kv head
 
 struct RowsArgs {
   Pool p;
@@ -96,12 +98,14 @@ __device__ __forceinline__ Unit find_unit(const RowsArgs& a, int id) {
 }
 
 // Bound by the loads that wait for each other -- the rows' offsets, the table, tokens and old
-// codes -- 4.8 us for one token of 32 rows; 4 rows of 8192 tokens (25 MB) in 9, 2.8 TB/s.
-template <bool kE4m3, bool kSingle>
+// codes.  kApart: a wave has a block's keys or its values, else both (one token of 32 rows
+// 4.2 us, with both 4.8; one row of 2048 tokens 5.0 and 5.3; 4 rows of 8192, 25 MB, 10.9
+// and 9.3, 2.7 TB/s).
+template <bool kE4m3, bool kSingle, bool kApart>
 __global__ __launch_bounds__(64 * kWaves) void append_kernel(RowsArgs a) {
-  const int id = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+  const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
   const int hk = blockIdx.y % a.p.kvh, layer = blockIdx.y / a.p.kvh;
-  const Unit u = find_unit<kSingle>(a, id);
+  const Unit u = find_unit<kSingle>(a, kApart ? w >> 1 : w);
   if (u.n <= 0 || u.lo < 0) return;
   const int slot0 = u.block << 4;                       // of the block
   const int lp = slot0 >> a.p.log2p;
@@ -112,7 +116,10 @@ __global__ __launch_bounds__(64 * kWaves) void append_kernel(RowsArgs a) {
                     a.v + layer * a.v_sl + hk * a.v_sh + u.tok * a.v_sn, a.v_sn,
                     a.cos == nullptr ? nullptr : a.cos + u.tok * a.cs_sn,
                     a.cos == nullptr ? nullptr : a.sin + u.tok * a.cs_sn, a.cs_sn};
-  append_block<kE4m3>(a.p, layer, hk, a.p.table[u.row * a.p.t_sb + lp], slot0, u.lo, end, t);
+  const int page = a.p.table[u.row * a.p.t_sb + lp];
+  if (!kApart) append_block<kE4m3, true, true>(a.p, layer, hk, page, slot0, u.lo, end, t);
+  else if (w & 1) append_block<kE4m3, false, true>(a.p, layer, hk, page, slot0, u.lo, end, t);
+  else append_block<kE4m3, true, false>(a.p, layer, hk, page, slot0, u.lo, end, t);
 }
 
 // A wave a block, the heads of a block side by side, so that a token's heads are written
@@ -244,16 +251,20 @@ int qf::kv8::append(const QfRows8& h, int cap, hipStream_t st) {
   a.sin = static_cast<const f16*>(h.sin);
   a.cs_sn = h.cs_sn;
   a.cap = std::min(a.cap, cap);
-  const dim3 grid((unsigned)((blocks + kWaves - 1) / kWaves), (unsigned)(h.pool.KVH * h.pool.layers));
-  const dim3 block(64 * kWaves);
-  const bool e4m3 = h.pool.code == QF_CODE_E4M3;
-  if (h.max_seqlen == 1) {
-    if (e4m3) hipLaunchKernelGGL((append_kernel<true, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((append_kernel<false, true>), grid, block, 0, st, a);
-  } else {
-    if (e4m3) hipLaunchKernelGGL((append_kernel<true, false>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((append_kernel<false, false>), grid, block, 0, st, a);
-  }
+  // Apart until the waves are more than run at once.
+  const int64_t pairs = h.pool.KVH * h.pool.layers;
+  const bool e4m3 = h.pool.code == QF_CODE_E4M3, apart = blocks * pairs <= kApartMost;
+  const dim3 grid((unsigned)(((apart ? 2 : 1) * blocks + kWaves - 1) / kWaves), (unsigned)pairs), block(64 * kWaves);
+  const auto launch = [&](auto code, auto single) {
+    if (apart) hipLaunchKernelGGL((append_kernel<code.value, single.value, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((append_kernel<code.value, single.value, false>), grid, block, 0, st, a);
+  };
+  const auto by_code = [&](auto single) {
+    if (e4m3) launch(std::true_type{}, single);
+    else launch(std::false_type{}, single);
+  };
+  if (h.max_seqlen == 1) by_code(std::true_type{});
+  else by_code(std::false_type{});
   return (int)hipGetLastError();
 }
 

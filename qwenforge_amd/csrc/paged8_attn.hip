@@ -469,20 +469,23 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Unit& u, Sourc
   }
 }
 
-// The unit's row's new tokens into its slots [first, end), a wave a block.  The waves of
-// a workgroup share a first-level cache: past the barrier they see what was written.
+// The unit's row's new tokens into its slots [first, end), one wave for a block's keys and one
+// for its values.  The waves of a workgroup share a first-level cache: past the barrier they
+// see what was written.
 template <bool kE4m3, bool kDecode>
 __device__ __forceinline__ void append_tokens(const AttnArgs& a, const Unit& u, const Source& src, int first,
                                               int end) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
-  for (int s0 = (first / kBlock + w) * kBlock; s0 < end; s0 += nw * kBlock) {
-    const int from = max(s0, first);
+  for (int s0 = (first / kBlock + w / 2) * kBlock; s0 < end; s0 += nw / 2 * kBlock) {
+    const int from = max(s0, first), to = min(end - s0, kBlock);
     const int64_t token = u.tok0 + from - first;
     const bool turn = !kDecode && a.cos != nullptr;
     const Tokens t = {a.kn + token * a.kn_st + u.hk * a.kn_sh, a.kn_st, a.vn + token * a.vn_st + u.hk * a.vn_sh,
                       a.vn_st, turn ? a.cos + token * a.cs_sn : nullptr, turn ? a.sin + token * a.cs_sn : nullptr,
                       a.cs_sn};
-    append_block<kE4m3>(a.p, 0, u.hk, src.row[s0 >> a.p.log2p], s0, from - s0, min(end - s0, kBlock), t);
+    const int page = src.row[s0 >> a.p.log2p];
+    if (w & 1) append_block<kE4m3, false, true>(a.p, 0, u.hk, page, s0, from - s0, to, t);
+    else append_block<kE4m3, true, false>(a.p, 0, u.hk, page, s0, from - s0, to, t);
   }
   s_waitcnt_vm(0);
   __threadfence_block();
