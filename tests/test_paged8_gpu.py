@@ -265,6 +265,32 @@ def test_layers_at_once(dev, code):
 
 
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("rows,longest", [(9, 1), (9, 37), (70, 1), (3, 700)])
+def test_many_layers_at_once(dev, rows, longest, code):
+    """More blocks than run at once, of new rows and of begun ones, with RoPE: as one layer at a time."""
+    gen = torch.Generator().manual_seed(110 + rows + longest)
+    layers, kvh, page = 24, 8, 64
+    lens = [longest] + [max(1, longest - 5 * r) if longest > 1 else 1 for r in range(1, rows)]
+    ctx = [[0, 5, 16, -1, 31, 77][r % 6] for r in range(rows)]
+    need = [max(c, 0) + n for n, c in zip(lens, ctx)]
+    n_pages = sum(-(-n // page) for n in need)
+    pools = make_pools(gen, n_pages, kvh, page, code, dev, layers=layers)
+    table, _ = make_table(gen, need, page, n_pages, -(-max(need) // page), dev)
+    total = sum(lens)
+    k, v = (spread(gen, layers, total, kvh, D).to(dev) for _ in range(2))
+    ang = torch.rand(total, 32, generator=gen) * 6
+    cos, sin = (torch.cat([f(ang), f(ang)], dim=1).half().to(dev) for f in (torch.cos, torch.sin))
+    cu = torch.tensor([sum(lens[:i]) for i in range(rows + 1)], dtype=torch.int32, device=dev)
+    at = torch.tensor(ctx, device=dev)
+    one = tuple(t.clone() for t in pools)
+    paged8.append_paged8(k, v, cu, longest, at, cos, sin, pools, table, lengths=lens)
+    for i in range(layers):
+        paged8.append_paged8(k[i], v[i], cu, longest, at, cos, sin, tuple(t[i] for t in one), table, lengths=lens)
+    for a, b in zip(pools, one):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
 def test_read_is_packed(dev, code):
     """Rows from the middle of blocks, empty, parked and past their pages."""
     gen = torch.Generator().manual_seed(11)
