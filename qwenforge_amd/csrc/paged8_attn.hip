@@ -1016,8 +1016,8 @@ Plan decode_plan(int B, int KVH, int cap) {
 // - where one unit of up to 32 query rows has all of a short row's queries, it appends the
 //   row's tokens too: 4 rows of 3 tokens behind 1000 slots 12.0, by a launch of its own
 //   13.0 (calls from Python 12.4 and 15.3); 32 of 2 behind 2000 15.3 and 17.8.  48 query
-//   rows take a wave longer than the launch unless the units fill the CUs: 4 of 5 behind
-//   2000 18.8 and 15.9, 64 of 5 behind 1000 16.2 and 18.6;
+//   rows take a wave longer than the launch unless there are units enough: 4 of 5 behind
+//   2000 18.4 and 15.6, 16 behind 1000 14.4 and 14.4, 32 15.0 and 16.0, 64 16.2 and 18.6;
 // - wide, in even pieces of all units (kv8_pieces.h), where those have 48 tiles or more, or
 //   24 of rows of 120: 2048 tokens behind 16384 slots 205, with each unit in as many equal
 //   ranges as fill the CUs once 214; 1750 tokens 169 and 193, 2400 218 and 289, 1024 behind
@@ -1056,7 +1056,7 @@ Plan extend_plan(int B, int KVH, int G, int total, int max_seqlen, int cap) {
   if (rows > 64 && n_units >= 3 * kCus / 2) return plan(8, 1);
   const int cols = rows <= 16 || (rows <= 64 && tiles <= 64) ? 1
                    : units(48) >= kCus && cap >= 4 * (int64_t)max_seqlen ? 3 : 2;
-  if (tiles <= 32 && (rows <= 32 || (rows <= 48 && (int64_t)B * KVH >= kCus / 2))) {
+  if (tiles <= 32 && (rows <= 32 || (rows <= 48 && (int64_t)B * KVH >= kCus / 4))) {
     Plan p = plan((int)((rows + 15) / 16), 1);
     p.appends = true;
     p.waves = 8;
