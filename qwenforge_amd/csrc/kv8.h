@@ -2,6 +2,7 @@
 #pragma once
 
 #include "qf_common.h"
+#include "kv8_pieces.h"
 #include "../../include/qf_paged8.h"
 
 namespace qf {
@@ -123,12 +124,12 @@ int check_rows(const QfRows8& rows);
 // qf_append_paged8 into the rows' slots below cap (paged8.hip).
 int append(const QfRows8& rows, int cap, hipStream_t st);
 
-// The sum of x over the lanes up to this one.
+// The sum of x >= 0 over the lanes up to this one, held at the largest int.
 __device__ __forceinline__ int scan_sum(int x) {
   const int lane = threadIdx.x & 63;
   for (int d = 1; d < 64; d <<= 1) {
     const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
+    if (lane >= d) x = add_capped(x, y);
   }
   return x;
 }

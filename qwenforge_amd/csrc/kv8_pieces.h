@@ -24,6 +24,15 @@ constexpr int kUnitRows = 128;
 constexpr int kUnitTiles = 2;      // what a unit's beginning and end cost, in tiles of 64 slots
 constexpr int kLeastCut = 4 * 64;  // slots on either side of a cut
 constexpr int kLeastTiles = 8;     // of a piece
+constexpr int kMostWork = (1 << 30) - 1;   // of a call's line
+
+// A sum of what is not negative, held at the largest int.  Offsets of rows are read on the
+// device, and those that overlap give sums that no check on the host bounds: one that
+// wrapped would make places out of range.
+QF_HD int add_capped(int a, int b) {
+  const unsigned s = (unsigned)a + (unsigned)b;
+  return (int)(s < 0x7fffffffu ? s : 0x7fffffffu);
+}
 
 // A row's units: unit q of a kv head costs first + 2 q (its newest token is number
 // 128 (q + 1) / G or so).
@@ -72,10 +81,22 @@ QF_HD int cut_slot(int off, int seen, int G, int shift) {
   return s < kLeastCut ? 0 : seen - s < kLeastCut ? seen : s;
 }
 
+// The line of a call whose units cost `sum` (add_capped).  Rows that do not overlap cost no
+// more than kMostWork; of others what lies past it is left out.
+QF_HD int line_length(int sum) { return sum < kMostWork ? sum : kMostWork; }
+
 QF_HD int piece_length(int work, int pieces, int G, int shift) {
   const int even = (int)((unsigned)(work + pieces - 1) / (unsigned)pieces);
   const int least = shift > 0 ? G : kLeastTiles * G;
   return even > least ? even : least;
+}
+
+// The piece of a workgroup, `pieces` being a multiple of 8: neighbouring pieces share an XCD
+// (workgroups go to the XCDs in turn) and its L2; those that have work are spread over all XCDs.
+QF_HD int piece_of(int workgroup, int pieces, int work, int len) {
+  const int eighth = (int)((unsigned)((work + len - 1) / len + 7) / 8u), nth = workgroup / 8;
+  return nth < eighth ? workgroup % 8 * eighth + nth
+                      : 8 * eighth + workgroup % 8 * (pieces / 8 - eighth) + nth - eighth;
 }
 
 // The unit of a row's kv head that has `x` of its line.

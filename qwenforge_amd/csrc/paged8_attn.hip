@@ -608,19 +608,17 @@ __device__ __forceinline__ bool find_piece(const AttnArgs& a, int& piece, int& x
     return __builtin_amdgcn_readlane(upto, 63);
   };
   int work = rows_from(0);
-  for (int i0 = 64; i0 < a.B; i0 += 64) work += rows_from(i0);
+  for (int i0 = 64; i0 < a.B; i0 += 64) work = add_capped(work, rows_from(i0));
+  work = line_length(work);
   len = same(piece_length(work, a.pieces, a.G, a.shift));
-  // Neighbouring pieces share an XCD (workgroups go to the XCDs in turn) and its L2; those
-  // that have work are spread over all XCDs.
-  const int eighth = same((int)((unsigned)((work + len - 1) / len + 7) / 8u)), nth = blockIdx.x / 8;
-  piece = nth < eighth ? blockIdx.x % 8 * eighth + nth : 8 * eighth + blockIdx.x % 8 * (a.pieces / 8 - eighth) + nth - eighth;
+  piece = same(piece_of((int)blockIdx.x, a.pieces, work, len));
   x = piece * len;
   end = min(x + len, work);
   if (x >= work) return false;
   int before = 0, i0 = 0;
   if (a.B > 64) rows_from(0);
   for (;;) {
-    const uint64_t hit = __ballot(x < before + upto);
+    const uint64_t hit = __ballot(x < add_capped(before, upto));
     if (hit != 0) {
       const int j = __builtin_ctzll(hit);
       int base = before + __builtin_amdgcn_readlane(upto - mine, j);
@@ -633,7 +631,7 @@ __device__ __forceinline__ bool find_piece(const AttnArgs& a, int& piece, int& x
       set_place(a, u, base + cost_before(u.w, u.q));
       return true;
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    before = add_capped(before, __builtin_amdgcn_readlane(upto, 63));
     i0 += 64;
     if (i0 >= a.B) return false;
     rows_from(i0);
