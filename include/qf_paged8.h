@@ -67,7 +67,8 @@ typedef struct {
 } QfPool8;
 
 /* Packed tokens of B rows: row b has tokens [cu_seqlens[b], cu_seqlens[b + 1]) of
- * `total`, at most max_seqlen, and they are its slots first[b * first_sb] + i. */
+ * `total`, at most max_seqlen (of a longer row the first max_seqlen; the others are tokens
+ * of no row), and they are its slots first[b * first_sb] + i. */
 typedef struct {
   QfPool8 pool;
   void* k;                   /* (layers, T, KVH, D): strides per layer, head, token */
@@ -180,8 +181,8 @@ typedef struct {
  * row b attends to slots [0, first[b] + i] of its pages -- all of them as the pages
  * hold them, the new ones too.  cos and sin rotate q as well.
  *
- * Rows of out for tokens of no row, and past a row's max_seqlen, are left as they were;
- * those of a parked row become zero.  cap is at most pages_per_row * page_size, a
+ * Rows of out for tokens of no row are left as they were; those of a parked row become
+ * zero.  cap is at most pages_per_row * page_size, a
  * bound on every row's first + tokens, from which the work is split; tokens past it
  * are not appended and see the slots below.  ws as above,
  * qf_prefill_extend_paged8_workspace bytes.

@@ -23,7 +23,8 @@ struct RowsArgs {
   const int32_t* cu;
   const int64_t* first;      // first slot of each row's tokens
   int64_t first_sb;
-  int B, total, cap;         // slots of a row from cap on are not there
+  int B, total, longest;     // no row has more than `longest` tokens
+  int cap;                   // slots of a row from cap on are not there
   const f16* cos;
   const f16* sin;
   int64_t cs_sn;
@@ -40,10 +41,10 @@ __device__ __forceinline__ int blocks_of(int64_t first, int n) {
   return n <= 0 ? 0 : (int)(((first < 0 ? 0 : first) % kBlock + n + kBlock - 1) / kBlock);
 }
 
-// Tokens [lo, hi) of row r, any contents of cu kept within the tokens.
+// Tokens [lo, hi) of row r, any contents of cu kept within the tokens and the longest row.
 __device__ __forceinline__ void row_tokens(const RowsArgs& a, int r, int& lo, int& hi) {
   lo = clampi(a.cu[r], 0, a.total);
-  hi = clampi(a.cu[r + 1], lo, a.total);
+  hi = clampi(a.cu[r + 1], lo, min(a.total, lo + a.longest));
 }
 
 // The id-th of the blocks that the rows' tokens touch, counted row by row.  kSingle: no
@@ -55,9 +56,9 @@ __device__ __forceinline__ Unit find_unit(const RowsArgs& a, int id) {
     int lo, hi;
     row_tokens(a, id, lo, hi);
     const int64_t first = a.first[id * a.first_sb];
-    if (first < 0) return {id, lo, min(hi - lo, 1), -1, 0};
+    if (first < 0) return {id, lo, hi - lo, -1, 0};
     const int64_t block = first / kBlock;
-    return {id, lo, min(hi - lo, 1), (int)(first % kBlock),
+    return {id, lo, hi - lo, (int)(first % kBlock),
             (int)(block < 0x7fffffff / kBlock ? block : 0x7fffffff / kBlock)};
   }
   const int lane = threadIdx.x & 63;
@@ -215,7 +216,7 @@ int make_rows(RowsArgs& a, int64_t& blocks, const QfRows8& h) {
   a.cu = h.cu_seqlens;
   a.first = h.first;
   a.first_sb = h.first_sb;
-  a.B = (int)h.B; a.total = (int)h.total;
+  a.B = (int)h.B; a.total = (int)h.total; a.longest = (int)h.max_seqlen;
   a.cap = row_cap(a.p);
   // A row's n tokens touch at most n / 16 + 2 blocks, one of them if n is 1.
   blocks = h.max_seqlen == 1 ? h.B : h.total / kBlock + 2 * std::min(h.B, h.total);

@@ -264,7 +264,8 @@ def append_paged8(key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tens
 
     Packed key and value (T, KVH, 64) fp16; ``cu_seqlens`` (B + 1,) int32,
     ``max_seqlen`` and ``lengths`` as in ``paged.prefill_extend_paged`` (a row may
-    have no tokens); ``context`` (B,) int64 is read on the device, and a row with a
+    have no tokens; of one that the device's offsets make longer than ``max_seqlen``
+    the first ``max_seqlen`` are taken); ``context`` (B,) int64 is read on the device, and a row with a
     negative one (parked) appends nothing.  ``cos``/``sin`` (T, 64): key is rotated
     before it is quantised.  With key and value (layers, T, KVH, 64) and the pools of
     as many layers (``PagedKv8Cache.all_pools``), all layers' tokens at once.
