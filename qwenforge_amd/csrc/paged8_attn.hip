@@ -35,6 +35,16 @@ namespace kv8 {
 constexpr int kTile = 64;                    // slots
 constexpr int kMaxSplits = 64;
 
+// Weights are held in fp16 for the matrix cores, as 2^(score - reference).  A reference is
+// set kHeadroom below the score that moves it and moved when scores come to be more than
+// kSlack above that again, so the largest weight of a state is 2^7 to 2^13, and the absolute
+// steps of others, 2^-24 below fp16's normal range, are 2^-31 of it or less.  (With the
+// largest at 1 slots 18 nats below it round to nothing: of 5400 slots beside one such, all
+// that they weigh together, 1e-4, was lost.)  The 3 bits up to fp16's largest are for the
+// rounding of the scores, which is 2 at 2^25.  A slack of 4 moves references often enough to
+// take 2% longer where rows are many and short, one of 8 half a percent less.
+constexpr float kHeadroom = 7.f, kSlack = 6.f;
+
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 // A unit of 128 query rows that pieces have to be joined for: `more` partials behind the
@@ -147,7 +157,7 @@ struct State {
   f16x8 q[kNC][2];      // dims 16 g + 8 h ..
   int lim[kNC];
   int seen;             // every column sees [0, seen)
-  float m[kNC];         // log2 units
+  float m[kNC];         // references, log2 units
   f32x4 l[kNC];
   f32x4 o[kNC][4];
 };
@@ -250,14 +260,14 @@ __device__ __forceinline__ void attend_tile(State<kNC>& s, f32x4 (&sc)[kNC][4], 
         if (i >= left) sc[b][i / 4][i % 4] = kNegInf;
     }
     mx[b] = max16(sc[b]) * f[b];
-    grew = grew || mx[b] > s.m[b] + kRescaleSlack;
+    grew = grew || mx[b] > s.m[b] + (kHeadroom + kSlack);
   }
   // Moves the references of the columns whose own scores grew past them.
   if (__any(grew)) {
 #pragma unroll
     for (int b = 0; b < kNC; ++b) {
       const float top = col_max(mx[b]);
-      const float m_new = top > s.m[b] + kRescaleSlack ? top : s.m[b];
+      const float m_new = top > s.m[b] + (kHeadroom + kSlack) ? top - kHeadroom : s.m[b];
       const float c = m_new == s.m[b] ? 1.f : fast_exp2(s.m[b] - m_new);
       s.l[b] *= c;
 #pragma unroll
@@ -269,8 +279,9 @@ __device__ __forceinline__ void attend_tile(State<kNC>& s, f32x4 (&sc)[kNC][4], 
   f16x8 p[kNC][2];
 #pragma unroll
   for (int b = 0; b < kNC; ++b) {
-    // p is rounded to fp16 for the matrix cores (off by 2^-11 of it at most, as the output
-    // is by its own rounding), and the sum adds the rounded ones: the weights add to one.
+    // p is rounded to fp16 for the matrix cores (off by 2^-11 of it, as the output is by its own
+    // rounding, or by 2^-25: see kHeadroom), and the sum adds the rounded ones: the weights
+    // add to one.
     const float neg_m = s.m[b] == kNegInf ? 0.f : -s.m[b];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
