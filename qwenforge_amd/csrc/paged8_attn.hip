@@ -950,7 +950,7 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a) {
   int n = 0;   // splits that hold a slot below lim
   if (lim > 0) {
     const int len = ((end + kTile - 1) / kTile + a.splits - 1) / a.splits * kTile;
-    n = (lim + len - 1) / len;
+    n = (lim - 1) / len + 1;
   }
   const int64_t p0 = th * a.splits * a.G + g;
   // All of a lane's partials at once.  Those past n hold anything, but are there.

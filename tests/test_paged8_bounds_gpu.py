@@ -52,3 +52,22 @@ def test_overlapping_rows_that_cost_more_than_the_line_holds(dev, code, monkeypa
     want = kv8.attend(q.reshape(-1, D).cpu().double().numpy(), k, v)
     # Weights off by 2^-11 each way and the output by 2^-11 of the largest value, fp32 sums beside them.
     assert np.abs(got.reshape(-1, D).cpu().double().numpy() - want).max() <= 3.1 * 2.0 ** -11 * np.abs(v).max()
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_rows_of_two_to_the_31_slots(dev, code):
+    """The longest rows that the calls take, all of one page: their slots' mean is the page's."""
+    page, ppr = 4096, 524287
+    kv = paged8.PagedKv8Cache(1, 1, 1, page, 1, 1, dev, code)
+    one = torch.ones(page, 1, D, device=dev, dtype=torch.float16)
+    cu = torch.tensor([0, page], dtype=torch.int32, device=dev)
+    zero = torch.zeros(1, dtype=torch.int64, device=dev)
+    table = torch.zeros(1, ppr, dtype=torch.int32, device=dev)
+    paged8.append_paged8(0 * one, one, cu, page, zero, None, None, kv.pools[0], table[:, :1].contiguous())
+    q = torch.randn(2, 3, D, generator=torch.Generator().manual_seed(1)).half().to(dev)
+    last = torch.tensor([page * ppr - 1], device=dev)
+    got = paged8.flash_decode_attention_paged8(q[:1, None], kv.pools[0], table, last)
+    assert torch.equal(got, torch.ones_like(got))
+    cu = torch.tensor([0, 2], dtype=torch.int32, device=dev)
+    got = paged8.prefill_extend_paged8(q, 0 * one[:2], one[:2], cu, 2, last - 1, None, None, kv.pools[0], table)
+    assert torch.equal(got, torch.ones_like(got))
