@@ -34,6 +34,9 @@ namespace kv8 {
 
 constexpr int kTile = 64;                    // slots
 constexpr int kMaxSplits = 64;
+// Least factor of the scores: no scores of finite halves are told apart by it, and times a
+// block's scale (2^-24 or more) it is not zero, by which masked ones would become NaN.
+constexpr float kLeastFactor = 0x1p-100f;
 
 // Weights are held in fp16 for the matrix cores, as 2^(score - reference).  A reference is
 // set kHeadroom below the score that moves it and moved when scores come to be more than
@@ -1144,7 +1147,7 @@ int fill_args(AttnArgs& a, const void* q, const QfPool8& pool, const int64_t* la
   a.last = last;
   a.last_sb = last_sb;
   a.B = (int)B; a.tokens = (int)tokens; a.G = (int)G;
-  a.scale_log2 = (float)scale * kLog2e;
+  a.scale_log2 = std::max((float)scale * kLog2e, kLeastFactor);
   a.m_unit = 1.f;
   return QF_OK;
 }
