@@ -569,7 +569,7 @@ __device__ __forceinline__ bool extend_unit(const AttnArgs& a, Unit& u) {
 
 // Few query rows: the waves take the tiles in turn.  Bound by the vector unit and by
 // latency: 16 rows of 9 to 301 tokens behind 2048 slots, in e4m3, issue it 37% of the time
-// with 1.1 waves a SIMD on average (48 us; their products alone 16), as rows end unevenly.
+// with 1.1 waves a SIMD on average (50 us; their products alone 16), as rows end unevenly.
 template <bool kE4m3, int kNC>
 __global__ __launch_bounds__(512, 2) void extend_kernel(AttnArgs a) {
   extern __shared__ f32x4 lds[];
@@ -681,9 +681,12 @@ struct Progress {
 //
 // What bounds it: a wave-step (32 query rows x 64 slots) is 36 matrix instructions of 16
 // cycles and some 180 vector ones, 32 of them exponentials; with three waves a SIMD the
-// vector unit issues 56% of the time, the matrix cores run 32% of it, and the clock is
-// lowered (2.0 GHz with int8 codes, 2.4 without load).  2048 tokens behind 16384 slots:
-// 620 to 660 TF/s in int8, 730 in e4m3.
+// vector unit issues 55% of the time, the matrix cores run 32% of it, and the clock is
+// lowered (2.0 GHz with int8 codes, 2.4 without load).  In even pieces the 168 registers of
+// three waves a SIMD are too few for the walk from unit to unit: 26 are spilled in int8, 21
+// in e4m3.  A reload behind each tile's exponentials waits for all loads that are out, and
+// in int8 every second tile waits for the K codes that it has just asked for, to spill them.
+// 2048 tokens behind 16384 slots: 620 to 660 TF/s in int8, 730 in e4m3.
 template <bool kE4m3, bool kEven>
 __device__ __forceinline__ void wide_unit(const AttnArgs& a, const Unit& u, int part, Progress& pr,
                                           f16x8 (&lds)[2][16][64]) {

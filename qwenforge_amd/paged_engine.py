@@ -203,7 +203,8 @@ class PagedDecodeEngine(DecodeEngine):
         ``rows[:, step]`` receives each replay's tokens (``n_cols`` columns).
         ``share_rows``: attention may share its workgroups out by the rows'
         lengths (``ops.flash_decode_attention``); without it a row's results do
-        not depend on the other rows.  ``prefix`` = (prefix_rows, prefix_len,
+        not depend on the other rows.  Over caches in 8 bits it changes nothing:
+        every row is cut into as many ranges.  ``prefix`` = (prefix_rows, prefix_len,
         prefix_table) of ``paged.flash_decode_attention_prefix_paged``: the step
         attends with it, the shared slots read once."""
         cfg = self.cfg
